@@ -308,6 +308,106 @@ int tf_attention_decode(const void* qkv, int32_t batch, int32_t heads, int32_t h
                         void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* paged key/value cache                                                      */
+
+/* Keys and values of one layer in pages shared by all requests: page p holds
+ * page_size consecutive tokens of one request as [kv_heads][page_size]
+ * [head_dim], and page p + 1 starts page_stride elements later (k and v may
+ * be interleaved in one buffer).  A request's pages are listed in its row of
+ * a page table: token t sits in slot t % page_size of page
+ * table[request][t / page_size].  dtype f16 or bf16; head_dim 64 or 128;
+ * page_size 8, 16, 32, 64, 128 or 256; k, v 16-byte aligned, page_stride a
+ * multiple of 8.  No counterpart in the reference, whose MLXSequenceCache
+ * (patches/executorch.patch:3357-3405) reserves one contiguous buffer for
+ * each request. */
+typedef struct tf_paged_kv {
+  void* k;
+  void* v;
+  int64_t pages;
+  int64_t page_stride;
+  int32_t kv_heads;
+  int32_t page_size;
+  int32_t head_dim;
+  int32_t dtype;
+} tf_paged_kv;
+
+/* Page table: int32 device memory, row r (of `requests`) starts at
+ * ids + r * stride and lists up to `columns` pages. */
+typedef struct tf_page_table {
+  const int32_t* ids;
+  int64_t stride;
+  int32_t requests;
+  int32_t columns;
+} tf_page_table;
+
+/* New tokens into the pages.  qkv: act [rows] rows of (heads + 2 kv_heads) *
+ * head_dim values q | k | v, `qkv_stride` values apart (a multiple of 8).
+ * Row r is the token at positions[r] of request requests[r] (int32 device
+ * arrays).  q and k are normalised over their full widths when q_norm / k_norm
+ * (f16 [heads * head_dim] / [kv_heads * head_dim]; both or neither) are given,
+ * then rotated by halves with base rope_theta (0: no rotation); k and v are
+ * written to the row's slot and q to q_out (act [rows][heads * head_dim]).
+ * All arithmetic is fp32 (the rotation's angle fp64) with one rounding at the
+ * end.  A row whose request, position or page id lies outside the table or
+ * the cache stores no key and no value; rows of one call must not share a
+ * slot.  heads * head_dim <= 16384. */
+int tf_paged_append(const void* qkv, int64_t qkv_stride, int64_t rows, int32_t heads, int act, const void* q_norm,
+                    const void* k_norm, float eps, float rope_theta, const int32_t* positions,
+                    const int32_t* requests, const tf_page_table* table, const tf_paged_kv* kv, void* q_out,
+                    void* stream);
+
+/* Plan of one attention call: how its rows and keys are divided over the
+ * GPU.  It depends on the lengths and the geometry alone, so a serving loop
+ * makes one plan per step and uses it in every layer.  The caller keeps the
+ * struct (plain data, filled by tf_paged_plan_size) and a device copy of the
+ * table that tf_paged_plan_fill writes to host memory. */
+typedef struct tf_paged_plan {
+  int64_t rows;             /* query rows of all requests                    */
+  size_t table_bytes;       /* device table, 16-byte aligned                 */
+  size_t workspace_bytes;   /* device scratch of a call (no initial contents) */
+  int64_t positions_offset; /* int32 [rows] inside the table: each row's
+                               position (kv length - new length + i)         */
+  int64_t requests_offset;  /* int32 [rows] inside the table: its request    */
+  int64_t segments_offset;
+  int64_t blocks_offset;
+  int32_t requests;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t page_size;
+  int32_t columns;          /* page-table columns the longest request needs  */
+  int32_t split_blocks;     /* thread blocks of the few-rows kernel          */
+  int32_t split_parts;      /* partial results it leaves for merging         */
+  int32_t counters;
+} tf_paged_plan;
+
+/* new_lengths[i] query rows and kv_lengths[i] cached tokens (the new ones
+ * included) for request i; host arrays.  Lengths of zero are allowed, and so
+ * is a kv length below the new length: the rows before token 0 attend
+ * nothing. */
+int tf_paged_plan_size(const int32_t* new_lengths, const int32_t* kv_lengths, int32_t requests, int32_t heads,
+                       int32_t kv_heads, int32_t head_dim, int32_t page_size, tf_paged_plan* plan);
+int tf_paged_plan_fill(const int32_t* new_lengths, const int32_t* kv_lengths, const tf_paged_plan* plan, void* table,
+                       size_t table_bytes);
+
+/* Attention of the planned rows over the pages (workspace): row i of request
+ * r attends keys 0 .. kv_len - new_len + i of that request,
+ * out = softmax(q K^T * scale) V, query head h reading key head
+ * h / (heads / kv_heads).  q: act rows of heads * head_dim values, q_stride
+ * apart (a multiple of 8); out: act [rows][heads * head_dim].  The cache has
+ * the activations' dtype, or f16 under bf16 activations (q is then rounded to
+ * f16).  A row that attends nothing, or whose every score is -inf, gives
+ * zeros; NaN and +inf scores give NaN.  Slots past a request's length are
+ * never used, whatever they hold.  plan_table is the device copy of the
+ * table; calls that overlap in time need tables and workspaces of their own
+ * (the kernels count arrivals in the table and leave it as they found it).
+ * Replaces the SDPA of MLXNativeGraniteMoEPrefill.h:471-483 for a paged
+ * cache. */
+int tf_paged_attention(const void* q, int64_t q_stride, const tf_page_table* table, const tf_paged_kv* kv,
+                       const tf_paged_plan* plan, void* plan_table, float scale, int act, void* out, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* model and session                                                          */
 
 /* OLMoE geometry; NativeModelConfig (overlays/executorch/backends/mlx/runtime/

@@ -47,6 +47,23 @@ class OLMoEConfig(C.Structure):
                 ("act", C.c_int32)]
 
 
+class PagedKV(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("pages", C.c_int64), ("page_stride", C.c_int64),
+                ("kv_heads", C.c_int32), ("page_size", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32)]
+
+
+class PageTable(C.Structure):
+    _fields_ = [("ids", C.c_void_p), ("stride", C.c_int64), ("requests", C.c_int32), ("columns", C.c_int32)]
+
+
+class PagedPlanDesc(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("table_bytes", C.c_size_t), ("workspace_bytes", C.c_size_t),
+                ("positions_offset", C.c_int64), ("requests_offset", C.c_int64), ("segments_offset", C.c_int64),
+                ("blocks_offset", C.c_int64), ("requests", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("page_size", C.c_int32), ("columns", C.c_int32),
+                ("split_blocks", C.c_int32), ("split_parts", C.c_int32), ("counters", C.c_int32)]
+
+
 P = C.c_void_p
 I32, I64, F32, SZ = C.c_int32, C.c_int64, C.c_float, C.c_size_t
 PSZ = C.POINTER(C.c_size_t)
@@ -109,6 +126,12 @@ SIGNATURES = {
     "tf_gather_rows": [P, C.c_int64, C.c_int32, P, C.c_int32, C.c_int64, C.c_int, P, P],
     "tf_session_capture": [P, P, P, C.c_int64],
     "tf_set_wait_limit": [C.c_int64],
+    "tf_paged_append": [P, I64, I64, I32, C.c_int, P, P, F32, F32, P, P, C.POINTER(PageTable), C.POINTER(PagedKV), P,
+                        P],
+    "tf_paged_plan_size": [P, P, I32, I32, I32, I32, I32, C.POINTER(PagedPlanDesc)],
+    "tf_paged_plan_fill": [P, P, C.POINTER(PagedPlanDesc), P, SZ],
+    "tf_paged_attention": [P, I64, C.POINTER(PageTable), C.POINTER(PagedKV), C.POINTER(PagedPlanDesc), P, F32,
+                           C.c_int, P, P, SZ, P],
 }
 
 _lib = None

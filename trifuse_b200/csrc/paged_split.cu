@@ -1,0 +1,537 @@
+// Paged attention for few packed rows per key head (single tokens, grouped
+// heads, short drafts): a memory-bound stream over the pages.
+//
+// out = softmax(q K^T * scale) V by one pass over the keys with a running
+// maximum m and sum l per row: a tile of scores s gives
+//   m' = max(m, max s),  O = O * 2^(m - m') + 2^(s - m') V,  l likewise,
+// in log2 units (scale * log2(e) folded into the scores' FMA).
+//
+// What bounds it: every key and value is read once (512 bytes per token and
+// key head at head_dim 128) against 2 * 16 * 128 multiply-adds per key on the
+// 16-row tile, so HBM is the bound and the products only have to keep out of
+// the way.  mma.sync m16n8k16 serves them from registers: a tcgen05 tile has
+// 128 rows of which at most 16 would be filled, and its scores would travel
+// through tensor memory for nothing.
+//
+// One block of four warps per SM walks its segments (paged.h).  The warps take
+// the segment's 32-key tiles in turn and never wait for one another inside a
+// segment: each has a ring of its own that lane-parallel TMA copies keep full
+// across segment boundaries (3 x 16 KB per warp in flight, 192 KB per SM; the
+// bandwidth-delay product needs about 45 KB per SM).  At a segment's end the
+// four warps' (m, l, O) are joined through shared memory, and the pieces of a
+// cut item through global memory by the last block to arrive.
+//
+// P is rounded to the cache's 16-bit type for the second product (its values
+// are at most 1, so its relative error is the type's, the same size as the
+// output's own rounding); scores, m, l and O stay fp32.
+#include <cuda.h>
+#include <math.h>
+#include <string.h>
+
+#include "common.cuh"
+#include "paged.h"
+#include "tc_ptx.cuh"
+
+namespace tf {
+
+namespace {
+
+using namespace tc;
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kRowBytes = 128;                        // one swizzled row: 64 values
+constexpr int kHalfBytes = kSplitKeys * kRowBytes;    // 64 columns of a tile's keys
+
+template <int D>
+struct Shape {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kTile = kHalves * kHalfBytes;  // bytes of a tile's keys (and of its values)
+  static constexpr int kStages = 384 / D;             // 48 KB per warp
+  static constexpr int kRing = kStages * 2 * kTile;
+  static constexpr int kPitch = D + 4;                // joined outputs: rows 4 words apart in the banks
+  static constexpr int kOffJoin = kWarps * kRing;
+  static constexpr int kOffStat = kOffJoin + kWarps * kSplitRows * kPitch * 4;
+  static constexpr int kOffBar = kOffStat + kWarps * kSplitRows * 2 * 4;
+  static constexpr int kSmem = kOffBar + kWarps * kStages * 8 + 16 + 1024;  // + alignment slack
+  static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
+};
+
+struct SplitParams {
+  CUtensorMap tm_k, tm_v;
+  const void* q;
+  int64_t q_stride;
+  const int32_t* ids;
+  int64_t ids_stride;
+  int32_t columns;
+  int32_t page_size;
+  int32_t page_shift;
+  int32_t box_rows;  // min(page_size, kSplitKeys)
+  int32_t group;     // query heads per key head
+  int32_t heads;
+  const PagedSegment* segments;
+  const int32_t* starts;
+  int* counters;
+  float* stat;  // [part][2][16]: m, l
+  float* part;  // [part][16][D]
+  void* out;
+  float scale_log2;
+  int* err;
+  const long long* wait_cycles;
+};
+
+// Waits for a phase of one of the warp's own copies, at most `limit` cycles.
+__device__ __forceinline__ bool wait_copy(uint64_t* bar, uint32_t parity, long long limit) {
+  const uint32_t suspend = limit < 2000000000LL ? 0u : kSuspendNs;  // a shortened limit polls
+  if (mbar_try(bar, parity, suspend)) return true;
+  const long long t0 = clock64();
+  while (clock64() - t0 < limit)
+    if (mbar_try(bar, parity, suspend)) return true;
+  return false;
+}
+
+__device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int x, int row, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+          "r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(page), "r"(smem_addr(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+template <typename C>
+__device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename C>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const C a = from_f<C>(lo), b = from_f<C>(hi);
+  uint32_t u;
+  if constexpr (sizeof(C) == 2) {
+    const uint16_t x = *reinterpret_cast<const uint16_t*>(&a), y = *reinterpret_cast<const uint16_t*>(&b);
+    u = (uint32_t)x | ((uint32_t)y << 16);
+  }
+  return u;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// max that keeps a NaN, so a row with a NaN score ends as NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// Weight of a part with maximum m against the joined maximum M: an empty part
+// (m = -inf) weighs nothing, also where every part is empty.
+__device__ __forceinline__ float part_weight(float m, float M) { return m == -INFINITY ? 0.f : exp2_fast(m - M); }
+
+// A warp's position in its block's work: tile `tile` of segment `seg`.
+struct Cursor {
+  int seg, end, tile, tile1;
+  int request, kv_head, kv_len;
+  __device__ __forceinline__ void load(const PagedSegment* s, int warp) {
+    const PagedSegment& g = s[seg];
+    tile = g.tile0 + warp;
+    tile1 = g.tile1;
+    request = g.request;
+    kv_head = g.kv_head;
+    kv_len = g.kv_len;
+  }
+  // Moves to the next tile that exists; false at the end of the block's work.
+  __device__ __forceinline__ bool settle(const PagedSegment* s, int warp) {
+    while (tile >= tile1) {
+      if (++seg >= end) return false;
+      load(s, warp);
+    }
+    return true;
+  }
+};
+
+template <typename T, typename C, int D>
+__global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_constant__ SplitParams p) {
+  using S = Shape<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t* ring = base + warp * S::kRing;
+  float* join = reinterpret_cast<float*>(base + S::kOffJoin);
+  float* stat = reinterpret_cast<float*>(base + S::kOffStat);  // [warp][2][16]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + S::kOffBar) + warp * S::kStages;
+  int* last_s = reinterpret_cast<int*>(base + S::kOffBar + kWarps * S::kStages * 8);
+
+  if (lane == 0) {
+    for (int i = 0; i < S::kStages; ++i) mbar_init(&bars[i], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
+
+  const int seg0 = p.starts[blockIdx.x], seg_end = p.starts[blockIdx.x + 1];
+  Cursor in;  // next tile to fetch
+  in.seg = seg0;
+  in.end = seg_end;
+  bool more = seg0 < seg_end;
+  if (more) {
+    in.load(p.segments, warp);
+    more = in.settle(p.segments, warp);
+  }
+  int fetched = 0, used = 0;
+
+  // Fetches one tile into the ring's next slot: lane i copies box i (of the
+  // tile's existing pages, keys before values, 64 columns each).
+  auto fetch = [&]() {
+    const int slot = fetched % S::kStages;
+    uint8_t* dst = ring + slot * 2 * S::kTile;
+    const int key0 = in.tile * kSplitKeys;
+    const int left = in.kv_len - key0;
+    const int want = left < kSplitKeys ? left : kSplitKeys;
+    const int boxes = (want + p.box_rows - 1) / p.box_rows;  // pages (or parts of one) that exist
+    const int box_bytes = p.box_rows * kRowBytes;
+    if (lane == 0) mbar_expect_tx(&bars[slot], (uint32_t)(boxes * box_bytes * S::kHalves * 2));
+    __syncwarp();
+    if (lane < boxes * S::kHalves * 2) {
+      const int b = lane / (S::kHalves * 2), what = lane % (S::kHalves * 2);
+      const int half = what % S::kHalves, is_v = what / S::kHalves;
+      const int key = key0 + b * p.box_rows;
+      const int column = key >> p.page_shift;
+      const int page = column < p.columns ? __ldg(p.ids + in.request * p.ids_stride + column) : -1;
+      const int row = in.kv_head * p.page_size + (key & (p.page_size - 1));
+      tma_page(dst + is_v * S::kTile + half * kHalfBytes + b * box_bytes, is_v ? &p.tm_v : &p.tm_k, half * 64, row,
+               page, &bars[slot]);
+    }
+    ++fetched;
+    in.tile += kWarps;
+    more = in.settle(p.segments, warp);
+  };
+  for (int i = 0; i < S::kStages && more; ++i) fetch();
+
+  const int g = lane >> 2, c2 = (lane & 3) * 2;  // MMA fragment row and column pair
+  const long long limit_cycles = *p.wait_cycles;
+  bool ok = true;
+  for (int seg = seg0; seg < seg_end; ++seg) {
+    const PagedSegment sg = p.segments[seg];
+    // Queries as the A operand: rows g and g + 8.
+    uint32_t qa[D / 16][4];
+    int limit[2];  // last key the rows see
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = g + 8 * i;
+      const int pr = sg.row0 + (r < sg.rows ? r : sg.rows - 1);
+      const int token = pr / p.group;
+      limit[i] = sg.kv_len - sg.new_len + token;
+      const T* qr = static_cast<const T*>(p.q) + (sg.q_row + token) * p.q_stride +
+                    (int64_t)(sg.kv_head * p.group + pr % p.group) * D;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t u = *reinterpret_cast<const uint32_t*>(qr + 16 * k + 8 * j + c2);
+          if constexpr (sizeof(T) == sizeof(C) && Act<T>::kDtype == Act<C>::kDtype) {
+            qa[k][2 * j + i] = u;
+          } else {
+            const T* t = reinterpret_cast<const T*>(&u);
+            qa[k][2 * j + i] = pack2<C>(to_f(t[0]), to_f(t[1]));
+          }
+        }
+    }
+    const int first_limit = sg.kv_len - sg.new_len + sg.row0 / p.group;  // what the first row sees
+    float o[D / 8][4];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (int tile = sg.tile0 + warp; tile < sg.tile1 && ok; tile += kWarps) {
+      const int slot = used % S::kStages;
+      ok = __all_sync(0xffffffffu, wait_copy(&bars[slot], (uint32_t)((used / S::kStages) & 1), limit_cycles));
+      if (!ok) {
+        if (lane == 0) atomicCAS(p.err, 0, 71);
+        break;
+      }
+      const uint32_t ks = smem_addr(ring + slot * 2 * S::kTile), vs = ks + S::kTile;
+      const int key0 = tile * kSplitKeys;
+      // Scores: 16 rows x 32 keys; a matrix of ldmatrix is 8 keys x 8 dims.
+      float s[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {  // 16 keys
+          uint32_t b[4];
+          const int row = 16 * n + (lane & 7) + ((lane >> 4) << 3);
+          const int chunk = (2 * k + ((lane >> 3) & 1)) & 7;
+          ldsm4(ks + (k >> 2) * kHalfBytes + row * kRowBytes + ((chunk ^ (row & 7)) << 4), b);
+          mma16816<C>(s[2 * n], qa[k], b[0], b[1]);
+          mma16816<C>(s[2 * n + 1], qa[k], b[2], b[3]);
+        }
+      }
+      float mx[2] = {-INFINITY, -INFINITY};
+      const bool ragged = key0 + kSplitKeys - 1 > first_limit;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float v = s[i][j] * p.scale_log2;
+          if (ragged && key0 + 8 * i + c2 + (j & 1) > limit[j >> 1]) v = -INFINITY;
+          s[i][j] = v;
+          mx[j >> 1] = max_nan(mx[j >> 1], v);
+        }
+      float keep[2], sub[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mx[i] = max_nan(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+        mx[i] = max_nan(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+        const float mn = max_nan(m[i], mx[i]);
+        // Rows that have seen no key yet keep m = -inf and add nothing.
+        sub[i] = mn == -INFINITY ? 0.f : mn;
+        keep[i] = exp2_fast(m[i] - sub[i]);
+        m[i] = mn;
+        l[i] *= keep[i];
+      }
+      uint32_t pa[2][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          e[j] = exp2_fast(s[i][j] - sub[j >> 1]);
+          l[j >> 1] += e[j];
+        }
+        pa[i >> 1][(i & 1) * 2] = pack2<C>(e[0], e[1]);
+        pa[i >> 1][(i & 1) * 2 + 1] = pack2<C>(e[2], e[3]);
+      }
+      if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          o[i][0] *= keep[0];
+          o[i][1] *= keep[0];
+          o[i][2] *= keep[1];
+          o[i][3] *= keep[1];
+        }
+      }
+      const int have = sg.kv_len - key0;
+      if (have < kSplitKeys) {
+        // Slots past the request's length hold anything, NaN included: 0 * NaN
+        // would reach the outputs, so their values become zeros.
+        uint8_t* v = ring + slot * 2 * S::kTile + S::kTile;
+        for (int i = have * kRowBytes / 16 + lane; i < kHalfBytes / 16; i += 32)
+#pragma unroll
+          for (int h = 0; h < S::kHalves; ++h)
+            *reinterpret_cast<uint4*>(v + h * kHalfBytes + 16 * i) = make_uint4(0, 0, 0, 0);
+        __syncwarp();
+      }
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {  // 16 dims
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {  // 16 keys
+          uint32_t b[4];
+          const int row = 16 * k + (lane & 15);
+          const int chunk = (2 * n + (lane >> 4)) & 7;
+          ldsm4_t(vs + (n >> 2) * kHalfBytes + row * kRowBytes + ((chunk ^ (row & 7)) << 4), b);
+          mma16816<C>(o[2 * n], pa[k], b[0], b[1]);
+          mma16816<C>(o[2 * n + 1], pa[k], b[2], b[3]);
+        }
+      }
+      // Every lane's shared loads fed an MMA above, so they have returned: the
+      // slot may be refilled.  Zeros written above precede the copy.
+      if (have < kSplitKeys) fence_proxy_async();
+      __syncwarp();
+      ++used;
+      if (more) fetch();
+    }
+
+    // Join the four warps' results.
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      if ((lane & 3) == 0) {
+        stat[warp * 32 + g + 8 * i] = m[i];
+        stat[warp * 32 + 16 + g + 8 * i] = l[i];
+      }
+      float* row = join + (warp * kSplitRows + g + 8 * i) * S::kPitch;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+        *reinterpret_cast<float2*>(row + 8 * n + c2) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+    }
+    __syncthreads();
+    for (int i = tid; i < sg.rows * D; i += kThreads) {
+      const int r = i / D, d = i % D;
+      float M = stat[r];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) M = max_nan(M, stat[w * 32 + r]);
+      float acc = 0.f, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = part_weight(stat[w * 32 + r], M);
+        acc = fmaf(f, join[(w * kSplitRows + r) * S::kPitch + d], acc);
+        sum = fmaf(f, stat[w * 32 + 16 + r], sum);
+      }
+      if (sg.part < 0) {
+        const int pr = sg.row0 + r;
+        T* orow = static_cast<T*>(p.out) + ((int64_t)(sg.q_row + pr / p.group) * p.heads + sg.kv_head * p.group +
+                                            pr % p.group) * D;
+        orow[d] = from_f<T>(sum == 0.f ? 0.f : acc / sum);
+      } else {
+        p.part[((int64_t)sg.part * kSplitRows + r) * D + d] = acc;
+        if (d == 0) {
+          p.stat[(int64_t)sg.part * 32 + r] = M;
+          p.stat[(int64_t)sg.part * 32 + 16 + r] = sum;
+        }
+      }
+    }
+    __syncthreads();
+    if (sg.part >= 0) {
+      // The last piece of these rows to finish merges all of them, in order.
+      if (tid == 0) {
+        __threadfence();
+        const int seen = atomicAdd(&p.counters[sg.counter], 1);
+        const int last = seen == sg.parts - 1;
+        if (last) p.counters[sg.counter] = 0;  // as the next call expects it
+        *last_s = last;
+      }
+      __syncthreads();
+      const bool last = *last_s != 0;
+      __syncthreads();
+      if (!last) continue;
+      __threadfence();
+      for (int i = tid; i < sg.rows * D; i += kThreads) {
+        const int r = i / D, d = i % D;
+        float M = -INFINITY;
+        for (int k = 0; k < sg.parts; ++k) M = max_nan(M, __ldcg(&p.stat[(int64_t)(sg.part0 + k) * 32 + r]));
+        float acc = 0.f, sum = 0.f;
+        for (int k = 0; k < sg.parts; ++k) {
+          const int64_t at = sg.part0 + k;
+          const float f = part_weight(__ldcg(&p.stat[at * 32 + r]), M);
+          acc = fmaf(f, __ldcg(&p.part[(at * kSplitRows + r) * D + d]), acc);
+          sum = fmaf(f, __ldcg(&p.stat[at * 32 + 16 + r]), sum);
+        }
+        const int pr = sg.row0 + r;
+        T* orow = static_cast<T*>(p.out) + ((int64_t)(sg.q_row + pr / p.group) * p.heads + sg.kv_head * p.group +
+                                            pr % p.group) * D;
+        orow[d] = from_f<T>(sum == 0.f ? 0.f : acc / sum);
+      }
+    }
+  }
+  // After an expired wait copies may still be in flight: they land before the
+  // block's shared memory goes to another (they always complete).
+  for (; used < fetched; ++used)
+    wait_copy(&bars[used % S::kStages], (uint32_t)((used / S::kStages) & 1), 2000000000LL);
+}
+
+template <typename T, typename C, int D>
+tf_status launch(const SplitParams& p, int blocks, cudaStream_t s) {
+  static PerDeviceOnce attr;
+  int dev = 0;
+  if (attr.needed(&dev)) {
+    TF_CUDA(cudaFuncSetAttribute(paged_split_kernel<T, C, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 Shape<D>::kSmem));
+    attr.mark(dev);
+  }
+  paged_split_kernel<T, C, D><<<blocks, kThreads, Shape<D>::kSmem, s>>>(p);
+  return check_launch("paged_split");
+}
+
+// cuTensorMapEncodeTiled, fetched from the driver at run time.
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static const EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  return fn;
+}
+
+}  // namespace
+
+tf_status make_page_map(void* map, const void* base, const tf_paged_kv& kv, int box_rows) {
+  const cuuint64_t dims[3] = {(cuuint64_t)kv.head_dim, (cuuint64_t)kv.kv_heads * kv.page_size, (cuuint64_t)kv.pages};
+  const cuuint64_t strides[2] = {(cuuint64_t)kv.head_dim * 2, (cuuint64_t)kv.page_stride * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+  const cuuint32_t elem[3] = {1, 1, 1};
+  const EncodeFn encode = encode_fn();
+  if (!encode) return set_error(TF_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const CUresult r = encode(
+      static_cast<CUtensorMap*>(map),
+      kv.dtype == TF_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+      const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(TF_ERR_CUDA, "paged attention: tensor map (%d)", (int)r);
+  return TF_OK;
+}
+
+tf_status launch_paged_split(const PagedArgs& a, cudaStream_t s) {
+  const tf_paged_plan& plan = *a.plan;
+  if (plan.split_blocks == 0) return TF_OK;
+  SplitParams p;
+  memset(&p, 0, sizeof(p));
+  p.box_rows = a.kv.page_size < kSplitKeys ? a.kv.page_size : kSplitKeys;
+  TF_TRY(make_page_map(&p.tm_k, a.kv.k, a.kv, p.box_rows));
+  TF_TRY(make_page_map(&p.tm_v, a.kv.v, a.kv, p.box_rows));
+  p.q = a.q;
+  p.q_stride = a.q_stride;
+  p.ids = a.table.ids;
+  p.ids_stride = a.table.stride;
+  p.columns = a.table.columns;
+  p.page_size = a.kv.page_size;
+  while ((1 << p.page_shift) < a.kv.page_size) ++p.page_shift;
+  p.group = plan.heads / plan.kv_heads;
+  p.heads = plan.heads;
+  p.segments = reinterpret_cast<const PagedSegment*>(a.plan_table + plan.segments_offset);
+  p.starts = reinterpret_cast<const int32_t*>(a.plan_table + plan.blocks_offset);
+  p.counters = reinterpret_cast<int*>(a.plan_table);
+  p.stat = reinterpret_cast<float*>(a.workspace);
+  p.part = p.stat + (int64_t)plan.split_parts * 2 * kSplitRows;
+  p.out = a.out;
+  p.scale_log2 = a.scale * kLog2e;
+  TF_TRY(tc_flags(&p.err, const_cast<long long**>(&p.wait_cycles)));
+#define TF_SPLIT(T, C)                                                                      \
+  return plan.head_dim == 128 ? launch<T, C, 128>(p, plan.split_blocks, s) : launch<T, C, 64>(p, plan.split_blocks, s)
+  if (a.act == TF_DTYPE_F16) TF_SPLIT(__half, __half);
+  if (a.kv.dtype == TF_DTYPE_F16) TF_SPLIT(__nv_bfloat16, __half);
+  TF_SPLIT(__nv_bfloat16, __nv_bfloat16);
+#undef TF_SPLIT
+}
+
+}  // namespace tf

@@ -16,7 +16,8 @@ import ctypes as C
 import torch
 from torch import Tensor
 
-from ._lib import (AffineWeight, DTYPE_BF16, DTYPE_F16, MoeArgs, RouterWeight, check, lib)
+from ._lib import (AffineWeight, DTYPE_BF16, DTYPE_F16, MoeArgs, PagedKV, PagedPlanDesc, PageTable, RouterWeight,
+                   check, lib)
 
 _ACT = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
 
@@ -420,6 +421,145 @@ def attention_decode(qkv: Tensor, q_norm: Tensor, k_norm: Tensor, positions: Ten
     check(lib().tf_attention_decode(_ptr(qkv.contiguous()), B, heads, D, _ptr(q_norm), _ptr(k_norm), eps,
                                     rope_theta, _ptr(pos), max_length, _ptr(k_cache), _ptr(v_cache), cap,
                                     scale, _act(qkv), _ptr(out), _ptr(ws), nb.value, _stream()))
+    return out
+
+
+# ---------------------------------------------------------------------------
+# paged key/value cache
+
+
+def _paged_kv(k_pages: Tensor, v_pages: Tensor) -> PagedKV:
+    """Descriptor of [pages, kv_heads, page_size, head_dim] caches; only the
+    first dimension may have a stride of its own."""
+    if k_pages.ndim != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+        raise ValueError("paged: k_pages and v_pages are [pages, kv_heads, page_size, head_dim] of one dtype")
+    if k_pages.dtype not in _ACT:
+        raise ValueError("paged: the cache must be float16 or bfloat16")
+    pages, heads, size, D = k_pages.shape
+    stride = k_pages.stride()
+    if stride != v_pages.stride() or stride[1:] != (size * D, D, 1):
+        raise ValueError("paged: a page must be contiguous, and k_pages and v_pages laid out alike")
+    return PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), pages, stride[0], heads, size, D, _ACT[k_pages.dtype])
+
+
+def _page_table(page_table: Tensor) -> PageTable:
+    if page_table.ndim != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1
+                                                                   and page_table.stride(1) != 1):
+        raise ValueError("paged: the page table is int32 [requests, pages] with contiguous rows")
+    requests, columns = page_table.shape
+    return PageTable(page_table.data_ptr(), max(page_table.stride(0), columns), requests, columns)
+
+
+def _same_device(*ts):
+    """Kernels launch on the current device's current stream: every tensor must live there."""
+    dev = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and (not t.is_cuda or t.device.index != dev):
+            _cuda(t)
+            raise ValueError("tensors must be on the current CUDA device")
+
+
+def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, positions: Tensor,
+                 requests: Tensor, heads: int, q_norm: Tensor | None = None, k_norm: Tensor | None = None,
+                 eps: float = 1e-5, rope_theta: float | None = None, out: Tensor | None = None) -> Tensor:
+    """New tokens into a paged cache: q and k RMS-normalised over their full
+    widths (when norms are given) and rotated by halves at ``positions`` (when
+    ``rope_theta`` is given), k and v written to the pages (updated in place),
+    q returned as [rows, heads, head_dim].
+
+    qkv: [rows, (heads + 2 kv_heads) * head_dim] rows q | k | v; positions and
+    requests: int32 [rows] on the device; page_table: int32 [requests, pages].
+    A row whose slot the table does not have is not stored."""
+    _same_device(qkv, k_pages, v_pages, page_table, positions, requests, q_norm, k_norm, out)
+    kv = _paged_kv(k_pages, v_pages)
+    D, width = kv.head_dim, (heads + 2 * kv.kv_heads) * kv.head_dim
+    if qkv.ndim != 2 or qkv.shape[1] != width:
+        raise ValueError("paged_append: qkv is [rows, (heads + 2 kv_heads) * head_dim]")
+    if qkv.stride(1) != 1 or qkv.stride(0) < width:
+        qkv = qkv.contiguous()
+    rows = qkv.shape[0]
+    for t in (positions, requests):
+        if t.dtype != torch.int32 or t.shape != (rows,) or not t.is_contiguous():
+            raise ValueError("paged_append: positions and requests are contiguous int32 [rows]")
+    for t, n in ((q_norm, heads * D), (k_norm, kv.kv_heads * D)):
+        if t is not None and (t.dtype != torch.float16 or t.shape != (n,) or not t.is_contiguous()):
+            raise ValueError("paged_append: norm weights are contiguous float16 over the full q and k widths")
+    if out is None:
+        out = torch.empty((rows, heads, D), dtype=qkv.dtype, device=qkv.device)
+    elif out.shape != (rows, heads, D) or out.dtype != qkv.dtype or not out.is_contiguous():
+        raise ValueError("paged_append: out is a contiguous [rows, heads, head_dim] of qkv's dtype")
+    table = _page_table(page_table)
+    check(lib().tf_paged_append(qkv.data_ptr(), qkv.stride(0) if rows > 1 else width, rows, heads, _act(qkv),
+                                None if q_norm is None else q_norm.data_ptr(),
+                                None if k_norm is None else k_norm.data_ptr(), eps,
+                                0.0 if rope_theta is None else rope_theta, positions.data_ptr(), requests.data_ptr(),
+                                table, kv, out.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    return out
+
+
+class PagedPlan:
+    """How one paged attention call is divided over the GPU, from the lengths
+    and the geometry alone: made once per step, used in every layer.
+
+    new_lengths[i] query rows and kv_lengths[i] cached tokens (the new ones
+    included) of request i, as sequences of ints.  ``positions`` and
+    ``requests`` are the rows' int32 device vectors for ``paged_append``.
+    The plan holds the calls' workspace, so calls that may run at the same
+    time (on several streams) need plans of their own."""
+
+    def __init__(self, new_lengths, kv_lengths, heads: int, kv_heads: int, head_dim: int, page_size: int,
+                 device=None):
+        n = len(new_lengths)
+        if len(kv_lengths) != n:
+            raise ValueError("paged plan: new_lengths and kv_lengths differ in length")
+        new, kv = (C.c_int32 * n)(*new_lengths), (C.c_int32 * n)(*kv_lengths)
+        self.desc = d = PagedPlanDesc()
+        check(lib().tf_paged_plan_size(new, kv, n, heads, kv_heads, head_dim, page_size, d))
+        host = torch.empty(max(d.table_bytes, 1), dtype=torch.uint8, pin_memory=True)
+        check(lib().tf_paged_plan_fill(new, kv, d, host.data_ptr(), d.table_bytes))
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        self.table = host.to(device, non_blocking=True)
+        self.workspace = torch.empty(max(d.workspace_bytes, 1), dtype=torch.uint8, device=device)
+        self._stream = torch.cuda.current_stream(device)
+        self._ready = self._stream.record_event()
+        self.rows, self.heads, self.head_dim = d.rows, heads, head_dim
+        at, size = d.positions_offset, 4 * d.rows
+        self.positions = self.table[at:at + size].view(torch.int32)
+        at = d.requests_offset
+        self.requests = self.table[at:at + size].view(torch.int32)
+
+    def _on(self, stream):
+        """Orders the plan's upload before work on another stream and keeps its memory until that work is done.
+        A capturing stream cannot wait for an event from outside; a graph's first replay comes after the
+        synchronization that opens its capture, and its owner keeps the plan."""
+        if stream != self._stream and not torch.cuda.is_current_stream_capturing():
+            stream.wait_event(self._ready)
+            self.table.record_stream(stream)
+            self.workspace.record_stream(stream)
+
+
+def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, plan: PagedPlan,
+                    scale: float | None = None, out: Tensor | None = None) -> Tensor:
+    """Attention of every request's new tokens over its pages: row i of a
+    request attends keys 0 .. kv_length - new_length + i; query heads share
+    key heads in groups.  q: [rows, heads, head_dim] (rows may be strided);
+    returns [rows, heads, head_dim].  Rows that attend nothing give zeros."""
+    _same_device(q, k_pages, v_pages, page_table, plan.table, out)
+    rows, heads, D = plan.rows, plan.heads, plan.head_dim
+    if q.shape != (rows, heads, D):
+        raise ValueError("paged_attention: q is [rows, heads, head_dim] of the plan")
+    if q.stride()[1:] != (D, 1) or q.stride(0) < heads * D or q.stride(0) % 8:
+        q = q.contiguous()
+    if out is None:
+        out = torch.empty((rows, heads, D), dtype=q.dtype, device=q.device)
+    elif out.shape != (rows, heads, D) or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("paged_attention: out is a contiguous [rows, heads, head_dim] of q's dtype")
+    stream = torch.cuda.current_stream()
+    plan._on(stream)
+    check(lib().tf_paged_attention(q.data_ptr(), q.stride(0) if rows > 1 else heads * D, _page_table(page_table),
+                                   _paged_kv(k_pages, v_pages), plan.desc, plan.table.data_ptr(),
+                                   D ** -0.5 if scale is None else scale, _act(q), out.data_ptr(),
+                                   plan.workspace.data_ptr(), plan.workspace.numel(), stream.cuda_stream))
     return out
 
 
