@@ -164,6 +164,25 @@ int tf_olmoe_topk_indices(const void* probs, int64_t rows, int32_t experts, int3
 int tf_take_along_last(const void* x, int64_t rows, int32_t width, const int32_t* indices,
                        int32_t k, int act, void* out, void* stream);
 
+/* What an answer reports about its tokens, from logits [rows] of `vocab`
+ * values (dtype f32, f16 or bf16) that start row_stride values apart:
+ *   logprob[r]  = log softmax(logits[r])[tokens[r]]
+ *   entropy[r]  = - sum p log p, in nats
+ *   rank[r]     = entries before tokens[r] in descending order (ties: lower
+ *                 index first); 0 is the argmax
+ *   top_logprob, top_token [rows][top]: the first `top` entries of that order
+ * tokens int64 [rows] on the device; the outputs are f32, f32, int32, f32 and
+ * int64.  top <= TF_MAX_TOP and <= vocab; with 0 the top arrays may be NULL.
+ * A token outside [0, vocab) gives logprob NaN and rank -1.  A row with a NaN
+ * or +inf logit, or nothing but -inf, gives NaN everywhere, rank -1, and its
+ * alternatives still in order (NaN last); single -inf logits have
+ * probability 0.  The rows need no alignment beyond the element's.  The
+ * reference's answers carry tokens only (patches/executorch.patch:1350-1353). */
+#define TF_MAX_TOP 64
+int tf_token_logprobs(const void* logits, int64_t row_stride, int64_t rows, int32_t vocab, int dtype,
+                      const int64_t* tokens, int32_t top, float* logprob, float* entropy, int32_t* rank,
+                      float* top_logprob, int64_t* top_token, void* stream);
+
 /* Top-k combine + residual: out[t] = act(residual[t] + act(sum_k act(y[inverse[t*k+j]]
  * * gates[t][j]))), the fp32 sum taken in k order from the k = 0 product.
  * y_sorted act [tokens*k][hidden] (rows in route-sort order), inverse int32

@@ -126,6 +126,7 @@ SIGNATURES = {
     "tf_gather_rows": [P, C.c_int64, C.c_int32, P, C.c_int32, C.c_int64, C.c_int, P, P],
     "tf_session_capture": [P, P, P, C.c_int64],
     "tf_set_wait_limit": [C.c_int64],
+    "tf_token_logprobs": [P, I64, I64, I32, C.c_int, P, I32, P, P, P, P, P, P],
     "tf_paged_append": [P, I64, I64, I32, C.c_int, P, P, F32, F32, P, P, C.POINTER(PageTable), C.POINTER(PagedKV), P,
                         P],
     "tf_paged_plan_size": [P, P, I32, I32, I32, I32, I32, C.POINTER(PagedPlanDesc)],

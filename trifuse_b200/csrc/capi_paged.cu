@@ -181,4 +181,23 @@ int tf_paged_attention(const void* q, int64_t q_stride, const tf_page_table* tab
   return launch_paged_split(a, st(stream));
 }
 
+int tf_token_logprobs(const void* logits, int64_t row_stride, int64_t rows, int32_t vocab, int dtype,
+                      const int64_t* tokens, int32_t top, float* logprob, float* entropy, int32_t* rank,
+                      float* top_logprob, int64_t* top_token, void* stream) {
+  if (!act_ok(dtype) && dtype != TF_DTYPE_F32)
+    return set_error(TF_ERR_INVALID_ARGUMENT, "token_logprobs: logits must be f32, f16 or bf16");
+  if (rows < 0 || vocab < 1 || vocab > 1 << 30 || row_stride < vocab)
+    return set_error(TF_ERR_SHAPE, "token_logprobs: rows %lld, vocab %d, stride %lld", (long long)rows, vocab,
+                     (long long)row_stride);
+  if (top < 0 || top > TF_MAX_TOP || top > vocab)
+    return set_error(TF_ERR_INVALID_ARGUMENT, "token_logprobs: top %d outside [0, min(%d, vocab)]", top, TF_MAX_TOP);
+  if (rows == 0) return TF_OK;
+  const size_t element = dtype == TF_DTYPE_F32 ? 4 : 2;
+  if (!logits || !tokens || !logprob || !entropy || !rank || (top && (!top_logprob || !top_token)) ||
+      reinterpret_cast<uintptr_t>(logits) % element)
+    return set_error(TF_ERR_INVALID_ARGUMENT, "token_logprobs: NULL or unaligned pointer");
+  return launch_token_logprobs(logits, row_stride, rows, vocab, dtype, tokens, top, logprob, entropy, rank,
+                               top_logprob, top_token, st(stream));
+}
+
 }  // extern "C"

@@ -214,6 +214,12 @@ int read_embed_error(bool clear);
 // tokens[r] = all(isfinite(logits[r])) ? argmax (lowest index on ties) : -1.
 tf_status launch_greedy(const float* logits, int64_t rows, int64_t vocab, int64_t* tokens, cudaStream_t s);
 
+// Log probability, entropy, rank and `top` alternatives of each row of logits
+// (dtype f32, f16 or bf16; rows row_stride values apart).
+tf_status launch_token_logprobs(const void* logits, int64_t row_stride, int64_t rows, int vocab, int dtype,
+                                const int64_t* tokens, int top, float* logprob, float* entropy, int32_t* rank,
+                                float* top_logprob, int64_t* top_token, cudaStream_t s);
+
 // y[i][:] = x[idx[i] / div][:] for i < n (act rows of `width`, width % 8 == 0).
 tf_status launch_gather_rows(const void* x, int64_t x_stride, const int32_t* idx, int div, int64_t n, int width,
                              int act, void* y, cudaStream_t s);

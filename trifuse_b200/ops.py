@@ -12,11 +12,12 @@ allocate outputs and scratch.
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 from torch import Tensor
 
-from ._lib import (AffineWeight, DTYPE_BF16, DTYPE_F16, MoeArgs, PagedKV, PagedPlanDesc, PageTable, RouterWeight,
+from ._lib import (AffineWeight, DTYPE_BF16, DTYPE_F16, DTYPE_F32, MoeArgs, PagedKV, PagedPlanDesc, PageTable, RouterWeight,
                    check, lib)
 
 _ACT = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
@@ -160,6 +161,49 @@ def greedy_tokens(logits: Tensor) -> Tensor:
     out = torch.empty(lc.shape[0], dtype=torch.int64, device=logits.device)
     check(lib().tf_greedy_tokens(_ptr(lc), lc.shape[0], V, _ptr(out), _stream()))
     return out.reshape(logits.shape[:-1])
+
+
+class TokenLogprobs(NamedTuple):
+    """What token_logprobs reports of each row."""
+    logprob: Tensor      # float32 [...]
+    entropy: Tensor      # float32 [...], nats
+    rank: Tensor         # int32 [...], 0 = argmax
+    top_logprob: Tensor  # float32 [..., top]
+    top_token: Tensor    # int64 [..., top]
+
+
+def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0) -> TokenLogprobs:
+    """Log probability of tokens [...] under logits [..., vocab] (float32,
+    float16 or bfloat16), the distribution's entropy, the token's rank, and the
+    ``top`` (at most 64) most probable tokens in order (ties: lower id first).
+
+    A token outside the vocabulary (-1 for "none") gives NaN and rank -1, as
+    does a row whose logits are NaN, +inf or all -inf."""
+    if logits.dtype != torch.float32 and logits.dtype not in _ACT:
+        raise ValueError("token_logprobs: logits must be float32, float16 or bfloat16")
+    if logits.ndim < 1 or tokens.shape != logits.shape[:-1] or tokens.dtype != torch.int64:
+        raise ValueError("token_logprobs: tokens are int64 with the shape of the logits' rows")
+    if type(top) is not int:
+        raise ValueError("token_logprobs: top is an int")
+    _same_device(logits, tokens)
+    shape, V = tokens.shape, logits.shape[-1]
+    if logits.ndim != 2:
+        logits = logits.reshape(-1, V)
+    if logits.stride(1) != 1 or logits.stride(0) < V:
+        logits = logits.contiguous()
+    rows = logits.shape[0]
+    tokens = tokens.contiguous()
+    dev = logits.device
+    scalars = torch.empty((3, rows), dtype=torch.float32, device=dev)
+    top_logprob = torch.empty((rows, top), dtype=torch.float32, device=dev) if top > 0 else scalars.new_empty((rows, 0))
+    top_token = torch.empty((rows, max(top, 0)), dtype=torch.int64, device=dev)
+    at = scalars.data_ptr()
+    check(lib().tf_token_logprobs(logits.data_ptr(), logits.stride(0) if rows > 1 else V, rows, V,
+                                  _ACT.get(logits.dtype, DTYPE_F32), tokens.data_ptr(), top, at, at + 4 * rows,
+                                  at + 8 * rows, top_logprob.data_ptr(), top_token.data_ptr(),
+                                  torch.cuda.current_stream().cuda_stream))
+    return TokenLogprobs(scalars[0].view(shape), scalars[1].view(shape), scalars[2].view(torch.int32).view(shape),
+                         top_logprob.view(*shape, top), top_token.view(*shape, top))
 
 
 def native_olmoe_softmax(x: Tensor) -> Tensor:
