@@ -7,22 +7,24 @@
 //   alternatives: the first k entries of that order (NaN last)
 //
 // What bounds it: each logit is read once; 50304 fp32 logits are 0.2 MB, 31 ns
-// of the whole GPU's bandwidth.  So the pass keeps every value in registers
-// for all of its uses: a tile of 8 vectors of 16 bytes a thread is loaded at
-// once, its maximum taken, then the exponentials and both sums relative to the
-// thread's running maximum (rescaled when that moves).  Differences are taken
-// before the scaling by log2 e, so the leading terms carry no rounding of m.
+// of the whole GPU's bandwidth, and with 16-bit logits the exponentials come
+// close behind (16 a clock on an SM: 0.7 of the time that the bytes take).  So
+// the pass spends about five issue slots a value: a tile of 8 vectors of 16
+// bytes a thread stays in registers for all of its uses while the next one
+// loads; the sums run on packed fp32 pairs against the thread's running
+// maximum (rescaled when that moves), and the maximum and the rank's
+// comparisons of 16-bit logits on packed pairs of their own type.
 //
 // The alternatives ride along as candidates: a composite key (ordered value
 // bits, then the inverted index) makes every entry distinct and ties fall to
 // the lowest index.  The first tile yields a lower bound of the k-th key (the
-// smallest over the warps of their ceil(k / 8)-th largest thread maximum: at
-// least k entries are at or above it), entries at or above the bound go to a
-// shared buffer, and pruning the buffer to its k best raises the bound to an
-// exact one.  After the first tile a thread whose maximum is below the bound
-// does nothing, so the pass stays a stream.  Should a tile's candidates not
-// fit the buffer (values in rising order, say), they enter in rounds of one
-// vector element a thread with a prune in between.
+// k-th largest of the warps' few largest thread maxima: k entries are at or
+// above it), entries at or above the bound go to a shared buffer, and pruning
+// the buffer to its k best raises the bound to an exact one.  After the first
+// tile a thread whose maximum is below the bound does nothing, so the pass
+// stays a stream.  Should the candidates not fit the buffer (values in rising
+// order, say), those since the last prune enter again in rounds of one entry a
+// thread with a prune in between.
 //
 // A row may be shared by a cluster of 1, 2, 4 or 8 blocks (few rows: the whole
 // GPU reads; one row of 50304 on one block would take its load latency 25
@@ -33,6 +35,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "tc_ptx.cuh"
 
 namespace tf {
 
@@ -42,7 +45,9 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kVectors = 8;     // 16-byte vectors a thread holds
+constexpr int kVectors = 8;     // 16-byte vectors of a thread's tile
+constexpr int kTile = kThreads * kVectors;
+constexpr int kStages = 2;      // tiles in shared memory
 constexpr int kMaxTop = 64;
 constexpr int kBuffer = 1024;   // candidates: the rounds need kMaxTop + kThreads, the cluster's join kMaxCluster * kMaxTop
 constexpr int kMaxCluster = 8;
@@ -61,6 +66,8 @@ struct LogprobParams {
   int32_t* rank;
   float* top_logprob;
   int64_t* top_token;
+  int* err;
+  const long long* wait_cycles;
 };
 
 // Order-preserving bits of a value: NaN lowest, then -inf; -0 counts as +0.
@@ -87,109 +94,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-template <typename T>
-struct Lane;
-template <>
-struct Lane<float> {
-  static constexpr int kPer = 4;
-  __device__ __forceinline__ static float get(const uint4& v, int i) {
-    return __uint_as_float(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w);
-  }
-  static constexpr uint32_t kNegInf = 0xff800000u;
-  __device__ __forceinline__ static float max_of(const uint4& v) {
-    return max_nan(max_nan(get(v, 0), get(v, 1)), max_nan(get(v, 2), get(v, 3)));
-  }
-};
-template <typename T>
-struct Lane16 {
-  static constexpr int kPer = 8;
-  __device__ __forceinline__ static uint32_t word(const uint4& v, int i) {
-    return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
-  }
-};
-template <>
-struct Lane<__half> : Lane16<__half> {
-  static constexpr uint32_t kNegInf = 0xfc00fc00u;
-  __device__ __forceinline__ static float get(const uint4& v, int i) {
-    const uint32_t w = word(v, i >> 1);
-    return __half2float(__ushort_as_half((unsigned short)((i & 1) ? w >> 16 : w & 0xffffu)));
-  }
-  __device__ __forceinline__ static float max_of(const uint4& v) {
-    const __half2* h = reinterpret_cast<const __half2*>(&v);
-    const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
-    return max_nan(__low2float(m), __high2float(m));
-  }
-};
-template <>
-struct Lane<__nv_bfloat16> : Lane16<__nv_bfloat16> {
-  static constexpr uint32_t kNegInf = 0xff80ff80u;
-  __device__ __forceinline__ static float get(const uint4& v, int i) {
-    const uint32_t w = word(v, i >> 1);
-    return __uint_as_float((i & 1) ? w & 0xffff0000u : w << 16);
-  }
-  __device__ __forceinline__ static float max_of(const uint4& v) {
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
-    return max_nan(__low2float(m), __high2float(m));
-  }
-};
-
-// Running sums relative to a maximum m, in log2 units: s = sum 2^d, w = sum d 2^d, d = (x - m) log2 e.
-struct Sums {
-  float m, s, w;
-  __device__ __forceinline__ void move(float to) {  // to >= m, or NaN
-    if (m == -INFINITY) {  // nothing but -inf so far: s = w = 0
-      m = to;
-    } else if (to != m) {
-      const float d = (m - to) * kLog2e, f = exp2_fast(d);
-      w = f == 0.f ? 0.f : f * fmaf(d, s, w);
-      s *= f;
-      m = to;
-    }
-  }
-  __device__ __forceinline__ void join(Sums o) {
-    const float to = max_nan(m, o.m);
-    move(to);
-    o.move(to);
-    s += o.s;
-    w += o.w;
-  }
-};
-
-struct Shared {
-  uint64_t buffer[kBuffer];
-  uint64_t best[kMaxTop];      // sorted k best of the last prune
-  uint64_t bound;              // entries below it are no candidates
-  int n;                       // candidates in the buffer
-  int overflow;
-  uint32_t warp_key[kWarps];
-  Sums warp_sums[kWarps];
-  int warp_before[kWarps];
-  Sums sums;   // the block's totals, which the cluster's first block collects
-  int before;
-};
-
-// Sorts the buffer's n distinct keys by counting, keeps the k best (in best[],
-// and at the buffer's front) and raises the bound.  Called by the whole block
-// after a barrier; ends with one.
-__device__ __forceinline__ void prune(Shared& sh, int k) {
-  const int n = sh.n;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint64_t mine = sh.buffer[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += sh.buffer[j] > mine;
-    if (rank < k) sh.best[rank] = mine;
-  }
-  __syncthreads();
-  const int keep = n < k ? n : k;
-  for (int i = threadIdx.x; i < keep; i += kThreads) sh.buffer[i] = sh.best[i];
-  if (threadIdx.x == 0) {
-    sh.n = keep;
-    if (n >= k) sh.bound = sh.best[k - 1] + 1;
-  }
-  __syncthreads();
-}
-
 __device__ __forceinline__ uint64_t pair(float a, float b) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -203,25 +107,208 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
 
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+// A 16-byte vector of logits: its values as floats, their maximum (NaN kept),
+// and how many lie above (or at) the given token's.
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int kPer = 4;
+  static constexpr uint32_t kNegInf = 0xff800000u;
+  __device__ __forceinline__ static float get(const uint4& v, int i) { return __uint_as_float(word(v, i)); }
+  __device__ __forceinline__ static float max_of(const uint4& v) {
+    return max_nan(max_nan(get(v, 0), get(v, 1)), max_nan(get(v, 2), get(v, 3)));
+  }
+  // Running maximum over vectors (NaN kept).
+  using Max = float;
+  __device__ __forceinline__ static Max lowest() { return -INFINITY; }
+  __device__ __forceinline__ static void raise(Max& m, const uint4& v) { m = max_nan(m, max_of(v)); }
+  __device__ __forceinline__ static float value(Max m) { return m; }
+  // Counts of values above (kAt: at or above) t, added up per thread.
+  using Count = int;
+  __device__ __forceinline__ static Count zero() { return 0; }
+  template <bool kAt>
+  __device__ __forceinline__ static void above(const uint4& v, float t, Count& n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n += kAt ? get(v, i) >= t : get(v, i) > t;
+  }
+  __device__ __forceinline__ static int total(Count n) { return n; }
+};
+template <typename T, typename T2>
+struct Vec16 {
+  static constexpr int kPer = 8;
+  __device__ __forceinline__ static float max_of(const uint4& v) {
+    Max m = lowest();
+    raise(m, v);
+    return value(m);
+  }
+  using Max = T2;
+  __device__ __forceinline__ static Max lowest() { return T2{from_f<T>(-INFINITY), from_f<T>(-INFINITY)}; }
+  __device__ __forceinline__ static void raise(Max& m, const uint4& v) {
+    const T2* h = reinterpret_cast<const T2*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __hmax2_nan(m, h[i]);
+  }
+  __device__ __forceinline__ static float value(Max m) { return max_nan(__low2float(m), __high2float(m)); }
+  // The comparisons give packed 0 and 1; a tile adds at most 4 * kVectors = 32
+  // to each half (bf16 counts exactly to 256).
+  using Count = T2;
+  __device__ __forceinline__ static Count zero() { return T2{from_f<T>(0.f), from_f<T>(0.f)}; }
+  template <bool kAt>
+  __device__ __forceinline__ static void above(const uint4& v, float t, Count& n) {
+    const T2* h = reinterpret_cast<const T2*>(&v);
+    const T tt = from_f<T>(t);  // exact: t is one of the row's values, or +inf
+    const T2 t2 = {tt, tt};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n = __hadd2(n, kAt ? __hge2(h[i], t2) : __hgt2(h[i], t2));
+  }
+  __device__ __forceinline__ static int total(Count n) { return (int)(__low2float(n) + __high2float(n)); }
+};
+template <>
+struct Vec<__half> : Vec16<__half, __half2> {
+  static constexpr uint32_t kNegInf = 0xfc00fc00u;
+  __device__ __forceinline__ static float get(const uint4& v, int i) {
+    const uint32_t w = word(v, i >> 1);
+    return __half2float(__ushort_as_half((unsigned short)((i & 1) ? w >> 16 : w & 0xffffu)));
+  }
+};
+template <>
+struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16, __nv_bfloat162> {
+  static constexpr uint32_t kNegInf = 0xff80ff80u;
+  __device__ __forceinline__ static float get(const uint4& v, int i) {
+    const uint32_t w = word(v, i >> 1);
+    return __uint_as_float((i & 1) ? w & 0xffff0000u : w << 16);
+  }
+};
+
+// Running sums relative to a maximum m, in log2 units: s = sum 2^d,
+// w = sum d 2^d, d = x log2 e + c by one fused multiply-add, c the rounded
+// -m log2 e.  At x = m that leaves a residue of c's rounding in d, the same for
+// every x; total() takes it out again (exactly, where one entry holds all of
+// the sum).  m = -inf: nothing but -inf so far.
+struct Sums {
+  float m, s, w;
+  __device__ __forceinline__ static float offset(float m) { return -__fmul_rn(m, kLog2e); }
+  __device__ __forceinline__ void move(float to) {  // to >= m, or NaN
+    if (m == -INFINITY) {
+      m = to;
+    } else if (to != m) {
+      const float d = offset(to) - offset(m), f = exp2_fast(d);
+      w = f == 0.f ? 0.f : f * fmaf(d, s, w);
+      s *= f;
+      m = to;
+    }
+  }
+  __device__ __forceinline__ void join(Sums o) {
+    const float to = max_nan(m, o.m);
+    move(to);
+    o.move(to);
+    s += o.s;
+    w += o.w;
+  }
+  // ln sum e^(x - m), and the entropy ln sum e^(x - m) - sum (x - m) p.
+  __device__ __forceinline__ void total(float& log_sum, float& entropy) const {
+    const float residue = fmaf(m, kLog2e, offset(m));
+    log_sum = logf(s / exp2_fast(residue));
+    entropy = log_sum - (w / s - residue) * kLn2;
+  }
+  // Adds a tile of vectors whose maximum is tmax.
+  template <typename T, int N>
+  __device__ __forceinline__ void add(const uint4 (&r)[N], float tmax) {
+    if (!(tmax <= m)) move(max_nan(m, tmax));
+    if (m == -INFINITY) return;
+    const float c = offset(m);
+    const uint64_t log2e = pair(kLog2e, kLog2e), c2 = pair(c, c);
+    uint64_t s2[2] = {0, 0}, w2[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < Vec<T>::kPer; j += 2) {
+        const uint64_t d = fma2(pair(Vec<T>::get(r[i], j), Vec<T>::get(r[i], j + 1)), log2e, c2);
+        float d0, d1;
+        unpair(d, d0, d1);
+        const uint64_t e = pair(exp2_fast(d0), exp2_fast(d1));
+        s2[(j >> 1) & 1] = add2(s2[(j >> 1) & 1], e);
+        w2[(j >> 1) & 1] = fma2(d, e, w2[(j >> 1) & 1]);
+      }
+    float a, b, tw;
+    unpair(add2(w2[0], w2[1]), a, b);
+    tw = a + b;
+    if (tw != tw) {
+      // A logit of -inf made 0 * -inf (or the row is NaN anyway): again, with
+      // d held above -150, where 2^d is zero in fp32.
+      tw = 0.f;
+#pragma unroll 1
+      for (int i = 0; i < N; ++i) {
+        uint4 v = r[0];
+#pragma unroll
+        for (int u = 1; u < N; ++u)
+          if (u == i) v = r[u];
+#pragma unroll
+        for (int j = 0; j < Vec<T>::kPer; ++j) {
+          const float d = fmaxf(fmaf(Vec<T>::get(v, j), kLog2e, c), -150.f);
+          tw = fmaf(d, exp2_fast(d), tw);
+        }
+      }
+    }
+    w += tw;
+    unpair(add2(s2[0], s2[1]), a, b);
+    s += a + b;
+  }
+};
+
+struct Shared {
+  uint64_t full[kStages], empty[kStages];
+  uint64_t buffer[kBuffer];
+  uint64_t best[kMaxTop];      // sorted k best of the last prune
+  int n;                       // candidates in the buffer
+  uint32_t warp_key[kMaxTop];  // the warps' largest thread maxima of the first tile
+  Sums warp_sums[kWarps];
+  int warp_before[kWarps];
+  Sums sums;   // the block's totals, which the cluster's first block collects
+  int before;
+};
+
+// Sorts the buffer's n distinct keys by counting and keeps the k best, in
+// best[] and at the buffer's front; returns the bound that they make (`bound`
+// while there are fewer than k).  Called by the whole block after a barrier;
+// ends with one.
+__device__ __forceinline__ uint64_t prune(Shared& sh, int k, uint64_t bound) {
+  const int n = sh.n;
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const uint64_t mine = sh.buffer[i];
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) rank += sh.buffer[j] > mine;
+    if (rank < k) sh.best[rank] = mine;
+  }
+  __syncthreads();
+  const int keep = n < k ? n : k;
+  for (int i = threadIdx.x; i < keep; i += kThreads) sh.buffer[i] = sh.best[i];
+  if (threadIdx.x == 0) sh.n = keep;
+  if (n >= k) bound = sh.best[k - 1] + 1;
+  __syncthreads();
+  return bound;
+}
+
 // Vector of kPer values from index e0, entries outside [0, V) read as -inf.
 template <typename T>
 __device__ __forceinline__ uint4 load_ragged(const T* x, int e0, int V) {
-  constexpr int kPer = Lane<T>::kPer;
+  constexpr int kPer = Vec<T>::kPer;
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    w[i] = Lane<T>::kNegInf;
+    w[i] = Vec<T>::kNegInf;
     if constexpr (kPer == 4) {
       if (e0 + i >= 0 && e0 + i < V) w[i] = reinterpret_cast<const uint32_t*>(x)[e0 + i];
     } else {
@@ -238,22 +325,67 @@ __device__ __forceinline__ uint4 load_ragged(const T* x, int e0, int V) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+__device__ __forceinline__ void copy_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          tc::smem_addr(dst)),
+      "l"(src), "r"(bytes), "r"(tc::smem_addr(bar))
+      : "memory");
+}
+
+// Waits for a slot's phase; after about a second (which only a stalled copy
+// could take) records an error code and goes on with what the slot holds.
+__device__ __forceinline__ void wait_slot(uint64_t* bar, uint32_t parity, const LogprobParams& p) {
+  if (tc::mbar_try(bar, parity)) return;
+  const long long t0 = clock64();
+  while (!tc::mbar_try(bar, parity))
+    if (clock64() - t0 > *p.wait_cycles) {
+      atomicCAS(p.err, 0, 72);
+      return;
+    }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const __grid_constant__ LogprobParams p) {
-  using L = Lane<T>;
+  using L = Vec<T>;
   constexpr int kPer = L::kPer;
+  extern __shared__ __align__(128) uint8_t ring[];  // [kStages][kTile] vectors
   __shared__ Shared sh;
   const cg::cluster_group cluster = cg::this_cluster();
   const int slices = (int)cluster.num_blocks(), slice = (int)cluster.block_rank();
-  const int64_t row = blockIdx.x / slices;
+  const int shift = __popc(slices - 1);  // slices is a power of two
+  const int64_t row = blockIdx.x >> shift;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
   const int V = p.vocab, k = p.top;
-  // Vectors are counted from the 16-byte boundary at or before the row.
+  // Vectors are counted from the 16-byte boundary at or before the row; those
+  // in [v_begin, v_end) of this slice lie wholly inside the row.  The row's
+  // ragged first and last vectors go to the first slice.
   const int head = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  const int vectors = (V + head + kPer - 1) / kPer;
-  const int v_begin = (int)((int64_t)vectors * slice / slices);
-  const int v_end = (int)((int64_t)vectors * (slice + 1) / slices);
+  const int whole0 = head ? 1 : 0, whole1 = (V + head) / kPer;
+  const int whole = whole1 > whole0 ? whole1 - whole0 : 0;
+  const int v_begin = whole0 + (int)(((int64_t)whole * slice) >> shift);
+  const int v_end = whole0 + (int)(((int64_t)whole * (slice + 1)) >> shift);
+  const int tiles = (v_end - v_begin + kTile - 1) / kTile;
+  const bool edges = slice == 0 && (head || (V + head) % kPer);
+
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      tc::mbar_init(&sh.full[i], 1);
+      tc::mbar_init(&sh.empty[i], kWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    sh.n = 0;
+  }
+  __syncthreads();
+  auto fetch = [&](int tile) {  // one thread
+    const int t0 = v_begin + tile * kTile, n = min(kTile, v_end - t0);
+    uint64_t* bar = &sh.full[tile % kStages];
+    tc::mbar_expect_tx(bar, (uint32_t)n * 16);
+    copy_bulk(ring + (tile % kStages) * (kTile * 16), x + ((int64_t)t0 * kPer - head), (uint32_t)n * 16, bar);
+  };
+  if (tid == 0)
+    for (int i = 0; i < kStages && i < tiles; ++i) fetch(i);
 
   const int64_t token64 = p.tokens[row];
   const bool given = token64 >= 0 && token64 < V;
@@ -265,186 +397,206 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const __grid_cons
     else
       xt = to_f(x[token]);
   }
-  if (tid == 0) {
-    sh.n = 0;
-    sh.overflow = 0;
-    sh.bound = 0;
-  }
-  __syncthreads();
 
   Sums acc = {-INFINITY, 0.f, 0.f};
   int before = 0;
   uint64_t bound = 0;
-  int kept = 0;  // candidates in the buffer when the tile began
-  for (int t0 = v_begin; t0 < v_end; t0 += kThreads * kVectors) {
-    uint4 r[kVectors];
+  float cut = -INFINITY;  // the bound's value: what is below is no candidate
+  int kept = 0;           // candidates that the last prune left
+  int group = v_begin;    // first vector after it
+  int crowded = 0;        // this thread saw more candidates than a prune is worth
+  auto set_bound = [&](uint64_t to) {
+    bound = to;
+    const uint32_t bits = (uint32_t)(to >> 32);
+    cut = bits ? order_value(bits) : -INFINITY;
+  };
+  // One vector's candidates.
+  auto offer = [&](const uint4& r, int e0) {
+    uint32_t some = 0;
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      const int v = t0 + tid + i * kThreads;
-      const int e0 = v * kPer - head;
-      if (v >= v_end)
-        r[i] = make_uint4(L::kNegInf, L::kNegInf, L::kNegInf, L::kNegInf);
-      else if (e0 >= 0 && e0 + kPer <= V)
-        r[i] = ld_stream_v4(x + e0);
-      else
-        r[i] = load_ragged<T>(x, e0, V);
+    for (int j = 0; j < kPer; ++j) some |= (L::get(r, j) < cut ? 0u : 1u) << j;
+    while (some) {
+      const int j = __ffs(some) - 1;
+      some &= some - 1;
+      float u = L::get(r, 0);
+#pragma unroll
+      for (int i = 1; i < kPer; ++i) u = i == j ? L::get(r, i) : u;
+      const uint64_t c = composite(u, (uint32_t)(e0 + j));
+      if (c < bound || e0 + j < 0 || e0 + j >= V) continue;
+      const int at = atomicAdd(&sh.n, 1);
+      if (at < kBuffer) sh.buffer[at] = c;
+      if (at >= 2 * k + 32) crowded = 1;
     }
-    float vmax[kVectors], tmax = -INFINITY;
+  };
+  auto rank_each = [&](const uint4& r, int e0) {
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      vmax[i] = L::max_of(r[i]);
-      tmax = max_nan(tmax, vmax[i]);
+    for (int j = 0; j < kPer; ++j) {
+      const float u = L::get(r, j);
+      before += u > xt || (u == xt && e0 + j >= 0 && e0 + j < token);
     }
-    // Sums.  d is held above -150, where 2^d is zero in fp32: a logit of -inf
-    // adds 0 to both sums and not 0 * -inf.
-    const float to = max_nan(acc.m, tmax);
-    acc.move(to);
-    if (to != -INFINITY) {
-      const uint64_t sub = pair(-to, -to), log2e = pair(kLog2e, kLog2e);
-      uint64_t s2[2] = {0, 0}, w2[2] = {0, 0};
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i)
-#pragma unroll
-        for (int j = 0; j < kPer; j += 2) {
-          float d0, d1;
-          unpair(mul2(add2(pair(L::get(r[i], j), L::get(r[i], j + 1)), sub), log2e), d0, d1);
-          d0 = fmaxf(d0, -150.f);
-          d1 = fmaxf(d1, -150.f);
-          const uint64_t e = pair(exp2_fast(d0), exp2_fast(d1));
-          s2[i & 1] = add2(s2[i & 1], e);
-          w2[i & 1] = fma2(pair(d0, d1), e, w2[i & 1]);
-        }
-      float a, b;
-      unpair(add2(s2[0], s2[1]), a, b);
-      acc.s += a + b;
-      unpair(add2(w2[0], w2[1]), a, b);
-      acc.w += a + b;
-    }
-    // Rank of the given token.
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      const int v = t0 + tid + i * kThreads, e0 = v * kPer - head;
-      if (vmax[i] < xt || v >= v_end) continue;
-      if (e0 > token) {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) before += L::get(r[i], j) > xt;
-      } else if (e0 >= 0 && e0 + kPer <= token) {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) before += L::get(r[i], j) >= xt;
-      } else {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const float v = L::get(r[i], j);
-          before += v > xt || (v == xt && e0 + j >= 0 && e0 + j < token);
-        }
-      }
-    }
-    if (k == 0) continue;
-    // Candidates.
-    if (t0 == v_begin) {
-      const int each = (k + kWarps - 1) / kWarps;
-      uint32_t key = t0 + tid < v_end ? order_bits(tmax) : 0u, kth = 0;
-      for (int i = 0; i < each; ++i) {
-        kth = __reduce_max_sync(0xffffffffu, key);
-        const uint32_t who = __ballot_sync(0xffffffffu, key == kth);
-        if (lane == __ffs(who) - 1) key = 0;
-      }
-      if (lane == 0) sh.warp_key[warp] = kth;
+  };
+  // Prunes the candidates of the vectors [group, to) if they became many (or
+  // the bound is still the rough first one).  Called by the whole block.
+  auto look = [&](int to, bool first) {
+    if (!__syncthreads_or(crowded || first)) return;
+    crowded = 0;
+    if (sh.n > kBuffer) {
+      // Those vectors again, kThreads entries at a time from memory.
       __syncthreads();
-      uint32_t low = sh.warp_key[0];
-#pragma unroll
-      for (int i = 1; i < kWarps; ++i) low = min(low, sh.warp_key[i]);
-      bound = (uint64_t)low << 32;
-      if (tid == 0) sh.bound = bound;
-    }
-    const uint32_t bound_bits = (uint32_t)(bound >> 32);
-    const float cut = bound_bits ? order_value(bound_bits) : -INFINITY;
-    if (!(tmax < cut)) {
-      int count = 0;
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i) {
-        if (vmax[i] < cut) continue;
-        const int v = t0 + tid + i * kThreads, e0 = v * kPer - head;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j)
-          count += v < v_end && e0 + j >= 0 && e0 + j < V && composite(L::get(r[i], j), (uint32_t)(e0 + j)) >= bound;
-      }
-      if (count) {
-        int at = atomicAdd(&sh.n, count);
-        if (at + count > kBuffer) {
-          sh.overflow = 1;
-        } else {
-#pragma unroll
-          for (int i = 0; i < kVectors; ++i) {
-            if (vmax[i] < cut) continue;
-            const int v = t0 + tid + i * kThreads, e0 = v * kPer - head;
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-              const uint64_t c = composite(L::get(r[i], j), (uint32_t)(e0 + j));
-              if (v < v_end && e0 + j >= 0 && e0 + j < V && c >= bound) sh.buffer[at++] = c;
-            }
-          }
-        }
-      }
-    }
-    __syncthreads();
-    const int n = sh.n;
-    const bool overflow = sh.overflow != 0;
-    __syncthreads();
-    if (overflow) {
-      // The tile again, kThreads entries at a time from memory.
-      if (tid == 0) {
-        sh.n = kept;
-        sh.overflow = 0;
-      }
+      if (tid == 0) sh.n = kept;
       __syncthreads();
-      const int v_last = min(v_end, t0 + kThreads * kVectors);
-      const int e_last = min(V, v_last * kPer - head);
-      for (int e = t0 * kPer - head; e < e_last; e += kThreads) {
+      const int e_last = to * kPer - head;
+      for (int e = group * kPer - head; e < e_last; e += kThreads) {
         const int mine = e + tid;
-        if (mine >= 0 && mine < e_last) {
-          float v;
+        if (mine < e_last) {
+          float u;
           if constexpr (kPer == 4)
-            v = reinterpret_cast<const float*>(x)[mine];
+            u = reinterpret_cast<const float*>(x)[mine];
           else
-            v = to_f(x[mine]);
-          const uint64_t c = composite(v, (uint32_t)mine);
+            u = to_f(x[mine]);
+          const uint64_t c = composite(u, (uint32_t)mine);
           if (c >= bound) sh.buffer[atomicAdd(&sh.n, 1)] = c;
         }
         __syncthreads();
         const bool full = sh.n > kBuffer - kThreads;
         __syncthreads();
         if (full) {
-          prune(sh, k);
-          bound = sh.bound;
+          set_bound(prune(sh, k, bound));
         }
       }
-      prune(sh, k);
-      bound = sh.bound;
-    } else if (n > 2 * k + 32 || t0 == v_begin) {
-      prune(sh, k);
-      bound = sh.bound;
     }
-    kept = sh.n;
-    __syncthreads();
+    kept = min(sh.n, k);
+    set_bound(prune(sh, k, bound));
+    group = to;
+  };
+
+  for (int tile = 0; tile < tiles; ++tile) {
+    const int t0 = v_begin + tile * kTile, slot = tile % kStages;
+    const uint4* src = reinterpret_cast<const uint4*>(ring + slot * (kTile * 16)) + tid;
+    const bool full = t0 + kTile <= v_end;
+    wait_slot(&sh.full[slot], (uint32_t)((tile / kStages) & 1), p);
+    uint4 r[kVectors];
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+      r[i] = full || t0 + tid + i * kThreads < v_end
+                 ? src[i * kThreads]
+                 : make_uint4(L::kNegInf, L::kNegInf, L::kNegInf, L::kNegInf);
+    auto most = L::lowest();
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) L::raise(most, r[i]);
+    const float tmax = L::value(most);
+    // The tile is in registers: its slot may be refilled.
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(&sh.empty[slot]);
+    if (tid == 0 && tile + kStages < tiles) {
+      wait_slot(&sh.empty[slot], (uint32_t)((tile / kStages) & 1), p);
+      fetch(tile + kStages);
+    }
+    if (full) {
+      acc.add<T>(r, tmax);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) {
+        const uint4 one[1] = {r[i]};
+        if (t0 + tid + i * kThreads < v_end) acc.add<T>(one, L::max_of(r[i]));
+      }
+    }
+    if (!(tmax < xt)) {
+      const int first = t0 * kPer - head;  // entry of the tile's first value
+      if (full && first > token) {
+        auto n = L::zero();
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) L::template above<false>(r[i], xt, n);
+        before += L::total(n);
+      } else if (full && first + kTile * kPer <= token) {
+        auto n = L::zero();
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) L::template above<true>(r[i], xt, n);
+        before += L::total(n);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+          const int v = t0 + tid + i * kThreads, e0 = v * kPer - head;
+          if (v >= v_end) continue;
+          auto n = L::zero();
+          if (e0 > token)
+            L::template above<false>(r[i], xt, n);
+          else if (e0 + kPer <= token)
+            L::template above<true>(r[i], xt, n);
+          else
+            rank_each(r[i], e0);
+          before += L::total(n);
+        }
+      }
+    }
+    if (k == 0) continue;
+    if (tile == 0) {
+      // A first bound: see the top of the file.  A thread without a value
+      // stands for the lowest key.
+      const int each = min(kMaxTop / kWarps, (k + kWarps - 1) / kWarps + 2);
+      uint32_t key = t0 + tid < v_end ? order_bits(tmax) : 0u;
+      for (int i = 0; i < each; ++i) {
+        const uint32_t most = __reduce_max_sync(0xffffffffu, key);
+        const uint32_t who = __ballot_sync(0xffffffffu, key == most);
+        if (lane == __ffs(who) - 1) key = 0;
+        if (lane == 0) sh.warp_key[i * kWarps + warp] = most;
+      }
+      __syncthreads();
+      // The k-th largest of the up to 64 keys, two a lane, equal ones in list
+      // order; every warp finds it for itself.
+      const int n = each * kWarps;
+      uint32_t kth = 0;
+      for (int mine = lane; mine < n; mine += 32) {
+        const uint32_t own = sh.warp_key[mine];
+        int ahead = 0;
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+          const uint32_t other = sh.warp_key[i];
+          ahead += other > own || (other == own && i < mine);
+        }
+        if (ahead == k - 1) kth = own;
+      }
+      set_bound((uint64_t)__reduce_max_sync(0xffffffffu, kth) << 32);
+    }
+    if (!(tmax < cut)) {
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) {
+        const int v = t0 + tid + i * kThreads;
+        if (v < v_end && !(L::max_of(r[i]) < cut)) offer(r[i], v * kPer - head);
+      }
+    }
+    look(min(v_end, t0 + kTile), tile == 0);
+  }
+  if (edges) {
+    // Thread 0 takes the row's first ragged vector, thread 1 its last.
+    const int v = tid == 0 ? 0 : whole1;
+    const bool mine = tid == 0 ? head != 0 : tid == 1 && (V + head) % kPer && !(head && whole1 == 0);
+    if (mine) {
+      const int e0 = v * kPer - head;
+      const uint4 r[1] = {load_ragged<T>(x, e0, V)};
+      acc.add<T>(r, L::max_of(r[0]));
+      rank_each(r[0], e0);
+      if (k) offer(r[0], e0);  // fits: a look leaves at most 2 k + 32 candidates
+    }
   }
 
-  // Block totals.
+  // Block totals: to the warp's maximum, then plain sums.
+  float top_of = acc.m;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) top_of = max_nan(top_of, __shfl_xor_sync(0xffffffffu, top_of, off));
+  acc.move(top_of);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
-    Sums o;
-    o.m = __shfl_xor_sync(0xffffffffu, acc.m, off);
-    o.s = __shfl_xor_sync(0xffffffffu, acc.s, off);
-    o.w = __shfl_xor_sync(0xffffffffu, acc.w, off);
-    acc.join(o);
-    before += __shfl_xor_sync(0xffffffffu, before, off);
+    acc.s += __shfl_xor_sync(0xffffffffu, acc.s, off);
+    acc.w += __shfl_xor_sync(0xffffffffu, acc.w, off);
   }
+  before = __reduce_add_sync(0xffffffffu, before);
   if (lane == 0) {
     sh.warp_sums[warp] = acc;
     sh.warp_before[warp] = before;
   }
   __syncthreads();
-  if (k) prune(sh, k);
+  if (k) prune(sh, k, 0);
   if (tid == 0) {
     Sums t = sh.warp_sums[0];
     int b = sh.warp_before[0];
@@ -480,23 +632,26 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const __grid_cons
         __syncthreads();
         if (tid == 0) sh.n = at;
         __syncthreads();
-        prune(sh, k);
+        prune(sh, k, 0);
       }
     }
     cluster.sync();  // the other blocks' shared memory stays until it has been read
     if (slice != 0) return;
   }
   __syncthreads();
+  if (tid > 0 && tid >= k) return;
   const Sums t = sh.sums;
-  const bool finite = fabsf(t.m) < INFINITY;  // no NaN, no +inf, not all -inf
-  const float log_sum = logf(t.s);
+  const bool finite = fabsf(Sums::offset(t.m)) < INFINITY;  // no NaN, no +inf, not all -inf
+  float log_sum, entropy;
+  t.total(log_sum, entropy);
   const float nan = __uint_as_float(0x7fc00000u);
   if (tid == 0) {
     p.logprob[row] = finite && given ? (xt - t.m) - log_sum : nan;
-    p.entropy[row] = finite ? log_sum - t.w / t.s * kLn2 : nan;
+    p.entropy[row] = finite ? entropy : nan;
     p.rank[row] = finite && given ? sh.before : -1;
   }
-  for (int i = tid; i < k; i += kThreads) {
+  if (tid < k) {
+    const int i = tid;
     const uint64_t c = sh.best[i];
     p.top_logprob[row * k + i] = finite ? (order_value((uint32_t)(c >> 32)) - t.m) - log_sum : nan;
     p.top_token[row * k + i] = (int64_t)(0xffffffffu - (uint32_t)c);
@@ -505,9 +660,17 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const __grid_cons
 
 template <typename T>
 tf_status launch(const LogprobParams& p, int slices, cudaStream_t s) {
+  static PerDeviceOnce once;
+  int dev = 0;
+  if (once.needed(&dev)) {
+    TF_CUDA(cudaFuncSetAttribute(logprobs_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kStages * kTile * 16));
+    once.mark(dev);
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(p.rows * slices));
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kStages * kTile * 16;
   cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -527,8 +690,9 @@ tf_status launch_token_logprobs(const void* logits, int64_t row_stride, int64_t 
                                 float* top_logprob, int64_t* top_token, cudaStream_t s) {
   if (rows == 0) return TF_OK;
   if (rows > 2147483647 / kMaxCluster) return set_error(TF_ERR_UNSUPPORTED, "token_logprobs: too many rows");
-  const LogprobParams p = {logits, row_stride, tokens, rows, vocab, top, logprob, entropy, rank, top_logprob,
-                           top_token};
+  LogprobParams p = {logits, row_stride, tokens, rows, vocab, top, logprob, entropy, rank, top_logprob, top_token,
+                     nullptr, nullptr};
+  TF_TRY(tc_flags(&p.err, const_cast<long long**>(&p.wait_cycles)));
   // Blocks a row: enough to fill the GPU (about three blocks an SM), each
   // with at least one vector a thread.
   const int vectors = vocab / (dtype == TF_DTYPE_F32 ? 4 : 8);
