@@ -388,8 +388,11 @@ typedef struct tf_paged_plan {
   int64_t positions_offset; /* int32 [rows] inside the table: each row's
                                position (kv length - new length + i)         */
   int64_t requests_offset;  /* int32 [rows] inside the table: its request    */
-  int64_t segments_offset;
-  int64_t blocks_offset;
+  int64_t split_segments_offset; /* the rest: the kernels' work lists        */
+  int64_t split_starts_offset;
+  int64_t tile_segments_offset;
+  int64_t tile_starts_offset;
+  int64_t merges_offset;
   int32_t requests;
   int32_t heads;
   int32_t kv_heads;
@@ -397,8 +400,11 @@ typedef struct tf_paged_plan {
   int32_t page_size;
   int32_t columns;          /* page-table columns the longest request needs  */
   int32_t split_blocks;     /* thread blocks of the few-rows kernel          */
-  int32_t split_parts;      /* partial results it leaves for merging         */
-  int32_t counters;
+  int32_t split_parts;      /* partial results that its pieces leave         */
+  int32_t split_counters;
+  int32_t tile_blocks;      /* the same of the tensor-core kernel            */
+  int32_t tile_parts;
+  int32_t merges;           /* row blocks that were cut                      */
 } tf_paged_plan;
 
 /* new_lengths[i] query rows and kv_lengths[i] cached tokens (the new ones

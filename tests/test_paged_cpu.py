@@ -70,11 +70,13 @@ def test_attention_and_append_refuse_before_any_launch():
     assert append(rows=0) == 0
 
 
-def segments(d, raw):
+def segments(d, raw, kind):
     import struct
-    starts = struct.unpack_from(f"<{d.split_blocks + 1}i", raw, d.blocks_offset)
-    return [(b, struct.unpack_from("<13i", raw, d.segments_offset + 64 * i))
-            for b in range(d.split_blocks) for i in range(starts[b], starts[b + 1])]
+    blocks, first, at = ((d.split_blocks, d.split_starts_offset, d.split_segments_offset) if kind == "split" else
+                         (d.tile_blocks, d.tile_starts_offset, d.tile_segments_offset))
+    starts = struct.unpack_from(f"<{blocks + 1}i", raw, first)
+    return [(b, struct.unpack_from("<13i", raw, at + 64 * i))
+            for b in range(blocks) for i in range(starts[b], starts[b + 1])]
 
 
 def test_every_row_meets_every_tile_once():
@@ -85,26 +87,31 @@ def test_every_row_meets_every_tile_once():
         kv = [rng.choice([0, n, n + rng.randint(0, 20000), max(0, n - 3)]) for n in new]
         H, Hk = rng.choice([(16, 16), (8, 1), (14, 2), (32, 8)])
         _, d, raw = plan(new, kv, H, Hk)
-        seen, parts = {}, {}
-        for block, g in segments(d, raw):
-            q_row, n, L, req, head, row0, rows, t0, t1, part, part0, count, counter = g
-            assert n == new[req] and L == kv[req] and q_row == sum(new[:req])
-            assert 0 < rows and row0 + rows <= n * (H // Hk)
-            seen.setdefault((req, head, row0, rows), []).append((t0, t1))
-            if count > 1:
-                assert part0 <= part < part0 + count <= d.split_parts and 0 <= counter < d.counters
-                assert part not in parts
-                parts[part] = counter
-            else:
-                assert part == -1
-        assert len(parts) == d.split_parts
         rows_seen = {}
-        for (req, head, row0, rows), spans in seen.items():
-            spans.sort()
-            last = kv[req] - new[req] + (row0 + rows - 1) // (H // Hk)
-            assert spans[0][0] == 0 and spans[-1][1] == (0 if last < 0 else last // 32 + 1)
-            assert all(a[1] == b[0] for a, b in zip(spans, spans[1:]))
-            rows_seen[(req, head)] = rows_seen.get((req, head), 0) + rows
+        for kind, most, keys, all_parts in (("split", 16, 32, d.split_parts), ("tile", 256, 128, d.tile_parts)):
+            seen, parts, cut = {}, {}, set()
+            load = {}
+            for block, g in segments(d, raw, kind):
+                q_row, n, L, req, head, row0, rows, t0, t1, part, part0, count, counter = g
+                assert n == new[req] and L == kv[req] and q_row == sum(new[:req])
+                assert 0 < rows <= most and row0 + rows <= n * (H // Hk)
+                load[block] = load.get(block, 0) + t1 - t0
+                seen.setdefault((req, head, row0, rows), []).append((t0, t1))
+                if count > 1:
+                    assert part0 <= part < part0 + count <= all_parts and part not in parts
+                    parts[part] = counter
+                    cut.add(part0)
+                else:
+                    assert part == -1
+            assert len(parts) == all_parts
+            assert len(cut) == (d.split_counters if kind == "split" else d.merges)
+            assert len(load) <= 148
+            for (req, head, row0, rows), spans in seen.items():
+                spans.sort()
+                last = kv[req] - new[req] + (row0 + rows - 1) // (H // Hk)
+                assert spans[0][0] == 0 and spans[-1][1] == (0 if last < 0 else last // keys + 1)
+                assert all(a[1] == b[0] for a, b in zip(spans, spans[1:]))
+                rows_seen[(req, head)] = rows_seen.get((req, head), 0) + rows
         for r in range(B):
             for h in range(Hk):
                 assert rows_seen.get((r, h), 0) == new[r] * (H // Hk)

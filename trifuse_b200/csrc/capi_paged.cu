@@ -178,7 +178,8 @@ int tf_paged_attention(const void* q, int64_t q_stride, const tf_page_table* tab
   a.act = act;
   a.out = out;
   a.workspace = static_cast<char*>(workspace);
-  return launch_paged_split(a, st(stream));
+  TF_TRY(launch_paged_split(a, st(stream)));
+  return launch_paged_tile(a, st(stream));
 }
 
 int tf_token_logprobs(const void* logits, int64_t row_stride, int64_t rows, int32_t vocab, int dtype,

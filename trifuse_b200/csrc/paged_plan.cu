@@ -148,55 +148,77 @@ Layout lay_out(const std::vector<Item>& items, const Schedule& s, const int32_t*
   return out;
 }
 
-Layout plan_split(const int32_t* new_lengths, const int32_t* kv_lengths, const tf_paged_plan& p) {
+// The work of one kernel: requests of more than kSplitRows packed rows per key
+// head go to the tensor-core kernel (whose 128-row products take the same time
+// however few rows they hold), the others to the few-rows kernel.
+Layout plan_kernel(const int32_t* new_lengths, const int32_t* kv_lengths, const tf_paged_plan& p, bool tile) {
   const int G = p.heads / p.kv_heads;
+  const int block_rows = tile ? kTileRows : kSplitRows, keys = tile ? kTileKeys : kSplitKeys;
   std::vector<Item> items;
   int32_t q_row = 0;
   for (int r = 0; r < p.requests; ++r) {
     const int n = new_lengths[r], kv = kv_lengths[r];
-    for (int64_t row0 = 0; row0 < (int64_t)n * G; row0 += kSplitRows) {
-      const int rows = (int)std::min<int64_t>(kSplitRows, (int64_t)n * G - row0);
-      const int64_t last = (int64_t)kv - n + (row0 + rows - 1) / G;  // last key the rows see
-      const int32_t tiles = last < 0 ? 0 : (int32_t)(last / kSplitKeys + 1);
-      for (int h = 0; h < p.kv_heads; ++h) items.push_back({r, h, (int32_t)row0, rows, q_row, tiles});
-    }
+    const int64_t rows = (int64_t)n * G;
+    if ((rows > kSplitRows) == tile)
+      for (int64_t row0 = 0; row0 < rows; row0 += block_rows) {
+        const int take = (int)std::min<int64_t>(block_rows, rows - row0);
+        const int64_t last = (int64_t)kv - n + (row0 + take - 1) / G;  // last key the rows see
+        const int32_t tiles = last < 0 ? 0 : (int32_t)(last / keys + 1);
+        for (int h = 0; h < p.kv_heads; ++h) items.push_back({r, h, (int32_t)row0, take, q_row, tiles});
+      }
     q_row += n;
   }
-  return lay_out(items, divide(items, current_sms(), 4, 8), new_lengths, kv_lengths);
+  // A segment starts in the time of some four small or one large tile; a piece
+  // should be worth its partial result (a large tile's keys and values are as
+  // many bytes as half a partial result).
+  const Schedule s = tile ? divide(items, current_sms(), 1, 4) : divide(items, current_sms(), 4, 8);
+  return lay_out(items, s, new_lengths, kv_lengths);
 }
 
-}  // namespace
+struct Plans {
+  Layout split, tile;
+  std::vector<PagedSegment> merges;
+  Plans(const int32_t* new_lengths, const int32_t* kv_lengths, const tf_paged_plan& p)
+      : split(plan_kernel(new_lengths, kv_lengths, p, false)), tile(plan_kernel(new_lengths, kv_lengths, p, true)) {
+    for (const PagedSegment& g : tile.segments)
+      if (g.part >= 0 && g.part == g.part0) merges.push_back(g);
+  }
+};
 
-tf_status paged_plan_size(const int32_t* new_lengths, const int32_t* kv_lengths, tf_paged_plan* p) {
-  const Layout l = plan_split(new_lengths, kv_lengths, *p);
-  p->split_blocks = (int32_t)l.starts.size() - 1;
-  p->split_parts = l.parts;
-  p->counters = l.counters;
-  // Table: arrival counters (zero between calls), segments, block starts,
-  // positions, requests.
-  size_t at = align_up((size_t)l.counters * 4, 16);
-  p->segments_offset = (int64_t)at;
-  at += l.segments.size() * sizeof(PagedSegment);
-  p->blocks_offset = (int64_t)at;
-  at = align_up(at + l.starts.size() * 4, 16);
+template <typename V>
+size_t put(char* table, size_t at, const std::vector<V>& v) {
+  if (table && !v.empty()) memcpy(table + at, v.data(), v.size() * sizeof(V));
+  return align_up(at + v.size() * sizeof(V), 16);
+}
+
+// Lays the table out, and fills it where `table` is given: the few-rows
+// kernel's arrival counters (zero between calls), the two kernels' segments and
+// block starts, the cut row blocks, the rows' positions and requests.
+void put_table(const Plans& plans, const int32_t* new_lengths, const int32_t* kv_lengths, tf_paged_plan* p,
+               char* table) {
+  p->split_blocks = (int32_t)plans.split.starts.size() - 1;
+  p->split_parts = plans.split.parts;
+  p->split_counters = plans.split.counters;
+  p->tile_blocks = (int32_t)plans.tile.starts.size() - 1;
+  p->tile_parts = plans.tile.parts;
+  p->merges = (int32_t)plans.merges.size();
+  size_t at = put(table, 0, std::vector<int32_t>(plans.split.counters, 0));
+  p->split_segments_offset = (int64_t)at;
+  at = put(table, at, plans.split.segments);
+  p->split_starts_offset = (int64_t)at;
+  at = put(table, at, plans.split.starts);
+  p->tile_segments_offset = (int64_t)at;
+  at = put(table, at, plans.tile.segments);
+  p->tile_starts_offset = (int64_t)at;
+  at = put(table, at, plans.tile.starts);
+  p->merges_offset = (int64_t)at;
+  at = put(table, at, plans.merges);
   p->positions_offset = (int64_t)at;
   at = align_up(at + (size_t)p->rows * 4, 16);
   p->requests_offset = (int64_t)at;
   p->table_bytes = align_up(at + (size_t)p->rows * 4, 16);
-  // Workspace: per part and row the running max and sum, then the outputs.
-  p->workspace_bytes = (size_t)l.parts * kSplitRows * (2 + p->head_dim) * 4;
-  return TF_OK;
-}
-
-tf_status paged_plan_fill(const int32_t* new_lengths, const int32_t* kv_lengths, const tf_paged_plan* p,
-                          char* table) {
-  const Layout l = plan_split(new_lengths, kv_lengths, *p);
-  if (p->split_blocks != (int32_t)l.starts.size() - 1 || p->split_parts != l.parts || p->counters != l.counters ||
-      p->blocks_offset - p->segments_offset != (int64_t)(l.segments.size() * sizeof(PagedSegment)))
-    return set_error(TF_ERR_STATE, "paged plan: lengths or device differ from those the plan was sized for");
-  memset(table, 0, p->table_bytes);
-  memcpy(table + p->segments_offset, l.segments.data(), l.segments.size() * sizeof(PagedSegment));
-  memcpy(table + p->blocks_offset, l.starts.data(), l.starts.size() * 4);
+  p->workspace_bytes = split_workspace_bytes(*p) + (size_t)p->tile_parts * kTileRows * (2 + p->head_dim) * 4;
+  if (!table) return;
   int32_t* pos = reinterpret_cast<int32_t*>(table + p->positions_offset);
   int32_t* req = reinterpret_cast<int32_t*>(table + p->requests_offset);
   for (int r = 0; r < p->requests; ++r)
@@ -204,6 +226,24 @@ tf_status paged_plan_fill(const int32_t* new_lengths, const int32_t* kv_lengths,
       *pos++ = kv_lengths[r] - new_lengths[r] + i;
       *req++ = r;
     }
+}
+
+}  // namespace
+
+tf_status paged_plan_size(const int32_t* new_lengths, const int32_t* kv_lengths, tf_paged_plan* p) {
+  put_table(Plans(new_lengths, kv_lengths, *p), new_lengths, kv_lengths, p, nullptr);
+  return TF_OK;
+}
+
+tf_status paged_plan_fill(const int32_t* new_lengths, const int32_t* kv_lengths, const tf_paged_plan* p,
+                          char* table) {
+  const Plans plans(new_lengths, kv_lengths, *p);
+  tf_paged_plan again = *p;
+  put_table(plans, new_lengths, kv_lengths, &again, nullptr);
+  if (memcmp(&again, p, sizeof(again)))
+    return set_error(TF_ERR_STATE, "paged plan: lengths or device differ from those the plan was sized for");
+  memset(table, 0, p->table_bytes);
+  put_table(plans, new_lengths, kv_lengths, &again, table);
   return TF_OK;
 }
 

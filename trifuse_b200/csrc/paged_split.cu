@@ -518,8 +518,8 @@ tf_status launch_paged_split(const PagedArgs& a, cudaStream_t s) {
   while ((1 << p.page_shift) < a.kv.page_size) ++p.page_shift;
   p.group = plan.heads / plan.kv_heads;
   p.heads = plan.heads;
-  p.segments = reinterpret_cast<const PagedSegment*>(a.plan_table + plan.segments_offset);
-  p.starts = reinterpret_cast<const int32_t*>(a.plan_table + plan.blocks_offset);
+  p.segments = reinterpret_cast<const PagedSegment*>(a.plan_table + plan.split_segments_offset);
+  p.starts = reinterpret_cast<const int32_t*>(a.plan_table + plan.split_starts_offset);
   p.counters = reinterpret_cast<int*>(a.plan_table);
   p.stat = reinterpret_cast<float*>(a.workspace);
   p.part = p.stat + (int64_t)plan.split_parts * 2 * kSplitRows;

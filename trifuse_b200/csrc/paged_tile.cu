@@ -1,0 +1,732 @@
+// Paged attention for many packed rows per key head (prompt chunks, whole
+// prompts) on the sm_100a tensor cores: tcgen05 with scores, weights and
+// outputs in tensor memory, keys and values by TMA from the pages.
+//
+// out = softmax(q K^T * scale) V over 128-key tiles with a running maximum m
+// and sum l per row; per tile s = q K^T, P = 2^(s * scale * log2 e - m),
+// O += P V, l += sum P.  The maximum is refreshed lazily: a row keeps the m it
+// used until a tile raises it by more than 8 (log2 units), so P <= 256 and O
+// is rescaled only on such tiles; O / l is the same quotient.
+//
+// What bounds it: 4 D flops per (row, key) pair on the tensor cores, and one
+// exponential per pair on a unit that gives 16 a clock and SM, which is just
+// as long (128 x 128 pairs: 1024 clocks of either at D = 128).  Hence
+//   * a block holds two halves of 128 rows, each with a softmax warpgroup of
+//     its own (thread = row), so one half's products run while the other's
+//     exponentials do, and a quarter of the exponentials are cubics on the FMA
+//     pipe;
+//   * one block per SM walks the segments of the plan (paged.h) and the roles
+//     run ahead across them: the next segment's queries and first scores are
+//     computed while this one's outputs are written.
+//
+// Roles (384 threads; registers move from the third warpgroup to the softmax):
+//   warps 0-3, 4-7  softmax of half A, B: read S from tensor memory, mask, write
+//              P in 16 bits over S's first columns; at a segment's end read O
+//              and write out (or the piece's partial result).
+//   warp 8     MMA: one elected lane issues, tile by tile,
+//              O_A += P_A V; S_A = Q_A K'; O_B += P_B V; S_B = Q_B K'
+//              with K' the next tile.  MMAs of one thread execute in issue
+//              order, so a next S may be issued over a P that the product
+//              before it still reads, and its completion implies that product's.
+//   warp 9     loader: page ids and TMA of the K and V tiles (128-byte
+//              swizzle) into one ring of tiles, K and V in turn.
+//   warps 10, 11  queries of half A, B: 16-byte copies into swizzled rows
+//              (converted where the cache's type differs).
+// Tensor memory columns: O_A [0, 128), O_B [128, 256), S_A [256, 384), S_B.
+//
+// P is rounded to the cache's 16-bit type, relative 2^-11 (f16) or 2^-8
+// (bf16), the size of the output's own rounding; l sums the unrounded values.
+// Every wait is bounded; an expired one records an error code (tf_device_error)
+// and all roles stop.
+#include <cuda.h>
+#include <math.h>
+#include <string.h>
+
+#include "common.cuh"
+#include "paged.h"
+#include "tc_ptx.cuh"
+
+namespace tf {
+
+namespace {
+
+using namespace tc;
+
+constexpr int kHalf = 128;  // rows of a half = TMEM lanes
+constexpr int kThreads = 384;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kQueryWarp = 10;
+constexpr uint32_t kColO = 0, kColS = 256;  // half x: + 128 x
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescale = 8.f;
+constexpr int kColBytes = kTileKeys * 128;  // 64 columns of a tile: 128 rows of 128 bytes
+
+template <int D>
+struct Shape {
+  static constexpr int kTile = D / 64 * kColBytes;  // bytes of 128 rows or keys
+  static constexpr int kSlots = D == 128 ? 5 : 8;   // ring of K and V tiles
+  static constexpr int kOffRing = 2 * kTile;        // after the two halves' queries
+  static constexpr int kOffBar = kOffRing + kSlots * kTile;
+  static constexpr int kSmem = kOffBar + 256 + 1024;  // + barriers + alignment slack
+  static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
+};
+
+struct TileParams {
+  CUtensorMap tm_k, tm_v;
+  const void* q;
+  int64_t q_stride;
+  const int32_t* ids;
+  int64_t ids_stride;
+  int32_t columns;
+  int32_t page_size, page_shift;
+  int32_t box_rows;  // min(page_size, kTileKeys)
+  int32_t group, heads;
+  const PagedSegment* segments;
+  const int32_t* starts;
+  float* stat;  // [part][2][256]: m, l
+  float* part;  // [part][256][D]
+  void* out;
+  float scale_log2;
+  int* err;
+  const long long* wait_cycles;
+};
+
+struct Control {
+  volatile int abort;
+  uint32_t suspend_ns;
+  long long limit;
+};
+
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Control* c, int* err, int code) {
+  const uint32_t susp = c->suspend_ns;
+  if (mbar_try(bar, parity, susp)) return true;
+  const long long t0 = clock64();
+  const long long limit = c->limit;
+  while (!mbar_try(bar, parity, susp)) {
+    if (c->abort) return false;
+    if (clock64() - t0 > limit) {
+      atomicCAS(err, 0, code);
+      c->abort = 1;
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, Control* c, int* err, int code) {
+  return __all_sync(0xffffffffu, wait_bar(bar, parity, c, err, code));
+}
+// The block's own copies and MMAs always complete: fixed limit, abort ignored.
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity, int* err) {
+  if (mbar_try(bar, parity)) return;
+  const long long t0 = clock64();
+  while (!mbar_try(bar, parity))
+    if (clock64() - t0 > 2000000000LL) {
+      atomicCAS(err, 0, 89);
+      return;
+    }
+}
+
+__device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int x, int row, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+          "r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(page), "r"(smem_addr(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float* v) {
+  uint32_t r[64];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// 2^x for x <= 8 on the FMA pipe: x = n + f, n = floor(x) (an add rounded down
+// against 1.5 * 2^23 leaves n in the low mantissa bits), 2^f on [0, 1) by a
+// cubic fitted by weighted least squares for relative error (8.6e-5, below
+// the 16-bit rounding of P), 2^n added to the exponent field.  Below -127 the
+// result is some 1e-38, nothing beside the row's largest weight.
+__device__ __forceinline__ float poly_exp2(float x) {
+  x = fmaxf(x, -127.f);
+  const float t = __fadd_rd(x, 12582912.f);
+  const float f = __fsub_rn(x, __fsub_rn(t, 12582912.f));
+  float p = fmaf(f, 0.07706641f, 0.22764570f);
+  p = fmaf(f, p, 0.69511662f);
+  p = fmaf(f, p, 1.f);
+  return __int_as_float(__float_as_int(p) + (__float_as_int(t) << 23));
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+template <typename C>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A segment as the roles see it: the tiles that each half meets.
+struct View {
+  int count[2];  // tiles of half A, B, from tile0
+  int tiles;     // the larger: tiles that are loaded
+  __device__ __forceinline__ View(const PagedSegment& g, int group) {
+    tiles = 0;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      count[x] = 0;
+      if (kHalf * x >= g.rows) continue;
+      const int last_row = g.row0 + min(kHalf * x + kHalf, g.rows) - 1;
+      const int last = g.kv_len - g.new_len + last_row / group;  // last key that the half's last row sees
+      const int nt = last < 0 ? 0 : last / kTileKeys + 1;
+      count[x] = max(0, min(nt, g.tile1) - g.tile0);
+      tiles = max(tiles, count[x]);
+    }
+  }
+};
+
+template <typename T, typename C, int D>
+__global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_constant__ TileParams p) {
+  using S = Shape<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + S::kOffBar);
+  uint64_t* q_full = bars;       // [2] a half's query warp wrote its rows
+  uint64_t* q_empty = bars + 2;  // [2] MMA: the half's last scores of a segment are done
+  uint64_t* s_full = bars + 4;   // [2] MMA: scores of a tile
+  uint64_t* p_full = bars + 6;   // [2] 128 threads: P written, O rescaled
+  uint64_t* o_full = bars + 8;   // [2] MMA: a segment's last product
+  uint64_t* o_free = bars + 10;  // [2] 128 threads: O read
+  uint64_t* kv_full = bars + 12;             // [slots] TMA
+  uint64_t* kv_empty = kv_full + S::kSlots;  // [slots] MMA: products of the tile done
+  uint64_t* done = kv_empty + S::kSlots;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  Control* ctl = reinterpret_cast<Control*>(done + 2);
+  static_assert((12 + 2 * S::kSlots + 2) * 8 + sizeof(Control) <= 256, "barrier block");
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int* err = p.err;
+  if (tid == 0) {
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&q_full[x], 32);
+      mbar_init(&q_empty[x], 1);
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_full[x], kHalf);
+      mbar_init(&o_full[x], 1);
+      mbar_init(&o_free[x], kHalf);
+    }
+    for (int i = 0; i < S::kSlots; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    mbar_init(done, 1);
+    const long long lim = *p.wait_cycles;
+    ctl->abort = 0;
+    ctl->limit = lim;
+    ctl->suspend_ns = lim < 2000000000LL ? 0u : kSuspendNs;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (warp == kLoadWarp && lane == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&p.tm_k)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&p.tm_v)) : "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int seg0 = p.starts[blockIdx.x], seg1 = p.starts[blockIdx.x + 1];
+
+  if (warp >= kMmaWarp) {
+    // 384 threads x 168 registers = 2 x 128 x 208 + 128 x 88.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == kLoadWarp) {
+      int n = 0;  // tiles fetched (K and V each count)
+      bool ok = true;
+      for (int seg = seg0; seg < seg1 && ok; ++seg) {
+        const PagedSegment g = p.segments[seg];
+        const View view(g, p.group);
+        const int32_t* ids = p.ids + g.request * p.ids_stride;
+        const int box_bytes = p.box_rows * 128;
+        for (int j = 0; j < view.tiles && ok; ++j) {
+          const int key0 = (g.tile0 + j) * kTileKeys;
+          const int left = g.kv_len - key0;
+          const int boxes = ((left < kTileKeys ? left : kTileKeys) + p.box_rows - 1) / p.box_rows;
+          // Lane i fetches box i (at most 16 of the tile's pages).
+          int page = -1, row = 0;
+          if (lane < boxes) {
+            const int key = key0 + lane * p.box_rows, column = key >> p.page_shift;
+            if (column < p.columns) page = __ldg(ids + column);
+            row = g.kv_head * p.page_size + (key & (p.page_size - 1));
+          }
+#pragma unroll
+          for (int v = 0; v < 2; ++v, ++n) {
+            const int slot = n % S::kSlots, turn = n / S::kSlots;
+            if (turn > 0 && !(ok = wait_warp(&kv_empty[slot], (uint32_t)((turn - 1) & 1), ctl, err, 81))) break;
+            if (lane == 0) mbar_expect_tx(&kv_full[slot], (uint32_t)(boxes * box_bytes * (D / 64)));
+            __syncwarp();
+            if (lane < boxes) {
+              uint8_t* dst = base + S::kOffRing + slot * S::kTile + lane * box_bytes;
+#pragma unroll
+              for (int h = 0; h < D / 64; ++h)
+                tma_page(dst + h * kColBytes, v ? &p.tm_v : &p.tm_k, 64 * h, row, page, &kv_full[slot]);
+            }
+          }
+        }
+      }
+      // Copies in flight land before the block exits.
+      for (int i = n > S::kSlots ? n - S::kSlots : 0; i < n; ++i)
+        drain(&kv_full[i % S::kSlots], (uint32_t)((i / S::kSlots) & 1), err);
+    } else if (warp == kMmaWarp) {
+      const uint32_t leader = elect_one();
+      const uint32_t fmt = Act<C>::kDtype == TF_DTYPE_BF16 ? (1u << 7) | (1u << 10) : 0u;  // A and B are bf16
+      const uint32_t id_qk = idesc_f16(kHalf, kTileKeys) | fmt;
+      const uint32_t id_pv = idesc_f16(kHalf, D) | (1u << 16) | fmt;  // B (V) MN-major
+      int n = 0;                                                      // ring position
+      uint32_t q_turn[2] = {0, 0}, p_turn[2] = {0, 0}, o_turn[2] = {0, 0};
+      bool ok = true;
+      auto scores = [&](int x, int slot) {
+        const uint32_t qa = smem_addr(base + x * S::kTile), ka = smem_addr(base + S::kOffRing + slot * S::kTile);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+          const uint32_t off = (uint32_t)((s >> 2) * kColBytes + (s & 3) * 32);
+          mma_f16(leader, tmem + kColS + 128 * x, sw128_desc(qa + off), sw128_desc(ka + off), id_qk, s > 0 ? 1u : 0u);
+        }
+        mma_commit(leader, &s_full[x]);
+      };
+      for (int seg = seg0; seg < seg1 && ok; ++seg) {
+        const PagedSegment g = p.segments[seg];
+        const View view(g, p.group);
+        if (view.tiles == 0) continue;
+        const int k0 = n % S::kSlots;
+        if (!(ok = wait_warp(&kv_full[k0], (uint32_t)((n / S::kSlots) & 1), ctl, err, 82))) break;
+        for (int x = 0; x < 2 && ok; ++x) {
+          if (view.count[x] == 0) continue;
+          if (!(ok = wait_warp(&q_full[x], q_turn[x] & 1, ctl, err, 83))) break;
+          ++q_turn[x];
+          tc_fence_after();
+          scores(x, k0);
+          if (view.count[x] == 1) mma_commit(leader, &q_empty[x]);
+        }
+        mma_commit(leader, &kv_empty[k0]);
+        ++n;
+        for (int j = 0; j < view.tiles && ok; ++j) {
+          const int vs = n % S::kSlots;
+          if (!(ok = wait_warp(&kv_full[vs], (uint32_t)((n / S::kSlots) & 1), ctl, err, 84))) break;
+          ++n;
+          uint8_t* vt = base + S::kOffRing + vs * S::kTile;
+          const int have = g.kv_len - (g.tile0 + j) * kTileKeys;
+          if (have < kTileKeys) {
+            // Slots past the request's length hold anything, NaN included:
+            // 0 * NaN would reach the outputs, so their values become zeros.
+            for (int i = have * 8 + lane; i < kTileKeys * 8; i += 32)
+#pragma unroll
+              for (int h = 0; h < D / 64; ++h)
+                *reinterpret_cast<uint4*>(vt + h * kColBytes + 16 * i) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async();
+            __syncwarp();
+          }
+          const uint32_t va = smem_addr(vt);
+          const bool more = j + 1 < view.tiles;
+          const int ks = n % S::kSlots;
+          const uint32_t k_parity = (uint32_t)((n / S::kSlots) & 1);
+          for (int x = 0; x < 2 && ok; ++x) {
+            if (j >= view.count[x]) continue;
+            if (!(ok = wait_warp(&p_full[x], p_turn[x] & 1, ctl, err, 85))) break;
+            ++p_turn[x];
+            if (j == 0) {
+              // O still holds the half's last segment until it has been read.
+              if (o_turn[x] > 0 && !(ok = wait_warp(&o_free[x], (o_turn[x] - 1) & 1, ctl, err, 86))) break;
+              ++o_turn[x];
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int s = 0; s < kTileKeys / 16; ++s)
+              mma_f16_ts(leader, tmem + kColO + 128 * x, tmem + kColS + 128 * x + 8 * s,
+                         sw128_mn_desc(va + s * 2048, kColBytes, 1024), id_pv, (j > 0 || s > 0) ? 1u : 0u);
+            if (j + 1 == view.count[x]) mma_commit(leader, &o_full[x]);
+            if (j + 1 < view.count[x]) {
+              if (!(ok = wait_warp(&kv_full[ks], k_parity, ctl, err, 87))) break;
+              scores(x, ks);
+              if (j + 2 == view.count[x]) mma_commit(leader, &q_empty[x]);
+            }
+          }
+          if (!ok) break;
+          mma_commit(leader, &kv_empty[vs]);
+          if (more) {
+            mma_commit(leader, &kv_empty[ks]);
+            ++n;
+          }
+        }
+      }
+      // Every MMA issued here completes before tensor memory is released.
+      mma_commit(leader, done);
+      drain(done, 0, err);
+    } else {
+      // ---- queries of half x.
+      const int x = warp - kQueryWarp;
+      uint8_t* dst = base + x * S::kTile;
+      uint32_t turn = 0;
+      constexpr int kChunks = D / 8, kRowsAt = 32 / kChunks;  // 16-byte chunks of a row, rows per pass
+      const int c = lane % kChunks;
+      bool ok = true;
+      for (int seg = seg0; seg < seg1 && ok; ++seg) {
+        const PagedSegment g = p.segments[seg];
+        const View view(g, p.group);
+        if (view.count[x] == 0) continue;
+        if (turn > 0 && !(ok = wait_warp(&q_empty[x], (turn - 1) & 1, ctl, err, 88))) break;
+        ++turn;
+        int r = lane / kChunks;
+        const int rows = min(kHalf, g.rows - kHalf * x);
+        const int pr = g.row0 + kHalf * x + min(r, rows - 1);  // addresses stay inside q
+        int token = pr / p.group, head = pr % p.group;
+        const T* q = static_cast<const T*>(p.q) + (int64_t)(g.q_row + token) * p.q_stride +
+                     (int64_t)(g.kv_head * p.group + head) * D + 8 * c;
+        // Row r of each 64-column half at r * 128, chunk c at (c ^ (r & 7)) * 16.
+        uint8_t* at = dst + (c >> 3) * kColBytes;
+#pragma unroll 8
+        for (int i = 0; i < kHalf / kRowsAt; ++i, r += kRowsAt) {
+          uint8_t* to = at + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+          if constexpr (Act<T>::kDtype == Act<C>::kDtype) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(to)), "l"(q),
+                         "r"(r < rows ? 16 : 0)
+                         : "memory");
+          } else {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < rows) {
+              float f[8];
+              unpack8<T>(ld_v4(q), f);
+              v = pack8<C>(f);
+            }
+            *reinterpret_cast<uint4*>(to) = v;
+          }
+          if (r + kRowsAt < rows) {  // the next row of this lane exists
+            head += kRowsAt;
+            q += (int64_t)kRowsAt * D;
+            while (head >= p.group) {
+              head -= p.group;
+              q += p.q_stride - (int64_t)p.group * D;
+            }
+          }
+        }
+        if constexpr (Act<T>::kDtype == Act<C>::kDtype) asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async();
+        mbar_arrive(&q_full[x]);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    // ---- softmax of half x: thread r owns row r = TMEM lane r.
+    const int x = warp >> 2;
+    const int r = tid - kHalf * x;
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t t_o = lane_base + kColO + 128 * x, t_s = lane_base + kColS + 128 * x;
+    uint32_t s_turn = 0, o_turn = 0;
+    bool ok = true;
+    for (int seg = seg0; seg < seg1 && ok; ++seg) {
+      const PagedSegment g = p.segments[seg];
+      if (kHalf * x >= g.rows) continue;
+      const View view(g, p.group);
+      const int count = view.count[x];
+      // Threads past the rows follow the last one; what they make is dropped.
+      const int pr = g.row0 + min(kHalf * x + r, g.rows - 1);
+      const int token = pr / p.group;
+      const int limit = g.kv_len - g.new_len + token;  // last key the row sees
+      const int first_limit = g.kv_len - g.new_len + (g.row0 + kHalf * x) / p.group;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < count; ++j) {
+        if (!(ok = wait_warp(&s_full[x], s_turn & 1, ctl, err, 90))) break;
+        ++s_turn;
+        tc_fence_after();
+        float sc[128];
+        tmem_ld64(t_s, sc);
+        tmem_ld64(t_s + 64, sc + 64);
+        const int key0 = (g.tile0 + j) * kTileKeys;
+        if (key0 + kTileKeys - 1 > first_limit) {
+          const int lim = limit - key0;  // later columns are masked
+#pragma unroll
+          for (int c = 0; c < 128; ++c) sc[c] = c > lim ? -INFINITY : sc[c];
+        }
+        // The maximum of the raw scores (the scale is positive), NaN kept.
+        float mp[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mp[i] = sc[i];
+#pragma unroll
+        for (int c = 4; c < 124; c += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mp[i] = max_nan(mp[i], sc[c + 2 * i], sc[c + 2 * i + 1]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mp[i] = max_nan(mp[i], sc[124 + i]);
+        float mx = max_nan(max_nan(mp[0], mp[1]), mp[2], mp[3]) * p.scale_log2;
+        if (mx == INFINITY) mx = __uint_as_float(0x7fc00000u);  // inf - inf: the row is NaN
+        float factor = 1.f;
+        if (!(mx <= m + kRescale)) {  // also for NaN, and for the first key seen
+          mx = max_nan(m, mx);  // a NaN stays
+          factor = fast_exp2(m - mx);
+          m = mx;
+          l *= factor;
+        }
+        // This tile's scores were issued after the last tile's product: O is
+        // stable, and P may overlay S.
+        if (j > 0 && __any_sync(0xffffffffu, factor != 1.f)) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            float o[32];
+            tmem_ld32(t_o + c, o);
+            uint32_t w[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * factor);
+            tmem_st16(t_o + c, w);
+            tmem_st16(t_o + c + 16, w + 16);
+          }
+        }
+        // Exponent arguments and sums on packed pairs, one exponential in
+        // four a cubic.
+        const float sub = m == -INFINITY ? 0.f : -m;
+        const uint64_t sl2 = f2_pack(p.scale_log2, p.scale_log2), nm = f2_pack(sub, sub);
+        uint64_t sp[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sp[i] = 0ull;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const int k0 = 64 * half + 2 * c;
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(sc[k0], sc[k0 + 1]), sl2, nm), x0, x1);
+            const float a = fast_exp2(x0), b = (c & 1) ? poly_exp2(x1) : fast_exp2(x1);
+            sp[c & 3] = f2_add(sp[c & 3], f2_pack(a, b));
+            pk[c] = pack2<C>(a, b);
+          }
+          tmem_st16(t_s + 32 * half, pk);
+          tmem_st16(t_s + 32 * half + 16, pk + 16);
+        }
+        float s0, s1;
+        f2_unpack(f2_add(f2_add(sp[0], sp[1]), f2_add(sp[2], sp[3])), s0, s1);
+        l += s0 + s1;
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_full[x]);
+      }
+      if (!ok) break;
+      const int row = kHalf * x + r;
+      const bool mine = row < g.rows;
+      if (count > 0) {
+        if (!(ok = wait_warp(&o_full[x], o_turn & 1, ctl, err, 91))) break;
+        ++o_turn;
+        tc_fence_after();
+      }
+      // A row that has seen no key above -inf gives zeros (its l holds nothing
+      // but the cubics' 1e-38).
+      const float inv = m == -INFINITY ? 0.f : 1.f / l;
+      T* orow = static_cast<T*>(p.out) +
+                ((int64_t)(g.q_row + token) * p.heads + g.kv_head * p.group + pr % p.group) * D;
+      float* prow = p.part + ((int64_t)g.part * kTileRows + row) * D;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        float o[32];
+        if (count > 0) {
+          tmem_ld32(t_o + c, o);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        }
+        if (!mine) continue;
+        if (g.part < 0) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            float f[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = m == -INFINITY ? 0.f : o[i + k] * inv;
+            *reinterpret_cast<uint4*>(orow + c + i) = pack8<T>(f);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(prow + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+      }
+      if (mine && g.part >= 0) {
+        p.stat[(int64_t)g.part * 2 * kTileRows + row] = m;
+        p.stat[(int64_t)g.part * 2 * kTileRows + kTileRows + row] = l;
+      }
+      if (count > 0) {
+        tc_fence_before();
+        mbar_arrive(&o_free[x]);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+}
+
+// Joins the pieces of cut row blocks: one warp per row, in piece order.
+constexpr int kMergeWarps = 8;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * kMergeWarps)
+    paged_merge_kernel(const PagedSegment* __restrict__ items, const float* __restrict__ stat,
+                       const float* __restrict__ part, int group, int heads, T* __restrict__ out) {
+  constexpr int kPer = D / 32;
+  const PagedSegment& g = items[blockIdx.y];
+  const int row = blockIdx.x * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= g.rows) return;
+  const float* st = stat + (int64_t)g.part0 * 2 * kTileRows + row;
+  float M = -INFINITY;
+  for (int i = 0; i < g.parts; ++i) M = max_nan(M, st[(int64_t)i * 2 * kTileRows]);
+  float acc[kPer], sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
+  for (int i = 0; i < g.parts; ++i) {
+    const float m = st[(int64_t)i * 2 * kTileRows];
+    if (m == -INFINITY) continue;
+    const float f = fast_exp2(m - M);
+    const float* o = part + ((int64_t)(g.part0 + i) * kTileRows + row) * D + kPer * lane;
+    sum = fmaf(f, st[(int64_t)i * 2 * kTileRows + kTileRows], sum);
+    if constexpr (kPer == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(o);
+      acc[0] = fmaf(f, v.x, acc[0]);
+      acc[1] = fmaf(f, v.y, acc[1]);
+      acc[2] = fmaf(f, v.z, acc[2]);
+      acc[3] = fmaf(f, v.w, acc[3]);
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(o);
+      acc[0] = fmaf(f, v.x, acc[0]);
+      acc[1] = fmaf(f, v.y, acc[1]);
+    }
+  }
+  const int pr = g.row0 + row;
+  T* to = out + ((int64_t)(g.q_row + pr / group) * heads + g.kv_head * group + pr % group) * D + kPer * lane;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) to[k] = from_f<T>(M == -INFINITY ? 0.f : acc[k] / sum);
+}
+
+template <typename T, typename C, int D>
+tf_status launch(const TileParams& p, const tf_paged_plan& plan, const PagedSegment* merges, cudaStream_t s) {
+  static PerDeviceOnce attr;
+  int dev = 0;
+  if (attr.needed(&dev)) {
+    TF_CUDA(cudaFuncSetAttribute(paged_tile_kernel<T, C, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 Shape<D>::kSmem));
+    attr.mark(dev);
+  }
+  paged_tile_kernel<T, C, D><<<plan.tile_blocks, kThreads, Shape<D>::kSmem, s>>>(p);
+  TF_TRY(check_launch("paged_tile"));
+  if (plan.merges == 0) return TF_OK;
+  // grid.y is below 65536: at most one cut item per block.
+  const dim3 grid(kTileRows / kMergeWarps, (unsigned)plan.merges);
+  paged_merge_kernel<T, D><<<grid, 32 * kMergeWarps, 0, s>>>(merges, p.stat, p.part, p.group, p.heads,
+                                                             static_cast<T*>(p.out));
+  return check_launch("paged_merge");
+}
+
+}  // namespace
+
+tf_status launch_paged_tile(const PagedArgs& a, cudaStream_t s) {
+  const tf_paged_plan& plan = *a.plan;
+  if (plan.tile_blocks == 0) return TF_OK;
+  TileParams p;
+  memset(&p, 0, sizeof(p));
+  p.box_rows = a.kv.page_size < kTileKeys ? a.kv.page_size : kTileKeys;
+  TF_TRY(make_page_map(&p.tm_k, a.kv.k, a.kv, p.box_rows));
+  TF_TRY(make_page_map(&p.tm_v, a.kv.v, a.kv, p.box_rows));
+  p.q = a.q;
+  p.q_stride = a.q_stride;
+  p.ids = a.table.ids;
+  p.ids_stride = a.table.stride;
+  p.columns = a.table.columns;
+  p.page_size = a.kv.page_size;
+  while ((1 << p.page_shift) < a.kv.page_size) ++p.page_shift;
+  p.group = plan.heads / plan.kv_heads;
+  p.heads = plan.heads;
+  p.segments = reinterpret_cast<const PagedSegment*>(a.plan_table + plan.tile_segments_offset);
+  p.starts = reinterpret_cast<const int32_t*>(a.plan_table + plan.tile_starts_offset);
+  p.stat = reinterpret_cast<float*>(a.workspace + split_workspace_bytes(plan));
+  p.part = p.stat + (int64_t)plan.tile_parts * 2 * kTileRows;
+  p.out = a.out;
+  p.scale_log2 = a.scale * kLog2e;
+  TF_TRY(tc_flags(&p.err, const_cast<long long**>(&p.wait_cycles)));
+  const PagedSegment* merges = reinterpret_cast<const PagedSegment*>(a.plan_table + plan.merges_offset);
+#define TF_TILE(T, C)                                                    \
+  return plan.head_dim == 128 ? launch<T, C, 128>(p, plan, merges, s)    \
+                              : launch<T, C, 64>(p, plan, merges, s)
+  if (a.act == TF_DTYPE_F16) TF_TILE(__half, __half);
+  if (a.kv.dtype == TF_DTYPE_F16) TF_TILE(__nv_bfloat16, __half);
+  TF_TILE(__nv_bfloat16, __nv_bfloat16);
+#undef TF_TILE
+}
+
+}  // namespace tf
