@@ -379,8 +379,8 @@ int tf_paged_append(const void* qkv, int64_t qkv_stride, int64_t rows, int32_t h
 /* Plan of one attention call: how its rows and keys are divided over the
  * GPU.  It depends on the lengths and the geometry alone, so a serving loop
  * makes one plan per step and uses it in every layer.  The caller keeps the
- * struct (plain data, filled by tf_paged_plan_size) and a device copy of the
- * table that tf_paged_plan_fill writes to host memory. */
+ * struct (plain data) and a device copy of the table that tf_paged_plan_make
+ * writes to host memory. */
 typedef struct tf_paged_plan {
   int64_t rows;             /* query rows of all requests                    */
   size_t table_bytes;       /* device table, 16-byte aligned                 */
@@ -410,11 +410,12 @@ typedef struct tf_paged_plan {
 /* new_lengths[i] query rows and kv_lengths[i] cached tokens (the new ones
  * included) for request i; host arrays.  Lengths of zero are allowed, and so
  * is a kv length below the new length: the rows before token 0 attend
- * nothing. */
-int tf_paged_plan_size(const int32_t* new_lengths, const int32_t* kv_lengths, int32_t requests, int32_t heads,
-                       int32_t kv_heads, int32_t head_dim, int32_t page_size, tf_paged_plan* plan);
-int tf_paged_plan_fill(const int32_t* new_lengths, const int32_t* kv_lengths, const tf_paged_plan* plan, void* table,
-                       size_t table_bytes);
+ * nothing.  Fills the plan, and the table (host memory) when its capacity is
+ * at least plan->table_bytes; otherwise TF_ERR_CAPACITY, for a second call
+ * with a larger one. */
+int tf_paged_plan_make(const int32_t* new_lengths, const int32_t* kv_lengths, int32_t requests, int32_t heads,
+                       int32_t kv_heads, int32_t head_dim, int32_t page_size, tf_paged_plan* plan, void* table,
+                       size_t table_capacity);
 
 /* Attention of the planned rows over the pages (workspace): row i of request
  * r attends keys 0 .. kv_len - new_len + i of that request,

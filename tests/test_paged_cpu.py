@@ -12,11 +12,11 @@ def plan(new, kv, H=8, Hk=2, D=128, page=16):
     n = len(new)
     a, b = (C.c_int32 * n)(*new), (C.c_int32 * n)(*kv)
     d = PagedPlanDesc()
-    status = lib().tf_paged_plan_size(a, b, n, H, Hk, D, page, C.byref(d))
-    if status:
+    status = lib().tf_paged_plan_make(a, b, n, H, Hk, D, page, C.byref(d), None, 0)
+    if status != 10:  # the size is known, the table was not given
         return status, None, None
     table = (C.c_uint8 * d.table_bytes)()
-    assert lib().tf_paged_plan_fill(a, b, C.byref(d), table, d.table_bytes) == 0, lib().tf_last_error()
+    assert lib().tf_paged_plan_make(a, b, n, H, Hk, D, page, C.byref(d), table, d.table_bytes) == 0
     return 0, d, bytes(table)
 
 
@@ -31,13 +31,16 @@ def test_geometry_refused(geometry, error):
     assert plan([1], [4], **geometry)[0] == error
 
 
-def test_fill_checks_the_lengths():
+def test_table_capacity():
     _, d, _ = plan([1, 2], [5, 600])
-    a, b = (C.c_int32 * 2)(1, 3), (C.c_int32 * 2)(5, 600)
-    table = (C.c_uint8 * d.table_bytes)()
-    assert lib().tf_paged_plan_fill(a, b, C.byref(d), table, d.table_bytes) == 9
-    b = (C.c_int32 * 2)(5, 600)
-    assert lib().tf_paged_plan_fill(a, b, C.byref(d), table, 8) == 1
+    a, b = (C.c_int32 * 2)(1, 2), (C.c_int32 * 2)(5, 600)
+    table = (C.c_uint8 * d.table_bytes)(*([7] * d.table_bytes))
+    again = PagedPlanDesc()
+    assert lib().tf_paged_plan_make(a, b, 2, 8, 2, 128, 16, C.byref(again), table, d.table_bytes - 1) == 10
+    assert again.table_bytes == d.table_bytes and set(bytes(table)) == {7}
+    assert lib().tf_paged_plan_make(a, b, 2, 8, 2, 128, 16, None, table, d.table_bytes) == 1
+    assert lib().tf_paged_plan_make(a, b, 2, 8, 2, 128, 16, C.byref(again), None, 8) == 1
+    assert lib().tf_paged_plan_make(None, b, 2, 8, 2, 128, 16, C.byref(again), None, 0) == 1
 
 
 def test_attention_and_append_refuse_before_any_launch():

@@ -13,6 +13,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libtrifuse_b200.so"
 
 TF_OK = 0
+TF_ERR_CAPACITY = 10
 STATUS = {0: "TF_OK", 1: "TF_ERR_INVALID_ARGUMENT", 2: "TF_ERR_SHAPE", 3: "TF_ERR_OUT_OF_MEMORY",
           4: "TF_ERR_CUDA", 5: "TF_ERR_NCCL", 6: "TF_ERR_TIMEOUT", 7: "TF_ERR_CANCELLED",
           8: "TF_ERR_UNSUPPORTED", 9: "TF_ERR_STATE", 10: "TF_ERR_CAPACITY"}
@@ -132,8 +133,7 @@ SIGNATURES = {
     "tf_token_logprobs": [P, I64, I64, I32, C.c_int, P, I32, P, P, P, P, P, P],
     "tf_paged_append": [P, I64, I64, I32, C.c_int, P, P, F32, F32, P, P, C.POINTER(PageTable), C.POINTER(PagedKV), P,
                         P],
-    "tf_paged_plan_size": [P, P, I32, I32, I32, I32, I32, C.POINTER(PagedPlanDesc)],
-    "tf_paged_plan_fill": [P, P, C.POINTER(PagedPlanDesc), P, SZ],
+    "tf_paged_plan_make": [P, P, I32, I32, I32, I32, I32, C.POINTER(PagedPlanDesc), P, SZ],
     "tf_paged_attention": [P, I64, C.POINTER(PageTable), C.POINTER(PagedKV), C.POINTER(PagedPlanDesc), P, F32,
                            C.c_int, P, P, SZ, P],
 }

@@ -105,9 +105,10 @@ int tf_paged_append(const void* qkv, int64_t qkv_stride, int64_t rows, int32_t h
   return launch_paged_append(a, st(stream));
 }
 
-int tf_paged_plan_size(const int32_t* new_lengths, const int32_t* kv_lengths, int32_t requests, int32_t heads,
-                       int32_t kv_heads, int32_t head_dim, int32_t page_size, tf_paged_plan* plan) {
-  if (!plan) return set_error(TF_ERR_INVALID_ARGUMENT, "paged plan: NULL plan");
+int tf_paged_plan_make(const int32_t* new_lengths, const int32_t* kv_lengths, int32_t requests, int32_t heads,
+                       int32_t kv_heads, int32_t head_dim, int32_t page_size, tf_paged_plan* plan, void* table,
+                       size_t table_capacity) {
+  if (!plan || (!table && table_capacity)) return set_error(TF_ERR_INVALID_ARGUMENT, "paged plan: NULL plan or table");
   TF_TRY(check_geometry(heads, kv_heads, head_dim, page_size));
   tf_paged_plan p{};
   TF_TRY(check_lengths(new_lengths, kv_lengths, requests, heads / kv_heads, &p.rows));
@@ -121,26 +122,9 @@ int tf_paged_plan_size(const int32_t* new_lengths, const int32_t* kv_lengths, in
     if (pages > p.columns) p.columns = pages;
   }
   try {
-    TF_TRY(paged_plan_size(new_lengths, kv_lengths, &p));
-  } catch (const std::bad_alloc&) {
-    return set_error(TF_ERR_OUT_OF_MEMORY, "paged plan: out of host memory");
-  }
-  *plan = p;
-  return TF_OK;
-}
-
-int tf_paged_plan_fill(const int32_t* new_lengths, const int32_t* kv_lengths, const tf_paged_plan* plan, void* table,
-                       size_t table_bytes) {
-  if (!plan || !table) return set_error(TF_ERR_INVALID_ARGUMENT, "paged plan: NULL plan or table");
-  if (table_bytes < plan->table_bytes)
-    return set_error(TF_ERR_INVALID_ARGUMENT, "paged plan: table of %zu bytes, %zu needed", table_bytes,
-                     plan->table_bytes);
-  TF_TRY(check_geometry(plan->heads, plan->kv_heads, plan->head_dim, plan->page_size));
-  int64_t rows = 0;
-  TF_TRY(check_lengths(new_lengths, kv_lengths, plan->requests, plan->heads / plan->kv_heads, &rows));
-  if (rows != plan->rows) return set_error(TF_ERR_STATE, "paged plan: lengths differ from those it was sized for");
-  try {
-    return paged_plan_fill(new_lengths, kv_lengths, plan, static_cast<char*>(table));
+    const tf_status s = paged_plan_make(new_lengths, kv_lengths, &p, static_cast<char*>(table), table_capacity);
+    *plan = p;
+    return s;
   } catch (const std::bad_alloc&) {
     return set_error(TF_ERR_OUT_OF_MEMORY, "paged plan: out of host memory");
   }

@@ -50,9 +50,9 @@ struct PagedArgs {
   char* workspace = nullptr;
 };
 
-tf_status paged_plan_size(const int32_t* new_lengths, const int32_t* kv_lengths, tf_paged_plan* plan);
-tf_status paged_plan_fill(const int32_t* new_lengths, const int32_t* kv_lengths, const tf_paged_plan* plan,
-                          char* table);
+// Fills the plan's remaining fields, and the table where it fits.
+tf_status paged_plan_make(const int32_t* new_lengths, const int32_t* kv_lengths, tf_paged_plan* plan, char* table,
+                          size_t table_capacity);
 // Tensor map over pages as [page][kv_head * page_size rows][head_dim], box
 // {64 values, box_rows rows, 1 page}, 128-byte swizzle; a page id outside
 // [0, pages) reads zeros.

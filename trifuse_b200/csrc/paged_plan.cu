@@ -12,7 +12,6 @@
 #include <string.h>
 
 #include <algorithm>
-#include <queue>
 #include <vector>
 
 #include "paged.h"
@@ -29,8 +28,10 @@ struct Piece {
   int32_t item, tile0, tile1;
 };
 
+// Pieces of all blocks, block by block.
 struct Schedule {
-  std::vector<std::vector<Piece>> blocks;
+  std::vector<Piece> pieces;
+  std::vector<int32_t> starts;  // first piece of each block, then the end
 };
 
 int current_sms() {
@@ -45,61 +46,76 @@ int current_sms() {
 
 // Divides the items over at most `blocks` blocks.  overhead: cost of starting
 // a segment, in tiles; min_piece: smallest piece worth cutting, in tiles.
-Schedule divide(const std::vector<Item>& items, int blocks, int overhead, int min_piece) {
+Schedule divide(const std::vector<Item>& items, int kv_heads, int blocks, int overhead, int min_piece) {
   Schedule out;
   int64_t total = 0;
   for (const Item& it : items) total += it.tiles + overhead;
   const int64_t mean = std::max<int64_t>((total + blocks - 1) / blocks, min_piece + overhead);
-  std::vector<int32_t> order(items.size());
-  for (size_t i = 0; i < order.size(); ++i) order[i] = (int32_t)i;
   // Longest first; equal items keep their order, so one request's key heads
-  // and row blocks run at the same time and share its pages through L2.
-  std::stable_sort(order.begin(), order.end(),
-                   [&](int32_t a, int32_t b) { return items[a].tiles > items[b].tiles; });
-  std::vector<std::vector<Piece>> whole(std::min<size_t>(blocks, items.size()));
-  using Load = std::pair<int64_t, int32_t>;
-  std::priority_queue<Load, std::vector<Load>, std::greater<Load>> loads;
-  for (size_t b = 0; b < whole.size(); ++b) loads.push({0, (int32_t)b});
-  int64_t most = 0;
+  // and row blocks run at the same time and share its pages through L2.  The
+  // key heads of a row block follow one another with equal lengths, so they
+  // are sorted as one.
+  std::vector<int32_t> order(items.size()), firsts;
+  firsts.reserve(items.size() / kv_heads);
+  for (size_t i = 0; i < items.size(); i += kv_heads) firsts.push_back((int32_t)i);
+  const auto longer = [&](int32_t a, int32_t b) { return items[a].tiles > items[b].tiles; };
+  if (!std::is_sorted(firsts.begin(), firsts.end(), longer)) std::stable_sort(firsts.begin(), firsts.end(), longer);
+  for (size_t i = 0; i < order.size(); ++i) order[i] = firsts[i / kv_heads] + (int32_t)(i % kv_heads);
+  // Loads as a binary heap of (load, block) in one 64-bit word; the least
+  // loaded block is raised in place.
+  const int used = (int)std::min<size_t>(blocks, items.size());
+  std::vector<uint64_t> heap(used);
+  for (int b = 0; b < used; ++b) heap[b] = (uint64_t)b;
+  std::vector<int32_t> owner(items.size()), count(used + 1, 0);
+  uint64_t most = 0;
   for (int32_t i : order) {
-    Load l = loads.top();
-    loads.pop();
-    whole[l.second].push_back({i, 0, items[i].tiles});
-    l.first += items[i].tiles + overhead;
-    most = std::max(most, l.first);
-    loads.push(l);
+    const uint64_t load = (heap[0] >> 20) + items[i].tiles + overhead;
+    const uint64_t b = heap[0] & 0xfffff;
+    owner[i] = (int32_t)b;
+    ++count[b + 1];
+    most = std::max(most, load);
+    const uint64_t word = load << 20 | b;
+    int at = 0;
+    for (int child; (child = 2 * at + 1) < used; at = child) {
+      if (child + 1 < used && heap[child + 1] < heap[child]) ++child;
+      if (heap[child] >= word) break;
+      heap[at] = heap[child];
+    }
+    heap[at] = word;
   }
-  if (most <= mean + mean / 16) {
-    out.blocks = std::move(whole);
+  if ((int64_t)most <= mean + mean / 16) {
+    for (int b = 0; b < used; ++b) count[b + 1] += count[b];
+    out.starts = count;
+    out.pieces.resize(items.size());
+    for (int32_t i : order) out.pieces[count[owner[i]]++] = {i, 0, items[i].tiles};
     return out;
   }
   // Every cut adds a segment, and a block may close short of a full share, so
   // the share grows until the pieces fit.
   for (int64_t share = mean + overhead;; share += share / 64 + 1) {
-    out.blocks.clear();
-    std::vector<Piece> cur;
+    out.pieces.clear();
+    out.starts.assign(1, 0);
     int64_t load = 0;
     for (int32_t i : order) {
       int32_t t = 0;
       do {
         const int64_t left = items[i].tiles - t;
         int64_t room = share - load - overhead;
-        if (room < min_piece && !cur.empty()) {
-          out.blocks.push_back(std::move(cur));
-          cur.clear();
+        if (room < min_piece && load > 0) {
+          out.starts.push_back((int32_t)out.pieces.size());
           load = 0;
           room = share - overhead;
         }
         int64_t take = std::min(left, room);
         // No crumbs: a rest below min_piece joins this piece.
         if (left - take < min_piece) take = left;
-        cur.push_back({i, t, (int32_t)(t + take)});
+        out.pieces.push_back({i, t, (int32_t)(t + take)});
         load += take + overhead;
         t += (int32_t)take;
       } while (t < items[i].tiles);
     }
-    if (!cur.empty()) out.blocks.push_back(std::move(cur));
-    if ((int)out.blocks.size() <= blocks) return out;
+    if (load > 0) out.starts.push_back((int32_t)out.pieces.size());
+    if ((int)out.starts.size() - 1 <= blocks) return out;
   }
 }
 
@@ -115,36 +131,33 @@ Layout lay_out(const std::vector<Item>& items, const Schedule& s, const int32_t*
   Layout out;
   std::vector<int32_t> pieces(items.size(), 0), part0(items.size(), -1), used(items.size(), 0),
       counter(items.size(), -1);
-  for (const auto& b : s.blocks)
-    for (const Piece& p : b) ++pieces[p.item];
+  for (const Piece& p : s.pieces) ++pieces[p.item];
   for (size_t i = 0; i < items.size(); ++i)
     if (pieces[i] > 1) {
       part0[i] = out.parts;
       out.parts += pieces[i];
       counter[i] = out.counters++;
     }
-  for (const auto& b : s.blocks) {
-    out.starts.push_back((int32_t)out.segments.size());
-    for (const Piece& p : b) {
-      const Item& it = items[p.item];
-      PagedSegment g{};
-      g.q_row = it.q_row;
-      g.new_len = new_lengths[it.request];
-      g.kv_len = kv_lengths[it.request];
-      g.request = it.request;
-      g.kv_head = it.kv_head;
-      g.row0 = it.row0;
-      g.rows = it.rows;
-      g.tile0 = p.tile0;
-      g.tile1 = p.tile1;
-      g.part = part0[p.item] < 0 ? -1 : part0[p.item] + used[p.item]++;
-      g.part0 = part0[p.item];
-      g.parts = pieces[p.item];
-      g.counter = counter[p.item];
-      out.segments.push_back(g);
-    }
+  out.segments.reserve(s.pieces.size());
+  for (const Piece& p : s.pieces) {
+    const Item& it = items[p.item];
+    PagedSegment g{};
+    g.q_row = it.q_row;
+    g.new_len = new_lengths[it.request];
+    g.kv_len = kv_lengths[it.request];
+    g.request = it.request;
+    g.kv_head = it.kv_head;
+    g.row0 = it.row0;
+    g.rows = it.rows;
+    g.tile0 = p.tile0;
+    g.tile1 = p.tile1;
+    g.part = part0[p.item] < 0 ? -1 : part0[p.item] + used[p.item]++;
+    g.part0 = part0[p.item];
+    g.parts = pieces[p.item];
+    g.counter = counter[p.item];
+    out.segments.push_back(g);
   }
-  out.starts.push_back((int32_t)out.segments.size());
+  out.starts = s.starts;
   return out;
 }
 
@@ -171,7 +184,8 @@ Layout plan_kernel(const int32_t* new_lengths, const int32_t* kv_lengths, const 
   // A segment starts in the time of some four small or one large tile; a piece
   // should be worth its partial result (a large tile's keys and values are as
   // many bytes as half a partial result).
-  const Schedule s = tile ? divide(items, current_sms(), 1, 4) : divide(items, current_sms(), 4, 8);
+  const Schedule s = tile ? divide(items, p.kv_heads, current_sms(), 1, 4)
+                          : divide(items, p.kv_heads, current_sms(), 4, 8);
   return lay_out(items, s, new_lengths, kv_lengths);
 }
 
@@ -230,20 +244,14 @@ void put_table(const Plans& plans, const int32_t* new_lengths, const int32_t* kv
 
 }  // namespace
 
-tf_status paged_plan_size(const int32_t* new_lengths, const int32_t* kv_lengths, tf_paged_plan* p) {
-  put_table(Plans(new_lengths, kv_lengths, *p), new_lengths, kv_lengths, p, nullptr);
-  return TF_OK;
-}
-
-tf_status paged_plan_fill(const int32_t* new_lengths, const int32_t* kv_lengths, const tf_paged_plan* p,
-                          char* table) {
+tf_status paged_plan_make(const int32_t* new_lengths, const int32_t* kv_lengths, tf_paged_plan* p, char* table,
+                          size_t table_capacity) {
   const Plans plans(new_lengths, kv_lengths, *p);
-  tf_paged_plan again = *p;
-  put_table(plans, new_lengths, kv_lengths, &again, nullptr);
-  if (memcmp(&again, p, sizeof(again)))
-    return set_error(TF_ERR_STATE, "paged plan: lengths or device differ from those the plan was sized for");
+  put_table(plans, new_lengths, kv_lengths, p, nullptr);
+  if (p->table_bytes > table_capacity)
+    return set_error(TF_ERR_CAPACITY, "paged plan: table of %zu bytes, %zu needed", table_capacity, p->table_bytes);
   memset(table, 0, p->table_bytes);
-  put_table(plans, new_lengths, kv_lengths, &again, table);
+  put_table(plans, new_lengths, kv_lengths, p, table);
   return TF_OK;
 }
 

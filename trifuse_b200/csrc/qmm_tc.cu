@@ -1313,8 +1313,18 @@ tf_status make_tma_2d(CUtensorMap* m, const void* base, CUtensorMapDataType dt, 
 }
 
 tf_status tc_flags(int** error, long long** wait_cycles) {
+  // Looked up once per device (below 64; the addresses are the module's).
+  static std::atomic<int*> errors[64];
+  static std::atomic<long long*> waits[64];
+  int dev = 0;
+  TF_CUDA(cudaGetDevice(&dev));
+  if (dev < 64 && (*error = errors[dev].load()) && (*wait_cycles = waits[dev].load())) return TF_OK;
   TF_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(error), g_tc_error));
   TF_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(wait_cycles), g_wait_cycles));
+  if (dev < 64) {
+    errors[dev].store(*error);
+    waits[dev].store(*wait_cycles);
+  }
   return TF_OK;
 }
 

@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from ._lib import (AffineWeight, DTYPE_BF16, DTYPE_F16, DTYPE_F32, MoeArgs, PagedKV, PagedPlanDesc, PageTable, RouterWeight,
-                   check, lib)
+                   TF_ERR_CAPACITY, check, lib)
 
 _ACT = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
 
@@ -185,25 +185,24 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0) -> TokenLogprob
         raise ValueError("token_logprobs: tokens are int64 with the shape of the logits' rows")
     if type(top) is not int:
         raise ValueError("token_logprobs: top is an int")
-    _same_device(logits, tokens)
+    stream = _launch_stream(logits, tokens)
     shape, V = tokens.shape, logits.shape[-1]
     if logits.ndim != 2:
         logits = logits.reshape(-1, V)
     if logits.stride(1) != 1 or logits.stride(0) < V:
         logits = logits.contiguous()
-    rows = logits.shape[0]
+    rows, k = logits.shape[0], max(top, 0)
     tokens = tokens.contiguous()
-    dev = logits.device
-    scalars = torch.empty((3, rows), dtype=torch.float32, device=dev)
-    top_logprob = torch.empty((rows, top), dtype=torch.float32, device=dev) if top > 0 else scalars.new_empty((rows, 0))
-    top_token = torch.empty((rows, max(top, 0)), dtype=torch.int64, device=dev)
-    at = scalars.data_ptr()
+    logprob = torch.empty_like(tokens, dtype=torch.float32)
+    entropy = torch.empty_like(logprob)
+    rank = torch.empty_like(tokens, dtype=torch.int32)
+    top_logprob = logprob.new_empty((*shape, k))
+    top_token = tokens.new_empty((*shape, k))
     check(lib().tf_token_logprobs(logits.data_ptr(), logits.stride(0) if rows > 1 else V, rows, V,
-                                  _ACT.get(logits.dtype, DTYPE_F32), tokens.data_ptr(), top, at, at + 4 * rows,
-                                  at + 8 * rows, top_logprob.data_ptr(), top_token.data_ptr(),
-                                  torch.cuda.current_stream().cuda_stream))
-    return TokenLogprobs(scalars[0].view(shape), scalars[1].view(shape), scalars[2].view(torch.int32).view(shape),
-                         top_logprob.view(*shape, top), top_token.view(*shape, top))
+                                  _ACT.get(logits.dtype, DTYPE_F32), tokens.data_ptr(), top, logprob.data_ptr(),
+                                  entropy.data_ptr(), rank.data_ptr(), top_logprob.data_ptr(), top_token.data_ptr(),
+                                  stream))
+    return TokenLogprobs(logprob, entropy, rank, top_logprob, top_token)
 
 
 def native_olmoe_softmax(x: Tensor) -> Tensor:
@@ -494,13 +493,14 @@ def _page_table(page_table: Tensor) -> PageTable:
     return PageTable(page_table.data_ptr(), max(page_table.stride(0), columns), requests, columns)
 
 
-def _same_device(*ts):
-    """Kernels launch on the current device's current stream: every tensor must live there."""
-    dev = torch.cuda.current_device()
+def _launch_stream(*ts) -> int:
+    """The current device's current stream (its handle); every tensor must live on that device."""
+    dev = torch._C._cuda_getDevice()
     for t in ts:
-        if t is not None and (not t.is_cuda or t.device.index != dev):
+        if t is not None and t.get_device() != dev:
             _cuda(t)
             raise ValueError("tensors must be on the current CUDA device")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, positions: Tensor,
@@ -514,7 +514,7 @@ def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tens
     qkv: [rows, (heads + 2 kv_heads) * head_dim] rows q | k | v; positions and
     requests: int32 [rows] on the device; page_table: int32 [requests, pages].
     A row whose slot the table does not have is not stored."""
-    _same_device(qkv, k_pages, v_pages, page_table, positions, requests, q_norm, k_norm, out)
+    stream = _launch_stream(qkv, k_pages, v_pages, page_table, positions, requests, q_norm, k_norm, out)
     kv = _paged_kv(k_pages, v_pages)
     D, width = kv.head_dim, (heads + 2 * kv.kv_heads) * kv.head_dim
     if qkv.ndim != 2 or qkv.shape[1] != width:
@@ -537,7 +537,7 @@ def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tens
                                 None if q_norm is None else q_norm.data_ptr(),
                                 None if k_norm is None else k_norm.data_ptr(), eps,
                                 0.0 if rope_theta is None else rope_theta, positions.data_ptr(), requests.data_ptr(),
-                                table, kv, out.data_ptr(), torch.cuda.current_stream().cuda_stream))
+                                table, kv, out.data_ptr(), stream))
     return out
 
 
@@ -558,25 +558,33 @@ class PagedPlan:
             raise ValueError("paged plan: new_lengths and kv_lengths differ in length")
         new, kv = (C.c_int32 * n)(*new_lengths), (C.c_int32 * n)(*kv_lengths)
         self.desc = d = PagedPlanDesc()
-        check(lib().tf_paged_plan_size(new, kv, n, heads, kv_heads, head_dim, page_size, d))
-        host = torch.empty(max(d.table_bytes, 1), dtype=torch.uint8, pin_memory=True)
-        check(lib().tf_paged_plan_fill(new, kv, d, host.data_ptr(), d.table_bytes))
+        guess = 65536 + 64 * n * max(kv_heads, 1) + 16 * sum(new)
+        while True:  # a second time when the table outgrows the guess
+            host = torch.empty(guess, dtype=torch.uint8, pin_memory=True)
+            status = lib().tf_paged_plan_make(new, kv, n, heads, kv_heads, head_dim, page_size, d, host.data_ptr(),
+                                              guess)
+            if status != TF_ERR_CAPACITY:
+                break
+            guess = d.table_bytes
+        check(status)
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-        self.table = host.to(device, non_blocking=True)
+        self.table = host[:d.table_bytes].to(device, non_blocking=True)
         self.workspace = torch.empty(max(d.workspace_bytes, 1), dtype=torch.uint8, device=device)
-        self._stream = torch.cuda.current_stream(device)
-        self._ready = self._stream.record_event()
+        stream = torch.cuda.current_stream(device)
+        self._made_on = stream.cuda_stream
+        self._ready = stream.record_event()
         self.rows, self.heads, self.head_dim = d.rows, heads, head_dim
         at, size = d.positions_offset, 4 * d.rows
         self.positions = self.table[at:at + size].view(torch.int32)
         at = d.requests_offset
         self.requests = self.table[at:at + size].view(torch.int32)
 
-    def _on(self, stream):
+    def _on(self, handle: int):
         """Orders the plan's upload before work on another stream and keeps its memory until that work is done.
         A capturing stream cannot wait for an event from outside; a graph's first replay comes after the
         synchronization that opens its capture, and its owner keeps the plan."""
-        if stream != self._stream and not torch.cuda.is_current_stream_capturing():
+        if handle != self._made_on and not torch.cuda.is_current_stream_capturing():
+            stream = torch.cuda.current_stream()
             stream.wait_event(self._ready)
             self.table.record_stream(stream)
             self.workspace.record_stream(stream)
@@ -588,7 +596,7 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Ten
     request attends keys 0 .. kv_length - new_length + i; query heads share
     key heads in groups.  q: [rows, heads, head_dim] (rows may be strided);
     returns [rows, heads, head_dim].  Rows that attend nothing give zeros."""
-    _same_device(q, k_pages, v_pages, page_table, plan.table, out)
+    stream = _launch_stream(q, k_pages, v_pages, page_table, plan.table, out)
     rows, heads, D = plan.rows, plan.heads, plan.head_dim
     if q.shape != (rows, heads, D):
         raise ValueError("paged_attention: q is [rows, heads, head_dim] of the plan")
@@ -598,12 +606,11 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Ten
         out = torch.empty((rows, heads, D), dtype=q.dtype, device=q.device)
     elif out.shape != (rows, heads, D) or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("paged_attention: out is a contiguous [rows, heads, head_dim] of q's dtype")
-    stream = torch.cuda.current_stream()
     plan._on(stream)
     check(lib().tf_paged_attention(q.data_ptr(), q.stride(0) if rows > 1 else heads * D, _page_table(page_table),
                                    _paged_kv(k_pages, v_pages), plan.desc, plan.table.data_ptr(),
                                    D ** -0.5 if scale is None else scale, _act(q), out.data_ptr(),
-                                   plan.workspace.data_ptr(), plan.workspace.numel(), stream.cuda_stream))
+                                   plan.workspace.data_ptr(), plan.desc.workspace_bytes, stream))
     return out
 
 
