@@ -13,8 +13,7 @@
 // as long (128 x 128 pairs: 1024 clocks of either at D = 128).  Hence
 //   * a block holds two halves of 128 rows, each with a softmax warpgroup of
 //     its own (thread = row), so one half's products run while the other's
-//     exponentials do, and a quarter of the exponentials are cubics on the FMA
-//     pipe;
+//     exponentials do;
 //   * one block per SM walks the segments of the plan (paged.h) and the roles
 //     run ahead across them: the next segment's queries and first scores are
 //     computed while this one's outputs are written.
@@ -23,15 +22,18 @@
 //   warps 0-3, 4-7  softmax of half A, B: read S from tensor memory, mask, write
 //              P in 16 bits over S's first columns; at a segment's end read O
 //              and write out (or the piece's partial result).
-//   warp 8     MMA: one elected lane issues, tile by tile,
-//              O_A += P_A V; S_A = Q_A K'; O_B += P_B V; S_B = Q_B K'
-//              with K' the next tile.  MMAs of one thread execute in issue
-//              order, so a next S may be issued over a P that the product
-//              before it still reads, and its completion implies that product's.
-//   warp 9     loader: page ids and TMA of the K and V tiles (128-byte
+//   warps 8, 9  MMA of half A, B: one elected lane issues, tile by tile,
+//              O += P V; S = Q K' with K' the next tile.  MMAs of one thread
+//              execute in issue order, so a next S may be issued over a P that
+//              the product before it still reads, and its completion implies
+//              that product's.  A warp each, because the waits between the
+//              products (some 150 clocks even when they are met) would leave
+//              the tensor cores idle: one warp for both took 3170 clocks a
+//              tile with the softmax taken out, of which 1840 were products.
+//   warp 10    loader: page ids and TMA of the K and V tiles (128-byte
 //              swizzle) into one ring of tiles, K and V in turn.
-//   warps 10, 11  queries of half A, B: 16-byte copies into swizzled rows
-//              (converted where the cache's type differs).
+//   warp 11    queries: 16-byte copies into swizzled rows (converted where the
+//              cache's type differs).
 // Tensor memory columns: O_A [0, 128), O_B [128, 256), S_A [256, 384), S_B.
 //
 // P is rounded to the cache's 16-bit type, relative 2^-11 (f16) or 2^-8
@@ -54,7 +56,7 @@ using namespace tc;
 
 constexpr int kHalf = 128;  // rows of a half = TMEM lanes
 constexpr int kThreads = 384;
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kQueryWarp = 10;
+constexpr int kMmaWarp = 8, kLoadWarp = 10;  // 8, 9: products of half A, B; 11: queries
 constexpr uint32_t kColO = 0, kColS = 256;  // half x: + 128 x
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;
@@ -66,7 +68,7 @@ struct Shape {
   static constexpr int kSlots = D == 128 ? 5 : 8;   // ring of K and V tiles
   static constexpr int kOffRing = 2 * kTile;        // after the two halves' queries
   static constexpr int kOffBar = kOffRing + kSlots * kTile;
-  static constexpr int kSmem = kOffBar + 256 + 1024;  // + barriers + alignment slack
+  static constexpr int kSmem = kOffBar + 512 + 1024;  // + barriers + alignment slack
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
@@ -92,16 +94,15 @@ struct TileParams {
 
 struct Control {
   volatile int abort;
-  uint32_t suspend_ns;
   long long limit;
 };
 
+// The first try is all that a met wait costs.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Control* c, int* err, int code) {
-  const uint32_t susp = c->suspend_ns;
-  if (mbar_try(bar, parity, susp)) return true;
+  if (mbar_try(bar, parity)) return true;
   const long long t0 = clock64();
   const long long limit = c->limit;
-  while (!mbar_try(bar, parity, susp)) {
+  while (!mbar_try(bar, parity)) {
     if (c->abort) return false;
     if (clock64() - t0 > limit) {
       atomicCAS(err, 0, code);
@@ -148,43 +149,29 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float* v) {
-  uint32_t r[64];
+// 32 columns, valid only after tmem_wait of the same registers.
+__device__ __forceinline__ void tmem_ld32_begin(uint32_t taddr, float* v) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
-      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
-      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+        "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
       : "r"(taddr)
       : "memory");
-#pragma unroll
-  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
+// Waits for every load begun; the registers pass through, so no use of them
+// can be scheduled before it.
+__device__ __forceinline__ void tmem_wait32(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]),
+                 "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]),
+                 "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]),
+                 "+f"(v[29]), "+f"(v[30]), "+f"(v[31])::"memory");
 }
 
-// 2^x for x <= 8 on the FMA pipe: x = n + f, n = floor(x) (an add rounded down
-// against 1.5 * 2^23 leaves n in the low mantissa bits), 2^f on [0, 1) by a
-// cubic fitted by weighted least squares for relative error (8.6e-5, below
-// the 16-bit rounding of P), 2^n added to the exponent field.  Below -127 the
-// result is some 1e-38, nothing beside the row's largest weight.
-__device__ __forceinline__ float poly_exp2(float x) {
-  x = fmaxf(x, -127.f);
-  const float t = __fadd_rd(x, 12582912.f);
-  const float f = __fsub_rn(x, __fsub_rn(t, 12582912.f));
-  float p = fmaf(f, 0.07706641f, 0.22764570f);
-  p = fmaf(f, p, 0.69511662f);
-  p = fmaf(f, p, 1.f);
-  return __int_as_float(__float_as_int(p) + (__float_as_int(t) << 23));
-}
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -259,15 +246,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
   uint64_t* q_full = bars;       // [2] a half's query warp wrote its rows
   uint64_t* q_empty = bars + 2;  // [2] MMA: the half's last scores of a segment are done
   uint64_t* s_full = bars + 4;   // [2] MMA: scores of a tile
-  uint64_t* p_full = bars + 6;   // [2] 128 threads: P written, O rescaled
-  uint64_t* o_full = bars + 8;   // [2] MMA: a segment's last product
-  uint64_t* o_free = bars + 10;  // [2] 128 threads: O read
-  uint64_t* kv_full = bars + 12;             // [slots] TMA
-  uint64_t* kv_empty = kv_full + S::kSlots;  // [slots] MMA: products of the tile done
-  uint64_t* done = kv_empty + S::kSlots;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
-  Control* ctl = reinterpret_cast<Control*>(done + 2);
-  static_assert((12 + 2 * S::kSlots + 2) * 8 + sizeof(Control) <= 256, "barrier block");
+  uint64_t* p_full = bars + 6;   // [2][2] 128 threads: a part of P written (before the first, O rescaled)
+  uint64_t* o_full = bars + 10;  // [2] MMA: a segment's last product
+  uint64_t* o_free = bars + 12;  // [2] 128 threads: O read
+  uint64_t* kv_full = bars + 14;             // [slots] TMA
+  uint64_t* kv_empty = kv_full + S::kSlots;  // [slots] each half: its products of the tile done
+  uint64_t* done = kv_empty + S::kSlots;     // [2] MMA: all products of a half
+  uint64_t* baton = done + 2;                // [2] the other half's products of a tile are issued
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(baton + 2);
+  Control* ctl = reinterpret_cast<Control*>(baton + 3);
+  static_assert((14 + 2 * S::kSlots + 5) * 8 + sizeof(Control) <= 512, "barrier block");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int* err = p.err;
@@ -276,19 +264,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
       mbar_init(&q_full[x], 32);
       mbar_init(&q_empty[x], 1);
       mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x], kHalf);
+      mbar_init(&p_full[2 * x], kHalf);
+      mbar_init(&p_full[2 * x + 1], kHalf);
       mbar_init(&o_full[x], 1);
       mbar_init(&o_free[x], kHalf);
+      mbar_init(&done[x], 1);
+      mbar_init(&baton[x], 1);
     }
     for (int i = 0; i < S::kSlots; ++i) {
       mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&kv_empty[i], 2);
     }
-    mbar_init(done, 1);
-    const long long lim = *p.wait_cycles;
     ctl->abort = 0;
-    ctl->limit = lim;
-    ctl->suspend_ns = lim < 2000000000LL ? 0u : kSuspendNs;
+    ctl->limit = *p.wait_cycles;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) {
@@ -346,48 +334,55 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
       // Copies in flight land before the block exits.
       for (int i = n > S::kSlots ? n - S::kSlots : 0; i < n; ++i)
         drain(&kv_full[i % S::kSlots], (uint32_t)((i / S::kSlots) & 1), err);
-    } else if (warp == kMmaWarp) {
+    } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+      // ---- products of half x.
+      const int x = warp - kMmaWarp;
       const uint32_t leader = elect_one();
       const uint32_t fmt = Act<C>::kDtype == TF_DTYPE_BF16 ? (1u << 7) | (1u << 10) : 0u;  // A and B are bf16
       const uint32_t id_qk = idesc_f16(kHalf, kTileKeys) | fmt;
       const uint32_t id_pv = idesc_f16(kHalf, D) | (1u << 16) | fmt;  // B (V) MN-major
-      int n = 0;                                                      // ring position
-      uint32_t q_turn[2] = {0, 0}, p_turn[2] = {0, 0}, o_turn[2] = {0, 0};
+      const uint32_t t_o = tmem + kColO + 128 * x, t_s = tmem + kColS + 128 * x;
+      const uint32_t qa = smem_addr(base + x * S::kTile);
+      int n = 0;  // ring position
+      uint32_t q_turn = 0, p_turn = 0, o_turn = 0, baton_turn = 0;
       bool ok = true;
-      auto scores = [&](int x, int slot) {
-        const uint32_t qa = smem_addr(base + x * S::kTile), ka = smem_addr(base + S::kOffRing + slot * S::kTile);
+      auto landed = [&](int at) {  // tile `at` of the ring is there
+        return wait_warp(&kv_full[at % S::kSlots], (uint32_t)((at / S::kSlots) & 1), ctl, err, 82);
+      };
+      auto scores = [&](int at) {
+        const int slot = at % S::kSlots;
+        const uint32_t ka = smem_addr(base + S::kOffRing + slot * S::kTile);
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) {
           const uint32_t off = (uint32_t)((s >> 2) * kColBytes + (s & 3) * 32);
-          mma_f16(leader, tmem + kColS + 128 * x, sw128_desc(qa + off), sw128_desc(ka + off), id_qk, s > 0 ? 1u : 0u);
+          mma_f16(leader, t_s, sw128_desc(qa + off), sw128_desc(ka + off), id_qk, s > 0 ? 1u : 0u);
         }
         mma_commit(leader, &s_full[x]);
+        mma_commit(leader, &kv_empty[slot]);
       };
       for (int seg = seg0; seg < seg1 && ok; ++seg) {
         const PagedSegment g = p.segments[seg];
         const View view(g, p.group);
-        if (view.tiles == 0) continue;
-        const int k0 = n % S::kSlots;
-        if (!(ok = wait_warp(&kv_full[k0], (uint32_t)((n / S::kSlots) & 1), ctl, err, 82))) break;
-        for (int x = 0; x < 2 && ok; ++x) {
-          if (view.count[x] == 0) continue;
-          if (!(ok = wait_warp(&q_full[x], q_turn[x] & 1, ctl, err, 83))) break;
-          ++q_turn[x];
+        const int count = view.count[x];
+        if (count > 0) {
+          if (!(ok = landed(n) && wait_warp(&q_full[x], q_turn & 1, ctl, err, 83))) break;
+          ++q_turn;
           tc_fence_after();
-          scores(x, k0);
-          if (view.count[x] == 1) mma_commit(leader, &q_empty[x]);
+          scores(n);
+          if (count == 1) mma_commit(leader, &q_empty[x]);
         }
-        mma_commit(leader, &kv_empty[k0]);
-        ++n;
-        for (int j = 0; j < view.tiles && ok; ++j) {
-          const int vs = n % S::kSlots;
-          if (!(ok = wait_warp(&kv_full[vs], (uint32_t)((n / S::kSlots) & 1), ctl, err, 84))) break;
-          ++n;
+        const int both = min(count, view.count[1 - x]);  // tiles that both halves meet
+        for (int j = 0; j < count && ok; ++j) {
+          // Ring: K of tile j at n, V of tile j, K of tile j + 1.
+          const bool more = j + 1 < count;
+          if (!(ok = landed(n + 1) && (!more || landed(n + 2)))) break;
+          const int vs = (n + 1) % S::kSlots;
           uint8_t* vt = base + S::kOffRing + vs * S::kTile;
           const int have = g.kv_len - (g.tile0 + j) * kTileKeys;
           if (have < kTileKeys) {
             // Slots past the request's length hold anything, NaN included:
-            // 0 * NaN would reach the outputs, so their values become zeros.
+            // 0 * NaN would reach the outputs, so their values become zeros
+            // (by both halves' warps, each before its own products).
             for (int i = have * 8 + lane; i < kTileKeys * 8; i += 32)
 #pragma unroll
               for (int h = 0; h < D / 64; ++h)
@@ -395,56 +390,56 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
             fence_proxy_async();
             __syncwarp();
           }
+          // O still holds the half's last segment until it has been read.
+          if (j == 0 && o_turn++ > 0 && !(ok = wait_warp(&o_free[x], o_turn & 1, ctl, err, 86))) break;
           const uint32_t va = smem_addr(vt);
-          const bool more = j + 1 < view.tiles;
-          const int ks = n % S::kSlots;
-          const uint32_t k_parity = (uint32_t)((n / S::kSlots) & 1);
-          for (int x = 0; x < 2 && ok; ++x) {
-            if (j >= view.count[x]) continue;
-            if (!(ok = wait_warp(&p_full[x], p_turn[x] & 1, ctl, err, 85))) break;
-            ++p_turn[x];
-            if (j == 0) {
-              // O still holds the half's last segment until it has been read.
-              if (o_turn[x] > 0 && !(ok = wait_warp(&o_free[x], (o_turn[x] - 1) & 1, ctl, err, 86))) break;
-              ++o_turn[x];
-            }
+          if (j < both && (x == 1 || j > 0)) {
+            if (!(ok = wait_warp(&baton[x], baton_turn & 1, ctl, err, 87))) break;
+            ++baton_turn;
+          }
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            if (!(ok = wait_warp(&p_full[2 * x + part], p_turn & 1, ctl, err, 85))) break;
             tc_fence_after();
 #pragma unroll
-            for (int s = 0; s < kTileKeys / 16; ++s)
-              mma_f16_ts(leader, tmem + kColO + 128 * x, tmem + kColS + 128 * x + 8 * s,
-                         sw128_mn_desc(va + s * 2048, kColBytes, 1024), id_pv, (j > 0 || s > 0) ? 1u : 0u);
-            if (j + 1 == view.count[x]) mma_commit(leader, &o_full[x]);
-            if (j + 1 < view.count[x]) {
-              if (!(ok = wait_warp(&kv_full[ks], k_parity, ctl, err, 87))) break;
-              scores(x, ks);
-              if (j + 2 == view.count[x]) mma_commit(leader, &q_empty[x]);
-            }
+            for (int s = 4 * part; s < 4 * part + 4; ++s)
+              mma_f16_ts(leader, t_o, t_s + 8 * s, sw128_mn_desc(va + s * 2048, kColBytes, 1024), id_pv,
+                         (j > 0 || s > 0) ? 1u : 0u);
           }
           if (!ok) break;
+          ++p_turn;
           mma_commit(leader, &kv_empty[vs]);
           if (more) {
-            mma_commit(leader, &kv_empty[ks]);
-            ++n;
+            scores(n + 2);
+            if (j + 2 == count) mma_commit(leader, &q_empty[x]);
+          } else {
+            mma_commit(leader, &o_full[x]);
           }
+          if (lane == 0 && (x == 0 ? j < both : j + 1 < both)) mbar_arrive(&baton[1 - x]);
+          n += 2;
         }
+        // Tiles that only the other half meets: released once they are there,
+        // so this warp never runs a turn of the ring ahead.
+        for (int j = count; j < view.tiles && ok; ++j)
+          for (int v = 0; v < 2 && ok; ++v, ++n)
+            if ((ok = landed(n)) && lane == 0) mbar_arrive(&kv_empty[n % S::kSlots]);
       }
       // Every MMA issued here completes before tensor memory is released.
-      mma_commit(leader, done);
-      drain(done, 0, err);
+      mma_commit(leader, &done[x]);
+      drain(&done[x], 0, err);
     } else {
-      // ---- queries of half x.
-      const int x = warp - kQueryWarp;
-      uint8_t* dst = base + x * S::kTile;
-      uint32_t turn = 0;
+      // ---- queries of both halves.
+      uint32_t turn[2] = {0, 0};
       constexpr int kChunks = D / 8, kRowsAt = 32 / kChunks;  // 16-byte chunks of a row, rows per pass
       const int c = lane % kChunks;
       bool ok = true;
       for (int seg = seg0; seg < seg1 && ok; ++seg) {
         const PagedSegment g = p.segments[seg];
         const View view(g, p.group);
+        for (int x = 0; x < 2; ++x) {
         if (view.count[x] == 0) continue;
-        if (turn > 0 && !(ok = wait_warp(&q_empty[x], (turn - 1) & 1, ctl, err, 88))) break;
-        ++turn;
+        if (turn[x] > 0 && !(ok = wait_warp(&q_empty[x], (turn[x] - 1) & 1, ctl, err, 88))) break;
+        ++turn[x];
         int r = lane / kChunks;
         const int rows = min(kHalf, g.rows - kHalf * x);
         const int pr = g.row0 + kHalf * x + min(r, rows - 1);  // addresses stay inside q
@@ -452,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
         const T* q = static_cast<const T*>(p.q) + (int64_t)(g.q_row + token) * p.q_stride +
                      (int64_t)(g.kv_head * p.group + head) * D + 8 * c;
         // Row r of each 64-column half at r * 128, chunk c at (c ^ (r & 7)) * 16.
-        uint8_t* at = dst + (c >> 3) * kColBytes;
+        uint8_t* at = base + x * S::kTile + (c >> 3) * kColBytes;
 #pragma unroll 8
         for (int i = 0; i < kHalf / kRowsAt; ++i, r += kRowsAt) {
           uint8_t* to = at + r * 128 + (((c & 7) ^ (r & 7)) << 4);
@@ -481,6 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
         if constexpr (Act<T>::kDtype == Act<C>::kDtype) asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async();
         mbar_arrive(&q_full[x]);
+        }
       }
     }
   } else {
@@ -508,8 +504,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
         ++s_turn;
         tc_fence_after();
         float sc[128];
-        tmem_ld64(t_s, sc);
-        tmem_ld64(t_s + 64, sc + 64);
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) tmem_ld32_begin(t_s + c, sc + c);
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) tmem_wait32(sc + c);
         const int key0 = (g.tile0 + j) * kTileKeys;
         if (key0 + kTileKeys - 1 > first_limit) {
           const int lim = limit - key0;  // later columns are masked
@@ -517,16 +515,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
           for (int c = 0; c < 128; ++c) sc[c] = c > lim ? -INFINITY : sc[c];
         }
         // The maximum of the raw scores (the scale is positive), NaN kept.
-        float mp[4];
+        float mp[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mp[i] = sc[i];
+        for (int i = 0; i < 8; ++i) mp[i] = max_nan(sc[2 * i], sc[2 * i + 1]);
 #pragma unroll
-        for (int c = 4; c < 124; c += 8)
+        for (int c = 16; c < 128; c += 16)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mp[i] = max_nan(mp[i], sc[c + 2 * i], sc[c + 2 * i + 1]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mp[i] = max_nan(mp[i], sc[124 + i]);
-        float mx = max_nan(max_nan(mp[0], mp[1]), mp[2], mp[3]) * p.scale_log2;
+          for (int i = 0; i < 8; ++i) mp[i] = max_nan(mp[i], sc[c + 2 * i], sc[c + 2 * i + 1]);
+        float mx = max_nan(max_nan(mp[0], mp[1], mp[2]), max_nan(mp[3], mp[4], mp[5]), max_nan(mp[6], mp[7])) *
+                   p.scale_log2;
         if (mx == INFINITY) mx = __uint_as_float(0x7fc00000u);  // inf - inf: the row is NaN
         float factor = 1.f;
         if (!(mx <= m + kRescale)) {  // also for NaN, and for the first key seen
@@ -549,8 +546,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
             tmem_st16(t_o + c + 16, w + 16);
           }
         }
-        // Exponent arguments and sums on packed pairs, one exponential in
-        // four a cubic.
+        // Exponent arguments and sums on packed pairs.  P goes out in two
+        // parts of 64 keys, so the product of the first runs while the
+        // second's exponentials do.
         const float sub = m == -INFINITY ? 0.f : -m;
         const uint64_t sl2 = f2_pack(p.scale_log2, p.scale_log2), nm = f2_pack(sub, sub);
         uint64_t sp[4];
@@ -562,21 +560,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
             const int k0 = 64 * half + 2 * c;
-            float x0, x1;
-            f2_unpack(f2_fma(f2_pack(sc[k0], sc[k0 + 1]), sl2, nm), x0, x1);
-            const float a = fast_exp2(x0), b = (c & 1) ? poly_exp2(x1) : fast_exp2(x1);
+            float a, b;
+            f2_unpack(f2_fma(f2_pack(sc[k0], sc[k0 + 1]), sl2, nm), a, b);
+            a = fast_exp2(a);
+            b = fast_exp2(b);
             sp[c & 3] = f2_add(sp[c & 3], f2_pack(a, b));
             pk[c] = pack2<C>(a, b);
           }
           tmem_st16(t_s + 32 * half, pk);
           tmem_st16(t_s + 32 * half + 16, pk + 16);
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(&p_full[2 * x + half]);
         }
         float s0, s1;
         f2_unpack(f2_add(f2_add(sp[0], sp[1]), f2_add(sp[2], sp[3])), s0, s1);
         l += s0 + s1;
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&p_full[x]);
       }
       if (!ok) break;
       const int row = kHalf * x + r;
@@ -586,8 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
         ++o_turn;
         tc_fence_after();
       }
-      // A row that has seen no key above -inf gives zeros (its l holds nothing
-      // but the cubics' 1e-38).
+      // A row that has seen no key above -inf gives zeros.
       const float inv = m == -INFINITY ? 0.f : 1.f / l;
       T* orow = static_cast<T*>(p.out) +
                 ((int64_t)(g.q_row + token) * p.heads + g.kv_head * p.group + pr % p.group) * D;
