@@ -20,8 +20,12 @@
 //
 // Roles (384 threads; registers move from the third warpgroup to the softmax):
 //   warps 0-3, 4-7  softmax of half A, B: read S from tensor memory, mask, write
-//              P in 16 bits over S's first columns; at a segment's end read O
-//              and write out (or the piece's partial result).
+//              P in 16 bits over S's first columns; after a segment's last
+//              scores copy the next segment's queries into shared memory
+//              (each thread its row, converted where the cache's type
+//              differs), then read O and write out (or the piece's partial
+//              result).  A warp of its own for the queries took 9000 clocks a
+//              half, most of a short segment.
 //   warps 8, 9  MMA of half A, B: one elected lane issues, tile by tile,
 //              O += P V; S = Q K' with K' the next tile.  MMAs of one thread
 //              execute in issue order, so a next S may be issued over a P that
@@ -32,8 +36,6 @@
 //              tile with the softmax taken out, of which 1840 were products.
 //   warp 10    loader: page ids and TMA of the K and V tiles (128-byte
 //              swizzle) into one ring of tiles, K and V in turn.
-//   warp 11    queries: 16-byte copies into swizzled rows (converted where the
-//              cache's type differs).
 // Tensor memory columns: O_A [0, 128), O_B [128, 256), S_A [256, 384), S_B.
 //
 // P is rounded to the cache's 16-bit type, relative 2^-11 (f16) or 2^-8
@@ -56,7 +58,7 @@ using namespace tc;
 
 constexpr int kHalf = 128;  // rows of a half = TMEM lanes
 constexpr int kThreads = 384;
-constexpr int kMmaWarp = 8, kLoadWarp = 10;  // 8, 9: products of half A, B; 11: queries
+constexpr int kMmaWarp = 8, kLoadWarp = 10;  // 8, 9: products of half A, B; 11 fills the warpgroup
 constexpr uint32_t kColO = 0, kColS = 256;  // half x: + 128 x
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;
@@ -85,7 +87,7 @@ struct TileParams {
   const PagedSegment* segments;
   const int32_t* starts;
   float* stat;  // [part][2][256]: m, l
-  float* part;  // [part][256][D]
+  float* part;  // [part][D / 4][256][4]: a warp's rows side by side
   void* out;
   float scale_log2;
   int* err;
@@ -243,26 +245,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + S::kOffBar);
-  uint64_t* q_full = bars;       // [2] a half's query warp wrote its rows
-  uint64_t* q_empty = bars + 2;  // [2] MMA: the half's last scores of a segment are done
-  uint64_t* s_full = bars + 4;   // [2] MMA: scores of a tile
-  uint64_t* p_full = bars + 6;   // [2][2] 128 threads: a part of P written (before the first, O rescaled)
-  uint64_t* o_full = bars + 10;  // [2] MMA: a segment's last product
-  uint64_t* o_free = bars + 12;  // [2] 128 threads: O read
-  uint64_t* kv_full = bars + 14;             // [slots] TMA
+  uint64_t* q_full = bars;       // [2] 128 threads: the half's query rows are written
+  uint64_t* s_full = bars + 2;   // [2] MMA: scores of a tile
+  uint64_t* p_full = bars + 4;   // [2][2] 128 threads: a part of P written (before the first, O rescaled)
+  uint64_t* o_full = bars + 8;   // [2] MMA: a segment's last product
+  uint64_t* o_free = bars + 10;  // [2] 128 threads: O read
+  uint64_t* kv_full = bars + 12;             // [slots] TMA
   uint64_t* kv_empty = kv_full + S::kSlots;  // [slots] each half: its products of the tile done
   uint64_t* done = kv_empty + S::kSlots;     // [2] MMA: all products of a half
   uint64_t* baton = done + 2;                // [2] the other half's products of a tile are issued
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(baton + 2);
   Control* ctl = reinterpret_cast<Control*>(baton + 3);
-  static_assert((14 + 2 * S::kSlots + 5) * 8 + sizeof(Control) <= 512, "barrier block");
+  static_assert((12 + 2 * S::kSlots + 5) * 8 + sizeof(Control) <= 512, "barrier block");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int* err = p.err;
   if (tid == 0) {
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&q_full[x], 32);
-      mbar_init(&q_empty[x], 1);
+      mbar_init(&q_full[x], kHalf);
       mbar_init(&s_full[x], 1);
       mbar_init(&p_full[2 * x], kHalf);
       mbar_init(&p_full[2 * x + 1], kHalf);
@@ -369,7 +369,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
           ++q_turn;
           tc_fence_after();
           scores(n);
-          if (count == 1) mma_commit(leader, &q_empty[x]);
         }
         const int both = min(count, view.count[1 - x]);  // tiles that both halves meet
         for (int j = 0; j < count && ok; ++j) {
@@ -411,7 +410,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
           mma_commit(leader, &kv_empty[vs]);
           if (more) {
             scores(n + 2);
-            if (j + 2 == count) mma_commit(leader, &q_empty[x]);
           } else {
             mma_commit(leader, &o_full[x]);
           }
@@ -427,57 +425,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
       // Every MMA issued here completes before tensor memory is released.
       mma_commit(leader, &done[x]);
       drain(&done[x], 0, err);
-    } else {
-      // ---- queries of both halves.
-      uint32_t turn[2] = {0, 0};
-      constexpr int kChunks = D / 8, kRowsAt = 32 / kChunks;  // 16-byte chunks of a row, rows per pass
-      const int c = lane % kChunks;
-      bool ok = true;
-      for (int seg = seg0; seg < seg1 && ok; ++seg) {
-        const PagedSegment g = p.segments[seg];
-        const View view(g, p.group);
-        for (int x = 0; x < 2; ++x) {
-        if (view.count[x] == 0) continue;
-        if (turn[x] > 0 && !(ok = wait_warp(&q_empty[x], (turn[x] - 1) & 1, ctl, err, 88))) break;
-        ++turn[x];
-        int r = lane / kChunks;
-        const int rows = min(kHalf, g.rows - kHalf * x);
-        const int pr = g.row0 + kHalf * x + min(r, rows - 1);  // addresses stay inside q
-        int token = pr / p.group, head = pr % p.group;
-        const T* q = static_cast<const T*>(p.q) + (int64_t)(g.q_row + token) * p.q_stride +
-                     (int64_t)(g.kv_head * p.group + head) * D + 8 * c;
-        // Row r of each 64-column half at r * 128, chunk c at (c ^ (r & 7)) * 16.
-        uint8_t* at = base + x * S::kTile + (c >> 3) * kColBytes;
-#pragma unroll 8
-        for (int i = 0; i < kHalf / kRowsAt; ++i, r += kRowsAt) {
-          uint8_t* to = at + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-          if constexpr (Act<T>::kDtype == Act<C>::kDtype) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(to)), "l"(q),
-                         "r"(r < rows ? 16 : 0)
-                         : "memory");
-          } else {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (r < rows) {
-              float f[8];
-              unpack8<T>(ld_v4(q), f);
-              v = pack8<C>(f);
-            }
-            *reinterpret_cast<uint4*>(to) = v;
-          }
-          if (r + kRowsAt < rows) {  // the next row of this lane exists
-            head += kRowsAt;
-            q += (int64_t)kRowsAt * D;
-            while (head >= p.group) {
-              head -= p.group;
-              q += p.q_stride - (int64_t)p.group * D;
-            }
-          }
-        }
-        if constexpr (Act<T>::kDtype == Act<C>::kDtype) asm volatile("cp.async.wait_all;" ::: "memory");
-        fence_proxy_async();
-        mbar_arrive(&q_full[x]);
-        }
-      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -488,6 +435,43 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
     const uint32_t t_o = lane_base + kColO + 128 * x, t_s = lane_base + kColS + 128 * x;
     uint32_t s_turn = 0, o_turn = 0;
     bool ok = true;
+    // Copies this thread's query row of the half's next segment with tiles,
+    // from segment `seg` on, into the K-major 128-byte swizzle: row r of each
+    // 64-column half at r * 128, 16-byte chunk c at (c ^ (r & 7)) * 16.  Rows
+    // past the segment's become zeros.
+    auto copy_queries = [&](int seg) {
+      for (; seg < seg1; ++seg) {
+        const PagedSegment g = p.segments[seg];
+        if (View(g, p.group).count[x] == 0) continue;
+        const bool mine = kHalf * x + r < g.rows;
+        const int pr = g.row0 + min(kHalf * x + r, g.rows - 1);
+        const T* q = static_cast<const T*>(p.q) + (int64_t)(g.q_row + pr / p.group) * p.q_stride +
+                     (int64_t)(g.kv_head * p.group + pr % p.group) * D;
+        uint8_t* to = base + x * S::kTile + r * 128;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          uint8_t* at = to + (c >> 3) * kColBytes + (((c & 7) ^ (r & 7)) << 4);
+          if constexpr (Act<T>::kDtype == Act<C>::kDtype) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(at)), "l"(q + 8 * c),
+                         "r"(mine ? 16 : 0)
+                         : "memory");
+          } else {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (mine) {
+              float f[8];
+              unpack8<T>(ld_v4(q + 8 * c), f);
+              v = pack8<C>(f);
+            }
+            *reinterpret_cast<uint4*>(at) = v;
+          }
+        }
+        if constexpr (Act<T>::kDtype == Act<C>::kDtype) asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async();
+        mbar_arrive(&q_full[x]);
+        return;
+      }
+    };
+    copy_queries(seg0);
     for (int seg = seg0; seg < seg1 && ok; ++seg) {
       const PagedSegment g = p.segments[seg];
       if (kHalf * x >= g.rows) continue;
@@ -581,6 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
       const int row = kHalf * x + r;
       const bool mine = row < g.rows;
       if (count > 0) {
+        copy_queries(seg + 1);  // the last scores are done, so the rows' place is free
         if (!(ok = wait_warp(&o_full[x], o_turn & 1, ctl, err, 91))) break;
         ++o_turn;
         tc_fence_after();
@@ -589,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
       const float inv = m == -INFINITY ? 0.f : 1.f / l;
       T* orow = static_cast<T*>(p.out) +
                 ((int64_t)(g.q_row + token) * p.heads + g.kv_head * p.group + pr % p.group) * D;
-      float* prow = p.part + ((int64_t)g.part * kTileRows + row) * D;
+      float* prow = p.part + (int64_t)g.part * kTileRows * D + row * 4;
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         float o[32];
@@ -611,7 +596,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
         } else {
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(prow + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            *reinterpret_cast<float4*>(prow + (c + i) * kTileRows) =
+                make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
       }
       if (mine && g.part >= 0) {
@@ -631,45 +617,40 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
-// Joins the pieces of cut row blocks: one warp per row, in piece order.
+// Joins the pieces of cut row blocks, in piece order.  A warp takes 32 rows
+// and 4 columns, so the pieces' outputs arrive 512 bytes at a time.
 constexpr int kMergeWarps = 8;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kMergeWarps)
     paged_merge_kernel(const PagedSegment* __restrict__ items, const float* __restrict__ stat,
                        const float* __restrict__ part, int group, int heads, T* __restrict__ out) {
-  constexpr int kPer = D / 32;
-  const PagedSegment& g = items[blockIdx.y];
-  const int row = blockIdx.x * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const PagedSegment& g = items[blockIdx.z];
+  const int row = blockIdx.x * 32 + (threadIdx.x & 31);
+  const int c = blockIdx.y * kMergeWarps + (threadIdx.x >> 5);  // columns 4 c ..
   if (row >= g.rows) return;
   const float* st = stat + (int64_t)g.part0 * 2 * kTileRows + row;
   float M = -INFINITY;
   for (int i = 0; i < g.parts; ++i) M = max_nan(M, st[(int64_t)i * 2 * kTileRows]);
-  float acc[kPer], sum = 0.f;
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
   for (int i = 0; i < g.parts; ++i) {
     const float m = st[(int64_t)i * 2 * kTileRows];
     if (m == -INFINITY) continue;
     const float f = fast_exp2(m - M);
-    const float* o = part + ((int64_t)(g.part0 + i) * kTileRows + row) * D + kPer * lane;
+    const float4 v = *reinterpret_cast<const float4*>(part + (int64_t)(g.part0 + i) * kTileRows * D +
+                                                      (c * kTileRows + row) * 4);
     sum = fmaf(f, st[(int64_t)i * 2 * kTileRows + kTileRows], sum);
-    if constexpr (kPer == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(o);
-      acc[0] = fmaf(f, v.x, acc[0]);
-      acc[1] = fmaf(f, v.y, acc[1]);
-      acc[2] = fmaf(f, v.z, acc[2]);
-      acc[3] = fmaf(f, v.w, acc[3]);
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(o);
-      acc[0] = fmaf(f, v.x, acc[0]);
-      acc[1] = fmaf(f, v.y, acc[1]);
-    }
+    acc.x = fmaf(f, v.x, acc.x);
+    acc.y = fmaf(f, v.y, acc.y);
+    acc.z = fmaf(f, v.z, acc.z);
+    acc.w = fmaf(f, v.w, acc.w);
   }
+  const float inv = M == -INFINITY ? 0.f : 1.f / sum;
   const int pr = g.row0 + row;
-  T* to = out + ((int64_t)(g.q_row + pr / group) * heads + g.kv_head * group + pr % group) * D + kPer * lane;
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) to[k] = from_f<T>(M == -INFINITY ? 0.f : acc[k] / sum);
+  T* to = out + ((int64_t)(g.q_row + pr / group) * heads + g.kv_head * group + pr % group) * D + 4 * c;
+  alignas(8) const T v[4] = {from_f<T>(acc.x * inv), from_f<T>(acc.y * inv), from_f<T>(acc.z * inv), from_f<T>(acc.w * inv)};
+  *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(v);
 }
 
 template <typename T, typename C, int D>
@@ -684,8 +665,8 @@ tf_status launch(const TileParams& p, const tf_paged_plan& plan, const PagedSegm
   paged_tile_kernel<T, C, D><<<plan.tile_blocks, kThreads, Shape<D>::kSmem, s>>>(p);
   TF_TRY(check_launch("paged_tile"));
   if (plan.merges == 0) return TF_OK;
-  // grid.y is below 65536: at most one cut item per block.
-  const dim3 grid(kTileRows / kMergeWarps, (unsigned)plan.merges);
+  // grid.z is below 65536: at most one cut item per block.
+  const dim3 grid(kTileRows / 32, D / 4 / kMergeWarps, (unsigned)plan.merges);
   paged_merge_kernel<T, D><<<grid, 32 * kMergeWarps, 0, s>>>(merges, p.stat, p.part, p.group, p.heads,
                                                              static_cast<T*>(p.out));
   return check_launch("paged_merge");
