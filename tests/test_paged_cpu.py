@@ -49,11 +49,11 @@ def test_attention_and_append_refuse_before_any_launch():
     kv = PagedKV(0x1000, 0x2000, 4, 2 * 16 * 128, 2, 16, 128, 1)
     tab = PageTable(0x3000, 3, 1, 3)
 
-    def attend(kv=kv, tab=tab, stride=1024, q=0x4000, ws=1 << 20, act=1, scale=0.1):
+    def attend(kv=kv, tab=tab, stride=1024, q=0x4000, ws=1 << 20, act=1, scale=0.1, out=0x6000):
         return L.tf_paged_attention(C.c_void_p(q), stride, C.byref(tab), C.byref(kv), C.byref(d), C.c_void_p(0x5000),
-                                    scale, act, C.c_void_p(0x6000), C.c_void_p(0x7000), ws, None)
+                                    scale, act, C.c_void_p(out), C.c_void_p(0x7000), ws, None)
 
-    assert attend(q=0) == 1 and attend(q=0x4008) == 1
+    assert attend(q=0) == 1 and attend(q=0x4008) == 1 and attend(out=0x6010) == 1
     assert attend(stride=1000) == 2 and attend(stride=1028) == 2
     assert attend(act=3) == 1 and attend(scale=-1.0) == 1
     assert attend(tab=PageTable(0x3000, 2, 1, 2)) == 2          # the request needs three pages

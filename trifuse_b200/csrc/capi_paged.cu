@@ -146,7 +146,7 @@ int tf_paged_attention(const void* q, int64_t q_stride, const tf_page_table* tab
   if (q_stride < (int64_t)plan->heads * plan->head_dim || q_stride % 8)
     return set_error(TF_ERR_SHAPE, "paged_attention: q stride %lld", (long long)q_stride);
   if (plan->rows == 0) return TF_OK;
-  if (!q || !out || !plan_table || !aligned16(q) || !aligned16(out) || !aligned16(plan_table))
+  if (!q || !out || !plan_table || !aligned16(q) || (reinterpret_cast<uintptr_t>(out) & 31u) || !aligned16(plan_table))
     return set_error(TF_ERR_INVALID_ARGUMENT, "paged_attention: NULL or unaligned pointer");
   if (workspace_bytes < plan->workspace_bytes ||
       (plan->workspace_bytes && (!workspace || !aligned16(workspace))))

@@ -220,6 +220,14 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// One whole 32-byte sector (a thread's rows are apart, so 16-byte stores would
+// touch every sector twice).
+__device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z),
+               "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
 // A segment as the roles see it: the tiles that each half meets.
 struct View {
   int count[2];  // tiles of half A, B, from tile0
@@ -435,31 +443,37 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
     const uint32_t t_o = lane_base + kColO + 128 * x, t_s = lane_base + kColS + 128 * x;
     uint32_t s_turn = 0, o_turn = 0;
     bool ok = true;
-    // Copies this thread's query row of the half's next segment with tiles,
-    // from segment `seg` on, into the K-major 128-byte swizzle: row r of each
-    // 64-column half at r * 128, 16-byte chunk c at (c ^ (r & 7)) * 16.  Rows
-    // past the segment's become zeros.
+    // Copies the query rows of the half's next segment with tiles, from
+    // segment `seg` on, into the K-major 128-byte swizzle: row i of each
+    // 64-column half at i * 128, 16-byte chunk c at (c ^ (i & 7)) * 16.  A warp
+    // copies its 32 rows whole rows at a time; rows past the segment's become
+    // zeros.
     auto copy_queries = [&](int seg) {
+      constexpr int kChunks = D / 8, kRowsAt = 32 / kChunks;  // chunks of a row, rows per pass
       for (; seg < seg1; ++seg) {
         const PagedSegment g = p.segments[seg];
         if (View(g, p.group).count[x] == 0) continue;
-        const bool mine = kHalf * x + r < g.rows;
         const int pr = g.row0 + min(kHalf * x + r, g.rows - 1);
-        const T* q = static_cast<const T*>(p.q) + (int64_t)(g.q_row + pr / p.group) * p.q_stride +
-                     (int64_t)(g.kv_head * p.group + pr % p.group) * D;
-        uint8_t* to = base + x * S::kTile + r * 128;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          uint8_t* at = to + (c >> 3) * kColBytes + (((c & 7) ^ (r & 7)) << 4);
+        const T* own = static_cast<const T*>(p.q) + (int64_t)(g.q_row + pr / p.group) * p.q_stride +
+                       (int64_t)(g.kv_head * p.group + pr % p.group) * D;
+        const int c = lane % kChunks;
+        uint8_t* to = base + x * S::kTile + (c >> 3) * kColBytes;
+#pragma unroll 8
+        for (int i = 0; i < 32 / kRowsAt; ++i) {
+          const int from = i * kRowsAt + lane / kChunks;  // lane whose row this is
+          const T* q = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(own), from)) + 8 * c;
+          const int row = (warp & 3) * 32 + from;
+          const bool real = kHalf * x + row < g.rows;
+          uint8_t* at = to + row * 128 + (((c & 7) ^ (row & 7)) << 4);
           if constexpr (Act<T>::kDtype == Act<C>::kDtype) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(at)), "l"(q + 8 * c),
-                         "r"(mine ? 16 : 0)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(at)), "l"(q),
+                         "r"(real ? 16 : 0)
                          : "memory");
           } else {
             uint4 v = make_uint4(0, 0, 0, 0);
-            if (mine) {
+            if (real) {
               float f[8];
-              unpack8<T>(ld_v4(q + 8 * c), f);
+              unpack8<T>(ld_v4(q), f);
               v = pack8<C>(f);
             }
             *reinterpret_cast<uint4*>(at) = v;
@@ -587,11 +601,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
         if (!mine) continue;
         if (g.part < 0) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            float f[8];
+          for (int i = 0; i < 32; i += 16) {
+            float f[16];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) f[k] = m == -INFINITY ? 0.f : o[i + k] * inv;
-            *reinterpret_cast<uint4*>(orow + c + i) = pack8<T>(f);
+            for (int k = 0; k < 16; ++k) f[k] = m == -INFINITY ? 0.f : o[i + k] * inv;
+            store32(orow + c + i, pack8<T>(f), pack8<T>(f + 8));
           }
         } else {
 #pragma unroll
