@@ -392,7 +392,10 @@ typedef struct tf_paged_plan {
   int64_t split_starts_offset;
   int64_t tile_segments_offset;
   int64_t tile_starts_offset;
-  int64_t merges_offset;
+  int64_t tile_merges_offset;
+  int64_t half_segments_offset;
+  int64_t half_starts_offset;
+  int64_t half_merges_offset;
   int32_t requests;
   int32_t heads;
   int32_t kv_heads;
@@ -404,7 +407,11 @@ typedef struct tf_paged_plan {
   int32_t split_counters;
   int32_t tile_blocks;      /* the same of the tensor-core kernel            */
   int32_t tile_parts;
-  int32_t merges;           /* row blocks that were cut                      */
+  int32_t tile_merges;      /* row blocks that were cut                      */
+  int32_t half_blocks;      /* the same of its form for up to 128 rows       */
+  int32_t half_parts;
+  int32_t half_merges;
+  int32_t reserved;
 } tf_paged_plan;
 
 /* new_lengths[i] query rows and kv_lengths[i] cached tokens (the new ones

@@ -75,8 +75,7 @@ def test_attention_and_append_refuse_before_any_launch():
 
 def segments(d, raw, kind):
     import struct
-    blocks, first, at = ((d.split_blocks, d.split_starts_offset, d.split_segments_offset) if kind == "split" else
-                         (d.tile_blocks, d.tile_starts_offset, d.tile_segments_offset))
+    blocks, first, at = (getattr(d, kind + name) for name in ("_blocks", "_starts_offset", "_segments_offset"))
     starts = struct.unpack_from(f"<{blocks + 1}i", raw, first)
     return [(b, struct.unpack_from("<13i", raw, at + 64 * i))
             for b in range(blocks) for i in range(starts[b], starts[b + 1])]
@@ -91,7 +90,8 @@ def test_every_row_meets_every_tile_once():
         H, Hk = rng.choice([(16, 16), (8, 1), (14, 2), (32, 8)])
         _, d, raw = plan(new, kv, H, Hk)
         rows_seen = {}
-        for kind, most, keys, all_parts in (("split", 16, 32, d.split_parts), ("tile", 256, 128, d.tile_parts)):
+        for kind, most, keys, all_parts in (("split", 16, 32, d.split_parts), ("half", 128, 128, d.half_parts),
+                                            ("tile", 256, 128, d.tile_parts)):
             seen, parts, cut = {}, {}, set()
             load = {}
             for block, g in segments(d, raw, kind):
@@ -107,8 +107,8 @@ def test_every_row_meets_every_tile_once():
                 else:
                     assert part == -1
             assert len(parts) == all_parts
-            assert len(cut) == (d.split_counters if kind == "split" else d.merges)
-            assert len(load) <= 148
+            assert len(cut) == (d.split_counters if kind == "split" else getattr(d, kind + "_merges"))
+            assert len(load) <= (296 if kind == "half" else 148)
             for (req, head, row0, rows), spans in seen.items():
                 spans.sort()
                 last = kv[req] - new[req] + (row0 + rows - 1) // (H // Hk)

@@ -61,11 +61,14 @@ class PagedPlanDesc(C.Structure):
     _fields_ = [("rows", C.c_int64), ("table_bytes", C.c_size_t), ("workspace_bytes", C.c_size_t),
                 ("positions_offset", C.c_int64), ("requests_offset", C.c_int64), ("split_segments_offset", C.c_int64),
                 ("split_starts_offset", C.c_int64), ("tile_segments_offset", C.c_int64),
-                ("tile_starts_offset", C.c_int64), ("merges_offset", C.c_int64), ("requests", C.c_int32),
+                ("tile_starts_offset", C.c_int64), ("tile_merges_offset", C.c_int64),
+                ("half_segments_offset", C.c_int64), ("half_starts_offset", C.c_int64),
+                ("half_merges_offset", C.c_int64), ("requests", C.c_int32),
                 ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32),
                 ("columns", C.c_int32), ("split_blocks", C.c_int32), ("split_parts", C.c_int32),
                 ("split_counters", C.c_int32), ("tile_blocks", C.c_int32), ("tile_parts", C.c_int32),
-                ("merges", C.c_int32)]
+                ("tile_merges", C.c_int32), ("half_blocks", C.c_int32), ("half_parts", C.c_int32),
+                ("half_merges", C.c_int32), ("reserved", C.c_int32)]
 
 
 P = C.c_void_p

@@ -35,6 +35,7 @@ static_assert(sizeof(PagedSegment) == 64, "segments are read as four 16-byte vec
 constexpr int kSplitRows = 16;  // packed rows of a segment of the few-rows kernel (one m16 MMA tile)
 constexpr int kSplitKeys = 32;  // keys per tile
 constexpr int kTileRows = 256;  // packed rows of a segment of the tensor-core kernel (two halves of 128)
+constexpr int kHalfRows = 128;  // of its form with one half
 constexpr int kTileKeys = 128;  // keys per tile
 
 struct PagedArgs {
@@ -60,7 +61,7 @@ tf_status make_page_map(void* map, const void* base, const tf_paged_kv& kv, int 
 tf_status launch_paged_split(const PagedArgs& a, cudaStream_t s);
 tf_status launch_paged_tile(const PagedArgs& a, cudaStream_t s);
 // Workspace of the few-rows kernel's parts: per part and row the maximum, the
-// sum, the outputs.  The tensor-core kernel's parts follow it.
+// sum, the outputs.  The tensor-core kernels' parts follow it.
 inline size_t split_workspace_bytes(const tf_paged_plan& p) {
   return (size_t)p.split_parts * kSplitRows * (2 + p.head_dim) * 4;
 }

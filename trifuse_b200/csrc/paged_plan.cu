@@ -161,18 +161,22 @@ Layout lay_out(const std::vector<Item>& items, const Schedule& s, const int32_t*
   return out;
 }
 
-// The work of one kernel: requests of more than kSplitRows packed rows per key
-// head go to the tensor-core kernel (whose 128-row products take the same time
-// however few rows they hold), the others to the few-rows kernel.
-Layout plan_kernel(const int32_t* new_lengths, const int32_t* kv_lengths, const tf_paged_plan& p, bool tile) {
+// The work of one kernel, chosen by a request's packed rows per key head: up to
+// kSplitRows go to the few-rows kernel, up to kHalfRows to the tensor-core
+// kernel with one half a block and two blocks an SM, more to the one with two
+// halves.
+enum Kind { kSplit, kHalves1, kHalves2 };
+
+Layout plan_kernel(const int32_t* new_lengths, const int32_t* kv_lengths, const tf_paged_plan& p, Kind kind) {
   const int G = p.heads / p.kv_heads;
-  const int block_rows = tile ? kTileRows : kSplitRows, keys = tile ? kTileKeys : kSplitKeys;
+  const int block_rows = kind == kSplit ? kSplitRows : kind == kHalves1 ? kHalfRows : kTileRows;
+  const int keys = kind == kSplit ? kSplitKeys : kTileKeys;
   std::vector<Item> items;
   int32_t q_row = 0;
   for (int r = 0; r < p.requests; ++r) {
     const int n = new_lengths[r], kv = kv_lengths[r];
     const int64_t rows = (int64_t)n * G;
-    if ((rows > kSplitRows) == tile)
+    if ((rows <= kSplitRows ? kSplit : rows <= kHalfRows ? kHalves1 : kHalves2) == kind)
       for (int64_t row0 = 0; row0 < rows; row0 += block_rows) {
         const int take = (int)std::min<int64_t>(block_rows, rows - row0);
         const int64_t last = (int64_t)kv - n + (row0 + take - 1) / G;  // last key the rows see
@@ -183,19 +187,26 @@ Layout plan_kernel(const int32_t* new_lengths, const int32_t* kv_lengths, const 
   }
   // A segment starts in the time of some four small or one large tile; a piece
   // should be worth its partial result (a large tile's keys and values are as
-  // many bytes as half a partial result).
-  const Schedule s = tile ? divide(items, p.kv_heads, current_sms(), 1, 4)
-                          : divide(items, p.kv_heads, current_sms(), 4, 8);
+  // many bytes as half a partial result of 256 rows).
+  const Schedule s = kind == kSplit ? divide(items, p.kv_heads, current_sms(), 4, 8)
+                                    : divide(items, p.kv_heads, current_sms() * (kind == kHalves1 ? 2 : 1), 1, 4);
   return lay_out(items, s, new_lengths, kv_lengths);
 }
 
 struct Plans {
-  Layout split, tile;
-  std::vector<PagedSegment> merges;
+  Layout split, half, tile;
+  std::vector<PagedSegment> half_merges, tile_merges;
   Plans(const int32_t* new_lengths, const int32_t* kv_lengths, const tf_paged_plan& p)
-      : split(plan_kernel(new_lengths, kv_lengths, p, false)), tile(plan_kernel(new_lengths, kv_lengths, p, true)) {
-    for (const PagedSegment& g : tile.segments)
-      if (g.part >= 0 && g.part == g.part0) merges.push_back(g);
+      : split(plan_kernel(new_lengths, kv_lengths, p, kSplit)),
+        half(plan_kernel(new_lengths, kv_lengths, p, kHalves1)),
+        tile(plan_kernel(new_lengths, kv_lengths, p, kHalves2)),
+        half_merges(cut(half)),
+        tile_merges(cut(tile)) {}
+  static std::vector<PagedSegment> cut(const Layout& l) {
+    std::vector<PagedSegment> out;
+    for (const PagedSegment& g : l.segments)
+      if (g.part >= 0 && g.part == g.part0) out.push_back(g);
+    return out;
   }
 };
 
@@ -206,8 +217,8 @@ size_t put(char* table, size_t at, const std::vector<V>& v) {
 }
 
 // Lays the table out, and fills it where `table` is given: the few-rows
-// kernel's arrival counters (zero between calls), the two kernels' segments and
-// block starts, the cut row blocks, the rows' positions and requests.
+// kernel's arrival counters (zero between calls), the kernels' segments, block
+// starts and cut row blocks, the rows' positions and requests.
 void put_table(const Plans& plans, const int32_t* new_lengths, const int32_t* kv_lengths, tf_paged_plan* p,
                char* table) {
   p->split_blocks = (int32_t)plans.split.starts.size() - 1;
@@ -215,7 +226,10 @@ void put_table(const Plans& plans, const int32_t* new_lengths, const int32_t* kv
   p->split_counters = plans.split.counters;
   p->tile_blocks = (int32_t)plans.tile.starts.size() - 1;
   p->tile_parts = plans.tile.parts;
-  p->merges = (int32_t)plans.merges.size();
+  p->tile_merges = (int32_t)plans.tile_merges.size();
+  p->half_blocks = (int32_t)plans.half.starts.size() - 1;
+  p->half_parts = plans.half.parts;
+  p->half_merges = (int32_t)plans.half_merges.size();
   size_t at = put(table, 0, std::vector<int32_t>(plans.split.counters, 0));
   p->split_segments_offset = (int64_t)at;
   at = put(table, at, plans.split.segments);
@@ -225,13 +239,20 @@ void put_table(const Plans& plans, const int32_t* new_lengths, const int32_t* kv
   at = put(table, at, plans.tile.segments);
   p->tile_starts_offset = (int64_t)at;
   at = put(table, at, plans.tile.starts);
-  p->merges_offset = (int64_t)at;
-  at = put(table, at, plans.merges);
+  p->tile_merges_offset = (int64_t)at;
+  at = put(table, at, plans.tile_merges);
+  p->half_segments_offset = (int64_t)at;
+  at = put(table, at, plans.half.segments);
+  p->half_starts_offset = (int64_t)at;
+  at = put(table, at, plans.half.starts);
+  p->half_merges_offset = (int64_t)at;
+  at = put(table, at, plans.half_merges);
   p->positions_offset = (int64_t)at;
   at = align_up(at + (size_t)p->rows * 4, 16);
   p->requests_offset = (int64_t)at;
   p->table_bytes = align_up(at + (size_t)p->rows * 4, 16);
-  p->workspace_bytes = split_workspace_bytes(*p) + (size_t)p->tile_parts * kTileRows * (2 + p->head_dim) * 4;
+  p->workspace_bytes = split_workspace_bytes(*p) +
+                       ((size_t)p->tile_parts * kTileRows + (size_t)p->half_parts * kHalfRows) * (2 + p->head_dim) * 4;
   if (!table) return;
   int32_t* pos = reinterpret_cast<int32_t*>(table + p->positions_offset);
   int32_t* req = reinterpret_cast<int32_t*>(table + p->requests_offset);

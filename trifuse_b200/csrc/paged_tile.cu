@@ -17,8 +17,13 @@
 //   * one block per SM walks the segments of the plan (paged.h) and the roles
 //     run ahead across them: the next segment's queries and first scores are
 //     computed while this one's outputs are written.
+// Requests of at most 128 packed rows run the same code with one half a block
+// and two blocks an SM: with half B empty, the chain scores - softmax -
+// products of half A alone would set the pace, at half of what the pages'
+// memory gives (24 requests of 35 rows over 8011 keys: 42 us against %HALF%).
 //
-// Roles (384 threads; registers move from the third warpgroup to the softmax):
+// Roles (two halves: 384 threads, registers move from the third warpgroup to
+// the softmax; one half: 192 threads):
 //   warps 0-3, 4-7  softmax of half A, B: read S from tensor memory, mask, write
 //              P in 16 bits over S's first columns; after a segment's last
 //              scores copy the next segment's queries into shared memory
@@ -26,7 +31,7 @@
 //              differs), then read O and write out (or the piece's partial
 //              result).  A warp of its own for the queries took 9000 clocks a
 //              half, most of a short segment.
-//   warps 8, 9  MMA of half A, B: one elected lane issues, tile by tile,
+//   MMA warps   of half A, B: one elected lane issues, tile by tile,
 //              O += P V; S = Q K' with K' the next tile.  MMAs of one thread
 //              execute in issue order, so a next S may be issued over a P that
 //              the product before it still reads, and its completion implies
@@ -34,9 +39,10 @@
 //              products (some 150 clocks even when they are met) would leave
 //              the tensor cores idle: one warp for both took 3170 clocks a
 //              tile with the softmax taken out, of which 1840 were products.
-//   warp 10    loader: page ids and TMA of the K and V tiles (128-byte
+//   loader     page ids and TMA of the K and V tiles (128-byte
 //              swizzle) into one ring of tiles, K and V in turn.
-// Tensor memory columns: O_A [0, 128), O_B [128, 256), S_A [256, 384), S_B.
+// Tensor memory columns: O_A [0, 128), O_B [128, 256), S_A [256, 384), S_B
+// (one half: O [0, 128), S [128, 256)).
 //
 // P is rounded to the cache's 16-bit type, relative 2^-11 (f16) or 2^-8
 // (bf16), the size of the output's own rounding; l sums the unrounded values.
@@ -57,21 +63,26 @@ namespace {
 using namespace tc;
 
 constexpr int kHalf = 128;  // rows of a half = TMEM lanes
-constexpr int kThreads = 384;
-constexpr int kMmaWarp = 8, kLoadWarp = 10;  // 8, 9: products of half A, B; 11 fills the warpgroup
-constexpr uint32_t kColO = 0, kColS = 256;  // half x: + 128 x
+constexpr uint32_t kColO = 0;  // half x's columns: O at kColO + 128 x, S after the halves' O
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;
 constexpr int kColBytes = kTileKeys * 128;  // 64 columns of a tile: 128 rows of 128 bytes
 
-template <int D>
+// A block of H halves: two of them one to an SM, or one half two to an SM.
+template <int D, int H>
 struct Shape {
   static constexpr int kTile = D / 64 * kColBytes;  // bytes of 128 rows or keys
-  static constexpr int kSlots = D == 128 ? 5 : 8;   // ring of K and V tiles
-  static constexpr int kOffRing = 2 * kTile;        // after the two halves' queries
+  static constexpr int kSlots = (H == 2 ? 160 : 64) * 1024 / kTile - (H == 2 && D == 64 ? 2 : 0);  // ring of K and V
+  static constexpr int kOffRing = H * kTile;        // after the halves' queries
   static constexpr int kOffBar = kOffRing + kSlots * kTile;
   static constexpr int kSmem = kOffBar + 512 + 1024;  // + barriers + alignment slack
-  static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
+  static_assert(kSmem <= 227 * 1024 / (3 - H) - (2 - H) * 1024, "shared memory of an SM");
+  // Warps: softmax 0 .. 4 H - 1, then the halves' MMA warps, then the loader
+  // (with two halves one more fills the third warpgroup).
+  static constexpr int kMmaWarp = 4 * H, kLoadWarp = 5 * H;
+  static constexpr int kThreads = H == 2 ? 384 : 192;
+  static constexpr uint32_t kColumns = 256 * H, kColS = 128 * H;
+  static constexpr int kRows = kHalf * H;
 };
 
 struct TileParams {
@@ -86,8 +97,8 @@ struct TileParams {
   int32_t group, heads;
   const PagedSegment* segments;
   const int32_t* starts;
-  float* stat;  // [part][2][256]: m, l
-  float* part;  // [part][D / 4][256][4]: a warp's rows side by side
+  float* stat;  // [part][2][rows of a block]: m, l
+  float* part;  // [part][D / 4][rows of a block][4]: a warp's rows side by side
   void* out;
   float scale_log2;
   int* err;
@@ -229,13 +240,14 @@ __device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b)
 }
 
 // A segment as the roles see it: the tiles that each half meets.
+template <int H>
 struct View {
-  int count[2];  // tiles of half A, B, from tile0
+  int count[H];  // tiles of half A, B, from tile0
   int tiles;     // the larger: tiles that are loaded
   __device__ __forceinline__ View(const PagedSegment& g, int group) {
     tiles = 0;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < H; ++x) {
       count[x] = 0;
       if (kHalf * x >= g.rows) continue;
       const int last_row = g.row0 + min(kHalf * x + kHalf, g.rows) - 1;
@@ -247,9 +259,10 @@ struct View {
   }
 };
 
-template <typename T, typename C, int D>
-__global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_constant__ TileParams p) {
-  using S = Shape<D>;
+template <typename T, typename C, int D, int H>
+__global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
+    paged_tile_kernel(const __grid_constant__ TileParams p) {
+  using S = Shape<D, H>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + S::kOffBar);
@@ -269,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int* err = p.err;
   if (tid == 0) {
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < H; ++x) {
       mbar_init(&q_full[x], kHalf);
       mbar_init(&s_full[x], 1);
       mbar_init(&p_full[2 * x], kHalf);
@@ -281,18 +294,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
     }
     for (int i = 0; i < S::kSlots; ++i) {
       mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 2);
+      mbar_init(&kv_empty[i], H);
     }
     ctl->abort = 0;
     ctl->limit = *p.wait_cycles;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kMmaWarp) {
+  if (warp == S::kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
-                 "r"(512));
+                 "r"(S::kColumns));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  if (warp == kLoadWarp && lane == 0) {
+  if (warp == S::kLoadWarp && lane == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&p.tm_k)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&p.tm_v)) : "memory");
   }
@@ -302,15 +315,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
   const uint32_t tmem = *tmem_slot;
   const int seg0 = p.starts[blockIdx.x], seg1 = p.starts[blockIdx.x + 1];
 
-  if (warp >= kMmaWarp) {
+  if (warp >= S::kMmaWarp) {
     // 384 threads x 168 registers = 2 x 128 x 208 + 128 x 88.
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == kLoadWarp) {
+    if constexpr (H == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == S::kLoadWarp) {
       int n = 0;  // tiles fetched (K and V each count)
       bool ok = true;
       for (int seg = seg0; seg < seg1 && ok; ++seg) {
         const PagedSegment g = p.segments[seg];
-        const View view(g, p.group);
+        const View<H> view(g, p.group);
         const int32_t* ids = p.ids + g.request * p.ids_stride;
         const int box_bytes = p.box_rows * 128;
         for (int j = 0; j < view.tiles && ok; ++j) {
@@ -342,14 +355,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
       // Copies in flight land before the block exits.
       for (int i = n > S::kSlots ? n - S::kSlots : 0; i < n; ++i)
         drain(&kv_full[i % S::kSlots], (uint32_t)((i / S::kSlots) & 1), err);
-    } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+    } else if (warp < S::kLoadWarp) {
       // ---- products of half x.
-      const int x = warp - kMmaWarp;
+      const int x = warp - S::kMmaWarp;
       const uint32_t leader = elect_one();
       const uint32_t fmt = Act<C>::kDtype == TF_DTYPE_BF16 ? (1u << 7) | (1u << 10) : 0u;  // A and B are bf16
       const uint32_t id_qk = idesc_f16(kHalf, kTileKeys) | fmt;
       const uint32_t id_pv = idesc_f16(kHalf, D) | (1u << 16) | fmt;  // B (V) MN-major
-      const uint32_t t_o = tmem + kColO + 128 * x, t_s = tmem + kColS + 128 * x;
+      const uint32_t t_o = tmem + kColO + 128 * x, t_s = tmem + S::kColS + 128 * x;
       const uint32_t qa = smem_addr(base + x * S::kTile);
       int n = 0;  // ring position
       uint32_t q_turn = 0, p_turn = 0, o_turn = 0, baton_turn = 0;
@@ -370,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
       };
       for (int seg = seg0; seg < seg1 && ok; ++seg) {
         const PagedSegment g = p.segments[seg];
-        const View view(g, p.group);
+        const View<H> view(g, p.group);
         const int count = view.count[x];
         if (count > 0) {
           if (!(ok = landed(n) && wait_warp(&q_full[x], q_turn & 1, ctl, err, 83))) break;
@@ -378,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
           tc_fence_after();
           scores(n);
         }
-        const int both = min(count, view.count[1 - x]);  // tiles that both halves meet
+        const int both = H == 2 ? min(count, view.count[(1 - x) & (H - 1)]) : 0;  // tiles that both halves meet
         for (int j = 0; j < count && ok; ++j) {
           // Ring: K of tile j at n, V of tile j, K of tile j + 1.
           const bool more = j + 1 < count;
@@ -435,12 +448,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
       drain(&done[x], 0, err);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    if constexpr (H == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax of half x: thread r owns row r = TMEM lane r.
     const int x = warp >> 2;
     const int r = tid - kHalf * x;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t t_o = lane_base + kColO + 128 * x, t_s = lane_base + kColS + 128 * x;
+    const uint32_t t_o = lane_base + kColO + 128 * x, t_s = lane_base + S::kColS + 128 * x;
     uint32_t s_turn = 0, o_turn = 0;
     bool ok = true;
     // Copies the query rows of the half's next segment with tiles, from
@@ -452,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
       constexpr int kChunks = D / 8, kRowsAt = 32 / kChunks;  // chunks of a row, rows per pass
       for (; seg < seg1; ++seg) {
         const PagedSegment g = p.segments[seg];
-        if (View(g, p.group).count[x] == 0) continue;
+        if (View<H>(g, p.group).count[x] == 0) continue;
         const int pr = g.row0 + min(kHalf * x + r, g.rows - 1);
         const T* own = static_cast<const T*>(p.q) + (int64_t)(g.q_row + pr / p.group) * p.q_stride +
                        (int64_t)(g.kv_head * p.group + pr % p.group) * D;
@@ -489,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
     for (int seg = seg0; seg < seg1 && ok; ++seg) {
       const PagedSegment g = p.segments[seg];
       if (kHalf * x >= g.rows) continue;
-      const View view(g, p.group);
+      const View<H> view(g, p.group);
       const int count = view.count[x];
       // Threads past the rows follow the last one; what they make is dropped.
       const int pr = g.row0 + min(kHalf * x + r, g.rows - 1);
@@ -588,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
       const float inv = m == -INFINITY ? 0.f : 1.f / l;
       T* orow = static_cast<T*>(p.out) +
                 ((int64_t)(g.q_row + token) * p.heads + g.kv_head * p.group + pr % p.group) * D;
-      float* prow = p.part + (int64_t)g.part * kTileRows * D + row * 4;
+      float* prow = p.part + (int64_t)g.part * S::kRows * D + row * 4;
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         float o[32];
@@ -610,13 +623,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
         } else {
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(prow + (c + i) * kTileRows) =
+            *reinterpret_cast<float4*>(prow + (c + i) * S::kRows) =
                 make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
       }
       if (mine && g.part >= 0) {
-        p.stat[(int64_t)g.part * 2 * kTileRows + row] = m;
-        p.stat[(int64_t)g.part * 2 * kTileRows + kTileRows + row] = l;
+        p.stat[(int64_t)g.part * 2 * S::kRows + row] = m;
+        p.stat[(int64_t)g.part * 2 * S::kRows + S::kRows + row] = l;
       }
       if (count > 0) {
         tc_fence_before();
@@ -627,15 +640,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tile_kernel(const __grid_co
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kMmaWarp)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  if (warp == S::kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kColumns));
 }
 
 // Joins the pieces of cut row blocks, in piece order.  A warp takes 32 rows
 // and 4 columns, so the pieces' outputs arrive 512 bytes at a time.
 constexpr int kMergeWarps = 8;
 
-template <typename T, int D>
+template <typename T, int D, int R>
 __global__ void __launch_bounds__(32 * kMergeWarps)
     paged_merge_kernel(const PagedSegment* __restrict__ items, const float* __restrict__ stat,
                        const float* __restrict__ part, int group, int heads, T* __restrict__ out) {
@@ -643,18 +656,18 @@ __global__ void __launch_bounds__(32 * kMergeWarps)
   const int row = blockIdx.x * 32 + (threadIdx.x & 31);
   const int c = blockIdx.y * kMergeWarps + (threadIdx.x >> 5);  // columns 4 c ..
   if (row >= g.rows) return;
-  const float* st = stat + (int64_t)g.part0 * 2 * kTileRows + row;
+  const float* st = stat + (int64_t)g.part0 * 2 * R + row;
   float M = -INFINITY;
-  for (int i = 0; i < g.parts; ++i) M = max_nan(M, st[(int64_t)i * 2 * kTileRows]);
+  for (int i = 0; i < g.parts; ++i) M = max_nan(M, st[(int64_t)i * 2 * R]);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
   for (int i = 0; i < g.parts; ++i) {
-    const float m = st[(int64_t)i * 2 * kTileRows];
+    const float m = st[(int64_t)i * 2 * R];
     if (m == -INFINITY) continue;
     const float f = fast_exp2(m - M);
-    const float4 v = *reinterpret_cast<const float4*>(part + (int64_t)(g.part0 + i) * kTileRows * D +
-                                                      (c * kTileRows + row) * 4);
-    sum = fmaf(f, st[(int64_t)i * 2 * kTileRows + kTileRows], sum);
+    const float4 v = *reinterpret_cast<const float4*>(part + (int64_t)(g.part0 + i) * R * D +
+                                                      (c * R + row) * 4);
+    sum = fmaf(f, st[(int64_t)i * 2 * R + R], sum);
     acc.x = fmaf(f, v.x, acc.x);
     acc.y = fmaf(f, v.y, acc.y);
     acc.z = fmaf(f, v.z, acc.z);
@@ -667,30 +680,57 @@ __global__ void __launch_bounds__(32 * kMergeWarps)
   *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(v);
 }
 
-template <typename T, typename C, int D>
-tf_status launch(const TileParams& p, const tf_paged_plan& plan, const PagedSegment* merges, cudaStream_t s) {
+// The work of one kind of block in a plan.
+struct Work {
+  int64_t segments, starts, merges;  // offsets in the table
+  int32_t blocks, parts, cuts;
+  float* stat;
+};
+
+template <typename T, typename C, int D, int H>
+tf_status launch(TileParams p, const Work& w, const char* table, cudaStream_t s) {
+  using S = Shape<D, H>;
+  if (w.blocks == 0) return TF_OK;
   static PerDeviceOnce attr;
   int dev = 0;
   if (attr.needed(&dev)) {
-    TF_CUDA(cudaFuncSetAttribute(paged_tile_kernel<T, C, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 Shape<D>::kSmem));
+    TF_CUDA(cudaFuncSetAttribute(paged_tile_kernel<T, C, D, H>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 S::kSmem));
     attr.mark(dev);
   }
-  paged_tile_kernel<T, C, D><<<plan.tile_blocks, kThreads, Shape<D>::kSmem, s>>>(p);
+  p.segments = reinterpret_cast<const PagedSegment*>(table + w.segments);
+  p.starts = reinterpret_cast<const int32_t*>(table + w.starts);
+  p.stat = w.stat;
+  p.part = p.stat + (int64_t)w.parts * 2 * S::kRows;
+  paged_tile_kernel<T, C, D, H><<<w.blocks, S::kThreads, S::kSmem, s>>>(p);
   TF_TRY(check_launch("paged_tile"));
-  if (plan.merges == 0) return TF_OK;
+  if (w.cuts == 0) return TF_OK;
   // grid.z is below 65536: at most one cut item per block.
-  const dim3 grid(kTileRows / 32, D / 4 / kMergeWarps, (unsigned)plan.merges);
-  paged_merge_kernel<T, D><<<grid, 32 * kMergeWarps, 0, s>>>(merges, p.stat, p.part, p.group, p.heads,
-                                                             static_cast<T*>(p.out));
+  const dim3 grid(S::kRows / 32, D / 4 / kMergeWarps, (unsigned)w.cuts);
+  paged_merge_kernel<T, D, S::kRows><<<grid, 32 * kMergeWarps, 0, s>>>(
+      reinterpret_cast<const PagedSegment*>(table + w.merges), p.stat, p.part, p.group, p.heads,
+      static_cast<T*>(p.out));
   return check_launch("paged_merge");
+}
+
+template <typename T, typename C, int D>
+tf_status launch_both(const TileParams& p, const PagedArgs& a, cudaStream_t s) {
+  const tf_paged_plan& plan = *a.plan;
+  float* stat = reinterpret_cast<float*>(a.workspace + split_workspace_bytes(plan));
+  const Work tile = {plan.tile_segments_offset, plan.tile_starts_offset, plan.tile_merges_offset,
+                     plan.tile_blocks, plan.tile_parts, plan.tile_merges, stat};
+  const Work half = {plan.half_segments_offset, plan.half_starts_offset, plan.half_merges_offset,
+                     plan.half_blocks, plan.half_parts, plan.half_merges,
+                     stat + (int64_t)plan.tile_parts * kTileRows * (2 + D)};
+  TF_TRY((launch<T, C, D, 2>(p, tile, a.plan_table, s)));
+  return launch<T, C, D, 1>(p, half, a.plan_table, s);
 }
 
 }  // namespace
 
 tf_status launch_paged_tile(const PagedArgs& a, cudaStream_t s) {
   const tf_paged_plan& plan = *a.plan;
-  if (plan.tile_blocks == 0) return TF_OK;
+  if (plan.tile_blocks == 0 && plan.half_blocks == 0) return TF_OK;
   TileParams p;
   memset(&p, 0, sizeof(p));
   p.box_rows = a.kv.page_size < kTileKeys ? a.kv.page_size : kTileKeys;
@@ -705,17 +745,10 @@ tf_status launch_paged_tile(const PagedArgs& a, cudaStream_t s) {
   while ((1 << p.page_shift) < a.kv.page_size) ++p.page_shift;
   p.group = plan.heads / plan.kv_heads;
   p.heads = plan.heads;
-  p.segments = reinterpret_cast<const PagedSegment*>(a.plan_table + plan.tile_segments_offset);
-  p.starts = reinterpret_cast<const int32_t*>(a.plan_table + plan.tile_starts_offset);
-  p.stat = reinterpret_cast<float*>(a.workspace + split_workspace_bytes(plan));
-  p.part = p.stat + (int64_t)plan.tile_parts * 2 * kTileRows;
   p.out = a.out;
   p.scale_log2 = a.scale * kLog2e;
   TF_TRY(tc_flags(&p.err, const_cast<long long**>(&p.wait_cycles)));
-  const PagedSegment* merges = reinterpret_cast<const PagedSegment*>(a.plan_table + plan.merges_offset);
-#define TF_TILE(T, C)                                                    \
-  return plan.head_dim == 128 ? launch<T, C, 128>(p, plan, merges, s)    \
-                              : launch<T, C, 64>(p, plan, merges, s)
+#define TF_TILE(T, C) return plan.head_dim == 128 ? launch_both<T, C, 128>(p, a, s) : launch_both<T, C, 64>(p, a, s)
   if (a.act == TF_DTYPE_F16) TF_TILE(__half, __half);
   if (a.kv.dtype == TF_DTYPE_F16) TF_TILE(__nv_bfloat16, __half);
   TF_TILE(__nv_bfloat16, __nv_bfloat16);
