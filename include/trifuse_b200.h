@@ -411,7 +411,8 @@ typedef struct tf_paged_plan {
   int32_t half_blocks;      /* the same of its form for up to 128 rows       */
   int32_t half_parts;
   int32_t half_merges;
-  int32_t reserved;
+  int32_t split_rows;       /* most packed rows of a request in the few-rows
+                               kernel                                        */
 } tf_paged_plan;
 
 /* new_lengths[i] query rows and kv_lengths[i] cached tokens (the new ones

@@ -68,7 +68,7 @@ class PagedPlanDesc(C.Structure):
                 ("columns", C.c_int32), ("split_blocks", C.c_int32), ("split_parts", C.c_int32),
                 ("split_counters", C.c_int32), ("tile_blocks", C.c_int32), ("tile_parts", C.c_int32),
                 ("tile_merges", C.c_int32), ("half_blocks", C.c_int32), ("half_parts", C.c_int32),
-                ("half_merges", C.c_int32), ("reserved", C.c_int32)]
+                ("half_merges", C.c_int32), ("split_rows", C.c_int32)]
 
 
 P = C.c_void_p

@@ -224,6 +224,8 @@ void put_table(const Plans& plans, const int32_t* new_lengths, const int32_t* kv
   p->split_blocks = (int32_t)plans.split.starts.size() - 1;
   p->split_parts = plans.split.parts;
   p->split_counters = plans.split.counters;
+  p->split_rows = 0;
+  for (const PagedSegment& g : plans.split.segments) p->split_rows = std::max(p->split_rows, g.rows);
   p->tile_blocks = (int32_t)plans.tile.starts.size() - 1;
   p->tile_parts = plans.tile.parts;
   p->tile_merges = (int32_t)plans.tile_merges.size();

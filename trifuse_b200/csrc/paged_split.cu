@@ -7,16 +7,19 @@
 // in log2 units (scale * log2(e) folded into the scores' FMA).
 //
 // What bounds it: every key and value is read once (512 bytes per token and
-// key head at head_dim 128) against 2 * 16 * 128 multiply-adds per key on the
-// 16-row tile, so HBM is the bound and the products only have to keep out of
-// the way.  mma.sync m16n8k16 serves them from registers: a tcgen05 tile has
-// 128 rows of which at most 16 would be filled, and its scores would travel
-// through tensor memory for nothing.
+// key head at head_dim 128), so HBM is the bound and the products only have to
+// keep out of the way.  mma.sync m16n8k16 serves them from registers: a tcgen05
+// tile has 128 rows of which at most 16 would be filled.  Its products are slow
+// here (some 32 clocks each), so keys take the 16-row side and the queries the
+// 8-column side:
+//   S^T = K Q^T,  O^T = V^T P^T      (K, V^T by ldmatrix, P^T by movmatrix)
+// Up to 8 packed rows then need half the products of 16 (kernel variants for
+// one and two 8-row groups), and 32 keys take less time than their bytes.
 //
 // One block of four warps per SM walks its segments (paged.h).  The warps take
 // the segment's 32-key tiles in turn and never wait for one another inside a
 // segment: each has a ring of its own that lane-parallel TMA copies keep full
-// across segment boundaries (3 x 16 KB per warp in flight, 192 KB per SM; the
+// across segment boundaries (48 KB per warp in flight, 192 KB per SM; the
 // bandwidth-delay product needs about 45 KB per SM).  At a segment's end the
 // four warps' (m, l, O) are joined through shared memory, and the pieces of a
 // cut item through global memory by the last block to arrive.
@@ -112,6 +115,13 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t* r) {
                : "memory");
 }
 
+// The 8x8 matrix of 16-bit values across the warp, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
 template <typename C>
 __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1);
 template <>
@@ -179,7 +189,7 @@ struct Cursor {
   }
 };
 
-template <typename T, typename C, int D>
+template <typename T, typename C, int D, int NT>  // NT: groups of 8 packed rows
 __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_constant__ SplitParams p) {
   using S = Shape<D>;
   extern __shared__ uint8_t smem_raw[];
@@ -207,6 +217,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
     more = in.settle(p.segments, warp);
   }
   int fetched = 0, used = 0;
+  // Box of this lane in a tile: which page's part, keys or values, which 64
+  // columns.  The page id of the next tile is looked up a tile ahead.
+  const int box = lane / (S::kHalves * 2), what = lane % (S::kHalves * 2);
+  int page = -1;
+  auto look_up = [&]() {
+    const int column = (in.tile * kSplitKeys + box * p.box_rows) >> p.page_shift;
+    page = column < p.columns ? __ldg(p.ids + in.request * p.ids_stride + column) : -1;
+  };
+  if (more) look_up();
 
   // Fetches one tile into the ring's next slot: lane i copies box i (of the
   // tile's existing pages, keys before values, 64 columns each).
@@ -220,58 +239,63 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
     const int box_bytes = p.box_rows * kRowBytes;
     if (lane == 0) mbar_expect_tx(&bars[slot], (uint32_t)(boxes * box_bytes * S::kHalves * 2));
     __syncwarp();
-    if (lane < boxes * S::kHalves * 2) {
-      const int b = lane / (S::kHalves * 2), what = lane % (S::kHalves * 2);
+    if (box < boxes) {
       const int half = what % S::kHalves, is_v = what / S::kHalves;
-      const int key = key0 + b * p.box_rows;
-      const int column = key >> p.page_shift;
-      const int page = column < p.columns ? __ldg(p.ids + in.request * p.ids_stride + column) : -1;
-      const int row = in.kv_head * p.page_size + (key & (p.page_size - 1));
-      tma_page(dst + is_v * S::kTile + half * kHalfBytes + b * box_bytes, is_v ? &p.tm_v : &p.tm_k, half * 64, row,
+      const int row = in.kv_head * p.page_size + ((key0 + box * p.box_rows) & (p.page_size - 1));
+      tma_page(dst + is_v * S::kTile + half * kHalfBytes + box * box_bytes, is_v ? &p.tm_v : &p.tm_k, half * 64, row,
                page, &bars[slot]);
     }
     ++fetched;
     in.tile += kWarps;
     more = in.settle(p.segments, warp);
+    if (more) look_up();
   };
   for (int i = 0; i < S::kStages && more; ++i) fetch();
 
-  const int g = lane >> 2, c2 = (lane & 3) * 2;  // MMA fragment row and column pair
+  const int g = lane >> 2, c2 = (lane & 3) * 2;  // MMA fragment row (or column) and column pair
   const long long limit_cycles = *p.wait_cycles;
   bool ok = true;
   for (int seg = seg0; seg < seg_end; ++seg) {
     const PagedSegment sg = p.segments[seg];
-    // Queries as the A operand: rows g and g + 8.
-    uint32_t qa[D / 16][4];
-    int limit[2];  // last key the rows see
+    // Queries as the B operand: packed row 8 t + g.
+    uint32_t qb[D / 16][NT][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = g + 8 * i;
-      const int pr = sg.row0 + (r < sg.rows ? r : sg.rows - 1);
-      const int token = pr / p.group;
-      limit[i] = sg.kv_len - sg.new_len + token;
-      const T* qr = static_cast<const T*>(p.q) + (sg.q_row + token) * p.q_stride +
+    for (int t = 0; t < NT; ++t) {
+      const int pr = sg.row0 + min(8 * t + g, sg.rows - 1);
+      const T* qr = static_cast<const T*>(p.q) + (sg.q_row + pr / p.group) * p.q_stride +
                     (int64_t)(sg.kv_head * p.group + pr % p.group) * D;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t u = *reinterpret_cast<const uint32_t*>(qr + 16 * k + 8 * j + c2);
-          if constexpr (sizeof(T) == sizeof(C) && Act<T>::kDtype == Act<C>::kDtype) {
-            qa[k][2 * j + i] = u;
+          if constexpr (Act<T>::kDtype == Act<C>::kDtype) {
+            qb[k][t][j] = u;
           } else {
-            const T* t = reinterpret_cast<const T*>(&u);
-            qa[k][2 * j + i] = pack2<C>(to_f(t[0]), to_f(t[1]));
+            const T* v = reinterpret_cast<const T*>(&u);
+            qb[k][t][j] = pack2<C>(to_f(v[0]), to_f(v[1]));
           }
         }
     }
+    int limit[NT][2];  // last key that rows 8 t + c2, + 1 see
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        limit[t][i] = sg.kv_len - sg.new_len + (sg.row0 + min(8 * t + c2 + i, sg.rows - 1)) / p.group;
     const int first_limit = sg.kv_len - sg.new_len + sg.row0 / p.group;  // what the first row sees
-    float o[D / 8][4];
+    float o[D / 16][NT][4];  // O^T: dims 16 d + g, + 8, rows 8 t + c2, + 1
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i)
+    for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[d][t][j] = 0.f;
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) m[t][i] = -INFINITY, l[t][i] = 0.f;
 
     for (int tile = sg.tile0 + warp; tile < sg.tile1 && ok; tile += kWarps) {
       const int slot = used % S::kStages;
@@ -282,67 +306,75 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
       }
       const uint32_t ks = smem_addr(ring + slot * 2 * S::kTile), vs = ks + S::kTile;
       const int key0 = tile * kSplitKeys;
-      // Scores: 16 rows x 32 keys; a matrix of ldmatrix is 8 keys x 8 dims.
-      float s[4][4];
+      // Scores S^T: keys 16 h + g, + 8, rows 8 t + c2, + 1.
+      float s[2][NT][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[h][t][j] = 0.f;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {  // 16 keys
-          uint32_t b[4];
-          const int row = 16 * n + (lane & 7) + ((lane >> 4) << 3);
-          const int chunk = (2 * k + ((lane >> 3) & 1)) & 7;
-          ldsm4(ks + (k >> 2) * kHalfBytes + row * kRowBytes + ((chunk ^ (row & 7)) << 4), b);
-          mma16816<C>(s[2 * n], qa[k], b[0], b[1]);
-          mma16816<C>(s[2 * n + 1], qa[k], b[2], b[3]);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t a[4];
+          const int row = 16 * h + (lane & 15);
+          const int chunk = (2 * k + (lane >> 4)) & 7;
+          ldsm4(ks + (k >> 2) * kHalfBytes + row * kRowBytes + ((chunk ^ (row & 7)) << 4), a);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma16816<C>(s[h][t], a, qb[k][t][0], qb[k][t][1]);
         }
       }
-      float mx[2] = {-INFINITY, -INFINITY};
       const bool ragged = key0 + kSplitKeys - 1 > first_limit;
+      uint32_t pb[2][NT][2];  // P^T as the B operand
+      float keep[NT][2];
+      bool moved = false;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int t = 0; t < NT; ++t) {
+        float sub[2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float v = s[i][j] * p.scale_log2;
-          if (ragged && key0 + 8 * i + c2 + (j & 1) > limit[j >> 1]) v = -INFINITY;
-          s[i][j] = v;
-          mx[j >> 1] = max_nan(mx[j >> 1], v);
+        for (int i = 0; i < 2; ++i) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = i; j < 4; j += 2) {
+              float v = s[h][t][j] * p.scale_log2;
+              if (ragged && key0 + 16 * h + g + 4 * (j - i) > limit[t][i]) v = -INFINITY;
+              s[h][t][j] = v;
+              mx = max_nan(mx, v);
+            }
+          mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float mn = max_nan(m[t][i], mx);
+          // Rows that have seen no key yet keep m = -inf and add nothing.
+          sub[i] = mn == -INFINITY ? 0.f : mn;
+          keep[t][i] = exp2_fast(m[t][i] - sub[i]);
+          moved |= keep[t][i] != 1.f;
+          m[t][i] = mn;
+          l[t][i] *= keep[t][i];
         }
-      float keep[2], sub[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        mx[i] = max_nan(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-        mx[i] = max_nan(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-        const float mn = max_nan(m[i], mx[i]);
-        // Rows that have seen no key yet keep m = -inf and add nothing.
-        sub[i] = mn == -INFINITY ? 0.f : mn;
-        keep[i] = exp2_fast(m[i] - sub[i]);
-        m[i] = mn;
-        l[i] *= keep[i];
+        for (int h = 0; h < 2; ++h) {
+          float e[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            e[j] = exp2_fast(s[h][t][j] - sub[j & 1]);
+            l[t][j & 1] += e[j];
+          }
+          pb[h][t][0] = transpose8(pack2<C>(e[0], e[1]));
+          pb[h][t][1] = transpose8(pack2<C>(e[2], e[3]));
+        }
       }
-      uint32_t pa[2][4];
+      if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float e[4];
+        for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          e[j] = exp2_fast(s[i][j] - sub[j >> 1]);
-          l[j >> 1] += e[j];
-        }
-        pa[i >> 1][(i & 1) * 2] = pack2<C>(e[0], e[1]);
-        pa[i >> 1][(i & 1) * 2 + 1] = pack2<C>(e[2], e[3]);
-      }
-      if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          o[i][0] *= keep[0];
-          o[i][1] *= keep[0];
-          o[i][2] *= keep[1];
-          o[i][3] *= keep[1];
-        }
+            for (int j = 0; j < 4; ++j) o[d][t][j] *= keep[t][j & 1];
       }
       const int have = sg.kv_len - key0;
       if (have < kSplitKeys) {
@@ -356,15 +388,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
         __syncwarp();
       }
 #pragma unroll
-      for (int n = 0; n < D / 16; ++n) {  // 16 dims
+      for (int d = 0; d < D / 16; ++d) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {  // 16 keys
-          uint32_t b[4];
-          const int row = 16 * k + (lane & 15);
-          const int chunk = (2 * n + (lane >> 4)) & 7;
-          ldsm4_t(vs + (n >> 2) * kHalfBytes + row * kRowBytes + ((chunk ^ (row & 7)) << 4), b);
-          mma16816<C>(o[2 * n], pa[k], b[0], b[1]);
-          mma16816<C>(o[2 * n + 1], pa[k], b[2], b[3]);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t a[4];
+          const int row = 16 * h + (lane & 7) + ((lane >> 4) << 3);
+          const int chunk = (2 * d + ((lane >> 3) & 1)) & 7;
+          ldsm4_t(vs + (d >> 2) * kHalfBytes + row * kRowBytes + ((chunk ^ (row & 7)) << 4), a);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma16816<C>(o[d][t], a, pb[h][t][0], pb[h][t][1]);
         }
       }
       // Every lane's shared loads fed an MMA above, so they have returned: the
@@ -377,18 +409,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
 
     // Join the four warps' results.
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-      if ((lane & 3) == 0) {
-        stat[warp * 32 + g + 8 * i] = m[i];
-        stat[warp * 32 + 16 + g + 8 * i] = l[i];
-      }
-      float* row = join + (warp * kSplitRows + g + 8 * i) * S::kPitch;
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n)
-        *reinterpret_cast<float2*>(row + 8 * n + c2) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
-    }
+      for (int i = 0; i < 2; ++i) {
+        l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], 4);
+        l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], 8);
+        l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], 16);
+        const int r = 8 * t + c2 + i;
+        if (g == 0) {
+          stat[warp * 32 + r] = m[t][i];
+          stat[warp * 32 + 16 + r] = l[t][i];
+        }
+        float* row = join + (warp * kSplitRows + r) * S::kPitch;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+          row[16 * d + g] = o[d][t][i];
+          row[16 * d + g + 8] = o[d][t][i + 2];
+        }
+      }
     __syncthreads();
     for (int i = tid; i < sg.rows * D; i += kThreads) {
       const int r = i / D, d = i % D;
@@ -454,17 +492,27 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
     wait_copy(&bars[used % S::kStages], (uint32_t)((used / S::kStages) & 1), 2000000000LL);
 }
 
-template <typename T, typename C, int D>
+template <typename T, typename C, int D, int NT>
 tf_status launch(const SplitParams& p, int blocks, cudaStream_t s) {
   static PerDeviceOnce attr;
   int dev = 0;
   if (attr.needed(&dev)) {
-    TF_CUDA(cudaFuncSetAttribute(paged_split_kernel<T, C, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    TF_CUDA(cudaFuncSetAttribute(paged_split_kernel<T, C, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  Shape<D>::kSmem));
     attr.mark(dev);
   }
-  paged_split_kernel<T, C, D><<<blocks, kThreads, Shape<D>::kSmem, s>>>(p);
+  paged_split_kernel<T, C, D, NT><<<blocks, kThreads, Shape<D>::kSmem, s>>>(p);
   return check_launch("paged_split");
+}
+
+template <typename T, typename C>
+tf_status launch_rows(const SplitParams& p, const tf_paged_plan& plan, cudaStream_t s) {
+  // Half the products where no request has more than 8 packed rows.
+  if (plan.split_rows <= 8)
+    return plan.head_dim == 128 ? launch<T, C, 128, 1>(p, plan.split_blocks, s)
+                                : launch<T, C, 64, 1>(p, plan.split_blocks, s);
+  return plan.head_dim == 128 ? launch<T, C, 128, 2>(p, plan.split_blocks, s)
+                              : launch<T, C, 64, 2>(p, plan.split_blocks, s);
 }
 
 // cuTensorMapEncodeTiled, fetched from the driver at run time.
@@ -526,12 +574,9 @@ tf_status launch_paged_split(const PagedArgs& a, cudaStream_t s) {
   p.out = a.out;
   p.scale_log2 = a.scale * kLog2e;
   TF_TRY(tc_flags(&p.err, const_cast<long long**>(&p.wait_cycles)));
-#define TF_SPLIT(T, C)                                                                      \
-  return plan.head_dim == 128 ? launch<T, C, 128>(p, plan.split_blocks, s) : launch<T, C, 64>(p, plan.split_blocks, s)
-  if (a.act == TF_DTYPE_F16) TF_SPLIT(__half, __half);
-  if (a.kv.dtype == TF_DTYPE_F16) TF_SPLIT(__nv_bfloat16, __half);
-  TF_SPLIT(__nv_bfloat16, __nv_bfloat16);
-#undef TF_SPLIT
+  if (a.act == TF_DTYPE_F16) return launch_rows<__half, __half>(p, plan, s);
+  if (a.kv.dtype == TF_DTYPE_F16) return launch_rows<__nv_bfloat16, __half>(p, plan, s);
+  return launch_rows<__nv_bfloat16, __nv_bfloat16>(p, plan, s);
 }
 
 }  // namespace tf
