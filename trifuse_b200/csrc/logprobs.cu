@@ -43,13 +43,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 constexpr int kVectors = 8;     // 16-byte vectors of a thread's tile
-constexpr int kTile = kThreads * kVectors;
 constexpr int kStages = 2;      // tiles in shared memory
 constexpr int kMaxTop = 64;
-constexpr int kBuffer = 1024;   // candidates: the rounds need kMaxTop + kThreads, the cluster's join kMaxCluster * kMaxTop
+constexpr int kBuffer = 512;    // candidates: two rounds of a block's threads, the cluster's join kMaxCluster * kMaxTop
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -209,12 +206,17 @@ struct Sums {
       m = to;
     }
   }
-  __device__ __forceinline__ void join(Sums o) {
-    const float to = max_nan(m, o.m);
+  // The sums of a warp's lanes: to their maximum, then plain additions.
+  __device__ __forceinline__ void join_warp() {
+    float to = m;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) to = max_nan(to, __shfl_xor_sync(0xffffffffu, to, off));
     move(to);
-    o.move(to);
-    s += o.s;
-    w += o.w;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, off);
+      w += __shfl_xor_sync(0xffffffffu, w, off);
+    }
   }
   // ln sum e^(x - m), and the entropy ln sum e^(x - m) - sum (x - m) p.
   __device__ __forceinline__ void total(float& log_sum, float& entropy) const {
@@ -267,23 +269,33 @@ struct Sums {
   }
 };
 
+// What a cluster's blocks leave in the first one's shared memory.
+struct Gather {
+  uint64_t best[kMaxCluster][kMaxTop];
+  Sums sums[kMaxCluster];
+  int before[kMaxCluster];
+  int n[kMaxCluster];
+};
+
+template <int W>
 struct Shared {
   uint64_t full[kStages], empty[kStages];
   uint64_t buffer[kBuffer];
   uint64_t best[kMaxTop];      // sorted k best of the last prune
   int n;                       // candidates in the buffer
   uint32_t warp_key[kMaxTop];  // the warps' largest thread maxima of the first tile
-  Sums warp_sums[kWarps];
-  int warp_before[kWarps];
-  Sums sums;   // the block's totals, which the cluster's first block collects
-  int before;
+  Sums sums[W];                // the warps' totals
+  int before[W];
+  Gather gather;
 };
 
 // Sorts the buffer's n distinct keys by counting and keeps the k best, in
 // best[] and at the buffer's front; returns the bound that they make (`bound`
 // while there are fewer than k).  Called by the whole block after a barrier;
 // ends with one.
-__device__ __forceinline__ uint64_t prune(Shared& sh, int k, uint64_t bound) {
+template <int W>
+__device__ __forceinline__ uint64_t prune(Shared<W>& sh, int k, uint64_t bound) {
+  constexpr int kThreads = 32 * W;
   const int n = sh.n;
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const uint64_t mine = sh.buffer[i];
@@ -345,12 +357,13 @@ __device__ __forceinline__ void wait_slot(uint64_t* bar, uint32_t parity, const 
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const __grid_constant__ LogprobParams p) {
+template <typename T, int W>
+__global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 5) logprobs_kernel(const __grid_constant__ LogprobParams p) {
+  constexpr int kWarps = W, kThreads = 32 * W, kTile = kThreads * kVectors;
   using L = Vec<T>;
   constexpr int kPer = L::kPer;
   extern __shared__ __align__(128) uint8_t ring[];  // [kStages][kTile] vectors
-  __shared__ Shared sh;
+  __shared__ Shared<W> sh;
   const cg::cluster_group cluster = cg::this_cluster();
   const int slices = (int)cluster.num_blocks(), slice = (int)cluster.block_rank();
   const int shift = __popc(slices - 1);  // slices is a power of two
@@ -580,67 +593,47 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const __grid_cons
     }
   }
 
-  // Block totals: to the warp's maximum, then plain sums.
-  float top_of = acc.m;
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) top_of = max_nan(top_of, __shfl_xor_sync(0xffffffffu, top_of, off));
-  acc.move(top_of);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    acc.s += __shfl_xor_sync(0xffffffffu, acc.s, off);
-    acc.w += __shfl_xor_sync(0xffffffffu, acc.w, off);
-  }
+  // Block totals, then the cluster's in its first block.
+  acc.join_warp();
   before = __reduce_add_sync(0xffffffffu, before);
   if (lane == 0) {
-    sh.warp_sums[warp] = acc;
-    sh.warp_before[warp] = before;
+    sh.sums[warp] = acc;
+    sh.before[warp] = before;
   }
   __syncthreads();
   if (k) prune(sh, k, 0);
-  if (tid == 0) {
-    Sums t = sh.warp_sums[0];
-    int b = sh.warp_before[0];
-    for (int i = 1; i < kWarps; ++i) {
-      t.join(sh.warp_sums[i]);
-      b += sh.warp_before[i];
-    }
-    sh.sums = t;
-    sh.before = b;
-  }
+  Sums t = {-INFINITY, 0.f, 0.f};
+  if (lane < W) t = sh.sums[lane];
+  t.join_warp();  // by every warp: each needs it for its outputs
+  before = __reduce_add_sync(0xffffffffu, lane < W ? sh.before[lane] : 0);
   if (slices > 1) {
-    cluster.sync();
-    if (slice == 0) {
-      if (tid == 0) {
-        Sums t = sh.sums;
-        int b = sh.before;
-        for (int i = 1; i < slices; ++i) {
-          const Shared* o = cluster.map_shared_rank(&sh, i);
-          t.join(o->sums);
-          b += o->before;
-        }
-        sh.sums = t;
-        sh.before = b;
-      }
-      if (k) {
-        int at = sh.n;
-        for (int i = 1; i < slices; ++i) {
-          const Shared* o = cluster.map_shared_rank(&sh, i);
-          const int n = o->n;
-          for (int j = tid; j < n; j += kThreads) sh.buffer[at + j] = o->best[j];
-          at += n;
-        }
-        __syncthreads();
-        if (tid == 0) sh.n = at;
-        __syncthreads();
-        prune(sh, k, 0);
-      }
+    Gather* to = &cluster.map_shared_rank(&sh, 0)->gather;
+    const int n = k ? sh.n : 0;
+    if (tid < n) to->best[slice][tid] = sh.best[tid];
+    if (tid == 0) {
+      to->sums[slice] = t;
+      to->before[slice] = before;
+      to->n[slice] = n;
     }
-    cluster.sync();  // the other blocks' shared memory stays until it has been read
+    cluster.sync();
     if (slice != 0) return;
+    t = {-INFINITY, 0.f, 0.f};
+    if (lane < slices) t = sh.gather.sums[lane];
+    t.join_warp();
+    before = __reduce_add_sync(0xffffffffu, lane < slices ? sh.gather.before[lane] : 0);
+    if (k) {
+      for (int i = tid; i < slices * kMaxTop; i += kThreads) {
+        const int from = i / kMaxTop, j = i % kMaxTop;
+        int at = j;
+        for (int u = 0; u < from; ++u) at += sh.gather.n[u];
+        if (j < sh.gather.n[from]) sh.buffer[at] = sh.gather.best[from][j];
+        if (from == slices - 1 && j == 0) sh.n = at + sh.gather.n[from];
+      }
+      __syncthreads();
+      prune(sh, k, 0);
+    }
   }
-  __syncthreads();
   if (tid > 0 && tid >= k) return;
-  const Sums t = sh.sums;
   const bool finite = fabsf(Sums::offset(t.m)) < INFINITY;  // no NaN, no +inf, not all -inf
   float log_sum, entropy;
   t.total(log_sum, entropy);
@@ -648,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const __grid_cons
   if (tid == 0) {
     p.logprob[row] = finite && given ? (xt - t.m) - log_sum : nan;
     p.entropy[row] = finite ? entropy : nan;
-    p.rank[row] = finite && given ? sh.before : -1;
+    p.rank[row] = finite && given ? before : -1;
   }
   if (tid < k) {
     const int i = tid;
@@ -658,19 +651,19 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const __grid_cons
   }
 }
 
-template <typename T>
+template <typename T, int W>
 tf_status launch(const LogprobParams& p, int slices, cudaStream_t s) {
+  constexpr int kThreads = 32 * W, kRing = kStages * kThreads * kVectors * 16;
   static PerDeviceOnce once;
   int dev = 0;
   if (once.needed(&dev)) {
-    TF_CUDA(cudaFuncSetAttribute(logprobs_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 kStages * kTile * 16));
+    TF_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing));
     once.mark(dev);
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(p.rows * slices));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kStages * kTile * 16;
+  cfg.dynamicSmemBytes = kRing;
   cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -678,7 +671,7 @@ tf_status launch(const LogprobParams& p, int slices, cudaStream_t s) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_kernel<T, W>, p);
   if (e != cudaSuccess) return set_error(TF_ERR_CUDA, "token_logprobs launch: %s", cudaGetErrorString(e));
   return check_launch("token_logprobs");
 }
@@ -694,15 +687,18 @@ tf_status launch_token_logprobs(const void* logits, int64_t row_stride, int64_t 
                      nullptr, nullptr};
   TF_TRY(tc_flags(&p.err, const_cast<long long**>(&p.wait_cycles)));
   // Blocks a row: enough to fill the GPU (about three blocks an SM), each
-  // with at least one vector a thread.
+  // with at least one vector a thread.  Whole rows go to blocks of 128 threads,
+  // five to an SM: more rows at once cover one another's waits for the prunes.
   const int vectors = vocab / (dtype == TF_DTYPE_F32 ? 4 : 8);
   int slices = 1;
-  while (slices < kMaxCluster && rows * slices * 2 <= 3 * 148 && vectors >= 2 * slices * kThreads) slices *= 2;
+  while (slices < kMaxCluster && rows * slices * 2 <= 3 * 148 && vectors >= 2 * slices * 256) slices *= 2;
+#define TF_LOGPROBS(T) return slices > 1 ? launch<T, 8>(p, slices, s) : launch<T, 4>(p, 1, s)
   switch (dtype) {
-    case TF_DTYPE_F32: return launch<float>(p, slices, s);
-    case TF_DTYPE_F16: return launch<__half>(p, slices, s);
-    default: return launch<__nv_bfloat16>(p, slices, s);
+    case TF_DTYPE_F32: TF_LOGPROBS(float);
+    case TF_DTYPE_F16: TF_LOGPROBS(__half);
+    default: TF_LOGPROBS(__nv_bfloat16);
   }
+#undef TF_LOGPROBS
 }
 
 }  // namespace tf
