@@ -19,12 +19,16 @@
 // bits, then the inverted index) makes every entry distinct and ties fall to
 // the lowest index.  The first tile yields a lower bound of the k-th key (the
 // k-th largest of the warps' few largest thread maxima: k entries are at or
-// above it), entries at or above the bound go to a shared buffer, and pruning
-// the buffer to its k best raises the bound to an exact one.  After the first
-// tile a thread whose maximum is below the bound does nothing, so the pass
-// stays a stream.  Should the candidates not fit the buffer (values in rising
-// order, say), those since the last prune enter again in rounds of one entry a
-// thread with a prune in between.
+// above it).  A thread whose maximum of a tile meets the bound queues the tile
+// and goes on; after 1, 2, 4, ... tiles the block looks through the queue (the
+// vectors come again, from L2), puts entries at or above the bound into a
+// buffer, and prunes that to its k best, which raises the bound to an exact
+// one.  (Looking through the vectors on the spot cost some 4000 clocks each
+// time: a hundred instructions that are rare enough to be fetched from memory.)
+// After the first tile few threads meet the bound, so the pass stays a stream.
+// Should queue or buffer run over (values in rising order, say), the entries
+// since the last prune come again in rounds of one a thread, with a prune in
+// between.
 //
 // A row may be shared by a cluster of 1, 2, 4 or 8 blocks (few rows: the whole
 // GPU reads; one row of 50304 on one block would take its load latency 25
@@ -46,7 +50,7 @@ namespace cg = cooperative_groups;
 constexpr int kVectors = 8;     // 16-byte vectors of a thread's tile
 constexpr int kStages = 2;      // tiles in shared memory
 constexpr int kMaxTop = 64;
-constexpr int kBuffer = 512;    // candidates: two rounds of a block's threads, the cluster's join kMaxCluster * kMaxTop
+constexpr int kQueue = 512;     // a thread's tiles that meet the bound between two looks
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -131,6 +135,16 @@ struct Vec<float> {
   __device__ __forceinline__ static Max lowest() { return -INFINITY; }
   __device__ __forceinline__ static void raise(Max& m, const uint4& v) { m = max_nan(m, max_of(v)); }
   __device__ __forceinline__ static float value(Max m) { return m; }
+  // Bit i set: value i is not below t.
+  __device__ __forceinline__ static uint32_t not_below(const uint4& v, float t) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m |= (get(v, i) < t ? 0u : 1u) << i;
+    return m;
+  }
+  __device__ __forceinline__ static float pick(const uint4& v, int i) {
+    return __uint_as_float(i < 2 ? (i == 0 ? v.x : v.y) : (i == 2 ? v.z : v.w));
+  }
   // Counts of values above (kAt: at or above) t, added up per thread.
   using Count = int;
   __device__ __forceinline__ static Count zero() { return 0; }
@@ -157,6 +171,25 @@ struct Vec16 {
     for (int i = 0; i < 4; ++i) m = __hmax2_nan(m, h[i]);
   }
   __device__ __forceinline__ static float value(Max m) { return max_nan(__low2float(m), __high2float(m)); }
+  // Bit i set: value i is not below t (t rounded to T, which for the value of
+  // an entry is exact; else a few more pass, for the exact test to drop).
+  __device__ __forceinline__ static uint32_t not_below(const uint4& v, float t) {
+    const T2* h = reinterpret_cast<const T2*>(&v);
+    const T tt = from_f<T>(t);
+    const T2 t2 = {tt, tt};
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t below = __hlt2_mask(h[i], t2);  // NaN: not below
+      m |= (~below & 0x00010001u) << (2 * i);
+    }
+    return (m & 0xffu) | (m >> 15 & 0xaau);  // even values, odd values
+  }
+  __device__ __forceinline__ static float pick(const uint4& v, int i) {
+    const uint32_t w = i < 4 ? (i < 2 ? v.x : v.y) : (i < 6 ? v.z : v.w);
+    const uint16_t u = (uint16_t)((i & 1) ? w >> 16 : w);
+    return to_f(*reinterpret_cast<const T*>(&u));
+  }
   // The comparisons give packed 0 and 1; a tile adds at most 4 * kVectors = 32
   // to each half (bf16 counts exactly to 256).
   using Count = T2;
@@ -279,14 +312,18 @@ struct Gather {
 
 template <int W>
 struct Shared {
+  // Two rounds of the block's threads, and the cluster's join where there is one.
+  static constexpr int kBuffer = W == 8 ? kMaxCluster * kMaxTop : 64 * W + kMaxTop;
   uint64_t full[kStages], empty[kStages];
   uint64_t buffer[kBuffer];
+  int queue[kQueue];  // tiles of threads (their first vector) that met the bound since the last look
+  int queued;
   uint64_t best[kMaxTop];      // sorted k best of the last prune
   int n;                       // candidates in the buffer
   uint32_t warp_key[kMaxTop];  // the warps' largest thread maxima of the first tile
   Sums sums[W];                // the warps' totals
   int before[W];
-  Gather gather;
+  Gather gather[W == 8];
 };
 
 // Sorts the buffer's n distinct keys by counting and keeps the k best, in
@@ -358,12 +395,13 @@ __device__ __forceinline__ void wait_slot(uint64_t* bar, uint32_t parity, const 
 }
 
 template <typename T, int W>
-__global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 5) logprobs_kernel(const __grid_constant__ LogprobParams p) {
+__global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const __grid_constant__ LogprobParams p) {
   constexpr int kWarps = W, kThreads = 32 * W, kTile = kThreads * kVectors;
   using L = Vec<T>;
+  using S = Shared<W>;
   constexpr int kPer = L::kPer;
   extern __shared__ __align__(128) uint8_t ring[];  // [kStages][kTile] vectors
-  __shared__ Shared<W> sh;
+  __shared__ S sh;
   const cg::cluster_group cluster = cg::this_cluster();
   const int slices = (int)cluster.num_blocks(), slice = (int)cluster.block_rank();
   const int shift = __popc(slices - 1);  // slices is a power of two
@@ -389,6 +427,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 5) logprobs_kernel(const 
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.n = 0;
+    sh.queued = 0;
   }
   __syncthreads();
   auto fetch = [&](int tile) {  // one thread
@@ -417,29 +456,11 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 5) logprobs_kernel(const 
   float cut = -INFINITY;  // the bound's value: what is below is no candidate
   int kept = 0;           // candidates that the last prune left
   int group = v_begin;    // first vector after it
-  int crowded = 0;        // this thread saw more candidates than a prune is worth
+  int queued = 0;         // this thread queued vectors since the last look
   auto set_bound = [&](uint64_t to) {
     bound = to;
     const uint32_t bits = (uint32_t)(to >> 32);
     cut = bits ? order_value(bits) : -INFINITY;
-  };
-  // One vector's candidates.
-  auto offer = [&](const uint4& r, int e0) {
-    uint32_t some = 0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) some |= (L::get(r, j) < cut ? 0u : 1u) << j;
-    while (some) {
-      const int j = __ffs(some) - 1;
-      some &= some - 1;
-      float u = L::get(r, 0);
-#pragma unroll
-      for (int i = 1; i < kPer; ++i) u = i == j ? L::get(r, i) : u;
-      const uint64_t c = composite(u, (uint32_t)(e0 + j));
-      if (c < bound || e0 + j < 0 || e0 + j >= V) continue;
-      const int at = atomicAdd(&sh.n, 1);
-      if (at < kBuffer) sh.buffer[at] = c;
-      if (at >= 2 * k + 32) crowded = 1;
-    }
   };
   auto rank_each = [&](const uint4& r, int e0) {
 #pragma unroll
@@ -448,13 +469,35 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 5) logprobs_kernel(const 
       before += u > xt || (u == xt && e0 + j >= 0 && e0 + j < token);
     }
   };
-  // Prunes the candidates of the vectors [group, to) if they became many (or
-  // the bound is still the rough first one).  Called by the whole block.
+  // One vector's candidates into the buffer.
+  auto offer = [&](const uint4& r, int e0) {
+    for (uint32_t some = L::not_below(r, cut); some; some &= some - 1) {
+      const int e = e0 + __ffs(some) - 1;
+      const uint64_t c = composite(L::pick(r, e - e0), (uint32_t)e);
+      if (c < bound || e < 0 || e >= V) continue;
+      const int at = atomicAdd(&sh.n, 1);
+      if (at < S::kBuffer) sh.buffer[at] = c;
+    }
+  };
+  // Takes the queued vectors' candidates, and prunes them if they became many
+  // (or the bound is still the rough first one).  Called by the whole block
+  // after the tiles up to vector `to`.
   auto look = [&](int to, bool first) {
-    if (!__syncthreads_or(crowded || first)) return;
-    crowded = 0;
-    if (sh.n > kBuffer) {
-      // Those vectors again, kThreads entries at a time from memory.
+    if (!__syncthreads_or(queued)) return;
+    queued = 0;
+    const int entries = sh.queued;
+    bool over = entries > kQueue;
+    if (!over) {
+      for (int i = tid; i < entries * kVectors; i += kThreads) {
+        const int v = sh.queue[i / kVectors] + (i % kVectors) * kThreads, e0 = v * kPer - head;
+        if (v < v_end) offer(ld_v4(x + e0), e0);
+      }
+      __syncthreads();
+      over = sh.n > S::kBuffer;
+    }
+    if (over) {
+      // The vectors since the last prune again, kThreads entries at a time
+      // from memory.
       __syncthreads();
       if (tid == 0) sh.n = kept;
       __syncthreads();
@@ -471,16 +514,21 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 5) logprobs_kernel(const 
           if (c >= bound) sh.buffer[atomicAdd(&sh.n, 1)] = c;
         }
         __syncthreads();
-        const bool full = sh.n > kBuffer - kThreads;
+        const bool full = sh.n > S::kBuffer - kThreads;
         __syncthreads();
         if (full) {
           set_bound(prune(sh, k, bound));
         }
       }
     }
-    kept = min(sh.n, k);
-    set_bound(prune(sh, k, bound));
-    group = to;
+    if (tid == 0) sh.queued = 0;
+    if (over || first || sh.n > 2 * k + 32) {
+      kept = min(sh.n, k);
+      set_bound(prune(sh, k, bound));
+      group = to;
+    } else {
+      __syncthreads();
+    }
   };
 
   for (int tile = 0; tile < tiles; ++tile) {
@@ -572,13 +620,12 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 5) logprobs_kernel(const 
       set_bound((uint64_t)__reduce_max_sync(0xffffffffu, kth) << 32);
     }
     if (!(tmax < cut)) {
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i) {
-        const int v = t0 + tid + i * kThreads;
-        if (v < v_end && !(L::max_of(r[i]) < cut)) offer(r[i], v * kPer - head);
-      }
+      queued = 1;
+      const int at = atomicAdd(&sh.queued, 1);
+      if (at < kQueue) sh.queue[at] = t0 + tid;
     }
-    look(min(v_end, t0 + kTile), tile == 0);
+    // After 1, 2, 4, 8, ... tiles: each group adds about k candidates.
+    if ((tile & (tile + 1)) == 0 || tile + 1 == tiles) look(min(v_end, t0 + kTile), tile == 0);
   }
   if (edges) {
     // Thread 0 takes the row's first ragged vector, thread 1 its last.
@@ -606,8 +653,8 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 5) logprobs_kernel(const 
   if (lane < W) t = sh.sums[lane];
   t.join_warp();  // by every warp: each needs it for its outputs
   before = __reduce_add_sync(0xffffffffu, lane < W ? sh.before[lane] : 0);
-  if (slices > 1) {
-    Gather* to = &cluster.map_shared_rank(&sh, 0)->gather;
+  if (W == 8 && slices > 1) {
+    Gather* to = cluster.map_shared_rank(&sh, 0)->gather;
     const int n = k ? sh.n : 0;
     if (tid < n) to->best[slice][tid] = sh.best[tid];
     if (tid == 0) {
@@ -618,16 +665,16 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 3 : 5) logprobs_kernel(const 
     cluster.sync();
     if (slice != 0) return;
     t = {-INFINITY, 0.f, 0.f};
-    if (lane < slices) t = sh.gather.sums[lane];
+    if (lane < slices) t = sh.gather[0].sums[lane];
     t.join_warp();
-    before = __reduce_add_sync(0xffffffffu, lane < slices ? sh.gather.before[lane] : 0);
+    before = __reduce_add_sync(0xffffffffu, lane < slices ? sh.gather[0].before[lane] : 0);
     if (k) {
       for (int i = tid; i < slices * kMaxTop; i += kThreads) {
         const int from = i / kMaxTop, j = i % kMaxTop;
         int at = j;
-        for (int u = 0; u < from; ++u) at += sh.gather.n[u];
-        if (j < sh.gather.n[from]) sh.buffer[at] = sh.gather.best[from][j];
-        if (from == slices - 1 && j == 0) sh.n = at + sh.gather.n[from];
+        for (int u = 0; u < from; ++u) at += sh.gather[0].n[u];
+        if (j < sh.gather[0].n[from]) sh.buffer[at] = sh.gather[0].best[from][j];
+        if (from == slices - 1 && j == 0) sh.n = at + sh.gather[0].n[from];
       }
       __syncthreads();
       prune(sh, k, 0);
@@ -686,12 +733,12 @@ tf_status launch_token_logprobs(const void* logits, int64_t row_stride, int64_t 
   LogprobParams p = {logits, row_stride, tokens, rows, vocab, top, logprob, entropy, rank, top_logprob, top_token,
                      nullptr, nullptr};
   TF_TRY(tc_flags(&p.err, const_cast<long long**>(&p.wait_cycles)));
-  // Blocks a row: enough to fill the GPU (about three blocks an SM), each
+  // Blocks a row: enough to fill the GPU (about two blocks an SM), each
   // with at least one vector a thread.  Whole rows go to blocks of 128 threads,
   // five to an SM: more rows at once cover one another's waits for the prunes.
   const int vectors = vocab / (dtype == TF_DTYPE_F32 ? 4 : 8);
   int slices = 1;
-  while (slices < kMaxCluster && rows * slices * 2 <= 3 * 148 && vectors >= 2 * slices * 256) slices *= 2;
+  while (slices < kMaxCluster && rows * slices * 2 <= 2 * 148 && vectors >= 2 * slices * 256) slices *= 2;
 #define TF_LOGPROBS(T) return slices > 1 ? launch<T, 8>(p, slices, s) : launch<T, 4>(p, 1, s)
   switch (dtype) {
     case TF_DTYPE_F32: TF_LOGPROBS(float);
