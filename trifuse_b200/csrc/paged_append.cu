@@ -10,8 +10,10 @@
 // traffic is the norm weights, from L2.  A unit is one row's q, k or v part,
 // taken by as many warps as hold it in registers at 32 values a thread, so
 // that a row is read once for the norm and the rotation alike, and its loads
-// are all in flight while the angles are computed.  Chunk c (8 values) of a
-// head and its rotation partner c ^ (D/16) sit in lanes of the same warp.
+// are all in flight while the angles are computed.  A thread holds 8 values of
+// a head's first half together with their rotation partners in the second, and
+// works on packed fp32 pairs: with the partners in another lane the shuffles
+// and selects took 190 instructions for 8 values, and issue was the limit.
 //
 // The angle is reduced in double precision (t / 2 pi, less its nearest whole
 // number) before the fp32 sine and cosine: in fp32 a position of 10^5 would
@@ -31,7 +33,50 @@ namespace tf {
 
 namespace {
 
-constexpr int kChunks = 4;  // 16-byte chunks a thread holds
+constexpr int kPairs = 2;  // pairs of 16-byte chunks (a head's halves) a thread holds
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)),
+        "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&r);
+}
+// Eight values as four packed pairs, and back with one rounding (by the paired
+// conversions: value by value they took half of the kernel's instructions).
+__device__ __forceinline__ float2 pair_of(uint32_t w, __half) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ float2 pair_of(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ uint32_t word_of(float2 f, __half) {
+  const __half2 h = __float22half2_rn(f);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t word_of(float2 f, __nv_bfloat16) {
+  const __nv_bfloat162 h = __float22bfloat162_rn(f);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ void unpack4(const uint4& v, float2* f) {
+  f[0] = pair_of(v.x, T());
+  f[1] = pair_of(v.y, T());
+  f[2] = pair_of(v.z, T());
+  f[3] = pair_of(v.w, T());
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack4(const float2* f) {
+  return make_uint4(word_of(f[0], T()), word_of(f[1], T()), word_of(f[2], T()), word_of(f[3], T()));
+}
 
 struct AppendParams {
   const void* qkv;
@@ -47,38 +92,54 @@ struct AppendParams {
   void* k;
   void* v;
   int64_t pages, page_stride;
-  int page_size;
+  int page_size, page_shift;
   void* q_out;
   unsigned q_blocks, k_blocks;  // blocks of the q units, then of the k units, then of the v units
-  int q_warps, kv_warps;        // warps of a unit
+  int q_shift, kv_shift;        // log2 of the warps of a unit
   int rotate;
   double turns[64];             // theta^(-2d/D) / (2 pi)
 };
 
 template <typename T, typename C, int D>
-__global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant__ AppendParams p) {
-  constexpr int kHeadChunks = D / 8;
-  __shared__ float2 rot[16][D / 2];  // (cos, sin) for each of the block's rows
-  __shared__ float total[16];        // warp sums of squares
+__global__ void __launch_bounds__(512, 2) paged_append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int kHalfChunks = D / 16;  // chunks of half a head
+  __shared__ float rot[2][16][D / 2];  // cos and sin for each of the block's rows
+  __shared__ float total[16];          // warp sums of squares
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int part = blockIdx.x < p.q_blocks ? 0 : blockIdx.x < p.q_blocks + p.k_blocks ? 1 : 2;
   const unsigned block = blockIdx.x - (part == 0 ? 0u : part == 1 ? p.q_blocks : p.q_blocks + p.k_blocks);
-  const int warps = part == 0 ? p.q_warps : p.kv_warps;
+  const int shift = part == 0 ? p.q_shift : p.kv_shift;
+  const int warps = 1 << shift;  // of a unit
   const int heads = part == 0 ? p.heads : p.kv_heads;
-  const int units = (int)(blockDim.x >> 5) / warps;  // rows of this block
-  const int unit = warp / warps;
+  const int units = (int)(blockDim.x >> 5) >> shift;  // rows of this block
+  const int unit = warp >> shift;
   const int64_t row = (int64_t)block * units + unit;
   const bool live = row < p.rows;
-  const int W = heads * D;
-  const int c0 = (warp % warps) * 32 + lane;  // this thread's chunks: c0 + 32 * warps * i
+  // This thread's pairs: first-half chunk `at` of heads head0, head0 + step.
+  const int index = (warp & (warps - 1)) * 32 + lane;
+  const int at = index % kHalfChunks, head0 = index / kHalfChunks, step = 32 * warps / kHalfChunks;
 
   const T* src = static_cast<const T*>(p.qkv) + (live ? row : 0) * p.qkv_stride +
-                 (int64_t)(part == 0 ? 0 : part == 1 ? p.heads : p.heads + p.kv_heads) * D;
-  uint4 raw[kChunks];
+                 (int64_t)(part == 0 ? 0 : part == 1 ? p.heads : p.heads + p.kv_heads) * D + 8 * at;
+  uint4 raw[kPairs][2];
 #pragma unroll
-  for (int i = 0; i < kChunks; ++i) {
-    const int c = c0 + 32 * warps * i;
-    raw[i] = live && 8 * c < W ? ld_stream_v4(src + 8 * c) : make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < kPairs; ++i) {
+    const int h = head0 + step * i;
+    const bool mine = live && h < heads;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      raw[i][j] = mine ? ld_stream_v4(src + h * D + j * (D / 2)) : make_uint4(0, 0, 0, 0);
+  }
+  // Where the row goes.  A row whose slot does not exist is not stored.
+  C* dst = nullptr;
+  if (part != 0 && live) {
+    const int pos = p.positions[row], req = p.requests[row];
+    const int column = pos >> p.page_shift;
+    if (pos >= 0 && req >= 0 && req < p.table.requests && column < p.table.columns) {
+      const int64_t page = p.table.ids[req * p.table.stride + column];
+      if (page >= 0 && page < p.pages)
+        dst = static_cast<C*>(part == 1 ? p.k : p.v) + page * p.page_stride + (int64_t)(pos & (p.page_size - 1)) * D;
+    }
   }
   const __half* norm = part == 0 ? p.q_norm : part == 1 ? p.k_norm : nullptr;
   const bool rotate = p.rotate && part < 2;
@@ -89,80 +150,81 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const __grid_constant
         const double t = (double)p.positions[r] * p.turns[i % (D / 2)];
         float sn, cs;
         sincospif(2.f * (float)(t - rint(t)), &sn, &cs);
-        rot[i / (D / 2)][i % (D / 2)] = make_float2(cs, sn);
+        rot[0][i / (D / 2)][i % (D / 2)] = cs;
+        rot[1][i / (D / 2)][i % (D / 2)] = sn;
       }
     }
   }
-  float scale = 1.f;
   if (norm) {
-    float sum = 0.f;
+    float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      float f[8];
-      unpack8<T>(raw[i], f);
+    for (int i = 0; i < kPairs; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum = fmaf(f[j], f[j], sum);
-    }
-    sum = warp_sum_butterfly(sum);
-    if (lane == 0) total[warp] = sum;
+      for (int j = 0; j < 2; ++j) {
+        float2 f[4];
+        unpack4<T>(raw[i][j], f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum = fma2(f[k], f[k], sum);
+      }
+    const float all = warp_sum_butterfly(sum.x + sum.y);
+    if (lane == 0) total[warp] = all;
   }
-  __syncthreads();
+  if (norm || rotate) __syncthreads();
+  float2 scale = make_float2(1.f, 1.f);
   if (norm) {
     float sum = 0.f;
     for (int w = 0; w < warps; ++w) sum += total[unit * warps + w];
-    scale = rms_scale(sum, W, p.eps);
+    scale.x = scale.y = rms_scale(sum, heads * D, p.eps);
   }
-  // Where the row goes.  A row whose slot does not exist is not stored.
-  T* q_row = nullptr;
-  C* dst = nullptr;
-  if (part == 0) {
-    q_row = static_cast<T*>(p.q_out) + row * W;
-  } else if (live) {
-    const int pos = p.positions[row], req = p.requests[row];
-    const int column = pos / p.page_size;
-    if (pos >= 0 && req >= 0 && req < p.table.requests && column < p.table.columns) {
-      const int64_t page = p.table.ids[req * p.table.stride + column];
-      if (page >= 0 && page < p.pages)
-        dst = static_cast<C*>(part == 1 ? p.k : p.v) + page * p.page_stride + (int64_t)(pos % p.page_size) * D;
+  float2 cs[4], sn[4];
+  if (rotate) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      cs[k] = *reinterpret_cast<const float2*>(&rot[0][unit][8 * at + 2 * k]);
+      sn[k] = *reinterpret_cast<const float2*>(&rot[1][unit][8 * at + 2 * k]);
     }
   }
 #pragma unroll
-  for (int i = 0; i < kChunks; ++i) {
-    const int c = c0 + 32 * warps * i;
-    const bool mine = live && 8 * c < W;
-    float f[8];
-    unpack8<T>(raw[i], f);
-    if (norm) {
-      float w[8];
-      unpack8<__half>(mine ? ld_v4(norm + 8 * c) : make_uint4(0, 0, 0, 0), w);
+  for (int i = 0; i < kPairs; ++i) {
+    const int h = head0 + step * i;
+    if (!live || h >= heads) continue;
+    float2 f[2][4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = f[j] * scale * w[j];
-    }
-    if (rotate) {
-      const bool first = (c % kHeadChunks) < kHeadChunks / 2;
-      const float2* cs = &rot[unit][(c % (kHeadChunks / 2)) * 8];
+    for (int j = 0; j < 2; ++j) {
+      unpack4<T>(raw[i][j], f[j]);
+      if (norm) {
+        float2 w[4];
+        unpack4<__half>(ld_v4(norm + h * D + j * (D / 2) + 8 * at), w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float other = __shfl_xor_sync(0xffffffffu, f[j], kHeadChunks / 2);
-        const float2 r = cs[j];
-        f[j] = first ? f[j] * r.x - other * r.y : other * r.y + f[j] * r.x;
+        for (int k = 0; k < 4; ++k) f[j][k] = mul2(mul2(f[j][k], scale), w[k]);
       }
     }
-    if (!mine) continue;
-    if (part == 0) {
-      *reinterpret_cast<uint4*>(q_row + 8 * c) = pack8<T>(f);
-    } else if (dst) {
-      const int h = c / kHeadChunks, d0 = (c % kHeadChunks) * 8;
-      *reinterpret_cast<uint4*>(dst + (int64_t)h * p.page_size * D + d0) = pack8<C>(f);
+    if (rotate) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 a = f[0][k], b = f[1][k];
+        const float2 minus = make_float2(-sn[k].x, -sn[k].y);
+        f[0][k] = fma2(a, cs[k], mul2(b, minus));
+        f[1][k] = fma2(a, sn[k], mul2(b, cs[k]));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (part == 0)
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.q_out) + (row * heads + h) * D + j * (D / 2) + 8 * at) =
+            pack4<T>(f[j]);
+      else if (dst)
+        *reinterpret_cast<uint4*>(dst + (int64_t)h * p.page_size * D + j * (D / 2) + 8 * at) = pack4<C>(f[j]);
     }
   }
 }
 
-// Warps that hold `width` values at kChunks chunks a thread: 1, 2, 4, 8 or 16.
-int unit_warps(int width) {
-  int w = 1;
-  while (w * 32 * kChunks * 8 < width) w *= 2;
-  return w;
+// log2 of the warps (1 to 16) that hold `width` values at kPairs pairs of
+// chunks a thread.
+int unit_shift(int width) {
+  int s = 0;
+  while ((32 << s) * kPairs * 16 < width) ++s;
+  return s;
 }
 
 }  // namespace
@@ -196,11 +258,13 @@ tf_status launch_paged_append(const AppendArgs& a, cudaStream_t s) {
     double f = 0.15915494309189535;  // 1 / (2 pi)
     for (int d = 0; d < D / 2; ++d, f *= step) p.turns[d] = f;
   }
-  p.q_warps = unit_warps(a.heads * D);
-  p.kv_warps = unit_warps(a.kv.kv_heads * D);
-  const int warps = p.q_warps > 8 ? p.q_warps : 8;  // per block
-  const int64_t qb = (a.rows + warps / p.q_warps - 1) / (warps / p.q_warps);
-  const int64_t kb = (a.rows + warps / p.kv_warps - 1) / (warps / p.kv_warps);
+  while ((1 << p.page_shift) < a.kv.page_size) ++p.page_shift;
+  p.q_shift = unit_shift(a.heads * D);
+  p.kv_shift = unit_shift(a.kv.kv_heads * D);
+  const int warps = p.q_shift > 3 ? 1 << p.q_shift : 8;  // per block
+  const int q_rows = warps >> p.q_shift, kv_rows = warps >> p.kv_shift;
+  const int64_t qb = (a.rows + q_rows - 1) / q_rows;
+  const int64_t kb = (a.rows + kv_rows - 1) / kv_rows;
   if (qb + 2 * kb > 2147483647LL) return set_error(TF_ERR_UNSUPPORTED, "paged_append: too many rows");
   p.q_blocks = (unsigned)qb;
   p.k_blocks = (unsigned)kb;

@@ -640,6 +640,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;");
   if (warp == S::kMmaWarp)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kColumns));
 }
@@ -650,23 +651,25 @@ constexpr int kMergeWarps = 8;
 
 template <typename T, int D, int R>
 __global__ void __launch_bounds__(32 * kMergeWarps)
-    paged_merge_kernel(const PagedSegment* __restrict__ items, const float* __restrict__ stat,
-                       const float* __restrict__ part, int group, int heads, T* __restrict__ out) {
-  const PagedSegment& g = items[blockIdx.z];
+    paged_merge_kernel(const PagedSegment* items, const float* stat, const float* part, int group, int heads,
+                       T* out) {
+  const PagedSegment g = items[blockIdx.z];
   const int row = blockIdx.x * 32 + (threadIdx.x & 31);
   const int c = blockIdx.y * kMergeWarps + (threadIdx.x >> 5);  // columns 4 c ..
   if (row >= g.rows) return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the pieces are written
   const float* st = stat + (int64_t)g.part0 * 2 * R + row;
+  const float* o = part + (int64_t)g.part0 * R * D + (c * R + row) * 4;
   float M = -INFINITY;
+#pragma unroll 4
   for (int i = 0; i < g.parts; ++i) M = max_nan(M, st[(int64_t)i * 2 * R]);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
+#pragma unroll 4
   for (int i = 0; i < g.parts; ++i) {
     const float m = st[(int64_t)i * 2 * R];
-    if (m == -INFINITY) continue;
-    const float f = fast_exp2(m - M);
-    const float4 v = *reinterpret_cast<const float4*>(part + (int64_t)(g.part0 + i) * R * D +
-                                                      (c * R + row) * 4);
+    const float f = m == -INFINITY ? 0.f : fast_exp2(m - M);  // an empty piece holds zeros
+    const float4 v = *reinterpret_cast<const float4*>(o + (int64_t)i * R * D);
     sum = fmaf(f, st[(int64_t)i * 2 * R + R], sum);
     acc.x = fmaf(f, v.x, acc.x);
     acc.y = fmaf(f, v.y, acc.y);
@@ -707,9 +710,20 @@ tf_status launch(TileParams p, const Work& w, const char* table, cudaStream_t s)
   if (w.cuts == 0) return TF_OK;
   // grid.z is below 65536: at most one cut item per block.
   const dim3 grid(S::kRows / 32, D / 4 / kMergeWarps, (unsigned)w.cuts);
-  paged_merge_kernel<T, D, S::kRows><<<grid, 32 * kMergeWarps, 0, s>>>(
-      reinterpret_cast<const PagedSegment*>(table + w.merges), p.stat, p.part, p.group, p.heads,
-      static_cast<T*>(p.out));
+  // The merge is launched while the pieces' last blocks still run and waits on
+  // the device for them.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(32 * kMergeWarps);
+  cfg.stream = s;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  TF_CUDA(cudaLaunchKernelEx(&cfg, paged_merge_kernel<T, D, S::kRows>,
+                             reinterpret_cast<const PagedSegment*>(table + w.merges), (const float*)p.stat,
+                             (const float*)p.part, p.group, p.heads, static_cast<T*>(p.out)));
   return check_launch("paged_merge");
 }
 
