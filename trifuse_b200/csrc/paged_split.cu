@@ -201,6 +201,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + S::kOffBar) + warp * S::kStages;
   int* last_s = reinterpret_cast<int*>(base + S::kOffBar + kWarps * S::kStages * 8);
 
+  // A tensor-core kernel of the same call may start where blocks have left.
+  asm volatile("griddepcontrol.launch_dependents;");
   if (lane == 0) {
     for (int i = 0; i < S::kStages; ++i) mbar_init(&bars[i], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");

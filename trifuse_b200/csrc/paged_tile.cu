@@ -640,7 +640,10 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // This kernel may have begun while the few-rows kernel before it still ran
+  // (it needs none of its results); what follows counts on both.
   asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (warp == S::kMmaWarp)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kColumns));
 }
@@ -691,7 +694,7 @@ struct Work {
 };
 
 template <typename T, typename C, int D, int H>
-tf_status launch(TileParams p, const Work& w, const char* table, cudaStream_t s) {
+tf_status launch(TileParams p, const Work& w, const char* table, bool early, cudaStream_t s) {
   using S = Shape<D, H>;
   if (w.blocks == 0) return TF_OK;
   static PerDeviceOnce attr;
@@ -705,21 +708,28 @@ tf_status launch(TileParams p, const Work& w, const char* table, cudaStream_t s)
   p.starts = reinterpret_cast<const int32_t*>(table + w.starts);
   p.stat = w.stat;
   p.part = p.stat + (int64_t)w.parts * 2 * S::kRows;
-  paged_tile_kernel<T, C, D, H><<<w.blocks, S::kThreads, S::kSmem, s>>>(p);
+  cudaLaunchAttribute overlap{};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)w.blocks);
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = s;
+  cfg.attrs = &overlap;
+  cfg.numAttrs = early ? 1 : 0;
+  TF_CUDA(cudaLaunchKernelEx(&cfg, paged_tile_kernel<T, C, D, H>, p));
   TF_TRY(check_launch("paged_tile"));
   if (w.cuts == 0) return TF_OK;
   // grid.z is below 65536: at most one cut item per block.
   const dim3 grid(S::kRows / 32, D / 4 / kMergeWarps, (unsigned)w.cuts);
   // The merge is launched while the pieces' last blocks still run and waits on
   // the device for them.
-  cudaLaunchConfig_t cfg{};
+  cfg = cudaLaunchConfig_t{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(32 * kMergeWarps);
   cfg.stream = s;
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &early;
+  cfg.attrs = &overlap;
   cfg.numAttrs = 1;
   TF_CUDA(cudaLaunchKernelEx(&cfg, paged_merge_kernel<T, D, S::kRows>,
                              reinterpret_cast<const PagedSegment*>(table + w.merges), (const float*)p.stat,
@@ -736,8 +746,10 @@ tf_status launch_both(const TileParams& p, const PagedArgs& a, cudaStream_t s) {
   const Work half = {plan.half_segments_offset, plan.half_starts_offset, plan.half_merges_offset,
                      plan.half_blocks, plan.half_parts, plan.half_merges,
                      stat + (int64_t)plan.tile_parts * kTileRows * (2 + D)};
-  TF_TRY((launch<T, C, D, 2>(p, tile, a.plan_table, s)));
-  return launch<T, C, D, 1>(p, half, a.plan_table, s);
+  // The first kernel after the few-rows kernel starts on the SMs that it leaves.
+  const bool after_split = plan.split_blocks > 0;
+  TF_TRY((launch<T, C, D, 2>(p, tile, a.plan_table, after_split, s)));
+  return launch<T, C, D, 1>(p, half, a.plan_table, after_split && plan.tile_blocks == 0, s);
 }
 
 }  // namespace
