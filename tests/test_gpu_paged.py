@@ -138,6 +138,17 @@ def test_rows_that_attend_nothing(ops):
         assert (got[: max(0, n - L)] == 0).all()
 
 
+def test_plan_takes_other_integers(ops):
+    """Lengths as tensors and numpy arrays; a length that would wrap is refused."""
+    import numpy as np
+    a = ops.PagedPlan(torch.tensor([1, 5]), np.array([40, 60]), 4, 2, 64, 16)
+    assert a.positions.tolist() == [39, 55, 56, 57, 58, 59]
+    with pytest.raises(ValueError):
+        ops.PagedPlan([1], [(1 << 32) + 5], 4, 2, 64, 16)
+    with pytest.raises(ValueError):
+        ops.PagedPlan([1, 2], [5], 4, 2, 64, 16)
+
+
 def test_no_rows(ops):
     k, v, table = make_cache([10, 0], 2, 64, 16, F16)
     plan = ops.PagedPlan([0, 0], [10, 0], 4, 2, 64, 16)
@@ -213,6 +224,23 @@ def test_strides_and_interleaved_pages(ops, n):
     assert torch.equal(got, want)
     out = torch.empty_like(want)
     assert ops.paged_attention(q, k, v, table, plan, out=out) is out and torch.equal(out, want)
+
+
+def test_rows_off_their_alignment(ops):
+    """q and qkv views that start in the middle of a 16-byte vector, or whose rows do."""
+    H, Hk, D, page, L = 4, 2, 64, 16, 40
+    k, v, table = make_cache([L], Hk, D, page, F16)
+    plan = ops.PagedPlan([3], [L], H, Hk, D, page)
+    g = torch.Generator().manual_seed(4)
+    wide = torch.randn(3, (H + 2 * Hk) * D + 13, generator=g).to(F16).cuda()
+    qkv = wide[:, 3:3 + (H + 2 * Hk) * D]
+    k2, v2 = k.clone(), v.clone()
+    q = ops.paged_append(qkv, k, v, table, plan.positions, plan.requests, H)
+    assert torch.equal(q, ops.paged_append(qkv.contiguous(), k2, v2, table, plan.positions, plan.requests, H))
+    assert torch.equal(k, k2) and torch.equal(v, v2)
+    view = wide[:, 3:3 + H * D].view(3, H, D)
+    assert torch.equal(ops.paged_attention(view, k, v, table, plan),
+                       ops.paged_attention(view.contiguous(), k, v, table, plan))
 
 
 def test_repeatable_and_plan_reused(ops):

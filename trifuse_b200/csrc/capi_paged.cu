@@ -1,6 +1,6 @@
 // C ABI of the paged key/value cache and of token log probabilities: argument
 // checks, all of them before any launch.
-#include <new>
+#include <exception>
 
 #include "internal.h"
 #include "paged.h"
@@ -125,7 +125,7 @@ int tf_paged_plan_make(const int32_t* new_lengths, const int32_t* kv_lengths, in
     const tf_status s = paged_plan_make(new_lengths, kv_lengths, &p, static_cast<char*>(table), table_capacity);
     *plan = p;
     return s;
-  } catch (const std::bad_alloc&) {
+  } catch (const std::exception&) {  // bad_alloc, or a length past what a vector holds
     return set_error(TF_ERR_OUT_OF_MEMORY, "paged plan: out of host memory");
   }
 }

@@ -493,14 +493,24 @@ def _page_table(page_table: Tensor) -> PageTable:
     return PageTable(page_table.data_ptr(), max(page_table.stride(0), columns), requests, columns)
 
 
-def _launch_stream(*ts) -> int:
+def _launch_stream(first: Tensor, *others) -> int:
     """The current device's current stream (its handle); every tensor must live on that device."""
-    dev = torch._C._cuda_getDevice()
-    for t in ts:
+    dev = first.get_device()
+    for t in others:
         if t is not None and t.get_device() != dev:
-            _cuda(t)
-            raise ValueError("tensors must be on the current CUDA device")
+            _cuda(first, *others)
+            raise ValueError("tensors must be on one CUDA device")
+    _cuda(first)
+    if dev != torch._C._cuda_getDevice():
+        raise ValueError("tensors must be on the current CUDA device")
     return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _rows16(t: Tensor, width: int) -> Tensor:
+    """t, or a copy of it where its rows (of `width` values) cannot be read 16 bytes at a time."""
+    if t.stride(0) < width or t.stride(0) % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
 
 
 def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, positions: Tensor,
@@ -519,8 +529,9 @@ def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tens
     D, width = kv.head_dim, (heads + 2 * kv.kv_heads) * kv.head_dim
     if qkv.ndim != 2 or qkv.shape[1] != width:
         raise ValueError("paged_append: qkv is [rows, (heads + 2 kv_heads) * head_dim]")
-    if qkv.stride(1) != 1 or qkv.stride(0) < width:
+    if qkv.stride(1) != 1:
         qkv = qkv.contiguous()
+    qkv = _rows16(qkv, width)
     rows = qkv.shape[0]
     for t in (positions, requests):
         if t.dtype != torch.int32 or t.shape != (rows,) or not t.is_contiguous():
@@ -529,7 +540,7 @@ def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tens
         if t is not None and (t.dtype != torch.float16 or t.shape != (n,) or not t.is_contiguous()):
             raise ValueError("paged_append: norm weights are contiguous float16 over the full q and k widths")
     if out is None:
-        out = torch.empty((rows, heads, D), dtype=qkv.dtype, device=qkv.device)
+        out = qkv.new_empty((rows, heads, D))
     elif out.shape != (rows, heads, D) or out.dtype != qkv.dtype or not out.is_contiguous():
         raise ValueError("paged_append: out is a contiguous [rows, heads, head_dim] of qkv's dtype")
     table = _page_table(page_table)
@@ -556,9 +567,12 @@ class PagedPlan:
         n = len(new_lengths)
         if len(kv_lengths) != n:
             raise ValueError("paged plan: new_lengths and kv_lengths differ in length")
+        new_lengths, kv_lengths = [int(x) for x in new_lengths], [int(x) for x in kv_lengths]
+        if n and max(max(new_lengths), max(kv_lengths)) >= 1 << 31:  # would wrap on the way to C
+            raise ValueError("paged plan: a length is above 2^31")
         new, kv = (C.c_int32 * n)(*new_lengths), (C.c_int32 * n)(*kv_lengths)
         self.desc = d = PagedPlanDesc()
-        guess = 65536 + 64 * n * max(kv_heads, 1) + 16 * sum(new)
+        guess = 65536 + 64 * n * max(kv_heads, 1) + 16 * max(sum(new_lengths), 0)
         while True:  # a second time when the table outgrows the guess
             host = torch.empty(guess, dtype=torch.uint8, pin_memory=True)
             status = lib().tf_paged_plan_make(new, kv, n, heads, kv_heads, head_dim, page_size, d, host.data_ptr(),
@@ -600,10 +614,11 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Ten
     rows, heads, D = plan.rows, plan.heads, plan.head_dim
     if q.shape != (rows, heads, D):
         raise ValueError("paged_attention: q is [rows, heads, head_dim] of the plan")
-    if q.stride()[1:] != (D, 1) or q.stride(0) < heads * D or q.stride(0) % 8:
+    if q.stride()[1:] != (D, 1):
         q = q.contiguous()
+    q = _rows16(q, heads * D)
     if out is None:
-        out = torch.empty((rows, heads, D), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != (rows, heads, D) or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("paged_attention: out is a contiguous [rows, heads, head_dim] of q's dtype")
     plan._on(stream)
