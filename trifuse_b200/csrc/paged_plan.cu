@@ -2,13 +2,17 @@
 // key-tile work of one call over the GPU's SMs.  Host code only.
 //
 // Every thread block gets a list of segments up front, so the kernels need no
-// work queue and a call's result does not depend on timing.  Whole items are
-// first placed longest-first on the least loaded block.  Where that leaves the
-// slowest block more than 1/16 above the mean (few or very unequal items),
-// the items are instead laid end to end and cut into equal shares; the pieces
-// of a cut item leave partial results that the last of them to finish merges.
-// A cut costs the partial results' traffic and the merge, a few percent of a
-// long item, so items stay whole where they balance anyway.
+// work queue and a call's result does not depend on timing.  Three ways to
+// divide the items are weighed by the load of the slowest block, in tiles:
+//   whole   every item whole, longest first on the least loaded block;
+//   even    long items cut into equal pieces of about a block's share, placed
+//           the same way;
+//   wrap    items laid end to end and cut into equal shares.
+// A cut piece costs a partial result and its merge beside a segment's start, so
+// items stay whole where they balance within 1/16 of the mean anyway.  (16
+// requests of 2048 tokens on 8 key heads, 128 items for 148 blocks: whole 30
+// us, wrapped 33; 24 x 5 drafted tokens over 2048, 48 items for 296: 18 us in
+// pieces of at least 4 tiles, 15 of at least 2.)
 #include <string.h>
 
 #include <algorithm>
@@ -44,36 +48,31 @@ int current_sms() {
   return n;
 }
 
-// Divides the items over at most `blocks` blocks.  overhead: cost of starting
-// a segment, in tiles; min_piece: smallest piece worth cutting, in tiles.
-Schedule divide(const std::vector<Item>& items, int kv_heads, int blocks, int overhead, int min_piece) {
+// What a kernel's segments cost beside their tiles, in tiles.
+struct Costs {
+  int start;      // any segment
+  int cut;        // a piece of a cut item: its partial result, its part of the merge
+  int join;       // a call that cuts at all
+  int min_piece;  // smallest piece worth cutting
+};
+
+// Places the pieces, in order, each on the least loaded block; most: the load
+// of the slowest.
+Schedule place(const std::vector<Piece>& pieces, const std::vector<int32_t>& cost, int blocks, int64_t* most) {
   Schedule out;
-  int64_t total = 0;
-  for (const Item& it : items) total += it.tiles + overhead;
-  const int64_t mean = std::max<int64_t>((total + blocks - 1) / blocks, min_piece + overhead);
-  // Longest first; equal items keep their order, so one request's key heads
-  // and row blocks run at the same time and share its pages through L2.  The
-  // key heads of a row block follow one another with equal lengths, so they
-  // are sorted as one.
-  std::vector<int32_t> order(items.size()), firsts;
-  firsts.reserve(items.size() / kv_heads);
-  for (size_t i = 0; i < items.size(); i += kv_heads) firsts.push_back((int32_t)i);
-  const auto longer = [&](int32_t a, int32_t b) { return items[a].tiles > items[b].tiles; };
-  if (!std::is_sorted(firsts.begin(), firsts.end(), longer)) std::stable_sort(firsts.begin(), firsts.end(), longer);
-  for (size_t i = 0; i < order.size(); ++i) order[i] = firsts[i / kv_heads] + (int32_t)(i % kv_heads);
   // Loads as a binary heap of (load, block) in one 64-bit word; the least
   // loaded block is raised in place.
-  const int used = (int)std::min<size_t>(blocks, items.size());
+  const int used = (int)std::min<size_t>(blocks, pieces.size());
   std::vector<uint64_t> heap(used);
   for (int b = 0; b < used; ++b) heap[b] = (uint64_t)b;
-  std::vector<int32_t> owner(items.size()), count(used + 1, 0);
-  uint64_t most = 0;
-  for (int32_t i : order) {
-    const uint64_t load = (heap[0] >> 20) + items[i].tiles + overhead;
-    const uint64_t b = heap[0] & 0xfffff;
+  std::vector<int32_t> owner(pieces.size());
+  out.starts.assign(used + 1, 0);
+  *most = 0;
+  for (size_t i = 0; i < pieces.size(); ++i) {
+    const uint64_t load = (heap[0] >> 20) + cost[i], b = heap[0] & 0xfffff;
     owner[i] = (int32_t)b;
-    ++count[b + 1];
-    most = std::max(most, load);
+    ++out.starts[b + 1];
+    *most = std::max<int64_t>(*most, (int64_t)load);
     const uint64_t word = load << 20 | b;
     int at = 0;
     for (int child; (child = 2 * at + 1) < used; at = child) {
@@ -83,40 +82,92 @@ Schedule divide(const std::vector<Item>& items, int kv_heads, int blocks, int ov
     }
     heap[at] = word;
   }
-  if ((int64_t)most <= mean + mean / 16) {
-    for (int b = 0; b < used; ++b) count[b + 1] += count[b];
-    out.starts = count;
-    out.pieces.resize(items.size());
-    for (int32_t i : order) out.pieces[count[owner[i]]++] = {i, 0, items[i].tiles};
-    return out;
+  for (int b = 0; b < used; ++b) out.starts[b + 1] += out.starts[b];
+  out.pieces.resize(pieces.size());
+  std::vector<int32_t> next(out.starts.begin(), out.starts.end());
+  for (size_t i = 0; i < pieces.size(); ++i) out.pieces[next[owner[i]]++] = pieces[i];
+  return out;
+}
+
+// Divides the items over at most `blocks` blocks.
+Schedule divide(const std::vector<Item>& items, int kv_heads, int blocks, const Costs& c) {
+  int64_t total = 0;
+  for (const Item& it : items) total += it.tiles + c.start;
+  const int64_t mean = std::max<int64_t>((total + blocks - 1) / blocks, c.min_piece + c.start);
+  // Longest first; equal items keep their order, so one request's key heads
+  // and row blocks run at the same time and share its pages through L2.  The
+  // key heads of a row block follow one another with equal lengths, so they
+  // are sorted as one.
+  std::vector<int32_t> firsts;
+  firsts.reserve(items.size() / kv_heads);
+  for (size_t i = 0; i < items.size(); i += kv_heads) firsts.push_back((int32_t)i);
+  const auto longer = [&](int32_t a, int32_t b) { return items[a].tiles > items[b].tiles; };
+  if (!std::is_sorted(firsts.begin(), firsts.end(), longer)) std::stable_sort(firsts.begin(), firsts.end(), longer);
+  std::vector<Piece> pieces;
+  std::vector<int32_t> cost;
+  for (int32_t f : firsts)
+    for (int h = 0; h < kv_heads; ++h) {
+      pieces.push_back({f + h, 0, items[f].tiles});
+      cost.push_back(items[f].tiles + c.start);
+    }
+  int64_t most = 0;
+  Schedule whole = place(pieces, cost, blocks, &most);
+  if (most <= mean + mean / 16) return whole;
+
+  const int64_t share = mean - c.start;
+  pieces.clear();
+  cost.clear();
+  for (int32_t f : firsts) {
+    const int64_t tiles = items[f].tiles;
+    const int64_t n = std::max<int64_t>(1, std::min((tiles + share - 1) / share, tiles / c.min_piece));
+    for (int64_t k = 0; k < n; ++k)
+      for (int h = 0; h < kv_heads; ++h) {
+        pieces.push_back({f + h, (int32_t)(tiles * k / n), (int32_t)(tiles * (k + 1) / n)});
+        cost.push_back((int32_t)(tiles * (k + 1) / n - tiles * k / n + c.start + (n > 1 ? c.cut : 0)));
+      }
   }
+  int64_t most_even = 0;
+  Schedule even = place(pieces, cost, blocks, &most_even);
+  most_even += c.join;
+
   // Every cut adds a segment, and a block may close short of a full share, so
   // the share grows until the pieces fit.
-  for (int64_t share = mean + overhead;; share += share / 64 + 1) {
-    out.pieces.clear();
-    out.starts.assign(1, 0);
+  Schedule wrap;
+  int64_t most_wrap = 0;
+  for (int64_t room_for = mean + c.start + c.cut;; room_for += room_for / 64 + 1) {
+    wrap.pieces.clear();
+    wrap.starts.assign(1, 0);
+    most_wrap = 0;
     int64_t load = 0;
-    for (int32_t i : order) {
-      int32_t t = 0;
-      do {
-        const int64_t left = items[i].tiles - t;
-        int64_t room = share - load - overhead;
-        if (room < min_piece && load > 0) {
-          out.starts.push_back((int32_t)out.pieces.size());
-          load = 0;
-          room = share - overhead;
-        }
-        int64_t take = std::min(left, room);
-        // No crumbs: a rest below min_piece joins this piece.
-        if (left - take < min_piece) take = left;
-        out.pieces.push_back({i, t, (int32_t)(t + take)});
-        load += take + overhead;
-        t += (int32_t)take;
-      } while (t < items[i].tiles);
-    }
-    if (load > 0) out.starts.push_back((int32_t)out.pieces.size());
-    if ((int)out.starts.size() - 1 <= blocks) return out;
+    for (int32_t f : firsts)
+      for (int h = 0; h < kv_heads; ++h) {
+        const int64_t tiles = items[f].tiles;
+        int64_t t = 0;
+        do {
+          const int64_t left = tiles - t;
+          int64_t room = room_for - load - c.start - c.cut;
+          if (room < c.min_piece && load > 0) {
+            wrap.starts.push_back((int32_t)wrap.pieces.size());
+            load = 0;
+            room = room_for - c.start - c.cut;
+          }
+          int64_t take = std::min(left, std::max<int64_t>(room, c.min_piece));
+          // No crumbs: a rest below min_piece takes as much from this piece,
+          // or joins it.
+          if (take < left && left - take < c.min_piece)
+            take = left >= 2 * c.min_piece ? left - c.min_piece : left;
+          wrap.pieces.push_back({f + h, (int32_t)t, (int32_t)(t + take)});
+          load += take + c.start + (take < tiles ? c.cut : 0);
+          most_wrap = std::max(most_wrap, load);
+          t += take;
+        } while (t < tiles);
+      }
+    if (load > 0) wrap.starts.push_back((int32_t)wrap.pieces.size());
+    if ((int)wrap.starts.size() - 1 <= blocks) break;
   }
+  most_wrap += c.join;
+  if (most <= most_even && most <= most_wrap) return whole;
+  return most_even <= most_wrap ? even : wrap;
 }
 
 struct Layout {
@@ -185,11 +236,10 @@ Layout plan_kernel(const int32_t* new_lengths, const int32_t* kv_lengths, const 
       }
     q_row += n;
   }
-  // A segment starts in the time of some four small or one large tile; a piece
-  // should be worth its partial result (a large tile's keys and values are as
-  // many bytes as half a partial result of 256 rows).
-  const Schedule s = kind == kSplit ? divide(items, p.kv_heads, current_sms(), 4, 8)
-                                    : divide(items, p.kv_heads, current_sms() * (kind == kHalves1 ? 2 : 1), 1, 4);
+  // In tiles of each kernel: 16 KB a small one, up to 64 KB a large one, whose
+  // pieces are merged by a kernel of their own.
+  const Costs costs = kind == kSplit ? Costs{2, 6, 0, 4} : Costs{1, 1, 2, 2};
+  const Schedule s = divide(items, p.kv_heads, current_sms() * (kind == kHalves1 ? 2 : 1), costs);
   return lay_out(items, s, new_lengths, kv_lengths);
 }
 
