@@ -54,10 +54,10 @@ struct PagedArgs {
 // Fills the plan's remaining fields, and the table where it fits.
 tf_status paged_plan_make(const int32_t* new_lengths, const int32_t* kv_lengths, tf_paged_plan* plan, char* table,
                           size_t table_capacity);
-// Tensor map over pages as [page][kv_head * page_size rows][head_dim], box
-// {64 values, box_rows rows, 1 page}, 128-byte swizzle; a page id outside
-// [0, pages) reads zeros.
-tf_status make_page_map(void* map, const void* base, const tf_paged_kv& kv, int box_rows);
+// Tensor map over pages as [page][64-column half][kv_head * page_size rows][64
+// columns], box of box_rows rows by box_columns columns of one page, 128-byte
+// swizzle; a page id outside [0, pages) reads zeros.
+tf_status make_page_map(void* map, const void* base, const tf_paged_kv& kv, int box_rows, int box_columns);
 tf_status launch_paged_split(const PagedArgs& a, cudaStream_t s);
 tf_status launch_paged_tile(const PagedArgs& a, cudaStream_t s);
 // Workspace of the few-rows kernel's parts: per part and row the maximum, the

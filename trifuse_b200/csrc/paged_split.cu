@@ -45,12 +45,11 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRowBytes = 128;                        // one swizzled row: 64 values
-constexpr int kHalfBytes = kSplitKeys * kRowBytes;    // 64 columns of a tile's keys
 
 template <int D>
 struct Shape {
   static constexpr int kHalves = D / 64;
-  static constexpr int kTile = kHalves * kHalfBytes;  // bytes of a tile's keys (and of its values)
+  static constexpr int kTile = kHalves * kSplitKeys * kRowBytes;  // bytes of a tile's keys (and of its values)
   static constexpr int kStages = 384 / D;             // 48 KB per warp
   static constexpr int kRing = kStages * 2 * kTile;
   static constexpr int kPitch = D + 4;                // joined outputs: rows 4 words apart in the banks
@@ -70,7 +69,7 @@ struct SplitParams {
   int32_t columns;
   int32_t page_size;
   int32_t page_shift;
-  int32_t box_rows;  // min(page_size, kSplitKeys)
+  int32_t box_rows, box_shift;  // min(page_size, kSplitKeys)
   int32_t group;     // query heads per key head
   int32_t heads;
   const PagedSegment* segments;
@@ -94,11 +93,12 @@ __device__ __forceinline__ bool wait_copy(uint64_t* bar, uint32_t parity, long l
   return false;
 }
 
-__device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int x, int row, int page, uint64_t* bar) {
+// `row` .. of a page, all columns: [64-column half][box row][128 bytes].
+__device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int row, int page, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
-          "r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(page), "r"(smem_addr(bar))
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(0), "r"(page), "r"(smem_addr(bar))
       : "memory");
 }
 
@@ -219,9 +219,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
     more = in.settle(p.segments, warp);
   }
   int fetched = 0, used = 0;
-  // Box of this lane in a tile: which page's part, keys or values, which 64
-  // columns.  The page id of the next tile is looked up a tile ahead.
-  const int box = lane / (S::kHalves * 2), what = lane % (S::kHalves * 2);
+  // Box of this lane in a tile: which page's part, keys or values.  The page id of the next tile is looked up a tile ahead.
+  const int box = lane >> 1, is_v = lane & 1;
+  const int half_bytes = p.box_rows * kRowBytes, box_bytes = half_bytes * S::kHalves;
   int page = -1;
   auto look_up = [&]() {
     const int column = (in.tile * kSplitKeys + box * p.box_rows) >> p.page_shift;
@@ -229,8 +229,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
   };
   if (more) look_up();
 
-  // Fetches one tile into the ring's next slot: lane i copies box i (of the
-  // tile's existing pages, keys before values, 64 columns each).
+  // Fetches one tile into the ring's next slot: lanes 2 i, 2 i + 1 copy the keys
+  // and the values of box i of the tile's existing pages.
   auto fetch = [&]() {
     const int slot = fetched % S::kStages;
     uint8_t* dst = ring + slot * 2 * S::kTile;
@@ -238,14 +238,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
     const int left = in.kv_len - key0;
     const int want = left < kSplitKeys ? left : kSplitKeys;
     const int boxes = (want + p.box_rows - 1) / p.box_rows;  // pages (or parts of one) that exist
-    const int box_bytes = p.box_rows * kRowBytes;
-    if (lane == 0) mbar_expect_tx(&bars[slot], (uint32_t)(boxes * box_bytes * S::kHalves * 2));
+    if (lane == 0) mbar_expect_tx(&bars[slot], (uint32_t)(boxes * box_bytes * 2));
     __syncwarp();
     if (box < boxes) {
-      const int half = what % S::kHalves, is_v = what / S::kHalves;
       const int row = in.kv_head * p.page_size + ((key0 + box * p.box_rows) & (p.page_size - 1));
-      tma_page(dst + is_v * S::kTile + half * kHalfBytes + box * box_bytes, is_v ? &p.tm_v : &p.tm_k, half * 64, row,
-               page, &bars[slot]);
+      tma_page(dst + is_v * S::kTile + box * box_bytes, is_v ? &p.tm_v : &p.tm_k, row, page, &bars[slot]);
     }
     ++fetched;
     in.tile += kWarps;
@@ -256,6 +253,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
 
   const int g = lane >> 2, c2 = (lane & 3) * 2;  // MMA fragment row (or column) and column pair
   const long long limit_cycles = *p.wait_cycles;
+  // Offset of key r in a tile, and those of the keys that this lane's ldmatrix
+  // addresses name.
+  auto key_at = [&](int r) { return (r >> p.box_shift) * box_bytes + (r & (p.box_rows - 1)) * kRowBytes; };
+  int k_at[2], v_at[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    k_at[h] = key_at(16 * h + (lane & 15));
+    v_at[h] = key_at(16 * h + (lane & 7) + ((lane >> 4) << 3));
+  }
   bool ok = true;
   for (int seg = seg0; seg < seg_end; ++seg) {
     const PagedSegment sg = p.segments[seg];
@@ -321,9 +327,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t a[4];
-          const int row = 16 * h + (lane & 15);
           const int chunk = (2 * k + (lane >> 4)) & 7;
-          ldsm4(ks + (k >> 2) * kHalfBytes + row * kRowBytes + ((chunk ^ (row & 7)) << 4), a);
+          ldsm4(ks + (k >> 2) * half_bytes + k_at[h] + ((chunk ^ (lane & 7)) << 4), a);
 #pragma unroll
           for (int t = 0; t < NT; ++t) mma16816<C>(s[h][t], a, qb[k][t][0], qb[k][t][1]);
         }
@@ -383,10 +388,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
         // Slots past the request's length hold anything, NaN included: 0 * NaN
         // would reach the outputs, so their values become zeros.
         uint8_t* v = ring + slot * 2 * S::kTile + S::kTile;
-        for (int i = have * kRowBytes / 16 + lane; i < kHalfBytes / 16; i += 32)
+        for (int i = have * 8 + lane; i < kSplitKeys * 8; i += 32)
 #pragma unroll
           for (int h = 0; h < S::kHalves; ++h)
-            *reinterpret_cast<uint4*>(v + h * kHalfBytes + 16 * i) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(v + key_at(i >> 3) + h * half_bytes + 16 * (i & 7)) = make_uint4(0, 0, 0, 0);
         __syncwarp();
       }
 #pragma unroll
@@ -394,9 +399,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t a[4];
-          const int row = 16 * h + (lane & 7) + ((lane >> 4) << 3);
           const int chunk = (2 * d + ((lane >> 3) & 1)) & 7;
-          ldsm4_t(vs + (d >> 2) * kHalfBytes + row * kRowBytes + ((chunk ^ (row & 7)) << 4), a);
+          ldsm4_t(vs + (d >> 2) * half_bytes + v_at[h] + ((chunk ^ (lane & 7)) << 4), a);
 #pragma unroll
           for (int t = 0; t < NT; ++t) mma16816<C>(o[d][t], a, pb[h][t][0], pb[h][t][1]);
         }
@@ -535,16 +539,17 @@ EncodeFn encode_fn() {
 
 }  // namespace
 
-tf_status make_page_map(void* map, const void* base, const tf_paged_kv& kv, int box_rows) {
-  const cuuint64_t dims[3] = {(cuuint64_t)kv.head_dim, (cuuint64_t)kv.kv_heads * kv.page_size, (cuuint64_t)kv.pages};
-  const cuuint64_t strides[2] = {(cuuint64_t)kv.head_dim * 2, (cuuint64_t)kv.page_stride * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
-  const cuuint32_t elem[3] = {1, 1, 1};
+tf_status make_page_map(void* map, const void* base, const tf_paged_kv& kv, int box_rows, int box_columns) {
+  const cuuint64_t dims[4] = {64, (cuuint64_t)kv.kv_heads * kv.page_size, (cuuint64_t)kv.head_dim / 64,
+                              (cuuint64_t)kv.pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)kv.head_dim * 2, 128, (cuuint64_t)kv.page_stride * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_columns / 64, 1};
+  const cuuint32_t elem[4] = {1, 1, 1, 1};
   const EncodeFn encode = encode_fn();
   if (!encode) return set_error(TF_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   const CUresult r = encode(
       static_cast<CUtensorMap*>(map),
-      kv.dtype == TF_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+      kv.dtype == TF_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
       const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(TF_ERR_CUDA, "paged attention: tensor map (%d)", (int)r);
@@ -557,8 +562,9 @@ tf_status launch_paged_split(const PagedArgs& a, cudaStream_t s) {
   SplitParams p;
   memset(&p, 0, sizeof(p));
   p.box_rows = a.kv.page_size < kSplitKeys ? a.kv.page_size : kSplitKeys;
-  TF_TRY(make_page_map(&p.tm_k, a.kv.k, a.kv, p.box_rows));
-  TF_TRY(make_page_map(&p.tm_v, a.kv.v, a.kv, p.box_rows));
+  while ((1 << p.box_shift) < p.box_rows) ++p.box_shift;
+  TF_TRY(make_page_map(&p.tm_k, a.kv.k, a.kv, p.box_rows, a.kv.head_dim));
+  TF_TRY(make_page_map(&p.tm_v, a.kv.v, a.kv, p.box_rows, a.kv.head_dim));
   p.q = a.q;
   p.q_stride = a.q_stride;
   p.ids = a.table.ids;

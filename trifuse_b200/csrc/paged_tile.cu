@@ -139,11 +139,13 @@ __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity, int* err) 
     }
 }
 
-__device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int x, int row, int page, uint64_t* bar) {
+// 64 columns (of half `half`) of `row` .. of a page.
+__device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int row, int half, int page,
+                                         uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
-          "r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(page), "r"(smem_addr(bar))
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(half), "r"(page), "r"(smem_addr(bar))
       : "memory");
 }
 
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
               uint8_t* dst = base + S::kOffRing + slot * S::kTile + lane * box_bytes;
 #pragma unroll
               for (int h = 0; h < D / 64; ++h)
-                tma_page(dst + h * kColBytes, v ? &p.tm_v : &p.tm_k, 64 * h, row, page, &kv_full[slot]);
+                tma_page(dst + h * kColBytes, v ? &p.tm_v : &p.tm_k, row, h, page, &kv_full[slot]);
             }
           }
         }
@@ -760,8 +762,8 @@ tf_status launch_paged_tile(const PagedArgs& a, cudaStream_t s) {
   TileParams p;
   memset(&p, 0, sizeof(p));
   p.box_rows = a.kv.page_size < kTileKeys ? a.kv.page_size : kTileKeys;
-  TF_TRY(make_page_map(&p.tm_k, a.kv.k, a.kv, p.box_rows));
-  TF_TRY(make_page_map(&p.tm_v, a.kv.v, a.kv, p.box_rows));
+  TF_TRY(make_page_map(&p.tm_k, a.kv.k, a.kv, p.box_rows, 64));
+  TF_TRY(make_page_map(&p.tm_v, a.kv.v, a.kv, p.box_rows, 64));
   p.q = a.q;
   p.q_stride = a.q_stride;
   p.ids = a.table.ids;
