@@ -474,23 +474,24 @@ def attention_decode(qkv: Tensor, q_norm: Tensor, k_norm: Tensor, positions: Ten
 def _paged_kv(k_pages: Tensor, v_pages: Tensor) -> PagedKV:
     """Descriptor of [pages, kv_heads, page_size, head_dim] caches; only the
     first dimension may have a stride of its own."""
-    if k_pages.ndim != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+    shape, dtype, stride = k_pages.shape, k_pages.dtype, k_pages.stride()
+    if len(shape) != 4 or shape != v_pages.shape or dtype != v_pages.dtype:
         raise ValueError("paged: k_pages and v_pages are [pages, kv_heads, page_size, head_dim] of one dtype")
-    if k_pages.dtype not in _ACT:
+    if dtype not in _ACT:
         raise ValueError("paged: the cache must be float16 or bfloat16")
-    pages, heads, size, D = k_pages.shape
-    stride = k_pages.stride()
-    if stride != v_pages.stride() or stride[1:] != (size * D, D, 1):
+    pages, heads, size, D = shape
+    step = stride[0]
+    if stride != (step, size * D, D, 1) or stride != v_pages.stride():
         raise ValueError("paged: a page must be contiguous, and k_pages and v_pages laid out alike")
-    return PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), pages, stride[0], heads, size, D, _ACT[k_pages.dtype])
+    return PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), pages, step, heads, size, D, _ACT[dtype])
 
 
 def _page_table(page_table: Tensor) -> PageTable:
-    if page_table.ndim != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1
-                                                                   and page_table.stride(1) != 1):
+    shape, stride = page_table.shape, page_table.stride()
+    if len(shape) != 2 or page_table.dtype != torch.int32 or (shape[1] > 1 and stride[1] != 1):
         raise ValueError("paged: the page table is int32 [requests, pages] with contiguous rows")
-    requests, columns = page_table.shape
-    return PageTable(page_table.data_ptr(), max(page_table.stride(0), columns), requests, columns)
+    requests, columns = shape
+    return PageTable(page_table.data_ptr(), max(stride[0], columns), requests, columns)
 
 
 def _launch_stream(first: Tensor, *others) -> int:
@@ -508,7 +509,8 @@ def _launch_stream(first: Tensor, *others) -> int:
 
 def _rows16(t: Tensor, width: int) -> Tensor:
     """t, or a copy of it where its rows (of `width` values) cannot be read 16 bytes at a time."""
-    if t.stride(0) < width or t.stride(0) % 8 or t.data_ptr() % 16:
+    step = t.stride(0)
+    if step < width or step % 8 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -526,29 +528,29 @@ def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tens
     A row whose slot the table does not have is not stored."""
     stream = _launch_stream(qkv, k_pages, v_pages, page_table, positions, requests, q_norm, k_norm, out)
     kv = _paged_kv(k_pages, v_pages)
-    D, width = kv.head_dim, (heads + 2 * kv.kv_heads) * kv.head_dim
+    D, kv_heads = kv.head_dim, kv.kv_heads
+    width = (heads + 2 * kv_heads) * D
     if qkv.ndim != 2 or qkv.shape[1] != width:
         raise ValueError("paged_append: qkv is [rows, (heads + 2 kv_heads) * head_dim]")
-    if qkv.stride(1) != 1:
-        qkv = qkv.contiguous()
-    qkv = _rows16(qkv, width)
+    qkv = _rows16(qkv if qkv.stride(1) == 1 else qkv.contiguous(), width)
     rows = qkv.shape[0]
-    for t in (positions, requests):
-        if t.dtype != torch.int32 or t.shape != (rows,) or not t.is_contiguous():
-            raise ValueError("paged_append: positions and requests are contiguous int32 [rows]")
-    for t, n in ((q_norm, heads * D), (k_norm, kv.kv_heads * D)):
-        if t is not None and (t.dtype != torch.float16 or t.shape != (n,) or not t.is_contiguous()):
-            raise ValueError("paged_append: norm weights are contiguous float16 over the full q and k widths")
+    i32 = torch.int32
+    if (positions.dtype != i32 or requests.dtype != i32 or not positions.shape == requests.shape == (rows,)
+            or not positions.is_contiguous() or not requests.is_contiguous()):
+        raise ValueError("paged_append: positions and requests are contiguous int32 [rows]")
+    qn = kn = None
+    if q_norm is not None or k_norm is not None:
+        for t, n in ((q_norm, heads * D), (k_norm, kv_heads * D)):
+            if t is not None and (t.dtype != torch.float16 or t.shape != (n,) or not t.is_contiguous()):
+                raise ValueError("paged_append: norm weights are contiguous float16 over the full q and k widths")
+        qn, kn = (None if t is None else t.data_ptr() for t in (q_norm, k_norm))
     if out is None:
         out = qkv.new_empty((rows, heads, D))
     elif out.shape != (rows, heads, D) or out.dtype != qkv.dtype or not out.is_contiguous():
         raise ValueError("paged_append: out is a contiguous [rows, heads, head_dim] of qkv's dtype")
-    table = _page_table(page_table)
-    check(lib().tf_paged_append(qkv.data_ptr(), qkv.stride(0) if rows > 1 else width, rows, heads, _act(qkv),
-                                None if q_norm is None else q_norm.data_ptr(),
-                                None if k_norm is None else k_norm.data_ptr(), eps,
-                                0.0 if rope_theta is None else rope_theta, positions.data_ptr(), requests.data_ptr(),
-                                table, kv, out.data_ptr(), stream))
+    check(lib().tf_paged_append(qkv.data_ptr(), qkv.stride(0) if rows > 1 else width, rows, heads, _act(qkv), qn, kn,
+                                eps, rope_theta or 0.0, positions.data_ptr(), requests.data_ptr(),
+                                _page_table(page_table), kv, out.data_ptr(), stream))
     return out
 
 
@@ -568,8 +570,8 @@ class PagedPlan:
         if len(kv_lengths) != n:
             raise ValueError("paged plan: new_lengths and kv_lengths differ in length")
         new_lengths, kv_lengths = [int(x) for x in new_lengths], [int(x) for x in kv_lengths]
-        if n and max(max(new_lengths), max(kv_lengths)) >= 1 << 31:  # would wrap on the way to C
-            raise ValueError("paged plan: a length is above 2^31")
+        if any(not -(1 << 31) <= x < 1 << 31 for x in new_lengths + kv_lengths):  # would wrap on the way to C
+            raise ValueError("paged plan: a length does not fit 32 bits")
         new, kv = (C.c_int32 * n)(*new_lengths), (C.c_int32 * n)(*kv_lengths)
         self.desc = d = PagedPlanDesc()
         guess = 65536 + 64 * n * max(kv_heads, 1) + 16 * max(sum(new_lengths), 0)
@@ -585,19 +587,24 @@ class PagedPlan:
         self.table = host[:d.table_bytes].to(device, non_blocking=True)
         self.workspace = torch.empty(max(d.workspace_bytes, 1), dtype=torch.uint8, device=device)
         stream = torch.cuda.current_stream(device)
-        self._made_on = stream.cuda_stream
+        self.made_on = stream.cuda_stream
         self._ready = stream.record_event()
-        self.rows, self.heads, self.head_dim = d.rows, heads, head_dim
+        self.shape = (d.rows, heads, head_dim)  # of q
+        self.rows = d.rows
+        self.table_ptr, self.workspace_ptr = self.table.data_ptr(), self.workspace.data_ptr()
+        self.workspace_bytes = d.workspace_bytes
         at, size = d.positions_offset, 4 * d.rows
         self.positions = self.table[at:at + size].view(torch.int32)
         at = d.requests_offset
         self.requests = self.table[at:at + size].view(torch.int32)
 
-    def _on(self, handle: int):
-        """Orders the plan's upload before work on another stream and keeps its memory until that work is done.
-        A capturing stream cannot wait for an event from outside; a graph's first replay comes after the
-        synchronization that opens its capture, and its owner keeps the plan."""
-        if handle != self._made_on and not torch.cuda.is_current_stream_capturing():
+    def order(self, handle: int):
+        """Orders the plan's upload before work on another stream (the current
+        one, of this handle) and keeps its memory until that work is done.  A
+        capturing stream cannot wait for an event from outside; a graph's first
+        replay comes after the synchronization that opens its capture, and its
+        owner keeps the plan."""
+        if handle != self.made_on and not torch.cuda.is_current_stream_capturing():
             stream = torch.cuda.current_stream()
             stream.wait_event(self._ready)
             self.table.record_stream(stream)
@@ -611,21 +618,22 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Ten
     key heads in groups.  q: [rows, heads, head_dim] (rows may be strided);
     returns [rows, heads, head_dim].  Rows that attend nothing give zeros."""
     stream = _launch_stream(q, k_pages, v_pages, page_table, plan.table, out)
-    rows, heads, D = plan.rows, plan.heads, plan.head_dim
-    if q.shape != (rows, heads, D):
+    shape = plan.shape
+    if q.shape != shape:
         raise ValueError("paged_attention: q is [rows, heads, head_dim] of the plan")
-    if q.stride()[1:] != (D, 1):
-        q = q.contiguous()
-    q = _rows16(q, heads * D)
+    rows, heads, D = shape
+    width = heads * D
+    q = _rows16(q if q.stride()[1:] == (D, 1) else q.contiguous(), width)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != (rows, heads, D) or out.dtype != q.dtype or not out.is_contiguous():
+    elif out.shape != shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("paged_attention: out is a contiguous [rows, heads, head_dim] of q's dtype")
-    plan._on(stream)
-    check(lib().tf_paged_attention(q.data_ptr(), q.stride(0) if rows > 1 else heads * D, _page_table(page_table),
-                                   _paged_kv(k_pages, v_pages), plan.desc, plan.table.data_ptr(),
+    if stream != plan.made_on:
+        plan.order(stream)
+    check(lib().tf_paged_attention(q.data_ptr(), q.stride(0) if rows > 1 else width, _page_table(page_table),
+                                   _paged_kv(k_pages, v_pages), plan.desc, plan.table_ptr,
                                    D ** -0.5 if scale is None else scale, _act(q), out.data_ptr(),
-                                   plan.workspace.data_ptr(), plan.desc.workspace_bytes, stream))
+                                   plan.workspace_ptr, plan.workspace_bytes, stream))
     return out
 
 
