@@ -23,6 +23,12 @@
 //
 // fp32 throughout, one rounding at the end: the rotated k is rounded straight
 // to the cache's type.
+//
+// Measured: 16384 rows of 16 + 2 x 16 heads of 128 with norms and rotation 85 us,
+// 4.8 TB/s (without either 70: the latency of a block's one pass, not the
+// arithmetic, is what is left); 64 rows 4.6 us.  At most 64 registers a thread:
+// four blocks an SM instead of three, 97 -> 88 us; 16 or 64 values a thread
+// instead of 32 gave 114 and 86.
 #include <math.h>
 #include <string.h>
 
