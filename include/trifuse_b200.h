@@ -433,8 +433,9 @@ int tf_paged_plan_make(const int32_t* new_lengths, const int32_t* kv_lengths, in
  * aligned.  The cache has
  * the activations' dtype, or f16 under bf16 activations (q is then rounded to
  * f16).  A row that attends nothing, or whose every score is -inf, gives
- * zeros; NaN and +inf scores give NaN.  Slots past a request's length are
- * never used, whatever they hold.  plan_table is the device copy of the
+ * zeros; NaN and +inf scores give NaN.  A value that is not finite reaches
+ * only the rows that see its token.  Slots past a request's length are never
+ * used, whatever they hold.  plan_table is the device copy of the
  * table; calls that overlap in time need tables and workspaces of their own
  * (the kernels count arrivals in the table and leave it as they found it).
  * Replaces the SDPA of MLXNativeGraniteMoEPrefill.h:471-483 for a paged

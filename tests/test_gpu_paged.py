@@ -182,6 +182,33 @@ def test_nan_and_infinite_scores(ops, n):
             check(clean, want, big, F16)
 
 
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("H,Hk,D,n,L", [(4, 4, 64, 2, 2), (4, 4, 128, 16, 700), (6, 2, 128, 5, 333), (8, 2, 64, 4, 5000),
+                                        (4, 2, 128, 40, 700), (2, 2, 64, 128, 9000), (4, 4, 128, 300, 300),
+                                        (4, 1, 128, 150, 6000), (3, 3, 64, 513, 900)])
+def test_masked_values_that_are_not_finite(ops, act, cache, H, Hk, D, n, L):
+    """A NaN or infinite value reaches the rows that see its token, in its column of its key head, and
+    nothing else changes by a bit."""
+    G, page = H // Hk, 16
+    k, v, table = make_cache([L, L], Hk, D, page, cache)
+    q = torch.randn(2 * n, H, D, generator=torch.Generator().manual_seed(3)).to(act).cuda()
+    plan = ops.PagedPlan([n, n], [L, L], H, Hk, D, page)
+    spots = [(0, L - 1, float("nan"), 0, 1), (0, L - 1 - n // 3, float("inf"), Hk - 1, D - 1),
+             (1, L - 1 - n // 2, -float("inf"), 0, D // 2 + 3), (1, L - n, float("nan"), Hk - 1, 7)]
+    for r, t, _, h, d in spots:
+        v[table[r, t // page].long(), h, t % page, d] = 0
+    clean = ops.paged_attention(q, k, v, table, plan)
+    hit = torch.zeros_like(clean, dtype=torch.bool)
+    for r, t, bad, h, d in spots:
+        v[table[r, t // page].long(), h, t % page, d] = bad
+        first = n * r + t - (L - n)
+        hit[first:n * (r + 1), h * G:(h + 1) * G, d] = True
+    got = ops.paged_attention(q, k, v, table, plan)
+    assert ops.device_error() == 0
+    assert torch.isfinite(clean).all() and not torch.isfinite(got[hit]).any()
+    assert torch.equal(got[~hit], clean[~hit])
+
+
 @pytest.mark.parametrize("n", [1, 200])
 def test_every_score_minus_infinity(ops, n):
     k, v, table = make_cache([n], 2, 64, 16, BF16)

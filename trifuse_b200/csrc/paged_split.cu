@@ -38,6 +38,7 @@
 
 #include "common.cuh"
 #include "paged.h"
+#include "paged_values.cuh"
 #include "tc_ptx.cuh"
 
 namespace tf {
@@ -399,6 +400,43 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
             *reinterpret_cast<uint4*>(v + key_at(i >> 3) + h * half_bytes + 16 * (i & 7)) = make_uint4(0, 0, 0, 0);
         __syncwarp();
       }
+      // Keys that some row does not see, with values that are not finite.
+      const int hidden = max(first_limit + 1 - key0, 0), hidden_end = min(have, kSplitKeys);
+      bool cleared = false;
+      if (hidden < hidden_end) {
+        uint8_t* v = ring + slot * 2 * S::kTile + S::kTile;
+        // A box's keys of one column half lie side by side.
+        for (int key = hidden; key < hidden_end;) {
+          const int next = min((key | (p.box_rows - 1)) + 1, hidden_end);
+#pragma unroll
+          for (int h = 0; h < S::kHalves; ++h)
+            cleared |= !all_finite<C>(v + key_at(key) + h * half_bytes, (next - key) * 8, lane);
+          key = next;
+        }
+        if (cleared) {
+#pragma unroll 1
+          for (int key = hidden; key < hidden_end; ++key)
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const int dim = (16 * d + 8 * half + g) & 63;
+                const C c = *reinterpret_cast<const C*>(v + key_at(key) + (d >> 2) * half_bytes +
+                                                        (((dim >> 3) ^ (key & 7)) << 4) + 2 * (dim & 7));
+                if (!not_finite(c)) continue;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                  for (int i = 0; i < 2; ++i)
+                    if (key0 + key <= limit[t][i]) o[d][t][2 * half + i] += to_f(c);
+              }
+          __syncwarp();
+          for (int key = hidden; key < hidden_end; ++key)
+#pragma unroll
+            for (int h = 0; h < S::kHalves; ++h) clear_not_finite<C>(v + key_at(key) + h * half_bytes, 8, lane);
+          __syncwarp();
+        }
+      }
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
 #pragma unroll
@@ -412,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
       }
       // Every lane's shared loads fed an MMA above, so they have returned: the
       // slot may be refilled.  Zeros written above precede the copy.
-      if (have < kSplitKeys) fence_proxy_async();
+      if (have < kSplitKeys || cleared) fence_proxy_async();
       __syncwarp();
       ++used;
       if (more) fetch();

@@ -55,14 +55,16 @@
 //
 // Measured: 2048 tokens after 14336 (32 query and 8 key heads of 128) 444 us,
 // 1.16 PFLOP/s, tensor pipe 64% at the 1.58 GHz that the power cap leaves; 8
-// prompts of 2048 tokens (16 heads) 163 us, 0.84 PFLOP/s (segments of 9 tiles on
-// average, whose ends cost 5600 clocks each).
+// prompts of 2048 tokens (16 heads) 168 us, 0.82 PFLOP/s (segments of 9 tiles on
+// average, whose ends cost 5600 clocks each; 163 us without looking the causal
+// edge's values through, paged_values.cuh).
 #include <cuda.h>
 #include <math.h>
 #include <string.h>
 
 #include "common.cuh"
 #include "paged.h"
+#include "paged_values.cuh"
 #include "tc_ptx.cuh"
 
 namespace tf {
@@ -104,6 +106,8 @@ struct TileParams {
   int32_t page_size, page_shift;
   int32_t box_rows;  // min(page_size, kTileKeys)
   int32_t group, heads;
+  const void* v;  // the value pages, for values that are not finite
+  int64_t pages, page_stride;
   const PagedSegment* segments;
   const int32_t* starts;
   float* stat;  // [part][2][rows of a block]: m, l
@@ -116,6 +120,7 @@ struct TileParams {
 
 struct Control {
   volatile int abort;
+  volatile int cleared;  // the block has cleared values that are not finite
   long long limit;
 };
 
@@ -270,6 +275,35 @@ struct View {
   }
 };
 
+// Adds to a row's stored result (or piece of one, `pitch` rows apart) the
+// values that are not finite, of the keys that it sees: a product may have had
+// zeros in their place.  Such keys lie past what the segment's first row sees.
+template <typename T, typename C, int D>
+__device__ __forceinline__ void add_cleared(const TileParams& p, const PagedSegment& g, int limit, T* out, float* part,
+                                         int pitch) {
+  const int begin = max(g.kv_len - g.new_len + g.row0 / p.group + 1, g.tile0 * kTileKeys);
+  const int end = min(min(limit + 1, g.kv_len), g.tile1 * kTileKeys);
+  for (int key = begin; key < end; ++key) {
+    const int column = key >> p.page_shift;
+    const int64_t page = column < p.columns ? p.ids[g.request * p.ids_stride + column] : -1;
+    if (page < 0 || page >= p.pages) continue;
+    const C* v = static_cast<const C*>(p.v) + page * p.page_stride +
+                 (int64_t)(g.kv_head * p.page_size + (key & (p.page_size - 1))) * D;
+    for (int c = 0; c < D; c += 8) {
+      const uint4 eight = ld_v4(v + c);
+      const C* value = reinterpret_cast<const C*>(&eight);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (not_finite(value[k])) {
+          if (out)
+            out[c + k] = from_f<T>(to_f(out[c + k]) + to_f(value[k]));
+          else
+            part[(c + k) / 4 * 4 * pitch + (c + k) % 4] += to_f(value[k]);
+        }
+    }
+  }
+}
+
 template <typename T, typename C, int D, int H>
 __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
     paged_tile_kernel(const __grid_constant__ TileParams p) {
@@ -280,7 +314,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
   uint64_t* q_full = bars;       // [2] 128 threads: the half's query rows are written
   uint64_t* s_full = bars + 2;   // [2] MMA: scores of a tile
   uint64_t* p_full = bars + 4;   // [2][2] 128 threads: a part of P written (before the first, O rescaled)
-  uint64_t* o_full = bars + 8;   // [2] MMA: a segment's last product
+  uint64_t* o_full = bars + 8;   // [2] MMA, and the warp that issues it: a segment's last product
   uint64_t* o_free = bars + 10;  // [2] 128 threads: O read
   uint64_t* kv_full = bars + 12;             // [slots] TMA
   uint64_t* kv_empty = kv_full + S::kSlots;  // [slots] each half: its products of the tile done
@@ -298,7 +332,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
       mbar_init(&s_full[x], 1);
       mbar_init(&p_full[2 * x], kHalf);
       mbar_init(&p_full[2 * x + 1], kHalf);
-      mbar_init(&o_full[x], 1);
+      mbar_init(&o_full[x], 2);
       mbar_init(&o_free[x], kHalf);
       mbar_init(&done[x], 1);
       mbar_init(&baton[x], 1);
@@ -308,6 +342,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
       mbar_init(&kv_empty[i], H);
     }
     ctl->abort = 0;
+    ctl->cleared = 0;
     ctl->limit = *p.wait_cycles;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -402,6 +437,8 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
           tc_fence_after();
           scores(n);
         }
+        // First key, from the segment's first, that not all rows of the half see.
+        const int hidden0 = g.kv_len - g.new_len + (g.row0 + kHalf * x) / p.group + 1 - g.tile0 * kTileKeys;
         const int both = H == 2 ? min(count, view.count[(1 - x) & (H - 1)]) : 0;  // tiles that both halves meet
         for (int j = 0; j < count && ok; ++j) {
           // Ring: K of tile j at n, V of tile j, K of tile j + 1.
@@ -420,6 +457,24 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
                 *reinterpret_cast<uint4*>(vt + h * kColBytes + 16 * i) = make_uint4(0, 0, 0, 0);
             fence_proxy_async();
             __syncwarp();
+          }
+          // Keys that some row of the half does not see, with values that are
+          // not finite (the other half may read them cleared as well).
+          const int hidden = max(hidden0 - j * kTileKeys, 0);
+          const int chunks = (min(have, kTileKeys) - hidden) * 8;  // of a column half
+          if (chunks > 0) {
+            uint8_t* first = vt + hidden * 128;
+            bool finite = true;
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) finite &= all_finite<C>(first + h * kColBytes, chunks, lane);
+            if (!finite) {
+              if (lane == 0) ctl->cleared = 1;
+              __threadfence_block();
+#pragma unroll
+              for (int h = 0; h < D / 64; ++h) clear_not_finite<C>(first + h * kColBytes, chunks, lane);
+              fence_proxy_async();
+              __syncwarp();
+            }
           }
           // O still holds the half's last segment until it has been read.
           if (j == 0 && o_turn++ > 0 && !(ok = wait_warp(&o_free[x], o_turn & 1, ctl, err, 86))) break;
@@ -444,6 +499,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
             scores(n + 2);
           } else {
             mma_commit(leader, &o_full[x]);
+            if (lane == 0) mbar_arrive(&o_full[x]);
           }
           if (lane == 0 && (x == 0 ? j < both : j + 1 < both)) mbar_arrive(&baton[1 - x]);
           n += 2;
@@ -608,6 +664,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
         ++o_turn;
         tc_fence_after();
       }
+      const bool cleared = ctl->cleared != 0;
       // A row that has seen no key above -inf gives zeros.
       const float inv = m == -INFINITY ? 0.f : 1.f / l;
       T* orow = static_cast<T*>(p.out) +
@@ -637,6 +694,11 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
             *reinterpret_cast<float4*>(prow + (c + i) * S::kRows) =
                 make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
+      }
+      if (cleared) {
+        if (mine && m != -INFINITY)
+          add_cleared<T, C, D>(p, g, limit, g.part < 0 ? orow : nullptr, prow, S::kRows);
+        __syncwarp();
       }
       if (mine && g.part >= 0) {
         p.stat[(int64_t)g.part * 2 * S::kRows + row] = m;
@@ -782,6 +844,9 @@ tf_status launch_paged_tile(const PagedArgs& a, cudaStream_t s) {
   while ((1 << p.page_shift) < a.kv.page_size) ++p.page_shift;
   p.group = plan.heads / plan.kv_heads;
   p.heads = plan.heads;
+  p.v = a.kv.v;
+  p.pages = a.kv.pages;
+  p.page_stride = a.kv.page_stride;
   p.out = a.out;
   p.scale_log2 = a.scale * kLog2e;
   TF_TRY(tc_flags(&p.err, const_cast<long long**>(&p.wait_cycles)));
