@@ -24,11 +24,13 @@
 // fp32 throughout, one rounding at the end: the rotated k is rounded straight
 // to the cache's type.
 //
-// Measured: 16384 rows of 16 + 2 x 16 heads of 128 with norms and rotation 85 us,
-// 4.8 TB/s (without either 70: the latency of a block's one pass, not the
-// arithmetic, is what is left); 64 rows 4.6 us.  At most 64 registers a thread:
-// four blocks an SM instead of three, 97 -> 88 us; 16 or 64 values a thread
-// instead of 32 gave 114 and 86.
+// Measured, L2 flushed: 16384 rows of 16 + 2 x 16 heads of 128 with norms and
+// rotation 82 us, 4.9 TB/s (without either 70: the latency of a block's one
+// pass, not the arithmetic, is what is left); 64 rows 3.9 us in a warm L2.  At
+// most 64 registers a thread: 82 us, without the cap 86 to 90; blocks of 4
+// warps where a row's parts fit them: 84 us, of 8 86, of 16 96; the norm
+// weights fetched before the sum is known: 84 -> 82; 64 values a thread instead
+// of 32: 92 against 88.
 #include <math.h>
 #include <string.h>
 
@@ -149,6 +151,14 @@ __global__ void __launch_bounds__(512, 2) paged_append_kernel(const __grid_const
   }
   const __half* norm = part == 0 ? p.q_norm : part == 1 ? p.k_norm : nullptr;
   const bool rotate = p.rotate && part < 2;
+  uint4 weight[kPairs][2];  // on their way during the angles and the sum
+  if (norm) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (head0 + step * i < heads) weight[i][j] = ld_v4(norm + (head0 + step * i) * D + j * (D / 2) + 8 * at);
+  }
   if (rotate) {
     for (int i = tid; i < units * (D / 2); i += (int)blockDim.x) {
       const int64_t r = (int64_t)block * units + i / (D / 2);
@@ -200,7 +210,7 @@ __global__ void __launch_bounds__(512, 2) paged_append_kernel(const __grid_const
       unpack4<T>(raw[i][j], f[j]);
       if (norm) {
         float2 w[4];
-        unpack4<__half>(ld_v4(norm + h * D + j * (D / 2) + 8 * at), w);
+        unpack4<__half>(weight[i][j], w);
 #pragma unroll
         for (int k = 0; k < 4; ++k) f[j][k] = mul2(mul2(f[j][k], scale), w[k]);
       }
@@ -267,7 +277,7 @@ tf_status launch_paged_append(const AppendArgs& a, cudaStream_t s) {
   while ((1 << p.page_shift) < a.kv.page_size) ++p.page_shift;
   p.q_shift = unit_shift(a.heads * D);
   p.kv_shift = unit_shift(a.kv.kv_heads * D);
-  const int warps = p.q_shift > 3 ? 1 << p.q_shift : 8;  // per block
+  const int warps = p.q_shift > 2 ? 1 << p.q_shift : 4;  // per block
   const int q_rows = warps >> p.q_shift, kv_rows = warps >> p.kv_shift;
   const int64_t qb = (a.rows + q_rows - 1) / q_rows;
   const int64_t kb = (a.rows + kv_rows - 1) / kv_rows;
