@@ -103,6 +103,25 @@ def test_orders(ops, dtype, make):
         check(ops, x, t, top)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("make", ["rising", "falling", "equal", "steps", "few threads", "late rise", "rising, with NaN"])
+@pytest.mark.parametrize("rows", [20, 160])
+def test_orders_of_long_rows(ops, dtype, make, rows):
+    """Many candidates past the first tiles, where rows are shared by a cluster and where they are not."""
+    V = 60001
+    i = torch.arange(V, dtype=F32)
+    noise = torch.randn(V, generator=torch.Generator().manual_seed(1))
+    own = (i // (4 if dtype == F32 else 8)) % 128
+    x = {"rising": i / 1000, "falling": -i / 1000, "equal": torch.zeros(V), "steps": (i // 9000) / 8,
+         "few threads": torch.where((own > 2) & (own < 10), 10 + i / 4096, noise),
+         "late rise": torch.where(i < 40000, noise, 5 + i / 8192),
+         "rising, with NaN": torch.where(i % 6007 == 5, math.nan, i / 1000)}[make]
+    x = x.repeat(rows, 1).to(dtype).cuda()
+    t = (torch.arange(rows, device="cuda") * 977) % V
+    for top in (1, 5, 20, 64):
+        check(ops, x, t, top)
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("V", [40, 5000, 50304])
 def test_infinities_and_nan(ops, dtype, V):

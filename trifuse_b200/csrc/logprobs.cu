@@ -20,24 +20,27 @@
 // the lowest index.  The first tile yields a lower bound of the k-th key (the
 // k-th largest of the warps' few largest thread maxima: k entries are at or
 // above it).  A thread whose maximum of a tile meets the bound queues the tile
-// and goes on; after 1, 2, 4, ... tiles the block looks through the queue (the
-// vectors come again, from L2), puts entries at or above the bound into a
-// buffer, and prunes that to its k best, which raises the bound to an exact
-// one.  (Looking through the vectors on the spot cost some 4000 clocks each
-// time: a hundred instructions that are rare enough to be fetched from memory.)
-// After the first tile few threads meet the bound, so the pass stays a stream.
-// Should queue or buffer run over (values in rising order, say), the entries
-// since the last prune come again in rounds of one a thread, with a prune in
-// between.
+// and goes on; after 1, 2, 4, ... tiles (for few alternatives from 4 on) the
+// block looks through the queue (the vectors come again, from L2), puts entries
+// at or above the bound into a buffer, and prunes that to its k best, which
+// raises the bound to an exact one.  (Looking through the vectors on the spot
+// cost some 4000 clocks each time: a hundred instructions that are rare enough
+// to be fetched from memory.)  After the first tile few threads meet the bound,
+// so the pass stays a stream.  Should queue or buffer run over (values in
+// rising order, say, or equal ones), the vectors since the last prune come
+// again: for a better bound, the k-th largest of the threads' best vectors,
+// then for what lies at or above it; and if the buffer runs over even so, in
+// rounds of one entry a thread with a prune in between.
 //
 // A row may be shared by a cluster of 1, 2, 4 or 8 blocks (few rows: the whole
 // GPU reads; one row of 50304 on one block would take its load latency 25
 // times over); the blocks' sums and candidates meet in the first block's hands
 // over distributed shared memory, so no scratch in device memory is needed.
 //
-// Measured: 4095 rows of 50304 bf16 logits 135 us with five alternatives (3.1
-// TB/s) and 92 with none (4.5 TB/s); 2048 rows of fp32 with twenty 108 us (3.8
-// TB/s); one row 10.8 us, 64 rows 13.
+// Measured: 4095 rows of 50304 bf16 logits 117 us with five alternatives (3.5
+// TB/s) and 92 with none (4.5 TB/s); 2048 rows of fp32 with twenty 94 us (4.4
+// TB/s), in rising order 500 (in rounds alone 9450); one row 10.5 us, 64 rows
+// 12.5.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -317,15 +320,17 @@ struct Gather {
 template <int W>
 struct Shared {
   // Two rounds of the block's threads, the cluster's join, and room for what a
-  // first tile offers (64 alternatives: 320 places ran over, 308 us against 252).
-  static constexpr int kBuffer = 512;
-  static_assert(kBuffer >= 64 * W && kBuffer >= kMaxCluster * kMaxTop, "candidates");
+  // first tile offers (64 alternatives: 320 places ran over, 308 us against 252),
+  // or 64 vectors of 8 values beside the kept ones (values in rising order).
+  static constexpr int kBuffer = 640;
+  static_assert(kBuffer >= 64 * W && kBuffer - 32 * W >= kMaxTop && kBuffer >= kMaxCluster * kMaxTop, "candidates");
   uint64_t full[kStages], empty[kStages];
   uint64_t buffer[kBuffer];
   int queue[kQueue];  // tiles of threads (their first vector) that met the bound since the last look
   int queued;
   uint64_t best[kMaxTop];      // sorted k best of the last prune
   int n;                       // candidates in the buffer
+  uint64_t rough;              // the k-th largest of the threads' best vectors
   uint32_t warp_key[kMaxTop];  // the warps' largest thread maxima of the first tile
   Sums sums[W];                // the warps' totals
   int before[W];
@@ -502,8 +507,36 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
       over = sh.n > S::kBuffer;
     }
     if (over) {
-      // The vectors since the last prune again, kThreads entries at a time
-      // from memory.
+      // The vectors since the last prune again, against a better bound.  A
+      // vector's maximum is an entry at or above (maximum, last index); the
+      // k-th largest of the threads' best vectors is below k entries.
+      __syncthreads();
+      uint64_t own = 0;
+#pragma unroll 1
+      for (int v = group + tid; v < to; v += kThreads) {
+        const int e0 = v * kPer - head;
+        own = max(own, composite(L::max_of(ld_v4(x + e0)), (uint32_t)(e0 + kPer - 1)));
+      }
+      uint64_t* keys = sh.buffer + (S::kBuffer - kThreads);  // past the kept ones
+      keys[tid] = own;
+      if (tid == 0) sh.n = kept;
+      __syncthreads();
+      int ahead = 0;
+#pragma unroll 8
+      for (int i = 0; i < kThreads; ++i) {
+        const uint64_t other = keys[i];
+        ahead += other > own || (other == own && i < tid);
+      }
+      if (ahead == k - 1) sh.rough = own;
+      __syncthreads();
+      set_bound(max(bound, sh.rough));
+#pragma unroll 1
+      for (int v = group + tid; v < to; v += kThreads) offer(ld_v4(x + (v * kPer - head)), v * kPer - head);
+      __syncthreads();
+      over = sh.n > S::kBuffer;
+    }
+    if (over) {
+      // Still too many (some threads' own): kThreads entries at a time.
       __syncthreads();
       if (tid == 0) sh.n = kept;
       __syncthreads();
@@ -537,6 +570,11 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
     }
   };
 
+  // With few alternatives the first tile's rough bound serves for a while: 4095
+  // rows of bf16 with 5 alternatives 121.5 us looking at once, 117.1 after two
+  // tiles, 116.3 after four; 20: 141.6, 134.2, 136.2; 64: 241, 248, 484 (the
+  // buffer runs over).
+  const int first_look = k <= 8 ? 4 : k <= 24 ? 2 : 1;
   for (int tile = 0; tile < tiles; ++tile) {
     const int t0 = v_begin + tile * kTile, slot = tile % kStages;
     const uint4* src = reinterpret_cast<const uint4*>(ring + slot * (kTile * 16)) + tid;
@@ -630,8 +668,10 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
       const int at = atomicAdd(&sh.queued, 1);
       if (at < kQueue) sh.queue[at] = t0 + tid;
     }
-    // After 1, 2, 4, 8, ... tiles: each group adds about k candidates.
-    if ((tile & (tile + 1)) == 0 || tile + 1 == tiles) look(min(v_end, t0 + kTile), tile == 0);
+    // After 1, 2, 4, 8, ... tiles, from first_look on: each group adds about k
+    // candidates.
+    if (((tile & (tile + 1)) == 0 && tile + 1 >= first_look) || tile + 1 == tiles)
+      look(min(v_end, t0 + kTile), group == v_begin);
   }
   if (edges) {
     // Thread 0 takes the row's first ragged vector, thread 1 its last.
