@@ -37,10 +37,10 @@
 // times over); the blocks' sums and candidates meet in the first block's hands
 // over distributed shared memory, so no scratch in device memory is needed.
 //
-// Measured: 4095 rows of 50304 bf16 logits 117 us with five alternatives (3.5
-// TB/s) and 92 with none (4.5 TB/s); 2048 rows of fp32 with twenty 94 us (4.4
-// TB/s), in rising order 500 (in rounds alone 9450); one row 10.5 us, 64 rows
-// 12.5.
+// Measured: 4095 rows of 50304 bf16 logits with five alternatives 133 us (3.1
+// TB/s; 117 where the given token is the largest, so that nothing is counted)
+// and 92 with none (4.5 TB/s); 2048 rows of fp32 with twenty 94 us (4.4 TB/s),
+// in rising order 500 (in rounds alone 9450); one row 10.5 us, 64 rows 12.5.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -571,9 +571,9 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
   };
 
   // With few alternatives the first tile's rough bound serves for a while: 4095
-  // rows of bf16 with 5 alternatives 121.5 us looking at once, 117.1 after two
-  // tiles, 116.3 after four; 20: 141.6, 134.2, 136.2; 64: 241, 248, 484 (the
-  // buffer runs over).
+  // rows of bf16, the largest token given, with 5 alternatives 121.5 us looking
+  // at once, 117.1 after two tiles, 116.3 after four; with 20 141.6, 134.2 and
+  // 136.2; with 64 241, 248 and 484 (the buffer runs over).
   const int first_look = k <= 8 ? 4 : k <= 24 ? 2 : 1;
   for (int tile = 0; tile < tiles; ++tile) {
     const int t0 = v_begin + tile * kTile, slot = tile % kStages;
