@@ -40,3 +40,27 @@ def test_clusters_on_a_busy_gpu(rows, dtype):
             for u, v in zip(want, r):
                 assert torch.equal(u, v)
     assert ops.device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,V", [(3, 50304), (200, 50304), (200, 9001), (1, 250001)])
+def test_expired_waits_are_told_and_do_no_harm(rows, V):
+    """With a wait limit of one cycle the waits for the copies run out: the error code is left, and the results are
+    those of the whole rows all the same, since no slot is read or refilled before its copy has landed."""
+    from trifuse_b200 import ops
+    from trifuse_b200._lib import check, lib
+    g = torch.Generator().manual_seed(V)
+    x = (torch.randn(rows, V, generator=g) * 2.5).cuda()
+    t = torch.randint(0, V, (rows,), generator=g).cuda()
+    want = ops.token_logprobs(x, t, top=20)
+    assert ops.device_error() == 0
+    check(lib().tf_set_wait_limit(1))
+    try:
+        got = ops.token_logprobs(x, t, top=20)
+        assert ops.device_error() in (0, 72)
+    finally:
+        check(lib().tf_set_wait_limit(0))
+    for u, v in zip(want, got):
+        assert torch.equal(u, v)
+    ops.token_logprobs(x, t, top=20)
+    assert ops.device_error() == 0

@@ -328,6 +328,7 @@ struct Shared {
   uint64_t buffer[kBuffer];
   int queue[kQueue];  // tiles of threads (their first vector) that met the bound since the last look
   int queued;
+  int stalled;                 // a copy that never came
   uint64_t best[kMaxTop];      // sorted k best of the last prune
   int n;                       // candidates in the buffer
   uint64_t rough;              // the k-th largest of the threads' best vectors
@@ -393,14 +394,22 @@ __device__ __forceinline__ void copy_bulk(void* dst, const void* src, uint32_t b
       : "memory");
 }
 
-// Waits for a slot's phase; after about a second (which only a stalled copy
-// could take) records an error code and goes on with what the slot holds.
-__device__ __forceinline__ void wait_slot(uint64_t* bar, uint32_t parity, const LogprobParams& p) {
-  if (tc::mbar_try(bar, parity)) return;
+// Waits for a slot's phase.  Past `limit` (about a second, which only a stalled
+// copy could take; a shortened limit polls) an error code is recorded, and the
+// wait goes on: a slot must not be read, refilled or left behind by the block
+// while its copy is in flight.  The copies always complete; were one not to, the
+// second wait ends as well, and the block neither waits nor copies any more.
+__device__ __forceinline__ void wait_slot(uint64_t* bar, uint32_t parity, long long limit, int* err,
+                                          volatile int* stalled) {
+  const uint32_t suspend = limit < 2000000000LL ? 0u : tc::kSuspendNs;
+  if (tc::mbar_try(bar, parity, suspend)) return;
   const long long t0 = clock64();
-  while (!tc::mbar_try(bar, parity))
-    if (clock64() - t0 > *p.wait_cycles) {
-      atomicCAS(p.err, 0, 72);
+  while (!tc::mbar_try(bar, parity, suspend))
+    if (clock64() - t0 > limit) {
+      atomicCAS(err, 0, 72);
+      const long long t1 = clock64();
+      while (!*stalled && !tc::mbar_try(bar, parity))
+        if (clock64() - t1 > 2000000000LL) *stalled = 1;
       return;
     }
 }
@@ -439,6 +448,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.n = 0;
     sh.queued = 0;
+    sh.stalled = 0;
   }
   // The first block's shared memory may be written once every block of the
   // cluster is known to run: announced here, waited for before the push.
@@ -453,6 +463,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
   if (tid == 0)
     for (int i = 0; i < kStages && i < tiles; ++i) fetch(i);
 
+  const long long limit = *p.wait_cycles;
   const int64_t token64 = p.tokens[row];
   const bool given = token64 >= 0 && token64 < V;
   const int token = given ? (int)token64 : -1;
@@ -582,7 +593,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
     const int t0 = v_begin + tile * kTile, slot = tile % kStages;
     const uint4* src = reinterpret_cast<const uint4*>(ring + slot * (kTile * 16)) + tid;
     const bool full = t0 + kTile <= v_end;
-    wait_slot(&sh.full[slot], (uint32_t)((tile / kStages) & 1), p);
+    wait_slot(&sh.full[slot], (uint32_t)((tile / kStages) & 1), limit, p.err, &sh.stalled);
     uint4 r[kVectors];
 #pragma unroll
     for (int i = 0; i < kVectors; ++i)
@@ -597,8 +608,8 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(&sh.empty[slot]);
     if (tid == 0 && tile + kStages < tiles) {
-      wait_slot(&sh.empty[slot], (uint32_t)((tile / kStages) & 1), p);
-      fetch(tile + kStages);
+      wait_slot(&sh.empty[slot], (uint32_t)((tile / kStages) & 1), limit, p.err, &sh.stalled);
+      if (!sh.stalled) fetch(tile + kStages);
     }
     if (full) {
       acc.add<T>(r, tmax);
