@@ -1,0 +1,28 @@
+"""What the paged operators' Python entries make of their arguments, as far as it shows without a GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+from trifuse_b200 import ops
+
+
+def read_back(desc):
+    """Page ids of a table's descriptor as the kernels would find them."""
+    return [[C.c_int32.from_address(desc.ids + 4 * (r * desc.stride + c)).value for c in range(desc.columns)]
+            for r in range(desc.requests)]
+
+
+@pytest.mark.parametrize("make", ["plain", "rows apart", "one row", "expanded", "overlapping", "one expanded row",
+                                  "every second row"])
+def test_page_table_rows_are_found_where_they_are(make):
+    base = torch.arange(100, 160, dtype=torch.int32)
+    table = {"plain": base[:21].view(3, 7), "rows apart": base[:40].view(4, 10)[:, 2:7], "one row": base[None, 3:9],
+             "expanded": base[None, :7].expand(5, 7), "overlapping": base.as_strided((4, 6), (2, 1)),
+             "one expanded row": base[None, :7].expand(1, 7), "every second row": base.view(6, 10)[::2]}[make]
+    desc = ops._page_table(table)
+    assert desc.stride >= desc.columns and (desc.requests, desc.columns) == tuple(table.shape)
+    held = desc.tensor.untyped_storage()
+    last = desc.ids + 4 * ((desc.requests - 1) * desc.stride + desc.columns)
+    assert held.data_ptr() <= desc.ids and last <= held.data_ptr() + held.nbytes(), "read past the storage"
+    assert read_back(desc) == table.tolist()

@@ -487,11 +487,19 @@ def _paged_kv(k_pages: Tensor, v_pages: Tensor) -> PagedKV:
 
 
 def _page_table(page_table: Tensor) -> PageTable:
+    """Descriptor of a page table; keep it until the launch (it may own a copy of the table)."""
     shape, stride = page_table.shape, page_table.stride()
     if len(shape) != 2 or page_table.dtype != torch.int32 or (shape[1] > 1 and stride[1] != 1):
         raise ValueError("paged: the page table is int32 [requests, pages] with contiguous rows")
     requests, columns = shape
-    return PageTable(page_table.data_ptr(), max(stride[0], columns), requests, columns)
+    step = stride[0]
+    if step < columns:  # of no meaning for one row; rows that share memory (an expanded row) are laid out apart
+        if requests > 1:
+            page_table = page_table.clone(memory_format=torch.contiguous_format)
+        step = columns
+    desc = PageTable(page_table.data_ptr(), step, requests, columns)
+    desc.tensor = page_table
+    return desc
 
 
 def _launch_stream(first: Tensor, *others) -> int:
