@@ -611,8 +611,9 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
           l *= factor;
         }
         // This tile's scores were issued after the last tile's product: O is
-        // stable, and P may overlay S.
-        if (j > 0 && __any_sync(0xffffffffu, factor != 1.f)) {
+        // stable, and P may overlay S.  (The vote is taken on the first tile too:
+        // it brings the warp together for the stores of P.)
+        if (__any_sync(0xffffffffu, factor != 1.f) && j > 0) {
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
             float o[32];
@@ -679,8 +680,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0.f;
         }
-        if (!mine) continue;
-        if (g.part < 0) {
+        if (mine && g.part < 0) {
 #pragma unroll
           for (int i = 0; i < 32; i += 16) {
             float f[16];
@@ -688,12 +688,13 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
             for (int k = 0; k < 16; ++k) f[k] = m == -INFINITY ? 0.f : o[i + k] * inv;
             store32(orow + c + i, pack8<T>(f), pack8<T>(f + 8));
           }
-        } else {
+        } else if (mine) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
             *reinterpret_cast<float4*>(prow + (c + i) * S::kRows) =
                 make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
+        __syncwarp();  // the next load takes the whole warp, also where the rows end inside it
       }
       if (cleared) {
         if (mine && m != -INFINITY)
