@@ -26,3 +26,18 @@ def test_page_table_rows_are_found_where_they_are(make):
     last = desc.ids + 4 * ((desc.requests - 1) * desc.stride + desc.columns)
     assert held.data_ptr() <= desc.ids and last <= held.data_ptr() + held.nbytes(), "read past the storage"
     assert read_back(desc) == table.tolist()
+
+
+def test_a_plans_vectors_are_ordered_where_they_are_asked_for(monkeypatch):
+    """positions and requests lie in the table that is still on its way: on another stream than the upload's they are
+    ordered after it, as paged_attention orders itself."""
+    plan = object.__new__(ops.PagedPlan)
+    plan.made_on, plan.device_index = 7, 0
+    plan._positions, plan._requests = torch.arange(3), torch.zeros(3)
+    ordered = []
+    monkeypatch.setattr(ops.PagedPlan, "order", lambda self, handle: ordered.append(handle))
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 7, raising=False)
+    assert plan.positions is plan._positions and plan.requests is plan._requests and not ordered
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 8, raising=False)
+    assert plan.positions is plan._positions and ordered == [8]
+    assert plan.requests is plan._requests and ordered == [8, 8]

@@ -568,9 +568,10 @@ class PagedPlan:
 
     new_lengths[i] query rows and kv_lengths[i] cached tokens (the new ones
     included) of request i, as sequences of ints.  ``positions`` and
-    ``requests`` are the rows' int32 device vectors for ``paged_append``.
-    The plan holds the calls' workspace, so calls that may run at the same
-    time (on several streams) need plans of their own."""
+    ``requests`` are the rows' int32 device vectors for ``paged_append``,
+    ordered after the plan's upload on the stream that is current when they are
+    asked for.  The plan holds the calls' workspace, so calls that may run at
+    the same time (on several streams) need plans of their own."""
 
     def __init__(self, new_lengths, kv_lengths, heads: int, kv_heads: int, head_dim: int, page_size: int,
                  device=None):
@@ -596,15 +597,30 @@ class PagedPlan:
         self.workspace = torch.empty(max(d.workspace_bytes, 1), dtype=torch.uint8, device=device)
         stream = torch.cuda.current_stream(device)
         self.made_on = stream.cuda_stream
+        self.device_index = self.table.get_device()
         self._ready = stream.record_event()
         self.shape = (d.rows, heads, head_dim)  # of q
         self.rows = d.rows
         self.table_ptr, self.workspace_ptr = self.table.data_ptr(), self.workspace.data_ptr()
         self.workspace_bytes = d.workspace_bytes
         at, size = d.positions_offset, 4 * d.rows
-        self.positions = self.table[at:at + size].view(torch.int32)
+        self._positions = self.table[at:at + size].view(torch.int32)
         at = d.requests_offset
-        self.requests = self.table[at:at + size].view(torch.int32)
+        self._requests = self.table[at:at + size].view(torch.int32)
+
+    def _here(self, vector: Tensor) -> Tensor:
+        handle = torch._C._cuda_getCurrentRawStream(self.device_index)
+        if handle != self.made_on:
+            self.order(handle)
+        return vector
+
+    @property
+    def positions(self) -> Tensor:
+        return self._here(self._positions)
+
+    @property
+    def requests(self) -> Tensor:
+        return self._here(self._requests)
 
     def order(self, handle: int):
         """Orders the plan's upload before work on another stream (the current
@@ -613,7 +629,7 @@ class PagedPlan:
         replay comes after the synchronization that opens its capture, and its
         owner keeps the plan."""
         if handle != self.made_on and not torch.cuda.is_current_stream_capturing():
-            stream = torch.cuda.current_stream()
+            stream = torch.cuda.current_stream(self.device_index)
             stream.wait_event(self._ready)
             self.table.record_stream(stream)
             self.workspace.record_stream(stream)
