@@ -41,3 +41,10 @@ def test_a_plans_vectors_are_ordered_where_they_are_asked_for(monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 8, raising=False)
     assert plan.positions is plan._positions and ordered == [8]
     assert plan.requests is plan._requests and ordered == [8, 8]
+
+
+def test_no_plan_is_made_inside_a_capture(monkeypatch):
+    """A captured upload would copy from a host buffer that other plans have since filled."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="captures a graph"):
+        ops.PagedPlan([1], [4], 4, 2, 64, 16)

@@ -581,6 +581,8 @@ class PagedPlan:
         new_lengths, kv_lengths = [int(x) for x in new_lengths], [int(x) for x in kv_lengths]
         if any(not -(1 << 31) <= x < 1 << 31 for x in new_lengths + kv_lengths):  # would wrap on the way to C
             raise ValueError("paged plan: a length does not fit 32 bits")
+        if torch.cuda.is_current_stream_capturing():  # a replay would read host memory that is long reused
+            raise RuntimeError("paged plan: made while the stream captures a graph; make it before the capture")
         new, kv = (C.c_int32 * n)(*new_lengths), (C.c_int32 * n)(*kv_lengths)
         self.desc = d = PagedPlanDesc()
         guess = 65536 + 64 * n * max(kv_heads, 1) + 16 * max(sum(new_lengths), 0)
