@@ -176,9 +176,9 @@ int tf_take_along_last(const void* x, int64_t rows, int32_t width, const int32_t
  * A token outside [0, vocab) gives logprob NaN and rank -1.  A row with a NaN
  * or +inf logit, or nothing but -inf, gives NaN everywhere, rank -1, and its
  * alternatives still in order (NaN last); single -inf logits have
- * probability 0, and a maximum beyond +-2.3e38 counts as infinite.  The rows
- * need no alignment beyond the element's.  The
- * reference's answers carry tokens only (patches/executorch.patch:1350-1353). */
+ * probability 0.  Finite logits may lie anywhere in their type's range (masks
+ * of its lowest value among them).  The rows need no alignment beyond the
+ * element's.  The reference's answers carry tokens only (patches/executorch.patch:1350-1353). */
 #define TF_MAX_TOP 64
 int tf_token_logprobs(const void* logits, int64_t row_stride, int64_t rows, int32_t vocab, int dtype,
                       const int64_t* tokens, int32_t top, float* logprob, float* entropy, int32_t* rank,

@@ -233,9 +233,16 @@ struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16, __nv_bfloat162> {
 // -m log2 e.  At x = m that leaves a residue of c's rounding in d, the same for
 // every x; total() takes it out again (exactly, where one entry holds all of
 // the sum).  m = -inf: nothing but -inf so far.
+//
+// Up to |m| = kFar the residue stays below 2^-3.  A thread that has met nothing
+// but a finite mask's values (-1e30, say) takes -kFar as its reference, which
+// serves unless the row ends up that low; rows whose maximum is further out
+// than kFar are summed again at the end, by far_sums().
+constexpr float kFar = 1048576.f;
+
 struct Sums {
   float m, s, w;
-  __device__ __forceinline__ static float offset(float m) { return -__fmul_rn(m, kLog2e); }
+  __device__ __forceinline__ static float offset(float m) { return -__fmul_rn(fmaxf(m, -kFar), kLog2e); }
   __device__ __forceinline__ void move(float to) {  // to >= m, or NaN
     if (m == -INFINITY) {
       m = to;
@@ -260,7 +267,7 @@ struct Sums {
   }
   // ln sum e^(x - m), and the entropy ln sum e^(x - m) - sum (x - m) p.
   __device__ __forceinline__ void total(float& log_sum, float& entropy) const {
-    const float residue = fmaf(m, kLog2e, offset(m));
+    const float residue = fabsf(m) > kFar ? 0.f : fmaf(m, kLog2e, offset(m));
     log_sum = logf(s / exp2_fast(residue));
     entropy = log_sum - (w / s - residue) * kLn2;
   }
@@ -308,6 +315,25 @@ struct Sums {
     s += a + b;
   }
 };
+
+// This thread's share of a row's sums relative to its maximum m, anywhere in the
+// type's range: x - m first (exact near m), so no residue; d is held above -150,
+// where 2^d is zero in fp32.
+template <typename T>
+__device__ __noinline__ Sums far_sums(const T* x, int V, float m, int threads) {
+  Sums a = {m, 0.f, 0.f};
+  for (int e = threadIdx.x; e < V; e += threads) {
+    float v;
+    if constexpr (sizeof(T) == 4)
+      v = x[e];
+    else
+      v = to_f(x[e]);
+    const float d = fmaxf((v - m) * kLog2e, -150.f), p = exp2_fast(d);
+    a.s += p;
+    a.w = fmaf(d, p, a.w);
+  }
+  return a;
+}
 
 // What a cluster's blocks leave in the first one's shared memory.
 struct Gather {
@@ -741,8 +767,18 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
       prune(sh, k, 0);
     }
   }
+  const bool finite = fabsf(t.m) < INFINITY;  // no NaN, no +inf, not all -inf
+  if (finite && fabsf(t.m) > kFar) {  // the same for the whole block (the cluster's first)
+    Sums far = far_sums(x, V, t.m, kThreads);
+    far.join_warp();
+    __syncthreads();
+    if (lane == 0) sh.sums[warp] = far;
+    __syncthreads();
+    t = {t.m, 0.f, 0.f};
+    if (lane < W) t = sh.sums[lane];
+    t.join_warp();
+  }
   if (tid > 0 && tid >= k) return;
-  const bool finite = fabsf(Sums::offset(t.m)) < INFINITY;  // no NaN, no +inf, not all -inf
   float log_sum, entropy;
   t.total(log_sum, entropy);
   const float nan = __uint_as_float(0x7fc00000u);
