@@ -35,7 +35,12 @@ class PagedCache:
         self.lengths: dict[int, int] = {}
 
     def grow(self, requests, counts):
-        """Room for counts[i] more tokens of requests[i]; all or nothing."""
+        """Room for counts[i] more tokens of requests[i], each listed once; all
+        or nothing."""
+        if len(requests) != len(counts) or any(n < 0 for n in counts):
+            raise ValueError("paged cache: a count of new tokens, not negative, for each request")
+        if len(set(requests)) != len(requests):  # its rows would be given the same slots twice
+            raise ValueError("paged cache: a request is listed twice")
         need = [max(0, -(-(self.lengths.get(r, 0) + n) // self.page_size) - len(self.pages.get(r, ())))
                 for r, n in zip(requests, counts)]
         if sum(need) > len(self.free):
