@@ -49,6 +49,18 @@ class PagedCache:
             self.pages.setdefault(r, []).extend(self.free.pop() for _ in range(n))
             self.lengths[r] = self.lengths.get(r, 0) + count
 
+    def take_back(self, requests, counts):
+        """Undoes the last grow of the same requests and counts."""
+        for r, count in reversed(list(zip(requests, counts))):
+            left = self.lengths[r] - count
+            keep = -(-left // self.page_size)
+            pages = self.pages[r]
+            self.free.extend(reversed(pages[keep:]))
+            del pages[keep:]
+            self.lengths[r] = left
+            if left == 0:
+                self.release(r)
+
     def release(self, request: int):
         self.free.extend(self.pages.pop(request, ()))
         self.lengths.pop(request, None)
@@ -84,10 +96,18 @@ class PagedOLMoE:
     def step(self, cache: PagedCache, requests, token_lists) -> Tensor:
         """Feeds token_lists[i] to requests[i] (a chunk of a prompt or one
         token) and returns the logits of every row, [rows, vocab] in the
-        activation dtype."""
-        cfg = self.cfg
+        activation dtype.  A step that raises leaves the cache's lengths and
+        pages as they were."""
         counts = [len(t) for t in token_lists]
         cache.grow(requests, counts)
+        try:
+            return self._forward(cache, requests, token_lists, counts)
+        except BaseException:
+            cache.take_back(requests, counts)
+            raise
+
+    def _forward(self, cache: PagedCache, requests, token_lists, counts) -> Tensor:
+        cfg = self.cfg
         table = cache.table(requests)
         plan = ops.PagedPlan(counts, [cache.lengths[r] for r in requests], cfg.heads, cfg.kv_heads, cfg.head_dim,
                              cache.page_size)
