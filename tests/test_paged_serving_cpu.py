@@ -63,3 +63,79 @@ def test_a_step_that_cannot_run_leaves_the_cache_as_it_was():
     with pytest.raises(Exception):
         model.step(cache, [0, 1], [[1] * 5, [2]])
     assert state(cache) == (list(range(6)), {}, {})
+
+
+VOCAB = 50
+
+
+class PagesOfTokens:
+    """A model whose keys are the token ids themselves, kept in the cache's slots: a row's logits depend on what its
+    page table finds there, so another request's tokens, or a shifted position, show."""
+
+    def __init__(self):
+        self.slots = {}
+
+    def step(self, cache, requests, parts):
+        import torch
+        cache.grow(requests, [len(p) for p in parts])
+        rows = []
+        for r, p in zip(requests, parts):
+            pages, size = cache.pages[r], cache.page_size
+            at = lambda j: (pages[j // size], j % size)  # noqa: E731
+            first = cache.lengths[r] - len(p)
+            for j, t in enumerate(p):
+                self.slots[at(first + j)] = t
+                seen = [self.slots[at(u)] for u in range(first + j + 1)]
+                rows.append([-((v - 7 * sum(seen) - 3 * len(seen)) % VOCAB) / 9.0 for v in range(VOCAB)])
+        return torch.tensor(rows)
+
+
+@pytest.fixture
+def plain_logprobs(monkeypatch):
+    import torch
+    from trifuse_b200 import ops
+
+    def token_logprobs(logits, tokens, top=0):
+        lp = torch.log_softmax(logits.double(), -1)
+        best, token = torch.sort(lp, descending=True, stable=True)
+        given = torch.where(tokens >= 0, lp.gather(1, tokens.clamp(min=0)[:, None])[:, 0], float("nan"))
+        return ops.TokenLogprobs(given, None, None, best[:, :top], token[:, :top])
+
+    monkeypatch.setattr(ops, "token_logprobs", token_logprobs)
+
+
+def batch(n=3):
+    from trifuse_b200.paged import Request
+    return [Request(list(range(3 + i, 9 + 2 * i)), 2 + i) for i in range(n)]
+
+
+def answers(requests):
+    return [(r.tokens, r.prompt_logprobs, r.logprobs, r.alternatives) for r in requests]
+
+
+def test_serve_gives_its_pages_back_when_a_step_fails(plain_logprobs):
+    """A call that runs out of pages leaves all of them free, and a smaller one on the same cache answers as on a new
+    one."""
+    from trifuse_b200.paged import serve
+    cache, model = small_cache(pages=5), PagesOfTokens()
+    with pytest.raises(RuntimeError, match="pages needed"):
+        serve(model, cache, batch(3), chunk=4)
+    assert state(cache) == (list(range(5)), {}, {})
+    got = serve(model, cache, batch(1), chunk=4)
+    want = serve(PagesOfTokens(), small_cache(pages=5), batch(1), chunk=4)
+    assert answers(got) == answers(want) and state(cache) == (list(range(5)), {}, {})
+
+
+@pytest.mark.parametrize("others", [[0, 1], [2], [0, 5], ["a"]])
+def test_serve_beside_requests_of_the_callers_own(plain_logprobs, others):
+    """Requests that the cache holds already keep their tokens, and are not taken for those served."""
+    from trifuse_b200.paged import serve
+    cache, model = small_cache(pages=30), PagesOfTokens()
+    model.step(cache, others, [[40 + i] * 3 for i in range(len(others))])
+    kept = {r: list(p) for r, p in cache.pages.items()}
+    got = serve(model, cache, batch(3), chunk=4)
+    want = serve(PagesOfTokens(), small_cache(pages=30), batch(3), chunk=4)
+    assert answers(got) == answers(want)
+    assert cache.pages == kept and cache.lengths == {r: 3 for r in others}
+    for i, r in enumerate(others):
+        assert [model.slots[kept[r][0], j] for j in range(3)] == [40 + i] * 3

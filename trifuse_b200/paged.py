@@ -12,6 +12,7 @@ alternatives.
 from __future__ import annotations
 
 import argparse
+import itertools
 from dataclasses import dataclass, field
 
 import torch
@@ -137,38 +138,46 @@ class Request:
 
 def serve(model: PagedOLMoE, cache: PagedCache, requests: list[Request], chunk: int = 256, top: int = 5):
     """Runs the requests to the end: each step takes up to `chunk` prompt
-    tokens of every request still reading and one token of every other."""
+    tokens of every request still reading and one token of every other.  The
+    cache may hold other requests; the pages of these are free again when the
+    call ends, also by an exception."""
     fed = [0] * len(requests)
     active = [i for i, r in enumerate(requests) if r.prompt]
-    while active:
-        parts = []
+    unused = (n for n in itertools.count() if n not in cache.lengths and n not in cache.pages)
+    names = dict(zip(active, unused))  # in the cache
+    try:
+        while active:
+            parts = []
+            for i in active:
+                known = requests[i].prompt + requests[i].tokens
+                parts.append(known[fed[i]: fed[i] + chunk])
+                fed[i] += len(parts[-1])
+            logits = model.step(cache, [names[i] for i in active], parts)
+            # The token that follows each row, where it is known; else none (-1).
+            follow = []
+            for i, p in zip(active, parts):
+                follow += (requests[i].prompt + requests[i].tokens)[fed[i] - len(p) + 1: fed[i] + 1]
+                follow += [-1] * (fed[i] >= len(requests[i].prompt) + len(requests[i].tokens))
+            got = ops.token_logprobs(logits, torch.tensor(follow, dtype=torch.int64).to(logits.device), top=max(top, 1))
+            logprob, best, token = got.logprob.tolist(), got.top_logprob.tolist(), got.top_token.tolist()
+            row = 0
+            for i, p in zip(list(active), parts):
+                r = requests[i]
+                last = row + len(p) - 1
+                if fed[i] - len(p) < len(r.prompt):
+                    r.prompt_logprobs += logprob[row: row + len(p) - (follow[last] < 0)]
+                if follow[last] < 0:  # everything known is read: the next token is the first alternative
+                    if len(r.tokens) < r.new_tokens:
+                        r.tokens.append(token[last][0])
+                        r.logprobs.append(best[last][0])
+                        r.alternatives.append(list(zip(token[last], best[last])))
+                    if len(r.tokens) >= r.new_tokens:
+                        active.remove(i)
+                        cache.release(names[i])
+                row += len(p)
+    finally:
         for i in active:
-            known = requests[i].prompt + requests[i].tokens
-            parts.append(known[fed[i]: fed[i] + chunk])
-            fed[i] += len(parts[-1])
-        logits = model.step(cache, active, parts)
-        # The token that follows each row, where it is known; else none (-1).
-        follow = []
-        for i, p in zip(active, parts):
-            follow += (requests[i].prompt + requests[i].tokens)[fed[i] - len(p) + 1: fed[i] + 1]
-            follow += [-1] * (fed[i] >= len(requests[i].prompt) + len(requests[i].tokens))
-        got = ops.token_logprobs(logits, torch.tensor(follow, dtype=torch.int64).to(logits.device), top=max(top, 1))
-        logprob, best, token = got.logprob.tolist(), got.top_logprob.tolist(), got.top_token.tolist()
-        row = 0
-        for i, p in zip(list(active), parts):
-            r = requests[i]
-            last = row + len(p) - 1
-            if fed[i] - len(p) < len(r.prompt):
-                r.prompt_logprobs += logprob[row: row + len(p) - (follow[last] < 0)]
-            if follow[last] < 0:  # everything known is read: the next token is the first alternative
-                if len(r.tokens) < r.new_tokens:
-                    r.tokens.append(token[last][0])
-                    r.logprobs.append(best[last][0])
-                    r.alternatives.append(list(zip(token[last], best[last])))
-                if len(r.tokens) >= r.new_tokens:
-                    active.remove(i)
-                    cache.release(i)
-            row += len(p)
+            cache.release(names[i])
     return requests
 
 
