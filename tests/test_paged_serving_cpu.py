@@ -139,3 +139,10 @@ def test_serve_beside_requests_of_the_callers_own(plain_logprobs, others):
     assert cache.pages == kept and cache.lengths == {r: 3 for r in others}
     for i, r in enumerate(others):
         assert [model.slots[kept[r][0], j] for j in range(3)] == [40 + i] * 3
+
+
+@pytest.mark.parametrize("top", [0, 1, 3])
+def test_as_many_alternatives_as_asked_for(plain_logprobs, top):
+    from trifuse_b200.paged import serve
+    for r in serve(PagesOfTokens(), small_cache(pages=30), batch(3), chunk=4, top=top):
+        assert [len(a) for a in r.alternatives] == [top] * r.new_tokens == [top] * len(r.tokens)

@@ -170,7 +170,7 @@ def serve(model: PagedOLMoE, cache: PagedCache, requests: list[Request], chunk: 
                     if len(r.tokens) < r.new_tokens:
                         r.tokens.append(token[last][0])
                         r.logprobs.append(best[last][0])
-                        r.alternatives.append(list(zip(token[last], best[last])))
+                        r.alternatives.append(list(zip(token[last], best[last]))[:top])
                     if len(r.tokens) >= r.new_tokens:
                         active.remove(i)
                         cache.release(names[i])
