@@ -146,3 +146,12 @@ def test_as_many_alternatives_as_asked_for(plain_logprobs, top):
     from trifuse_b200.paged import serve
     for r in serve(PagesOfTokens(), small_cache(pages=30), batch(3), chunk=4, top=top):
         assert [len(a) for a in r.alternatives] == [top] * r.new_tokens == [top] * len(r.tokens)
+
+
+@pytest.mark.parametrize("chunk", [0, -1, -3])
+def test_a_chunk_of_nothing_is_refused(plain_logprobs, chunk):
+    from trifuse_b200.paged import serve
+    cache, requests = small_cache(), batch(1)
+    with pytest.raises(ValueError, match="chunk"):
+        serve(PagesOfTokens(), cache, requests, chunk=chunk)
+    assert not cache.lengths and answers(requests) == [([], [], [], [])]

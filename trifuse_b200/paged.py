@@ -141,6 +141,8 @@ def serve(model: PagedOLMoE, cache: PagedCache, requests: list[Request], chunk: 
     tokens of every request still reading and one token of every other.  The
     cache may hold other requests; the pages of these are free again when the
     call ends, also by an exception."""
+    if chunk < 1:
+        raise ValueError("serve: chunk is a positive number of tokens")
     fed = [0] * len(requests)
     active = [i for i, r in enumerate(requests) if r.prompt]
     unused = (n for n in itertools.count() if n not in cache.lengths and n not in cache.pages)
