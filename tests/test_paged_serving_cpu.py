@@ -155,3 +155,23 @@ def test_a_chunk_of_nothing_is_refused(plain_logprobs, chunk):
     with pytest.raises(ValueError, match="chunk"):
         serve(PagesOfTokens(), cache, requests, chunk=chunk)
     assert not cache.lengths and answers(requests) == [([], [], [], [])]
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_logits_that_are_no_distribution_give_no_token(plain_logprobs, bad):
+    """A row with a NaN or +inf, or nothing but -inf, has no next token: told, as the session tells it."""
+    from trifuse_b200 import TriFuseError
+    from trifuse_b200.paged import serve
+
+    class Bad(PagesOfTokens):
+        def step(self, cache, requests, parts):
+            logits = super().step(cache, requests, parts)
+            if cache.lengths[requests[0]] == 8:
+                logits[0, 4 if bad > 0 or bad != bad else slice(None)] = bad
+            return logits
+
+    cache, requests = small_cache(), batch(1)  # a prompt of 6
+    requests[0].new_tokens = 9
+    with pytest.raises(TriFuseError, match="not finite"):
+        serve(Bad(), cache, requests, chunk=8)
+    assert len(requests[0].tokens) == 2 and not cache.lengths and len(cache.free) == 6

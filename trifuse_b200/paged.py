@@ -13,12 +13,14 @@ from __future__ import annotations
 
 import argparse
 import itertools
+import math
 from dataclasses import dataclass, field
 
 import torch
 from torch import Tensor
 
 from . import ops
+from ._lib import TriFuseError
 from .model import Config
 
 
@@ -170,6 +172,8 @@ def serve(model: PagedOLMoE, cache: PagedCache, requests: list[Request], chunk: 
                     r.prompt_logprobs += logprob[row: row + len(p) - (follow[last] < 0)]
                 if follow[last] < 0:  # everything known is read: the next token is the first alternative
                     if len(r.tokens) < r.new_tokens:
+                        if math.isnan(best[last][0]):  # as Session.generate_greedy refuses such a row
+                            raise TriFuseError(9, "serve: logits that are not finite give no next token")
                         r.tokens.append(token[last][0])
                         r.logprobs.append(best[last][0])
                         r.alternatives.append(list(zip(token[last], best[last]))[:top])
