@@ -175,3 +175,25 @@ def test_logits_that_are_no_distribution_give_no_token(plain_logprobs, bad):
     with pytest.raises(TriFuseError, match="not finite"):
         serve(Bad(), cache, requests, chunk=8)
     assert len(requests[0].tokens) == 2 and not cache.lengths and len(cache.free) == 6
+
+
+@pytest.mark.parametrize("chunk", [2, 4, 100])
+@pytest.mark.parametrize("fails_at", [1, 2, 3, 4])
+def test_a_call_that_was_cut_short_may_be_repeated(plain_logprobs, chunk, fails_at):
+    """The same requests again: each prompt token's log probability once, and the answers of an undisturbed call."""
+    from trifuse_b200.paged import serve
+
+    class Once(PagesOfTokens):
+        steps = 0
+
+        def step(self, *a):
+            self.steps += 1
+            if self.steps == fails_at:
+                raise RuntimeError("once")
+            return super().step(*a)
+
+    cache, requests, model = small_cache(pages=30), batch(3), Once()
+    with pytest.raises(RuntimeError, match="once"):
+        serve(model, cache, requests, chunk=chunk)
+    got = serve(model, cache, requests, chunk=chunk)
+    assert answers(got) == answers(serve(PagesOfTokens(), small_cache(pages=30), batch(3), chunk=chunk))

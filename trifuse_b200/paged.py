@@ -142,13 +142,17 @@ def serve(model: PagedOLMoE, cache: PagedCache, requests: list[Request], chunk: 
     """Runs the requests to the end: each step takes up to `chunk` prompt
     tokens of every request still reading and one token of every other.  The
     cache may hold other requests; the pages of these are free again when the
-    call ends, also by an exception."""
+    call ends, also by an exception, and requests that were cut short may be
+    passed again: they go on after the tokens that they have.  A request without
+    a prompt is left as it is."""
     if chunk < 1:
         raise ValueError("serve: chunk is a positive number of tokens")
     fed = [0] * len(requests)
     active = [i for i, r in enumerate(requests) if r.prompt]
     unused = (n for n in itertools.count() if n not in cache.lengths and n not in cache.pages)
     names = dict(zip(active, unused))  # in the cache
+    for i in active:
+        requests[i].prompt_logprobs = []
     try:
         while active:
             parts = []
@@ -168,8 +172,7 @@ def serve(model: PagedOLMoE, cache: PagedCache, requests: list[Request], chunk: 
             for i, p in zip(list(active), parts):
                 r = requests[i]
                 last = row + len(p) - 1
-                if fed[i] - len(p) < len(r.prompt):
-                    r.prompt_logprobs += logprob[row: row + len(p) - (follow[last] < 0)]
+                r.prompt_logprobs += logprob[row: row + max(0, min(len(p), len(r.prompt) - 1 - (fed[i] - len(p))))]
                 if follow[last] < 0:  # everything known is read: the next token is the first alternative
                     if len(r.tokens) < r.new_tokens:
                         if math.isnan(best[last][0]):  # as Session.generate_greedy refuses such a row
