@@ -427,8 +427,8 @@ int tf_paged_plan_make(const int32_t* new_lengths, const int32_t* kv_lengths, in
 
 /* Attention of the planned rows over the pages (workspace): row i of request
  * r attends keys 0 .. kv_len - new_len + i of that request,
- * out = softmax(q K^T * scale) V, query head h reading key head
- * h / (heads / kv_heads).  q: act rows of heads * head_dim values, q_stride
+ * out = softmax(q K^T * scale) V (scale positive, up to 2.3e38), query head h
+ * reading key head h / (heads / kv_heads).  q: act rows of heads * head_dim values, q_stride
  * apart (a multiple of 8); out: act [rows][heads * head_dim], 32-byte
  * aligned.  The cache has
  * the activations' dtype, or f16 under bf16 activations (q is then rounded to

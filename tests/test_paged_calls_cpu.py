@@ -48,3 +48,14 @@ def test_no_plan_is_made_inside_a_capture(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="captures a graph"):
         ops.PagedPlan([1], [4], 4, 2, 64, 16)
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3.0e38, float("inf"), float("nan"), 0.0, -1.0, 1e-60])
+def test_scales_that_overflow_inside_are_refused(scale):
+    """The kernels fold log2(e) into the scale: beyond 2.3e38 every score would be 0 * inf."""
+    from trifuse_b200._lib import PagedKV, PageTable, lib
+    from tests.test_paged_cpu import plan
+    _, d, _ = plan([1], [40])
+    kv, tab = PagedKV(0x1000, 0x2000, 4, 2 * 16 * 128, 2, 16, 128, 1), PageTable(0x3000, 3, 1, 3)
+    assert lib().tf_paged_attention(C.c_void_p(0x4000), 1024, C.byref(tab), C.byref(kv), C.byref(d), C.c_void_p(0x5000),
+                                    scale, 1, C.c_void_p(0x6000), C.c_void_p(0x7000), 1 << 20, None) == 1

@@ -141,8 +141,9 @@ int tf_paged_attention(const void* q, int64_t q_stride, const tf_page_table* tab
   if (table->requests < plan->requests || table->columns < plan->columns)
     return set_error(TF_ERR_SHAPE, "paged_attention: page table %d x %d, the plan needs %d x %d", table->requests,
                      table->columns, plan->requests, plan->columns);
-  if (!(scale > 0) || !(scale <= 3.0e38f))
-    return set_error(TF_ERR_INVALID_ARGUMENT, "paged_attention: scale must be positive");
+  // The kernels work with scale * log2(e) in fp32.
+  if (!(scale > 0) || !(scale <= 2.3e38f))
+    return set_error(TF_ERR_INVALID_ARGUMENT, "paged_attention: scale must be positive and below 2.3e38");
   if (q_stride < (int64_t)plan->heads * plan->head_dim || q_stride % 8)
     return set_error(TF_ERR_SHAPE, "paged_attention: q stride %lld", (long long)q_stride);
   if (plan->rows == 0) return TF_OK;
