@@ -59,3 +59,36 @@ def test_scales_that_overflow_inside_are_refused(scale):
     kv, tab = PagedKV(0x1000, 0x2000, 4, 2 * 16 * 128, 2, 16, 128, 1), PageTable(0x3000, 3, 1, 3)
     assert lib().tf_paged_attention(C.c_void_p(0x4000), 1024, C.byref(tab), C.byref(kv), C.byref(d), C.c_void_p(0x5000),
                                     scale, 1, C.c_void_p(0x6000), C.c_void_p(0x7000), 1 << 20, None) == 1
+
+
+@pytest.fixture
+def host_plans(monkeypatch):
+    """Plans as far as the host makes them: the tables' allocations by size, none of them pinned."""
+    sizes, empty = [], torch.empty
+
+    def allocate(n, pin_memory=False, **kw):
+        sizes.append(n)
+        if n > 1 << 26:
+            raise MemoryError(n)
+        return empty(n, **kw)
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch, "empty", allocate)
+    return sizes
+
+
+@pytest.mark.parametrize("new,kv,H,Hk", [([1 << 30], [1], 8, 2), ([1, -5], [1, 1], 8, 2), ([1], [1], 1 << 30, 1 << 30),
+                                         ([(1 << 31) - 1] * 4, [1] * 4, 8, 2)])
+def test_nothing_large_is_allocated_for_a_plan_that_is_refused(host_plans, new, kv, H, Hk):
+    """The planner's refusal, not one of the allocator after gigabytes of pinned memory."""
+    from trifuse_b200 import TriFuseError
+    with pytest.raises((ValueError, TriFuseError)):
+        ops.PagedPlan(new, kv, H, Hk, 128, 16)
+    assert max(host_plans) <= 1 << 23
+
+
+def test_a_plan_larger_than_the_first_allocation(host_plans):
+    """800,000 rows: the table is made again at the size that the planner gives."""
+    with pytest.raises((RuntimeError, AssertionError)):  # the upload, where there is no device
+        ops.PagedPlan([400000, 400000], [400000, 500000], 8, 8, 128, 16, device="cuda:99")
+    assert len(host_plans) == 2 and host_plans[0] <= 1 << 23 and host_plans[1] >= 8 * 800000

@@ -585,7 +585,8 @@ class PagedPlan:
             raise RuntimeError("paged plan: made while the stream captures a graph; make it before the capture")
         new, kv = (C.c_int32 * n)(*new_lengths), (C.c_int32 * n)(*kv_lengths)
         self.desc = d = PagedPlanDesc()
-        guess = 65536 + 64 * n * max(kv_heads, 1) + 16 * max(sum(new_lengths), 0)
+        # At most 4 MB before the planner has checked what it is to plan.
+        guess = 65536 + min(64 * n * max(kv_heads, 1) + 16 * max(sum(new_lengths), 0), 1 << 22)
         while True:  # a second time when the table outgrows the guess
             host = torch.empty(guess, dtype=torch.uint8, pin_memory=True)
             status = lib().tf_paged_plan_make(new, kv, n, heads, kv_heads, head_dim, page_size, d, host.data_ptr(),
