@@ -92,3 +92,10 @@ def test_a_plan_larger_than_the_first_allocation(host_plans):
     with pytest.raises((RuntimeError, AssertionError)):  # the upload, where there is no device
         ops.PagedPlan([400000, 400000], [400000, 500000], 8, 8, 128, 16, device="cuda:99")
     assert len(host_plans) == 2 and host_plans[0] <= 1 << 23 and host_plans[1] >= 8 * 800000
+
+
+@pytest.mark.parametrize("lengths", [[2.5], [1.0], ["1"], [None]])
+def test_lengths_that_are_no_integers_are_refused(host_plans, lengths):
+    for new, kv in ((lengths, [40]), ([1], lengths)):
+        with pytest.raises(TypeError):
+            ops.PagedPlan(new, kv, 4, 2, 64, 16)

@@ -12,6 +12,7 @@ allocate outputs and scratch.
 from __future__ import annotations
 
 import ctypes as C
+from operator import index
 from typing import NamedTuple
 
 import torch
@@ -578,7 +579,7 @@ class PagedPlan:
         n = len(new_lengths)
         if len(kv_lengths) != n:
             raise ValueError("paged plan: new_lengths and kv_lengths differ in length")
-        new_lengths, kv_lengths = [int(x) for x in new_lengths], [int(x) for x in kv_lengths]
+        new_lengths, kv_lengths = [index(x) for x in new_lengths], [index(x) for x in kv_lengths]
         if any(not -(1 << 31) <= x < 1 << 31 for x in new_lengths + kv_lengths):  # would wrap on the way to C
             raise ValueError("paged plan: a length does not fit 32 bits")
         if torch.cuda.is_current_stream_capturing():  # a replay would read host memory that is long reused
