@@ -1,0 +1,33 @@
+"""Arguments of the paged operators and of token_logprobs that need care at the entry: outputs and weights off their
+alignment, integers of other types, caches of one head or one page."""
+import numpy as np
+import pytest
+import torch
+
+from tests.test_gpu_paged import BF16, F16, append_reference, check, make_cache, near, reference, run
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from trifuse_b200 import ops as _ops
+    return _ops
+
+
+@pytest.mark.parametrize("offset", [0, 1, 4, 8, 16])
+@pytest.mark.parametrize("n", [1, 40, 300])
+def test_outputs_off_their_alignment(ops, offset, n):
+    """out as a view that starts `offset` values into its storage: the same values, and nothing beside them."""
+    H, Hk, D, page = 4, 2, 64, 16
+    q, k, v, table, plan, want = run(ops, [n], [n + 5], H, Hk, D, page, F16, F16)
+    wide = torch.full((n * H * D + 64,), 7.0, dtype=F16, device="cuda")
+    out = wide[offset:offset + n * H * D].view(n, H, D)
+    assert ops.paged_attention(q, k, v, table, plan, out=out) is out and torch.equal(out, want)
+    assert (wide[:offset] == 7).all() and (wide[offset + n * H * D:] == 7).all()
+    qkv = torch.randn(n, (H + 2 * Hk) * D, generator=torch.Generator().manual_seed(n)).to(F16).cuda()
+    want = ops.paged_append(qkv, k, v, table, plan.positions, plan.requests, H, rope_theta=1e4)
+    wide.fill_(7.0)
+    got = ops.paged_append(qkv, k, v, table, plan.positions, plan.requests, H, rope_theta=1e4, out=out)
+    assert got is out and torch.equal(out, want)
+    assert (wide[:offset] == 7).all() and (wide[offset + n * H * D:] == 7).all()

@@ -524,6 +524,13 @@ def _rows16(t: Tensor, width: int) -> Tensor:
     return t
 
 
+def _aligned_out(out: Tensor | None, shape, like: Tensor, align: int) -> Tensor:
+    """`out`, or a new tensor where there is none or the kernel cannot store to it (the caller copies it over)."""
+    if out is None or out.data_ptr() % align:
+        return like.new_empty(shape)
+    return out
+
+
 def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, positions: Tensor,
                  requests: Tensor, heads: int, q_norm: Tensor | None = None, k_norm: Tensor | None = None,
                  eps: float = 1e-5, rope_theta: float | None = None, out: Tensor | None = None) -> Tensor:
@@ -553,14 +560,13 @@ def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tens
             if t is not None and (t.dtype != torch.float16 or t.shape != (n,) or not t.is_contiguous()):
                 raise ValueError("paged_append: norm weights are contiguous float16 over the full q and k widths")
         qn, kn = (None if t is None else t.data_ptr() for t in (q_norm, k_norm))
-    if out is None:
-        out = qkv.new_empty((rows, heads, D))
-    elif out.shape != (rows, heads, D) or out.dtype != qkv.dtype or not out.is_contiguous():
+    if out is not None and (out.shape != (rows, heads, D) or out.dtype != qkv.dtype or not out.is_contiguous()):
         raise ValueError("paged_append: out is a contiguous [rows, heads, head_dim] of qkv's dtype")
+    q = _aligned_out(out, (rows, heads, D), qkv, 16)
     check(lib().tf_paged_append(qkv.data_ptr(), qkv.stride(0) if rows > 1 else width, rows, heads, _act(qkv), qn, kn,
                                 eps, rope_theta or 0.0, positions.data_ptr(), requests.data_ptr(),
-                                _page_table(page_table), kv, out.data_ptr(), stream))
-    return out
+                                _page_table(page_table), kv, q.data_ptr(), stream))
+    return q if out is None or q is out else out.copy_(q)
 
 
 class PagedPlan:
@@ -652,17 +658,16 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Ten
     rows, heads, D = shape
     width = heads * D
     q = _rows16(q if q.stride()[1:] == (D, 1) else q.contiguous(), width)
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != shape or out.dtype != q.dtype or not out.is_contiguous():
+    if out is not None and (out.shape != shape or out.dtype != q.dtype or not out.is_contiguous()):
         raise ValueError("paged_attention: out is a contiguous [rows, heads, head_dim] of q's dtype")
     if stream != plan.made_on:
         plan.order(stream)
+    o = _aligned_out(out, shape, q, 32)
     check(lib().tf_paged_attention(q.data_ptr(), q.stride(0) if rows > 1 else width, _page_table(page_table),
                                    _paged_kv(k_pages, v_pages), plan.desc, plan.table_ptr,
-                                   D ** -0.5 if scale is None else scale, _act(q), out.data_ptr(),
+                                   D ** -0.5 if scale is None else scale, _act(q), o.data_ptr(),
                                    plan.workspace_ptr, plan.workspace_bytes, stream))
-    return out
+    return o if out is None or o is out else out.copy_(o)
 
 
 def set_qmm_path(path: int):
