@@ -31,3 +31,19 @@ def test_outputs_off_their_alignment(ops, offset, n):
     got = ops.paged_append(qkv, k, v, table, plan.positions, plan.requests, H, rope_theta=1e4, out=out)
     assert got is out and torch.equal(out, want)
     assert (wide[:offset] == 7).all() and (wide[offset + n * H * D:] == 7).all()
+
+
+@pytest.mark.parametrize("offset", [1, 4, 8])
+def test_norm_weights_off_their_alignment(ops, offset):
+    """Both weights as slices of one buffer of parameters."""
+    H, Hk, D, page, n = 4, 2, 64, 16, 5
+    k, v, table = make_cache([n], Hk, D, page, F16)
+    plan = ops.PagedPlan([n], [n], H, Hk, D, page)
+    g = torch.Generator().manual_seed(offset)
+    buffer = (1 + 0.2 * torch.randn(offset + (H + Hk) * D + 3, generator=g)).to(F16).cuda()
+    qn, kn = buffer[offset:offset + H * D], buffer[offset + H * D + 3:offset + (H + Hk) * D + 3]
+    qkv = torch.randn(n, (H + 2 * Hk) * D, generator=g).to(F16).cuda()
+    q = ops.paged_append(qkv, k, v, table, plan.positions, plan.requests, H, q_norm=qn, k_norm=kn, rope_theta=1e4)
+    wq, wk, _ = append_reference(qkv, H, Hk, D, plan.positions, qn, kn, 1e-5, 1e4)
+    near(q, wq)
+    near(k[table[0].long()].transpose(1, 2).reshape(-1, Hk, D)[:n], wk)

@@ -559,6 +559,7 @@ def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tens
         for t, n in ((q_norm, heads * D), (k_norm, kv_heads * D)):
             if t is not None and (t.dtype != torch.float16 or t.shape != (n,) or not t.is_contiguous()):
                 raise ValueError("paged_append: norm weights are contiguous float16 over the full q and k widths")
+        q_norm, k_norm = (t if t is None or t.data_ptr() % 16 == 0 else t.clone() for t in (q_norm, k_norm))
         qn, kn = (None if t is None else t.data_ptr() for t in (q_norm, k_norm))
     if out is not None and (out.shape != (rows, heads, D) or out.dtype != qkv.dtype or not out.is_contiguous()):
         raise ValueError("paged_append: out is a contiguous [rows, heads, head_dim] of qkv's dtype")
