@@ -47,3 +47,15 @@ def test_norm_weights_off_their_alignment(ops, offset):
     wq, wk, _ = append_reference(qkv, H, Hk, D, plan.positions, qn, kn, 1e-5, 1e4)
     near(q, wq)
     near(k[table[0].long()].transpose(1, 2).reshape(-1, Hk, D)[:n], wk)
+
+
+def test_top_of_any_integer_type(ops):
+    x = torch.randn(3, 500, generator=torch.Generator().manual_seed(1)).cuda()
+    t = torch.tensor([1, 2, 3], device="cuda")
+    want = ops.token_logprobs(x, t, top=7)
+    for top in (np.int64(7), np.int32(7), torch.tensor(7)):
+        for a, b in zip(want, ops.token_logprobs(x, t, top=top)):
+            assert torch.equal(a, b)
+    for top in (7.0, np.float32(7), "7", None, np.int64(65)):
+        with pytest.raises(ValueError):
+            ops.token_logprobs(x, t, top=top)

@@ -185,7 +185,9 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0) -> TokenLogprob
     if logits.ndim < 1 or tokens.shape != logits.shape[:-1] or tokens.dtype != torch.int64:
         raise ValueError("token_logprobs: tokens are int64 with the shape of the logits' rows")
     if type(top) is not int:
-        raise ValueError("token_logprobs: top is an int")
+        if not hasattr(type(top), "__index__"):
+            raise ValueError("token_logprobs: top is an int")
+        top = index(top)
     stream = _launch_stream(logits, tokens)
     shape, V = tokens.shape, logits.shape[-1]
     if logits.ndim != 2:
