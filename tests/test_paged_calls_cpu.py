@@ -99,3 +99,18 @@ def test_lengths_that_are_no_integers_are_refused(host_plans, lengths):
     for new, kv in ((lengths, [40]), ([1], lengths)):
         with pytest.raises(TypeError):
             ops.PagedPlan(new, kv, 4, 2, 64, 16)
+
+
+@pytest.mark.parametrize("make", ["one head, slots first", "one page of a wide buffer", "one page, expanded", "plain"])
+def test_strides_of_single_heads_and_pages_do_not_matter(make):
+    """A page that is contiguous is taken, whatever stride its dimensions of one carry."""
+    base = torch.zeros(4, 16, 2, 64, dtype=torch.float16)
+    k = {"one head, slots first": base[..., :1, :].contiguous().transpose(1, 2),
+         "one page of a wide buffer": base.view(-1).as_strided((1, 2, 16, 64), (8, 1024, 64, 1)),
+         "one page, expanded": base[0].reshape(2, 16, 64)[None].expand(1, 2, 16, 64),
+         "plain": base.view(4, 2, 16, 64)}[make]
+    d = ops._paged_kv(k, k)
+    assert (d.pages, d.kv_heads, d.page_size, d.head_dim) == tuple(k.shape) and d.k == k.data_ptr()
+    assert d.page_stride >= d.kv_heads * 16 * 64 and (d.pages == 1 or d.page_stride == k.stride(0))
+    with pytest.raises(ValueError):
+        ops._paged_kv(base.transpose(1, 2), base.transpose(1, 2))  # two heads inside each slot

@@ -483,8 +483,13 @@ def _paged_kv(k_pages: Tensor, v_pages: Tensor) -> PagedKV:
     if dtype not in _ACT:
         raise ValueError("paged: the cache must be float16 or bfloat16")
     pages, heads, size, D = shape
+    if heads == 1 or pages == 1:  # the stride of a dimension of one is of no meaning
+        stride, other = ((t[0] if pages > 1 else heads * size * D, t[1] if heads > 1 else size * D, t[2], t[3])
+                         for t in (stride, v_pages.stride()))
+    else:
+        other = v_pages.stride()
     step = stride[0]
-    if stride != (step, size * D, D, 1) or stride != v_pages.stride():
+    if stride != (step, size * D, D, 1) or stride != other:
         raise ValueError("paged: a page must be contiguous, and k_pages and v_pages laid out alike")
     return PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), pages, step, heads, size, D, _ACT[dtype])
 
