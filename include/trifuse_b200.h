@@ -428,18 +428,18 @@ int tf_paged_plan_make(const int32_t* new_lengths, const int32_t* kv_lengths, in
 /* Attention of the planned rows over the pages (workspace): row i of request
  * r attends keys 0 .. kv_len - new_len + i of that request,
  * out = softmax(q K^T * scale) V (scale positive, up to 2.3e38), query head h
- * reading key head h / (heads / kv_heads).  q: act rows of heads * head_dim values, q_stride
- * apart (a multiple of 8); out: act [rows][heads * head_dim], 32-byte
- * aligned.  The cache has
- * the activations' dtype, or f16 under bf16 activations (q is then rounded to
- * f16).  A row that attends nothing, or whose every score is -inf, gives
- * zeros; NaN and +inf scores give NaN.  A value that is not finite reaches
- * only the rows that see its token.  Slots past a request's length are never
- * used, whatever they hold.  plan_table is the device copy of the
- * table; calls that overlap in time need tables and workspaces of their own
- * (the kernels count arrivals in the table and leave it as they found it).
- * Replaces the SDPA of MLXNativeGraniteMoEPrefill.h:471-483 for a paged
- * cache. */
+ * reading key head h / (heads / kv_heads).  q: act rows of heads * head_dim
+ * values, q_stride apart (a multiple of 8); out: act [rows][heads * head_dim],
+ * 32-byte aligned.  The cache has the activations' dtype, or f16 under bf16
+ * activations: q is then rounded to f16, a (row, head) with values beyond its
+ * range after division by a power of two that its scores get back.  A row that
+ * attends nothing, or whose every score is -inf, gives zeros; NaN and +inf
+ * scores give NaN.  A value that is not finite reaches only the rows that see
+ * its token.  Slots past a request's length are never used, whatever they
+ * hold.  plan_table is the device copy of the table; calls that overlap in
+ * time need tables and workspaces of their own (the kernels count arrivals in
+ * the table and leave it as they found it).  Replaces the SDPA of
+ * MLXNativeGraniteMoEPrefill.h:471-483 for a paged cache. */
 int tf_paged_attention(const void* q, int64_t q_stride, const tf_page_table* table, const tf_paged_kv* kv,
                        const tf_paged_plan* plan, void* plan_table, float scale, int act, void* out, void* workspace,
                        size_t workspace_bytes, void* stream);

@@ -281,15 +281,33 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
 #pragma unroll
       for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t u = *reinterpret_cast<const uint32_t*>(qr + 16 * k + 8 * j + c2);
-          if constexpr (Act<T>::kDtype == Act<C>::kDtype) {
-            qb[k][t][j] = u;
-          } else {
-            const T* v = reinterpret_cast<const T*>(&u);
-            qb[k][t][j] = pack2<C>(to_f(v[0]), to_f(v[1]));
+        for (int j = 0; j < 2; ++j)
+          qb[k][t][j] = *reinterpret_cast<const uint32_t*>(qr + 16 * k + 8 * j + c2);
+    }
+    float scale[NT][2];  // of the scores of rows 8 t + c2, + 1
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      scale[t][0] = scale[t][1] = p.scale_log2;
+      if constexpr (Act<T>::kDtype != Act<C>::kDtype) {
+        uint32_t most = 0;  // of row 8 t + g, whose values four lanes share
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) most = magnitude(qb[k][t][j], most);
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int over = beyond_f16(most);
+        const float down = power2(-over);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) scale[t][i] *= power2(__shfl_sync(0xffffffffu, over, 4 * (c2 + i)));
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const T* v = reinterpret_cast<const T*>(&qb[k][t][j]);
+            qb[k][t][j] = pack2<C>(to_f(v[0]) * down, to_f(v[1]) * down);
           }
-        }
+      }
     }
     int limit[NT][2];  // last key that rows 8 t + c2, + 1 see
 #pragma unroll
@@ -353,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int j = i; j < 4; j += 2) {
-              float v = s[h][t][j] * p.scale_log2;
+              float v = s[h][t][j] * scale[t][i];
               if (ragged && key0 + 16 * h + g + 4 * (j - i) > limit[t][i]) v = -INFINITY;
               s[h][t][j] = v;
               mx = max_nan(mx, v);

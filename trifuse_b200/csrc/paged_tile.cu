@@ -527,7 +527,8 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
     // segment `seg` on, into the K-major 128-byte swizzle: row i of each
     // 64-column half at i * 128, 16-byte chunk c at (c ^ (i & 7)) * 16.  A warp
     // copies its 32 rows whole rows at a time; rows past the segment's become
-    // zeros.
+    // zeros.  Leaves what the own row's scores are to be multiplied with.
+    float boost = 1.f;
     auto copy_queries = [&](int seg) {
       constexpr int kChunks = D / 8, kRowsAt = 32 / kChunks;  // chunks of a row, rows per pass
       for (; seg < seg1; ++seg) {
@@ -538,25 +539,52 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
                        (int64_t)(g.kv_head * p.group + pr % p.group) * D;
         const int c = lane % kChunks;
         uint8_t* to = base + x * S::kTile + (c >> 3) * kColBytes;
-#pragma unroll 8
-        for (int i = 0; i < 32 / kRowsAt; ++i) {
-          const int from = i * kRowsAt + lane / kChunks;  // lane whose row this is
-          const T* q = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(own), from)) + 8 * c;
-          const int row = (warp & 3) * 32 + from;
-          const bool real = kHalf * x + row < g.rows;
-          uint8_t* at = to + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-          if constexpr (Act<T>::kDtype == Act<C>::kDtype) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(at)), "l"(q),
-                         "r"(real ? 16 : 0)
-                         : "memory");
-          } else {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (real) {
-              float f[8];
-              unpack8<T>(ld_v4(q), f);
-              v = pack8<C>(f);
+        constexpr int kBatch = 8;  // rows' loads in flight
+        static_assert(32 / kRowsAt % kBatch == 0, "batches");
+        boost = 1.f;
+#pragma unroll 1
+        for (int i0 = 0; i0 < 32 / kRowsAt; i0 += kBatch) {
+          uint4 values[kBatch];
+          uint32_t most[kBatch], all = 0;
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            const int from = (i0 + b) * kRowsAt + lane / kChunks;  // lane whose row this is
+            const T* q = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(own), from)) + 8 * c;
+            const int row = (warp & 3) * 32 + from;
+            const bool real = kHalf * x + row < g.rows;
+            if constexpr (Act<T>::kDtype == Act<C>::kDtype) {
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                               smem_addr(to + row * 128 + (((c & 7) ^ (row & 7)) << 4))),
+                           "l"(q), "r"(real ? 16 : 0)
+                           : "memory");
+            } else {
+              values[b] = real ? ld_v4(q) : make_uint4(0, 0, 0, 0);
             }
-            *reinterpret_cast<uint4*>(at) = v;
+          }
+          if constexpr (Act<T>::kDtype != Act<C>::kDtype) {
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+              const uint4 v = values[b];
+              most[b] = magnitude(v.w, magnitude(v.z, magnitude(v.y, magnitude(v.x, 0))));
+              all = max(all, most[b]);
+            }
+            const bool wide = __any_sync(0xffffffffu, beyond_f16(all) > 0);
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+              float f[8];
+              unpack8<T>(values[b], f);
+              if (wide) {
+#pragma unroll
+                for (int off = 1; off < kChunks; off <<= 1) most[b] = max(most[b], __shfl_xor_sync(0xffffffffu, most[b], off));
+                const int over = beyond_f16(most[b]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) f[k] *= power2(-over);
+                const int mine = __shfl_sync(0xffffffffu, over, lane % kRowsAt * kChunks);
+                if (lane / kRowsAt == i0 + b) boost = power2(mine);
+              }
+              const int row = (warp & 3) * 32 + (i0 + b) * kRowsAt + lane / kChunks;
+              *reinterpret_cast<uint4*>(to + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = pack8<C>(f);
+            }
           }
         }
         if constexpr (Act<T>::kDtype == Act<C>::kDtype) asm volatile("cp.async.wait_all;" ::: "memory");
@@ -576,6 +604,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
       const int token = pr / p.group;
       const int limit = g.kv_len - g.new_len + token;  // last key the row sees
       const int first_limit = g.kv_len - g.new_len + (g.row0 + kHalf * x) / p.group;
+      const float scale = Act<T>::kDtype == Act<C>::kDtype ? p.scale_log2 : p.scale_log2 * boost;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < count; ++j) {
         if (!(ok = wait_warp(&s_full[x], s_turn & 1, ctl, err, 90))) break;
@@ -601,7 +630,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
 #pragma unroll
           for (int i = 0; i < 8; ++i) mp[i] = max_nan(mp[i], sc[c + 2 * i], sc[c + 2 * i + 1]);
         float mx = max_nan(max_nan(mp[0], mp[1], mp[2]), max_nan(mp[3], mp[4], mp[5]), max_nan(mp[6], mp[7])) *
-                   p.scale_log2;
+                   scale;
         if (mx == INFINITY) mx = __uint_as_float(0x7fc00000u);  // inf - inf: the row is NaN
         float factor = 1.f;
         if (!(mx <= m + kRescale)) {  // also for NaN, and for the first key seen
@@ -629,7 +658,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
         // parts of 64 keys, so the product of the first runs while the
         // second's exponentials do.
         const float sub = m == -INFINITY ? 0.f : -m;
-        const uint64_t sl2 = f2_pack(p.scale_log2, p.scale_log2), nm = f2_pack(sub, sub);
+        const uint64_t sl2 = f2_pack(scale, scale), nm = f2_pack(sub, sub);
         uint64_t sp[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) sp[i] = 0ull;

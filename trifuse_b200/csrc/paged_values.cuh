@@ -85,4 +85,18 @@ __device__ __forceinline__ void clear_not_finite(uint8_t* chunks, int n, int lan
   }
 }
 
+// Queries of bf16 for a cache of f16, whose largest value is 65504: a row with
+// larger ones goes to the product divided by a power of two, which its scores
+// get back with the scale (exact both ways).  Rows within the range, that is
+// all but unheard-of ones, are converted as they are.
+//
+// The largest magnitude, as bf16 bits, of two packed values.
+__device__ __forceinline__ uint32_t magnitude(uint32_t w, uint32_t most) {
+  return max(most, max(w & 0x7fffu, w >> 16 & 0x7fffu));
+}
+// The power (0 or more) by which a row of that magnitude must be divided.
+__device__ __forceinline__ int beyond_f16(uint32_t most) { return max((int)(most >> 7) - (127 + 15), 0); }
+// 2^n, n in [-126, 127].
+__device__ __forceinline__ float power2(int n) { return __uint_as_float((uint32_t)(127 + n) << 23); }
+
 }  // namespace tf
