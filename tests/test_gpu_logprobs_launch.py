@@ -11,7 +11,7 @@ def test_blocks_meet_before_they_write_into_the_first_ones_memory():
     """In the source: a cluster-wide arrive before the pass and its wait before the first remote write."""
     text = (Path(__file__).resolve().parent.parent / "trifuse_b200" / "csrc" / "logprobs.cu").read_text()
     kernel = text[text.index("logprobs_kernel("):]
-    arrive, wait = kernel.index("cluster.barrier_arrive()"), kernel.index("cluster.barrier_wait()")
+    arrive, wait = kernel.index("barrier.cluster.arrive"), kernel.index("barrier.cluster.wait")
     remote = re.search(r"\bto->\w+\[slice\]", kernel).start()
     assert arrive < kernel.index("auto fetch") < wait < remote < kernel.index("cluster.sync()")
 

@@ -505,8 +505,9 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
     sh.stalled = 0;
   }
   // The first block's shared memory may be written once every block of the
-  // cluster is known to run: announced here, waited for before the push.
-  if (W == 8 && slices > 1) cluster.barrier_arrive();
+  // cluster is known to run: announced here (nothing has been written for
+  // another block, so without an order), waited for before the push.
+  if (W == 8 && slices > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   __syncthreads();
   auto fetch = [&](int tile) {  // one thread
     const int t0 = v_begin + tile * kTile, n = min(kTile, v_end - t0);
@@ -768,7 +769,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
   if (W == 8 && slices > 1) {
     Gather* to = cluster.map_shared_rank(&sh, 0)->gather;
     const int n = k ? sh.n : 0;
-    cluster.barrier_wait();  // the first block has started
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the first block has started
     if (tid < n) to->best[slice][tid] = sh.best[tid];
     if (tid == 0) {
       to->sums[slice] = t;
