@@ -42,7 +42,8 @@
 //              halves took 3214 clocks with one warp for both and 2260 with two
 //              (2048 at the peak rate).  The halves take turns issuing (baton),
 //              which keeps one's softmax beside the other's products; without
-//              it both ran in step, 4090 clocks a tile against 3500.
+//              it both ran in step, 4090 clocks a tile against 3500.  Neither
+//              passes it a second time before the other has seen the first.
 //   loader     page ids and TMA of the K and V tiles (128-byte
 //              swizzle) into one ring of tiles, K and V in turn.
 // Tensor memory columns: O_A [0, 128), O_B [128, 256), S_A [256, 384), S_B
@@ -479,9 +480,16 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
           // O still holds the half's last segment until it has been read.
           if (j == 0 && o_turn++ > 0 && !(ok = wait_warp(&o_free[x], o_turn & 1, ctl, err, 86))) break;
           const uint32_t va = smem_addr(vt);
-          if (j < both && (x == 1 || j > 0)) {
-            if (!(ok = wait_warp(&baton[x], baton_turn & 1, ctl, err, 87))) break;
+          if (j < both) {
+            // Half A waits for B's turn before its own, but for the block's first.
+            if ((x == 1 || baton_turn > 0) &&
+                !(ok = wait_warp(&baton[x], (baton_turn - (1 - x)) & 1, ctl, err, 87)))
+              break;
             ++baton_turn;
+            // At a segment's end half B says that it has seen A's: without a word
+            // A would pass the baton again in the next segment, and B, held up
+            // by its outputs, would miss a phase and wait for good.
+            if (x == 1 && j + 1 == both && lane == 0) mbar_arrive(&baton[0]);
           }
 #pragma unroll
           for (int part = 0; part < 2; ++part) {
