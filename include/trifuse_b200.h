@@ -368,7 +368,8 @@ typedef struct tf_page_table {
  * then rotated by halves with base rope_theta (0: no rotation); k and v are
  * written to the row's slot and q to q_out (act [rows][heads * head_dim]).
  * All arithmetic is fp32 (the rotation's angle fp64) with one rounding at the
- * end.  A row whose request, position or page id lies outside the table or
+ * end.  (In an f16 cache keys and values of bf16 activations beyond 65504
+ * become infinite.)  A row whose request, position or page id lies outside the table or
  * the cache stores no key and no value; rows of one call must not share a
  * slot.  heads * head_dim <= 16384. */
 int tf_paged_append(const void* qkv, int64_t qkv_stride, int64_t rows, int32_t heads, int act, const void* q_norm,

@@ -37,10 +37,13 @@
 // times over); the blocks' sums and candidates meet in the first block's hands
 // over distributed shared memory, so no scratch in device memory is needed.
 //
-// Measured: 4095 rows of 50304 bf16 logits with five alternatives 133 us (3.1
-// TB/s; 117 where the given token is the largest, so that nothing is counted)
-// and 92 with none (4.5 TB/s); 2048 rows of fp32 with twenty 94 us (4.4 TB/s),
-// in rising order 500 (in rounds alone 9450); one row 10.5 us, 64 rows 12.5.
+// Measured: 4095 rows of 50304 bf16 logits with five alternatives 132 us (3.1
+// TB/s; 116 where the given token is the largest, so that nothing is counted)
+// and 97 with none (4.3 TB/s); with 64 251; 2048 rows of fp32 with twenty 103 us
+// (93 with the largest token), in rising order 496 (in rounds alone 9450); one
+// row 11 us, 64 rows 13.  At 18 warps an SM it is latency that is left: a
+// scheduler issues in half of its clocks, and warps wait for their own dependent
+// instructions, for instructions to be fetched and at the prunes' barriers.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -363,7 +366,8 @@ struct Gather {
 template <int W>
 struct Shared {
   // Two rounds of the block's threads, the cluster's join, and room for what a
-  // first tile offers (64 alternatives: 320 places ran over, 308 us against 252),
+  // first tile offers (64 alternatives, drawn tokens given: 320 places ran over,
+  // 308 us against 252),
   // or 64 vectors of 8 values beside the kept ones (values in rising order).
   static constexpr int kBuffer = 640;
   static_assert(kBuffer >= 64 * W && kBuffer - 32 * W >= kMaxTop && kBuffer >= kMaxCluster * kMaxTop, "candidates");

@@ -28,10 +28,10 @@
 // are at most 1, so its relative error is the type's, the same size as the
 // output's own rounding); scores, m, l and O stay fp32.
 //
-// Measured: 64 decodes of 4096 tokens, 16 heads, pages of 64: 308 us, 7.0 TB/s;
+// Measured: 64 decodes of 4096 tokens, 16 heads, pages of 64: 311 us, 6.9 TB/s;
 // 37 ragged decodes of up to 32768 tokens, 8 key heads, pages of 16: 279 us, 6.0
 // TB/s (277 with the products taken out: 4 KB pages set that); one decode of 600
-// tokens 7.3 us, of one token 4.3.
+// tokens 7.2 us, of one token 4.0.
 #include <cuda.h>
 #include <math.h>
 #include <string.h>

@@ -28,7 +28,7 @@
 //   warps 0-3, 4-7  softmax of half A, B: read S from tensor memory, mask, write
 //              P in 16 bits over S's first columns; after a segment's last
 //              scores copy the next segment's queries into shared memory
-//              (each thread its row, converted where the cache's type
+//              (whole rows by a warp, converted where the cache's type
 //              differs), then read O and write out (or the piece's partial
 //              result).  A warp of its own for the queries took 9000 clocks a
 //              half, most of a short segment.
@@ -54,11 +54,12 @@
 // Every wait is bounded; an expired one records an error code (tf_device_error)
 // and all roles stop.
 //
-// Measured: 2048 tokens after 14336 (32 query and 8 key heads of 128) 444 us,
-// 1.16 PFLOP/s, tensor pipe 64% at the 1.58 GHz that the power cap leaves; 8
-// prompts of 2048 tokens (16 heads) 168 us, 0.82 PFLOP/s (segments of 9 tiles on
-// average, whose ends cost 5600 clocks each; 163 us without looking the causal
-// edge's values through, paged_values.cuh).
+// Measured: 2048 tokens after 14336 (32 query and 8 key heads of 128) 426 us,
+// 1.21 PFLOP/s (444 us under a profiler: tensor pipe 64% at the 1.58 GHz that the
+// power cap leaves); 8 prompts of 2048 tokens (16 heads) 166 us, 0.83 PFLOP/s
+// (segments of 9 tiles on average, whose ends cost 5600 clocks each; 4 us of it
+// for looking the causal edge's values through, paged_values.cuh), 182 us with
+// bf16 queries over an f16 cache.
 #include <cuda.h>
 #include <math.h>
 #include <string.h>
