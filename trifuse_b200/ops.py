@@ -483,11 +483,10 @@ def _paged_kv(k_pages: Tensor, v_pages: Tensor) -> PagedKV:
     if dtype not in _ACT:
         raise ValueError("paged: the cache must be float16 or bfloat16")
     pages, heads, size, D = shape
+    other = v_pages.stride()
     if heads == 1 or pages == 1:  # the stride of a dimension of one is of no meaning
         stride, other = ((t[0] if pages > 1 else heads * size * D, t[1] if heads > 1 else size * D, t[2], t[3])
-                         for t in (stride, v_pages.stride()))
-    else:
-        other = v_pages.stride()
+                         for t in (stride, other))
     step = stride[0]
     if stride != (step, size * D, D, 1) or stride != other:
         raise ValueError("paged: a page must be contiguous, and k_pages and v_pages laid out alike")
@@ -495,17 +494,16 @@ def _paged_kv(k_pages: Tensor, v_pages: Tensor) -> PagedKV:
 
 
 def _page_table(page_table: Tensor) -> PageTable:
-    """Descriptor of a page table; keep it until the launch (it may own a copy of the table)."""
+    """Descriptor of a page table; keep both until the launch."""
     shape, stride = page_table.shape, page_table.stride()
     if len(shape) != 2 or page_table.dtype != torch.int32 or (shape[1] > 1 and stride[1] != 1):
         raise ValueError("paged: the page table is int32 [requests, pages] with contiguous rows")
     requests, columns = shape
-    step = stride[0]
-    if step < columns:  # of no meaning for one row; rows that share memory (an expanded row) are laid out apart
-        if requests > 1:
-            page_table = page_table.clone(memory_format=torch.contiguous_format)
-        step = columns
-    desc = PageTable(page_table.data_ptr(), step, requests, columns)
+    if stride[0] >= columns:
+        return PageTable(page_table.data_ptr(), stride[0], requests, columns)
+    if requests > 1:  # rows that share memory (an expanded row) are laid out apart
+        page_table = page_table.clone(memory_format=torch.contiguous_format)
+    desc = PageTable(page_table.data_ptr(), columns, requests, columns)  # the stride of one row is of no meaning
     desc.tensor = page_table
     return desc
 
@@ -529,13 +527,6 @@ def _rows16(t: Tensor, width: int) -> Tensor:
     if step < width or step % 8 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
-
-
-def _aligned_out(out: Tensor | None, shape, like: Tensor, align: int) -> Tensor:
-    """`out`, or a new tensor where there is none or the kernel cannot store to it (the caller copies it over)."""
-    if out is None or out.data_ptr() % align:
-        return like.new_empty(shape)
-    return out
 
 
 def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, positions: Tensor,
@@ -566,15 +557,21 @@ def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tens
         for t, n in ((q_norm, heads * D), (k_norm, kv_heads * D)):
             if t is not None and (t.dtype != torch.float16 or t.shape != (n,) or not t.is_contiguous()):
                 raise ValueError("paged_append: norm weights are contiguous float16 over the full q and k widths")
-        q_norm, k_norm = (t if t is None or t.data_ptr() % 16 == 0 else t.clone() for t in (q_norm, k_norm))
         qn, kn = (None if t is None else t.data_ptr() for t in (q_norm, k_norm))
-    if out is not None and (out.shape != (rows, heads, D) or out.dtype != qkv.dtype or not out.is_contiguous()):
+        if (qn or 0) % 16 or (kn or 0) % 16:
+            q_norm, k_norm = (None if t is None else t.clone() for t in (q_norm, k_norm))
+            qn, kn = (None if t is None else t.data_ptr() for t in (q_norm, k_norm))
+    q = out
+    if out is None:
+        q = qkv.new_empty((rows, heads, D))
+    elif out.shape != (rows, heads, D) or out.dtype != qkv.dtype or not out.is_contiguous():
         raise ValueError("paged_append: out is a contiguous [rows, heads, head_dim] of qkv's dtype")
-    q = _aligned_out(out, (rows, heads, D), qkv, 16)
+    elif out.data_ptr() % 16:  # the kernel cannot store there: copied over
+        q = torch.empty_like(out)
     check(lib().tf_paged_append(qkv.data_ptr(), qkv.stride(0) if rows > 1 else width, rows, heads, _act(qkv), qn, kn,
                                 eps, rope_theta or 0.0, positions.data_ptr(), requests.data_ptr(),
                                 _page_table(page_table), kv, q.data_ptr(), stream))
-    return q if out is None or q is out else out.copy_(q)
+    return q if out is None or out is q else out.copy_(q)
 
 
 class PagedPlan:
@@ -666,16 +663,20 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Ten
     rows, heads, D = shape
     width = heads * D
     q = _rows16(q if q.stride()[1:] == (D, 1) else q.contiguous(), width)
-    if out is not None and (out.shape != shape or out.dtype != q.dtype or not out.is_contiguous()):
+    o = out
+    if out is None:
+        o = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("paged_attention: out is a contiguous [rows, heads, head_dim] of q's dtype")
+    elif out.data_ptr() % 32:  # the kernel cannot store there: copied over
+        o = torch.empty_like(out)
     if stream != plan.made_on:
         plan.order(stream)
-    o = _aligned_out(out, shape, q, 32)
     check(lib().tf_paged_attention(q.data_ptr(), q.stride(0) if rows > 1 else width, _page_table(page_table),
                                    _paged_kv(k_pages, v_pages), plan.desc, plan.table_ptr,
                                    D ** -0.5 if scale is None else scale, _act(q), o.data_ptr(),
                                    plan.workspace_ptr, plan.workspace_bytes, stream))
-    return o if out is None or o is out else out.copy_(o)
+    return o if out is None or out is o else out.copy_(o)
 
 
 def set_qmm_path(path: int):
