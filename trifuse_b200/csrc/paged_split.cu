@@ -24,9 +24,9 @@
 // four warps' (m, l, O) are joined through shared memory, and the pieces of a
 // cut item through global memory by the last block to arrive.
 //
-// P is rounded to the cache's 16-bit type for the second product (its values
-// are at most 1, so its relative error is the type's, the same size as the
-// output's own rounding); scores, m, l and O stay fp32.
+// P is rounded to the cache's 16-bit type for the second product (its relative
+// error is the type's, the same size as the output's own rounding, in f16 down
+// to 2^-21 of the row's largest, paged_values.cuh); scores, m, l and O stay fp32.
 //
 // Measured: 64 decodes of 4096 tokens, 16 heads, pages of 64: 311 us, 6.9 TB/s;
 // 37 ragged decodes of up to 32768 tokens, 8 key heads, pages of 16: 279 us, 6.0
@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_split_kernel(const __grid_c
           mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          const float mn = max_nan(m[t][i], mx);
+          const float mn = max_nan(m[t][i], lifted<C>(mx));
           // Rows that have seen no key yet keep m = -inf and add nothing.
           sub[i] = mn == -INFINITY ? 0.f : mn;
           keep[t][i] = exp2_fast(m[t][i] - sub[i]);

@@ -5,8 +5,9 @@
 // out = softmax(q K^T * scale) V over 128-key tiles with a running maximum m
 // and sum l per row; per tile s = q K^T, P = 2^(s * scale * log2 e - m),
 // O += P V, l += sum P.  The maximum is refreshed lazily: a row keeps the m it
-// used until a tile raises it by more than 8 (log2 units), so P <= 256 and O
-// is rescaled only on such tiles; O / l is the same quotient.
+// used until a tile raises it by more than 8 (log2 units), so P <= 2^8 (in f16
+// 2^15: m lies 7 below the maximum, paged_values.cuh) and O is rescaled only on
+// such tiles; O / l is the same quotient.
 //
 // What bounds it: 4 D flops per (row, key) pair on the tensor cores, and one
 // exponential per pair on a unit that gives 16 a clock and SM, which is just
@@ -49,8 +50,9 @@
 // Tensor memory columns: O_A [0, 128), O_B [128, 256), S_A [256, 384), S_B
 // (one half: O [0, 128), S [128, 256)).
 //
-// P is rounded to the cache's 16-bit type, relative 2^-11 (f16) or 2^-8
-// (bf16), the size of the output's own rounding; l sums the unrounded values.
+// P is rounded to the cache's 16-bit type, relative 2^-11 (f16, down to 2^-21 of
+// the row's largest) or 2^-8 (bf16), the size of the output's own rounding; l
+// sums the unrounded values.
 // Every wait is bounded; an expired one records an error code (tf_device_error)
 // and all roles stop.
 //
@@ -78,7 +80,7 @@ using namespace tc;
 constexpr int kHalf = 128;  // rows of a half = TMEM lanes
 constexpr uint32_t kColO = 0;  // half x's columns: O at kColO + 128 x, S after the halves' O
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRescale = 8.f;  // log2 units that P may exceed 1 by
+constexpr float kRescale = 8.f;  // log2 units that a row's maximum may rise by before O is rescaled
 constexpr int kColBytes = kTileKeys * 128;  // 64 columns of a tile: 128 rows of 128 bytes
 
 // A block of H halves: two of them one to an SM, or one half two to an SM.
@@ -642,6 +644,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
                    scale;
         if (mx == INFINITY) mx = __uint_as_float(0x7fc00000u);  // inf - inf: the row is NaN
         float factor = 1.f;
+        mx = lifted<C>(mx);
         if (!(mx <= m + kRescale)) {  // also for NaN, and for the first key seen
           mx = max_nan(m, mx);  // a NaN stays
           factor = fast_exp2(m - mx);

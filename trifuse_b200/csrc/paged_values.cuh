@@ -41,6 +41,21 @@ struct PairOf<__nv_bfloat16> {
   static constexpr uint32_t kExponent = 0x7f80u;
 };
 
+// Weights P = 2^(s - m) go to the second product in the cache's 16-bit type.  f16
+// ends at 2^-24: against a row's maximum, 60000 weights just below 2^-25 would
+// all vanish, 0.2 per cent of the row beside one key that outweighs the rest.
+// So for f16 the reference m lies kLift (log2 units) below the maximum, and P
+// uses the type's upper range as well; sums and outputs carry the same factor,
+// which the quotient drops.  bf16 reaches as far as fp32.  (Not for maxima so
+// large that the difference would round, up to a P past 65504.)
+constexpr float kLift = 7.f;
+
+template <typename C>
+__device__ __forceinline__ float lifted(float maximum) {
+  if constexpr (PairOf<C>::kExponent != 0x7c00u) return maximum;
+  return maximum - (fabsf(maximum) < 1048576.f ? kLift : 0.f);
+}
+
 template <typename C>
 __device__ __forceinline__ bool not_finite(C v) {
   const uint32_t w = *reinterpret_cast<const uint16_t*>(&v);
