@@ -5,8 +5,8 @@
 // out = softmax(q K^T * scale) V over 128-key tiles with a running maximum m
 // and sum l per row; per tile s = q K^T, P = 2^(s * scale * log2 e - m),
 // O += P V, l += sum P.  The maximum is refreshed lazily: a row keeps the m it
-// used until a tile raises it by more than 8 (log2 units), so P <= 2^8 (in f16
-// 2^15: m lies 7 below the maximum, paged_values.cuh) and O is rescaled only on
+// used until a tile raises it by more than 7 (log2 units), so P <= 2^7 (in f16
+// 2^14: m lies 7 below the maximum, paged_values.cuh) and O is rescaled only on
 // such tiles; O / l is the same quotient.
 //
 // What bounds it: 4 D flops per (row, key) pair on the tensor cores, and one
@@ -80,7 +80,9 @@ using namespace tc;
 constexpr int kHalf = 128;  // rows of a half = TMEM lanes
 constexpr uint32_t kColO = 0;  // half x's columns: O at kColO + 128 x, S after the halves' O
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRescale = 8.f;  // log2 units that a row's maximum may rise by before O is rescaled
+// Log2 units that a row's maximum may rise by before O is rescaled (with 8 a sum
+// near 2^28, where fp32 has steps of 16, would round up to twice as much).
+constexpr float kRescale = 7.f;
 constexpr int kColBytes = kTileKeys * 128;  // 64 columns of a tile: 128 rows of 128 bytes
 
 // A block of H halves: two of them one to an SM, or one half two to an SM.
@@ -643,6 +645,14 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
         float mx = max_nan(max_nan(mp[0], mp[1], mp[2]), max_nan(mp[3], mp[4], mp[5]), max_nan(mp[6], mp[7])) *
                    scale;
         if (mx == INFINITY) mx = __uint_as_float(0x7fc00000u);  // inf - inf: the row is NaN
+        // Far out the product with the scale is rounded by more than the
+        // exponential bears: there each score takes the maximum's rounding.
+        float unit = scale;
+        if (__any_sync(0xffffffffu, fabsf(mx) > kFar)) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c) sc[c] *= scale;
+          unit = 1.f;
+        }
         float factor = 1.f;
         mx = lifted<C>(mx);
         if (!(mx <= m + kRescale)) {  // also for NaN, and for the first key seen
@@ -670,7 +680,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
         // parts of 64 keys, so the product of the first runs while the
         // second's exponentials do.
         const float sub = m == -INFINITY ? 0.f : -m;
-        const uint64_t sl2 = f2_pack(scale, scale), nm = f2_pack(sub, sub);
+        const uint64_t sl2 = f2_pack(unit, unit), nm = f2_pack(sub, sub);
         uint64_t sp[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) sp[i] = 0ull;

@@ -49,11 +49,12 @@ struct PairOf<__nv_bfloat16> {
 // which the quotient drops.  bf16 reaches as far as fp32.  (Not for maxima so
 // large that the difference would round, up to a P past 65504.)
 constexpr float kLift = 7.f;
+constexpr float kFar = 1048576.f;  // 2^20: fp32's steps are an eighth there
 
 template <typename C>
 __device__ __forceinline__ float lifted(float maximum) {
   if constexpr (PairOf<C>::kExponent != 0x7c00u) return maximum;
-  return maximum - (fabsf(maximum) < 1048576.f ? kLift : 0.f);
+  return maximum - (fabsf(maximum) < kFar ? kLift : 0.f);
 }
 
 template <typename C>
