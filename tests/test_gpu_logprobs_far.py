@@ -86,3 +86,15 @@ def test_every_logit_the_lowest(ops):
         r = check(ops, x, torch.tensor([0, 7, 4999], device="cuda"), 5)
         assert torch.allclose(r.logprob, torch.full_like(r.logprob, -math.log(5000)), atol=1e-5)
         assert r.rank.tolist() == [0, 7, 4999] and r.top_token[1].tolist() == [0, 1, 2, 3, 4]
+
+
+@pytest.mark.parametrize("centre", [1e5, -1e6, 2e6, 5e6])
+@pytest.mark.parametrize("rows,V", [(170, 57973), (230, 150001), (3, 250001)])
+def test_long_rows_of_a_few_values(ops, centre, rows, V):
+    """Logits a few steps of fp32 apart: hundreds of equal exponentials to a thread, whose sum may not drift."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    for std in (0.3, 2.5):
+        x = torch.randn(rows, V, generator=g, device="cuda") * std + centre
+        t = torch.randint(0, V, (rows,), generator=g, device="cuda")
+        for top in (0, 8):
+            check(ops, x, t, top)

@@ -347,11 +347,15 @@ __device__ __noinline__ Sums far_sums(const T* x, int V, Sums* warps) {
   Sums a = {-INFINITY, 0.f, 0.f};
   for (int e = threadIdx.x; e < V; e += 32 * W) a.m = fmaxf(a.m, value(e));
   a = join(a);
+  // In fp64: hundreds of equal terms to a thread would drift in fp32.
+  double sum = 0., weighted = 0.;
   for (int e = threadIdx.x; e < V; e += 32 * W) {
     const float d = fmaxf((value(e) - a.m) * kLog2e, -150.f), p = exp2_fast(d);
-    a.s += p;
-    a.w = fmaf(d, p, a.w);
+    sum += p;
+    weighted += d * p;
   }
+  a.s = (float)sum;
+  a.w = (float)weighted;
   return join(a);
 }
 
