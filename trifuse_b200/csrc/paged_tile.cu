@@ -56,9 +56,9 @@
 // Every wait is bounded; an expired one records an error code (tf_device_error)
 // and all roles stop.
 //
-// Measured: 2048 tokens after 14336 (32 query and 8 key heads of 128) 426 us,
-// 1.21 PFLOP/s (444 us under a profiler: tensor pipe 64% at the 1.58 GHz that the
-// power cap leaves); 8 prompts of 2048 tokens (16 heads) 166 us, 0.83 PFLOP/s
+// Measured: 2048 tokens after 14336 (32 query and 8 key heads of 128) 424 us,
+// 1.22 PFLOP/s (444 us under a profiler: tensor pipe 64% at the 1.58 GHz that the
+// power cap leaves); 8 prompts of 2048 tokens (16 heads) 163 us, 0.84 PFLOP/s
 // (segments of 9 tiles on average, whose ends cost 5600 clocks each; 4 us of it
 // for looking the causal edge's values through, paged_values.cuh), 182 us with
 // bf16 queries over an f16 cache.
