@@ -45,8 +45,8 @@ def test_clusters_on_a_busy_gpu(rows, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,V", [(3, 50304), (200, 50304), (200, 9001), (1, 250001)])
 def test_expired_waits_are_told_and_do_no_harm(rows, V):
-    """With a wait limit of one cycle the waits for the copies run out: the error code is left, and the results are
-    those of the whole rows all the same, since no slot is read or refilled before its copy has landed."""
+    """With a wait limit of one cycle a wait that its first try does not meet runs out and leaves the error code; the
+    results are those of the whole rows all the same, since no slot is read or refilled before its copy has landed."""
     from trifuse_b200 import ops
     from trifuse_b200._lib import check, lib
     g = torch.Generator().manual_seed(V)
