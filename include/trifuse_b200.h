@@ -66,7 +66,9 @@ typedef enum tf_status {
 typedef enum tf_dtype {
   TF_DTYPE_F16 = 1,
   TF_DTYPE_BF16 = 2,
-  TF_DTYPE_F32 = 3
+  TF_DTYPE_F32 = 3,
+  TF_DTYPE_I8 = 4,  /* codes of an 8-bit cache */
+  TF_DTYPE_E4M3 = 5
 } tf_dtype;
 
 /* MLX affine-quantized weight, stacked over experts when experts > 0.
@@ -444,6 +446,88 @@ int tf_paged_plan_make(const int32_t* new_lengths, const int32_t* kv_lengths, in
 int tf_paged_attention(const void* q, int64_t q_stride, const tf_page_table* table, const tf_paged_kv* kv,
                        const tf_paged_plan* plan, void* plan_table, float scale, int act, void* out, void* workspace,
                        size_t workspace_bytes, void* stream);
+
+/* Scales of a paged cache held in 8 bits: tf_paged_kv with dtype TF_DTYPE_I8
+ * (codes -127 .. 127) or TF_DTYPE_E4M3 (finite codes), page_size from 16,
+ * page_stride a multiple of 16.  The tokens of a page are scaled in blocks of
+ * TF_SCALE_TOKENS: the value of a code is code * scale[page][kv_head]
+ * [slot / TF_SCALE_TOKENS], f32 in device memory, page p + 1 page_stride
+ * values after page p. */
+#define TF_SCALE_TOKENS 16
+typedef struct tf_paged_scales {
+  float* k;
+  float* v;
+  int64_t page_stride;
+} tf_paged_scales;
+
+/* tf_paged_append into an 8-bit cache.  For each key head the new tokens of a
+ * block get the scale
+ *   s = max(the block's scale, if it holds earlier tokens of the request;
+ *           largest magnitude of the new ones / 127 (I8) or 448 (E4M3)),
+ * at least 2^-126 where that magnitude is not zero, and the codes of their
+ * values / s, rounded to nearest even; where s grew, the earlier tokens' codes
+ * become code * old / s, rounded the same way.  A NaN or an infinity makes the
+ * block's scale NaN (and its own code 0), until the block is begun anew.  Codes
+ * of later slots stay as they are.
+ * Rows of one request whose tokens share a block must be adjacent, their
+ * positions rising by one; a row at another position begins anew, and two
+ * such groups in one block in one call leave its contents undefined. */
+int tf_paged_append_8bit(const void* qkv, int64_t qkv_stride, int64_t rows, int32_t heads, int act,
+                         const void* q_norm, const void* k_norm, float eps, float rope_theta,
+                         const int32_t* positions, const int32_t* requests, const tf_page_table* table,
+                         const tf_paged_kv* kv, const tf_paged_scales* scales, void* q_out, void* stream);
+
+/* tf_paged_attention over an 8-bit cache; the same plans serve both.  The
+ * codes enter the products as f16, which holds them exactly; the scales go to
+ * the scores and weights (or, for many rows, to the f16 operands, which then
+ * are rounded once).  A NaN scale makes the rows NaN that see a token of its
+ * block, and only those. */
+int tf_paged_attention_8bit(const void* q, int64_t q_stride, const tf_page_table* table, const tf_paged_kv* kv,
+                            const tf_paged_scales* scales, const tf_paged_plan* plan, void* plan_table, float scale,
+                            int act, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Pages of a cache copied inside it, in every layer and array: page dst[i]
+ * becomes page src[i].  An array holds layers x pages pages of page_bytes
+ * contiguous bytes each, layer l and page p at base + l * layer_stride +
+ * p * page_stride bytes (device memory; keys, values and scales of one cache
+ * are arrays of one call).  src and dst are host arrays, read before the call
+ * returns; a pair of equal pages does nothing, else a page may be written once
+ * and not be read as well. */
+#define TF_MAX_COPY_ARRAYS 8
+typedef struct tf_copy_array {
+  void* base;
+  int64_t layer_stride;
+  int64_t page_stride;
+  int64_t page_bytes;
+} tf_copy_array;
+int tf_paged_copy(const tf_copy_array* arrays, int32_t count, int32_t layers, int64_t pages, const int32_t* src,
+                  const int32_t* dst, int64_t pairs, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* beam search                                                                */
+
+/* The best `count` continuations of each request over its beams and the
+ * vocabulary.  logits (dtype f32, f16 or bf16): row requests * beams + b,
+ * row_stride values apart; scores f32 [requests][beams], the beams' log
+ * probabilities so far.  A continuation of beam b by token t has the score
+ *   scores[b] + log softmax(logits[b])[t];
+ * of those that are finite the first `count` in falling order go to score
+ * f32, parent int32 (b) and token int64 (t), all [requests][count] (equal
+ * scores: the lower beam first; inside a beam the larger logit, then the lower
+ * token).  Where there are fewer, the rest is -inf, -1, -1.  finished (uint8
+ * [requests][beams], may be NULL): such a beam has ended and competes with its
+ * score as it is, as one continuation by the token `end`; its logits are not
+ * read.  A beam whose score is not finite, or whose logits hold a NaN or +inf
+ * or nothing but -inf, has no continuations.  Scores that lie within 3e-5 of
+ * one another are told apart in 64 bits.  beams <= TF_MAX_BEAMS, count <=
+ * TF_MAX_TOP.  The workspace is device scratch (16-byte aligned, no initial
+ * contents).  The reference generates greedily (patches/executorch.patch:
+ * 1350-1353). */
+#define TF_MAX_BEAMS 64
+int tf_beam_select_workspace_size(int64_t requests, int32_t beams, int32_t vocab, int32_t count, size_t* bytes);
+int tf_beam_select(const void* logits, int64_t row_stride, int64_t requests, int32_t beams, int32_t vocab, int dtype,
+                   const float* scores, const uint8_t* finished, int64_t end, int32_t count, float* score,
+                   int32_t* parent, int64_t* token, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* model and session                                                          */

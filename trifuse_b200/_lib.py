@@ -17,7 +17,7 @@ TF_ERR_CAPACITY = 10
 STATUS = {0: "TF_OK", 1: "TF_ERR_INVALID_ARGUMENT", 2: "TF_ERR_SHAPE", 3: "TF_ERR_OUT_OF_MEMORY",
           4: "TF_ERR_CUDA", 5: "TF_ERR_NCCL", 6: "TF_ERR_TIMEOUT", 7: "TF_ERR_CANCELLED",
           8: "TF_ERR_UNSUPPORTED", 9: "TF_ERR_STATE", 10: "TF_ERR_CAPACITY"}
-DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 1, 2, 3
+DTYPE_F16, DTYPE_BF16, DTYPE_F32, DTYPE_I8, DTYPE_E4M3 = 1, 2, 3, 4, 5
 HOST_INPUTS, HOST_OUTPUT = 1, 2
 
 
@@ -51,6 +51,15 @@ class OLMoEConfig(C.Structure):
 class PagedKV(C.Structure):
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("pages", C.c_int64), ("page_stride", C.c_int64),
                 ("kv_heads", C.c_int32), ("page_size", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32)]
+
+
+class PagedScales(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64)]
+
+
+class CopyArray(C.Structure):
+    _fields_ = [("base", C.c_void_p), ("layer_stride", C.c_int64), ("page_stride", C.c_int64),
+                ("page_bytes", C.c_int64)]
 
 
 class PageTable(C.Structure):
@@ -136,6 +145,13 @@ SIGNATURES = {
     "tf_token_logprobs": [P, I64, I64, I32, C.c_int, P, I32, P, P, P, P, P, P],
     "tf_paged_append": [P, I64, I64, I32, C.c_int, P, P, F32, F32, P, P, C.POINTER(PageTable), C.POINTER(PagedKV), P,
                         P],
+    "tf_paged_append_8bit": [P, I64, I64, I32, C.c_int, P, P, F32, F32, P, P, C.POINTER(PageTable),
+                             C.POINTER(PagedKV), C.POINTER(PagedScales), P, P],
+    "tf_paged_attention_8bit": [P, I64, C.POINTER(PageTable), C.POINTER(PagedKV), C.POINTER(PagedScales),
+                                C.POINTER(PagedPlanDesc), P, F32, C.c_int, P, P, SZ, P],
+    "tf_paged_copy": [C.POINTER(CopyArray), I32, I32, I64, P, P, I64, P],
+    "tf_beam_select_workspace_size": [I64, I32, I32, I32, PSZ],
+    "tf_beam_select": [P, I64, I64, I32, I32, C.c_int, P, P, I64, I32, P, P, P, P, SZ, P],
     "tf_paged_plan_make": [P, P, I32, I32, I32, I32, I32, C.POINTER(PagedPlanDesc), P, SZ],
     "tf_paged_attention": [P, I64, C.POINTER(PageTable), C.POINTER(PagedKV), C.POINTER(PagedPlanDesc), P, F32,
                            C.c_int, P, P, SZ, P],

@@ -220,6 +220,10 @@ tf_status launch_token_logprobs(const void* logits, int64_t row_stride, int64_t 
                                 const int64_t* tokens, int top, float* logprob, float* entropy, int32_t* rank,
                                 float* top_logprob, int64_t* top_token, cudaStream_t s);
 
+// Pages dst[i] = src[i] (host arrays) of `count` arrays, in every layer.
+tf_status launch_paged_copy(const tf_copy_array* arrays, int count, int layers, int64_t pages, const int32_t* src,
+                            const int32_t* dst, int64_t pairs, cudaStream_t s);
+
 // y[i][:] = x[idx[i] / div][:] for i < n (act rows of `width`, width % 8 == 0).
 tf_status launch_gather_rows(const void* x, int64_t x_stride, const int32_t* idx, int div, int64_t n, int width,
                              int act, void* y, cudaStream_t s);

@@ -37,6 +37,10 @@
 // times over); the blocks' sums and candidates meet in the first block's hands
 // over distributed shared memory, so no scratch in device memory is needed.
 //
+// Beam selection (beams.cu) takes its rows from the same pass: the maximum, the
+// log of the sum and the candidates as keys, without the weighted sum and the
+// rank; rows of beams that have ended or stand at -inf are not read.
+//
 // Measured: 4095 rows of 50304 bf16 logits with five alternatives 132 us (3.1
 // TB/s; 116 where the given token is the largest, so that nothing is counted)
 // and 97 with none (4.3 TB/s); with 64 251; 2048 rows of fp32 with twenty 103 us
@@ -47,6 +51,7 @@
 #include <cooperative_groups.h>
 #include <math.h>
 
+#include "beams.h"
 #include "common.cuh"
 #include "internal.h"
 #include "tc_ptx.cuh"
@@ -79,18 +84,12 @@ struct LogprobParams {
   int64_t* top_token;
   int* err;
   const long long* wait_cycles;
+  const float* scores;      // of beams
+  const uint8_t* finished;  // or NULL
+  BeamRow* beam_rows;
+  uint64_t* beam_keys;      // [rows][top]
 };
 
-// Order-preserving bits of a value: NaN lowest, then -inf; -0 counts as +0.
-__device__ __forceinline__ uint32_t order_bits(float v) {
-  const uint32_t u = __float_as_uint(v + 0.f);
-  if (v != v) return 0u;
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-}
-__device__ __forceinline__ float order_value(uint32_t k) {
-  if (k == 0u) return __uint_as_float(0x7fc00000u);
-  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
-}
 __device__ __forceinline__ uint64_t composite(float v, uint32_t index) {
   return ((uint64_t)order_bits(v) << 32) | (0xffffffffu - index);
 }
@@ -274,8 +273,13 @@ struct Sums {
     log_sum = logf(s / exp2_fast(residue));
     entropy = log_sum - (w / s - residue) * kLn2;
   }
+  // The logarithm alone, in fp64: sums of other rows are compared with it.
+  __device__ __forceinline__ double log_sum() const {
+    const float residue = fabsf(m) >= kFar ? 0.f : fmaf(m, kLog2e, offset(m));
+    return log((double)s) - (double)residue * 0.6931471805599453;
+  }
   // Adds a tile of vectors whose maximum is tmax.
-  template <typename T, int N>
+  template <typename T, bool kWeighted, int N>
   __device__ __forceinline__ void add(const uint4 (&r)[N], float tmax) {
     if (!(tmax <= m)) {
       const float to = max_nan(m, tmax);
@@ -294,9 +298,14 @@ struct Sums {
         unpair(d, d0, d1);
         const uint64_t e = pair(exp2_fast(d0), exp2_fast(d1));
         s2[(j >> 1) & 1] = add2(s2[(j >> 1) & 1], e);
-        w2[(j >> 1) & 1] = fma2(d, e, w2[(j >> 1) & 1]);
+        if (kWeighted) w2[(j >> 1) & 1] = fma2(d, e, w2[(j >> 1) & 1]);
       }
     float a, b, tw;
+    if (!kWeighted) {
+      unpair(add2(s2[0], s2[1]), a, b);
+      s += a + b;
+      return;
+    }
     unpair(add2(w2[0], w2[1]), a, b);
     tw = a + b;
     if (tw != tw) {
@@ -476,7 +485,7 @@ __device__ __forceinline__ bool wait_slot(uint64_t* bar, uint32_t parity, const 
   return tc::mbar_try(bar, parity, 0) || wait_long(bar, parity, p.wait_cycles, p.err, stalled);
 }
 
-template <typename T, int W>
+template <typename T, int W, bool kBeams>
 __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const __grid_constant__ LogprobParams p) {
   constexpr int kWarps = W, kThreads = 32 * W, kTile = kThreads * kVectors;
   using L = Vec<T>;
@@ -491,6 +500,13 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
   const int V = p.vocab, k = p.top;
+  if constexpr (kBeams) {
+    // A beam that has ended, or is none: the whole cluster leaves.
+    if (!(fabsf(p.scores[row]) < INFINITY) || (p.finished && p.finished[row])) {
+      if (slice == 0 && tid == 0) p.beam_rows[row] = BeamRow{0., 0.f, 0};
+      return;
+    }
+  }
   // Vectors are counted from the 16-byte boundary at or before the row; those
   // in [v_begin, v_end) of this slice lie wholly inside the row.  The row's
   // ragged first and last vectors go to the first slice.
@@ -526,7 +542,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
   if (tid == 0)
     for (int i = 0; i < kStages && i < tiles; ++i) fetch(i);
 
-  const int64_t token64 = p.tokens[row];
+  const int64_t token64 = kBeams ? -1 : p.tokens[row];
   const bool given = token64 >= 0 && token64 < V;
   const int token = given ? (int)token64 : -1;
   float xt = INFINITY;  // nothing comes before it
@@ -673,15 +689,15 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
       if (wait_slot(&sh.empty[slot], (uint32_t)((tile / kStages) & 1), p, &sh.stalled)) fetch(tile + kStages);
     }
     if (full) {
-      acc.add<T>(r, tmax);
+      acc.template add<T, !kBeams>(r, tmax);
     } else {
 #pragma unroll
       for (int i = 0; i < kVectors; ++i) {
         const uint4 one[1] = {r[i]};
-        if (t0 + tid + i * kThreads < v_end) acc.add<T>(one, L::max_of(r[i]));
+        if (t0 + tid + i * kThreads < v_end) acc.template add<T, !kBeams>(one, L::max_of(r[i]));
       }
     }
-    if (!(tmax < xt)) {
+    if (!kBeams && !(tmax < xt)) {
       const int first = t0 * kPer - head;  // entry of the tile's first value
       if (full && first > token) {
         auto n = L::zero();
@@ -755,12 +771,13 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
     if (mine) {
       const int e0 = v * kPer - head;
       const uint4 r[1] = {load_ragged<T>(x, e0, V)};
-      acc.add<T>(r, L::max_of(r[0]));
-      rank_each(r[0], e0);
+      acc.template add<T, !kBeams>(r, L::max_of(r[0]));
+      if (!kBeams) rank_each(r[0], e0);
       if (k) offer(r[0], e0);  // fits: a look leaves at most 2 k + 32 candidates
     }
   }
 
+  if (kBeams) asm volatile("griddepcontrol.launch_dependents;");
   // Block totals, then the cluster's in its first block.
   acc.join_warp();
   before = __reduce_add_sync(0xffffffffu, before);
@@ -806,6 +823,11 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
   const bool far = finite && fabsf(t.m) >= kFar;  // the same for the whole block
   if (far) t = far_sums<T, W>(x, V, sh.sums);
   if (tid > 0 && tid >= k) return;
+  if constexpr (kBeams) {
+    if (tid < k) p.beam_keys[row * k + tid] = sh.best[tid];
+    if (tid == 0) p.beam_rows[row] = finite ? BeamRow{t.log_sum(), t.m, k} : BeamRow{0., 0.f, 0};
+    return;
+  }
   float log_sum, entropy;
   t.total(log_sum, entropy);
   const float nan = __uint_as_float(0x7fc00000u);
@@ -822,13 +844,13 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 5) logprobs_kernel(const 
   }
 }
 
-template <typename T, int W>
+template <typename T, int W, bool kBeams>
 tf_status launch(const LogprobParams& p, int slices, cudaStream_t s) {
   constexpr int kThreads = 32 * W, kRing = kStages * kThreads * kVectors * 16;
   static PerDeviceOnce once;
   int dev = 0;
   if (once.needed(&dev)) {
-    TF_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing));
+    TF_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, W, kBeams>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing));
     once.mark(dev);
   }
   cudaLaunchConfig_t cfg{};
@@ -842,9 +864,30 @@ tf_status launch(const LogprobParams& p, int slices, cudaStream_t s) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_kernel<T, W>, p);
-  if (e != cudaSuccess) return set_error(TF_ERR_CUDA, "token_logprobs launch: %s", cudaGetErrorString(e));
-  return check_launch("token_logprobs");
+  const char* name = kBeams ? "beam_select" : "token_logprobs";
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_kernel<T, W, kBeams>, p);
+  if (e != cudaSuccess) return set_error(TF_ERR_CUDA, "%s launch: %s", name, cudaGetErrorString(e));
+  return check_launch(name);
+}
+
+template <bool kBeams>
+tf_status launch_rows(LogprobParams& p, int dtype, cudaStream_t s) {
+  if (p.rows > 2147483647 / kMaxCluster)
+    return set_error(TF_ERR_UNSUPPORTED, "%s: too many rows", kBeams ? "beam_select" : "token_logprobs");
+  TF_TRY(tc_flags(&p.err, const_cast<long long**>(&p.wait_cycles)));
+  // Blocks a row: enough to fill the GPU (about two blocks an SM), each
+  // with at least one vector a thread.  Whole rows go to blocks of 128 threads,
+  // five to an SM: more rows at once cover one another's waits for the prunes.
+  const int vectors = p.vocab / (dtype == TF_DTYPE_F32 ? 4 : 8);
+  int slices = 1;
+  while (slices < kMaxCluster && p.rows * slices * 2 <= 2 * 148 && vectors >= 2 * slices * 256) slices *= 2;
+#define TF_LOGPROBS(T) return slices > 1 ? launch<T, 8, kBeams>(p, slices, s) : launch<T, 4, kBeams>(p, 1, s)
+  switch (dtype) {
+    case TF_DTYPE_F32: TF_LOGPROBS(float);
+    case TF_DTYPE_F16: TF_LOGPROBS(__half);
+    default: TF_LOGPROBS(__nv_bfloat16);
+  }
+#undef TF_LOGPROBS
 }
 
 }  // namespace
@@ -853,23 +896,22 @@ tf_status launch_token_logprobs(const void* logits, int64_t row_stride, int64_t 
                                 const int64_t* tokens, int top, float* logprob, float* entropy, int32_t* rank,
                                 float* top_logprob, int64_t* top_token, cudaStream_t s) {
   if (rows == 0) return TF_OK;
-  if (rows > 2147483647 / kMaxCluster) return set_error(TF_ERR_UNSUPPORTED, "token_logprobs: too many rows");
-  LogprobParams p = {logits, row_stride, tokens, rows, vocab, top, logprob, entropy, rank, top_logprob, top_token,
-                     nullptr, nullptr};
-  TF_TRY(tc_flags(&p.err, const_cast<long long**>(&p.wait_cycles)));
-  // Blocks a row: enough to fill the GPU (about two blocks an SM), each
-  // with at least one vector a thread.  Whole rows go to blocks of 128 threads,
-  // five to an SM: more rows at once cover one another's waits for the prunes.
-  const int vectors = vocab / (dtype == TF_DTYPE_F32 ? 4 : 8);
-  int slices = 1;
-  while (slices < kMaxCluster && rows * slices * 2 <= 2 * 148 && vectors >= 2 * slices * 256) slices *= 2;
-#define TF_LOGPROBS(T) return slices > 1 ? launch<T, 8>(p, slices, s) : launch<T, 4>(p, 1, s)
-  switch (dtype) {
-    case TF_DTYPE_F32: TF_LOGPROBS(float);
-    case TF_DTYPE_F16: TF_LOGPROBS(__half);
-    default: TF_LOGPROBS(__nv_bfloat16);
-  }
-#undef TF_LOGPROBS
+  LogprobParams p = {logits, row_stride, tokens, rows, vocab, top, logprob, entropy, rank, top_logprob, top_token};
+  return launch_rows<false>(p, dtype, s);
+}
+
+tf_status launch_beam_rows(const BeamArgs& a, cudaStream_t s) {
+  LogprobParams p = {};
+  p.logits = a.logits;
+  p.row_stride = a.row_stride;
+  p.rows = a.requests * a.beams;
+  p.vocab = a.vocab;
+  p.top = a.each();
+  p.scores = a.scores;
+  p.finished = a.finished;
+  p.beam_rows = a.rows();
+  p.beam_keys = a.keys();
+  return launch_rows<true>(p, a.dtype, s);
 }
 
 }  // namespace tf

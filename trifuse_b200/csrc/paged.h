@@ -37,6 +37,7 @@ constexpr int kSplitKeys = 32;  // keys per tile
 constexpr int kTileRows = 256;  // packed rows of a segment of the tensor-core kernel (two halves of 128)
 constexpr int kHalfRows = 128;  // of its form with one half
 constexpr int kTileKeys = 128;  // keys per tile
+constexpr int kScaleTokens = TF_SCALE_TOKENS;  // tokens that share a scale of an 8-bit cache
 
 struct PagedArgs {
   const void* q = nullptr;
@@ -49,6 +50,7 @@ struct PagedArgs {
   int act = TF_DTYPE_F16;
   void* out = nullptr;
   char* workspace = nullptr;
+  tf_paged_scales scales{};  // of an 8-bit cache
 };
 
 // Fills the plan's remaining fields, and the table where it fits.
@@ -58,8 +60,13 @@ tf_status paged_plan_make(const int32_t* new_lengths, const int32_t* kv_lengths,
 // columns], box of box_rows rows by box_columns columns of one page, 128-byte
 // swizzle; a page id outside [0, pages) reads zeros.
 tf_status make_page_map(void* map, const void* base, const tf_paged_kv& kv, int box_rows, int box_columns);
+// The same over 8-bit codes: [page][kv_head * page_size rows][head_dim], box of
+// box_rows whole rows, 128-byte swizzle at head_dim 128, 64-byte at 64.
+tf_status make_code_map(void* map, const void* base, const tf_paged_kv& kv, int box_rows);
 tf_status launch_paged_split(const PagedArgs& a, cudaStream_t s);
 tf_status launch_paged_tile(const PagedArgs& a, cudaStream_t s);
+tf_status launch_paged_split_8bit(const PagedArgs& a, cudaStream_t s);
+tf_status launch_paged_tile_8bit(const PagedArgs& a, cudaStream_t s);
 // Workspace of the few-rows kernel's parts: per part and row the maximum, the
 // sum, the outputs.  The tensor-core kernels' parts follow it.
 inline size_t split_workspace_bytes(const tf_paged_plan& p) {
@@ -83,5 +90,7 @@ struct AppendArgs {
   void* q_out = nullptr;
 };
 tf_status launch_paged_append(const AppendArgs& a, cudaStream_t s);
+tf_status launch_paged_append_8bit(const AppendArgs& a, const tf_paged_scales& scales, cudaStream_t s);
+
 
 }  // namespace tf

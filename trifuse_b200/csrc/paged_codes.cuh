@@ -1,0 +1,75 @@
+// Codes of an 8-bit cache: the storage types I8 and E4M3, narrowing and
+// widening.  Both widen to f16 without rounding (integers up to 127; e4m3 has
+// 4 bits of precision and magnitudes from 2^-9 to 448).
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace tf {
+
+struct I8 {
+  uint8_t bits;
+};
+struct E4M3 {
+  uint8_t bits;
+};
+
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
+
+template <typename S>
+struct Code;
+
+template <>
+struct Code<I8> {
+  static constexpr tf_dtype kDtype = TF_DTYPE_I8;
+  static constexpr float kLargest = 127.f;
+  // A byte c + 128 under 0x64 is the f16 number 1024 + 128 + c.
+  __device__ __forceinline__ static uint32_t lift(uint32_t biased, uint32_t select) {
+    return half2_bits(__hsub2(bits_half2(__byte_perm(biased, 0x64646464u, select)), bits_half2(0x64806480u)));
+  }
+  // Four codes -> f16 pairs (0, 1) and (2, 3).
+  __device__ __forceinline__ static void widen(uint32_t w, uint32_t& a, uint32_t& b) {
+    const uint32_t u = w ^ 0x80808080u;
+    a = lift(u, 0x4140);
+    b = lift(u, 0x4342);
+  }
+  // Four codes -> f16 pairs (0, 2) and (1, 3).
+  __device__ __forceinline__ static void widen_cross(uint32_t w, uint32_t& a, uint32_t& b) {
+    const uint32_t u = w ^ 0x80808080u;
+    a = lift(u, 0x4240);
+    b = lift(u, 0x4341);
+  }
+  // Four values -> codes, the first in the lowest byte.
+  __device__ __forceinline__ static uint32_t narrow(float x, float y, float z, float w) {
+    const auto one = [](float v) { return (uint32_t)__float2int_rn(fminf(fmaxf(v, -127.f), 127.f)) & 0xffu; };
+    return one(x) | one(y) << 8 | one(z) << 16 | one(w) << 24;
+  }
+};
+
+template <>
+struct Code<E4M3> {
+  static constexpr tf_dtype kDtype = TF_DTYPE_E4M3;
+  static constexpr float kLargest = 448.f;
+  __device__ __forceinline__ static uint32_t pair(uint32_t two) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(r) : "r"(two));
+    return r;
+  }
+  __device__ __forceinline__ static void widen(uint32_t w, uint32_t& a, uint32_t& b) {
+    a = pair(w & 0xffffu);
+    b = pair(w >> 16);
+  }
+  __device__ __forceinline__ static void widen_cross(uint32_t w, uint32_t& a, uint32_t& b) {
+    widen(__byte_perm(w, 0, 0x3120), a, b);
+  }
+  __device__ __forceinline__ static uint32_t narrow(float x, float y, float z, float w) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(z, w), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+  }
+};
+
+}  // namespace tf

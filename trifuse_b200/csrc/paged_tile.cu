@@ -53,6 +53,17 @@
 // P is rounded to the cache's 16-bit type, relative 2^-11 (f16, down to 2^-21 of
 // the row's largest) or 2^-8 (bf16), the size of the output's own rounding; l
 // sums the unrounded values.
+// An 8-bit cache (storage I8 or E4M3, C = f16) adds a warpgroup (one half: two
+// warps) that widens the tiles on their way: TMA brings codes into a small ring,
+// the wideners write them as f16, exactly, into the ring that the products read.
+// The scales of a tile's 16-token blocks go to the softmax: s_k into the factor
+// of the exponent's argument and of the block's maximum, and s_v / r into the
+// weights as a summand log2(s_v / r) of the argument, which the row's sum takes
+// out again block by block: P' = 2^(s s_k - m + log2(s_v / r)), l += (r / s_v)
+// sum P', O += P' V.  That costs a few instructions a block, none a score, and
+// rounds nothing but P'.  r is a power of two at or above all value scales of the
+// segment so far; O is rescaled where it grows, along with the maximum.
+//
 // Every wait is bounded; an expired one records an error code (tf_device_error)
 // and all roles stop.
 //
@@ -66,8 +77,11 @@
 #include <math.h>
 #include <string.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "paged.h"
+#include "paged_codes.cuh"
 #include "paged_values.cuh"
 #include "tc_ptx.cuh"
 
@@ -85,19 +99,33 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 7.f;
 constexpr int kColBytes = kTileKeys * 128;  // 64 columns of a tile: 128 rows of 128 bytes
 
-// A block of H halves: two of them one to an SM, or one half two to an SM.
-template <int D, int H>
+// A block of H halves: two of them one to an SM, or one half two to an SM.  St:
+// what the pages hold; the products' type C, or codes.
+template <int D, int H, typename C, typename St>
 struct Shape {
+  static constexpr bool kCoded = !std::is_same<St, C>::value;
   static constexpr int kTile = D / 64 * kColBytes;  // bytes of 128 rows or keys
-  static constexpr int kSlots = (H == 2 ? 160 : 64) * 1024 / kTile - (H == 2 && D == 64 ? 2 : 0);  // ring of K and V
+  // Ring of K and V.
+  static constexpr int kSlots = kCoded ? (H == 2 ? (D == 128 ? 4 : 6) : D == 128 ? 2 : 4)
+                                       : (H == 2 ? 160 : 64) * 1024 / kTile - (H == 2 && D == 64 ? 2 : 0);
+  // Ring of codes: a slot holds that many keys (or values).
+  static constexpr int kRawKeys = H == 1 && D == 128 ? 64 : kTileKeys;
+  static constexpr int kRaw = kRawKeys * D;
+  static constexpr int kRawSlots = kCoded ? (D == 128 ? 2 : H == 2 ? 4 : 2) : 0;
   static constexpr int kOffRing = H * kTile;        // after the halves' queries
-  static constexpr int kOffBar = kOffRing + kSlots * kTile;
-  static constexpr int kSmem = kOffBar + 512 + 1024;  // + barriers + alignment slack
-  static_assert(kSmem <= 227 * 1024 / (3 - H) - (2 - H) * 1024, "shared memory of an SM");
+  static constexpr int kOffRaw = kOffRing + kSlots * kTile;
+  static constexpr int kOffBar = kOffRaw + kRawSlots * kRaw;
+  static constexpr int kBarBytes = kCoded ? 1024 * H : 512;
+  // + barriers + alignment slack.  (Two blocks of codes on an SM have no room for
+  // the slack; without static shared memory the base is aligned, and checked.)
+  static constexpr int kSlack = kCoded && H == 1 ? 0 : 1024;
+  static constexpr int kSmem = kOffBar + kBarBytes + kSlack;
+  static_assert(kSmem <= 227 * 1024 / (3 - H) - (2 - H) * (kCoded ? 512 : 1024), "shared memory of an SM");
   // Warps: softmax 0 .. 4 H - 1, then the halves' MMA warps, then the loader
-  // (with two halves one more fills the third warpgroup).
+  // (with two halves one more fills the third warpgroup), then the wideners.
   static constexpr int kMmaWarp = 4 * H, kLoadWarp = 5 * H;
-  static constexpr int kThreads = H == 2 ? 384 : 192;
+  static constexpr int kWidenWarp = H == 2 ? 12 : 6, kWideners = H == 2 ? 128 : 64;
+  static constexpr int kThreads = (H == 2 ? 384 : 192) + (kCoded ? kWideners : 0);
   static constexpr uint32_t kColumns = 256 * H, kColS = 128 * H;
   static constexpr int kRows = kHalf * H;
 };
@@ -110,7 +138,7 @@ struct TileParams {
   int64_t ids_stride;
   int32_t columns;
   int32_t page_size, page_shift;
-  int32_t box_rows;  // min(page_size, kTileKeys)
+  int32_t box_rows;  // min(page_size, kTileKeys), of codes min(page_size, 64)
   int32_t group, heads;
   const void* v;  // the value pages, for values that are not finite
   int64_t pages, page_stride;
@@ -122,6 +150,9 @@ struct TileParams {
   float scale_log2;
   int* err;
   const long long* wait_cycles;
+  const float* k_scales;  // of codes
+  const float* v_scales;
+  int64_t scale_stride;
 };
 
 struct Control {
@@ -167,6 +198,43 @@ __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int 
       "[%6];" ::"r"(smem_addr(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(half), "r"(page), "r"(smem_addr(bar))
       : "memory");
+}
+
+// `row` .. of a page of codes, all columns.
+__device__ __forceinline__ void tma_codes(void* dst, const CUtensorMap* map, int row, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(page), "r"(smem_addr(bar))
+      : "memory");
+}
+// One value, or zero, into shared memory; the barrier's phase waits for the
+// copies that a thread has begun before it arrives.
+__device__ __forceinline__ void copy_value(float* dst, const float* src, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(real ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void arrive_with_copies(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+// The power of two at or above a positive finite value (at most 2^127).
+__device__ __forceinline__ float power_above(float v) {
+  return __uint_as_float(min((__float_as_uint(v) + 0x7fffffu) & 0x7f800000u, 0x7f000000u));
+}
+constexpr float kLeastRef = 1.17549435e-38f;  // 2^-126
+// What the wideners say of a tile of codes.  Zero scales and ratios stay above
+// 2^-100 and 2^-60, where nothing is left of what they scale.
+struct TileScales {
+  float k[8];      // s_k of each block of 16 keys
+  float v_log[8];  // log2(s_v / r)
+  float v_inv[8];  // r / s_v
+  float v_ref;     // r
+  float pad[7];
+};
+// The reference of scales: a power of two at or above those that are finite.
+__device__ __forceinline__ float raise_ref(float ref, float scale) {
+  return scale > ref && scale < INFINITY ? power_above(scale) : ref;
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
@@ -310,12 +378,17 @@ __device__ __forceinline__ void add_cleared(const TileParams& p, const PagedSegm
   }
 }
 
-template <typename T, typename C, int D, int H>
-__global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
+template <typename T, typename C, int D, int H, typename St>
+__global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
     paged_tile_kernel(const __grid_constant__ TileParams p) {
-  using S = Shape<D, H>;
+  using S = Shape<D, H, C, St>;
+  constexpr bool kCoded = S::kCoded;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  if (S::kSlack == 0 && base != smem_raw) {  // does not happen
+    if (threadIdx.x == 0) atomicCAS(p.err, 0, 92);
+    return;
+  }
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + S::kOffBar);
   uint64_t* q_full = bars;       // [2] 128 threads: the half's query rows are written
   uint64_t* s_full = bars + 2;   // [2] MMA: scores of a tile
@@ -328,14 +401,19 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
   uint64_t* baton = done + 2;                // [2] the other half's products of a tile are issued
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(baton + 2);
   Control* ctl = reinterpret_cast<Control*>(baton + 3);
+  uint64_t* raw_full = baton + 6;               // [raw slots] TMA, and each lane's scales
+  uint64_t* raw_empty = raw_full + S::kRawSlots;  // [raw slots] each warp of the wideners
+  float* scales = reinterpret_cast<float*>(raw_empty + S::kRawSlots);  // [4 tiles][k, v][8]
+  TileScales* told = reinterpret_cast<TileScales*>(scales + 64);  // [4 tiles]
   static_assert((12 + 2 * S::kSlots + 5) * 8 + sizeof(Control) <= 512, "barrier block");
+  static_assert(!kCoded || (20 + 2 * S::kSlots + 2 * S::kRawSlots) * 8 + 256 + 4 * sizeof(TileScales) <= S::kBarBytes, "barrier block");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int* err = p.err;
   if (tid == 0) {
     for (int x = 0; x < H; ++x) {
       mbar_init(&q_full[x], kHalf);
-      mbar_init(&s_full[x], 1);
+      mbar_init(&s_full[x], kCoded ? 2 : 1);
       mbar_init(&p_full[2 * x], kHalf);
       mbar_init(&p_full[2 * x + 1], kHalf);
       mbar_init(&o_full[x], 2);
@@ -344,8 +422,12 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
       mbar_init(&baton[x], 1);
     }
     for (int i = 0; i < S::kSlots; ++i) {
-      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_full[i], kCoded ? S::kWideners : 1);
       mbar_init(&kv_empty[i], H);
+    }
+    for (int i = 0; i < S::kRawSlots; ++i) {
+      mbar_init(&raw_full[i], 33);
+      mbar_init(&raw_empty[i], S::kWideners / 32);
     }
     ctl->abort = 0;
     ctl->cleared = 0;
@@ -368,9 +450,150 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
   const int seg0 = p.starts[blockIdx.x], seg1 = p.starts[blockIdx.x + 1];
 
   if (warp >= S::kMmaWarp) {
-    // 384 threads x 168 registers = 2 x 128 x 208 + 128 x 88.
-    if constexpr (H == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == S::kLoadWarp) {
+    // 384 threads x 168 registers = 2 x 128 x 208 + 128 x 88; with codes 512 x 128 =
+    // 2 x 128 x 200 + 128 x 56 + 128 x 56, or 256 x 128 = 128 x 200 + 128 x 56.
+    if constexpr (kCoded)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    else if constexpr (H == 2)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (kCoded && warp == S::kLoadWarp) {
+      if constexpr (kCoded) {
+      constexpr int kChunks = kTileKeys / S::kRawKeys;
+      int m = 0, t = 0;  // chunks and tiles fetched
+      bool ok = true;
+      for (int seg = seg0; seg < seg1 && ok; ++seg) {
+        const PagedSegment g = p.segments[seg];
+        const View<H> view(g, p.group);
+        const int32_t* ids = p.ids + g.request * p.ids_stride;
+        const int box_bytes = p.box_rows * D;
+        for (int j = 0; j < view.tiles && ok; ++j, ++t) {
+          const int key0 = (g.tile0 + j) * kTileKeys;
+          // Lane i brings the scale of block i % 8 of the tile's keys (i < 8) or values
+          // (i < 16).
+          int64_t scale_page = -1;
+          const int scale_key = key0 + (lane & 7) * kScaleTokens;
+          if (lane < 16 && scale_key < g.kv_len && scale_key >> p.page_shift < p.columns)
+            scale_page = __ldg(ids + (scale_key >> p.page_shift));
+#pragma unroll 1
+          for (int c = 0; c < 2 * kChunks && ok; ++c, ++m) {
+            const bool v = c >= kChunks;
+            const int slot = m % S::kRawSlots, turn = m / S::kRawSlots;
+            const int chunk0 = key0 + c % kChunks * S::kRawKeys;
+            const int left = min(g.kv_len - chunk0, S::kRawKeys);
+            const int boxes = left > 0 ? (left + p.box_rows - 1) / p.box_rows : 0;
+            // Lane i fetches box i (at most 8 of the chunk's pages).
+            int page = -1, row = 0;
+            if (lane < boxes) {
+              const int key = chunk0 + lane * p.box_rows, column = key >> p.page_shift;
+              if (column < p.columns) page = __ldg(ids + column);
+              row = g.kv_head * p.page_size + (key & (p.page_size - 1));
+            }
+            if (turn > 0 && !(ok = wait_warp(&raw_empty[slot], (uint32_t)((turn - 1) & 1), ctl, err, 93))) break;
+            if (lane == 0) mbar_expect_tx(&raw_full[slot], (uint32_t)(boxes * box_bytes));
+            __syncwarp();
+            if (lane < boxes)
+              tma_codes(base + S::kOffRaw + slot * S::kRaw + lane * box_bytes, v ? &p.tm_v : &p.tm_k, row, page,
+                        &raw_full[slot]);
+            if (c == 0 && lane < 16) {
+              const bool real = scale_page >= 0 && scale_page < p.pages;
+              const float* from = lane < 8 ? p.k_scales : p.v_scales;
+              if (real)
+                from += scale_page * p.scale_stride + g.kv_head * (p.page_size / kScaleTokens) +
+                        (scale_key & (p.page_size - 1)) / kScaleTokens;
+              copy_value(scales + (t & 3) * 16 + lane, from, real);
+            }
+            arrive_with_copies(&raw_full[slot]);
+          }
+        }
+      }
+      // Copies in flight land before the block exits.
+      for (int i = m > S::kRawSlots ? m - S::kRawSlots : 0; i < m; ++i)
+        drain(&raw_full[i % S::kRawSlots], (uint32_t)((i / S::kRawSlots) & 1), err);
+      }
+    } else if (kCoded && warp >= S::kWidenWarp) {
+      if constexpr (kCoded) {
+      constexpr int kChunks = kTileKeys / S::kRawKeys;
+      constexpr int kRowVectors = D / 16;  // 16-byte vectors of a row of codes
+      const int me = tid - 32 * S::kWidenWarp;
+      int n = 0, m = 0, t = 0;  // slots of the ring, chunks, tiles
+      bool ok = true;
+      for (int seg = seg0; seg < seg1 && ok; ++seg) {
+        const PagedSegment g = p.segments[seg];
+        const View<H> view(g, p.group);
+        float ref = kLeastRef;  // r: of the segment's values so far
+        for (int j = 0; j < view.tiles && ok; ++j, ++t) {
+          const int have = g.kv_len - (g.tile0 + j) * kTileKeys;
+#pragma unroll 1
+          for (int v = 0; v < 2 && ok; ++v, ++n) {
+            const int slot = n % S::kSlots, turn = n / S::kSlots;
+            if (turn > 0 && !(ok = wait_warp(&kv_empty[slot], (uint32_t)((turn - 1) & 1), ctl, err, 94))) break;
+            uint8_t* dst = base + S::kOffRing + slot * S::kTile;
+#pragma unroll 1
+            for (int c = 0; c < kChunks; ++c, ++m) {
+              const int raw = m % S::kRawSlots;
+              if (!(ok = wait_warp(&raw_full[raw], (uint32_t)((m / S::kRawSlots) & 1), ctl, err, 95))) break;
+              if (c == 0 && v == 0 && warp == S::kWidenWarp) {
+                // Lane i speaks of block i; four tiles of this are enough, because a tile's
+                // keys are overwritten only once its weights are there.
+                const float* from = scales + (t & 3) * 16;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ref = raise_ref(ref, from[8 + i]);
+                if (lane < 8) {
+                  TileScales& to = told[t & 3];
+                  const float k = from[lane], v_scale = from[8 + lane];
+                  const float ratio = v_scale * (1.f / ref);
+                  to.k[lane] = fabsf(k) < INFINITY ? fmaxf(k, 7.8886091e-31f) : __uint_as_float(0x7fc00000u);
+                  const bool finite = fabsf(v_scale) < INFINITY;
+                  const float some = fmaxf(ratio, 8.6736174e-19f);
+                  to.v_log[lane] = finite ? log2f(some) : __uint_as_float(0x7fc00000u);
+                  to.v_inv[lane] = finite ? 1.f / some : __uint_as_float(0x7fc00000u);
+                  if (lane == 0) to.v_ref = ref;
+                }
+              }
+              const uint8_t* src = base + S::kOffRaw + raw * S::kRaw;
+              // Vectors in flight: each thread has kRawKeys * D / 16 / kWideners of a chunk.
+              constexpr int kBatch = 4;
+              static_assert(S::kRawKeys * kRowVectors % (kBatch * S::kWideners) == 0, "batches");
+#pragma unroll 1
+              for (int i0 = me; i0 < S::kRawKeys * kRowVectors; i0 += kBatch * S::kWideners) {
+                uint4 w[kBatch];
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b) {
+                  const int i = i0 + b * S::kWideners, r = i / kRowVectors, vec = i % kRowVectors;
+                  w[b] = *reinterpret_cast<const uint4*>(
+                      src + r * D + ((D == 128 ? vec ^ (r & 7) : vec ^ ((r >> 1) & 3)) << 4));
+                }
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b) {
+                  const int i = i0 + b * S::kWideners, r = i / kRowVectors, vec = i % kRowVectors;
+                  const int row = c * S::kRawKeys + r;
+                  // Past the request's length anything may lie, NaN included: zeros.
+                  if (row >= have) w[b] = make_uint4(0, 0, 0, 0);
+                  uint4 out[2];
+                  Code<St>::widen(w[b].x, out[0].x, out[0].y);
+                  Code<St>::widen(w[b].y, out[0].z, out[0].w);
+                  Code<St>::widen(w[b].z, out[1].x, out[1].y);
+                  Code<St>::widen(w[b].w, out[1].z, out[1].w);
+                  // The first and second column halves lie in the same banks: their threads
+                  // store their two vectors in opposite order.
+                  const int half = vec >> 2, pair = (vec & 3) * 2;
+                  uint8_t* to = dst + half * kColBytes + row * 128;
+                  const int x = half & 1;
+                  *reinterpret_cast<uint4*>(to + (((pair + x) ^ (row & 7)) << 4)) = x ? out[1] : out[0];
+                  *reinterpret_cast<uint4*>(to + (((pair + 1 - x) ^ (row & 7)) << 4)) = x ? out[0] : out[1];
+                }
+              }
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&raw_empty[raw]);
+            }
+            if (!ok) break;
+            fence_proxy_async();
+            mbar_arrive(&kv_full[slot]);
+          }
+        }
+      }
+      }
+    } else if (!kCoded && warp == S::kLoadWarp) {
       int n = 0;  // tiles fetched (K and V each count)
       bool ok = true;
       for (int seg = seg0; seg < seg1 && ok; ++seg) {
@@ -431,6 +654,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
           mma_f16(leader, t_s, sw128_desc(qa + off), sw128_desc(ka + off), id_qk, s > 0 ? 1u : 0u);
         }
         mma_commit(leader, &s_full[x]);
+        if (kCoded && lane == 0) mbar_arrive(&s_full[x]);  // what the wideners said of the tile has been seen
         mma_commit(leader, &kv_empty[slot]);
       };
       for (int seg = seg0; seg < seg1 && ok; ++seg) {
@@ -453,7 +677,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
           const int vs = (n + 1) % S::kSlots;
           uint8_t* vt = base + S::kOffRing + vs * S::kTile;
           const int have = g.kv_len - (g.tile0 + j) * kTileKeys;
-          if (have < kTileKeys) {
+          if (!kCoded && have < kTileKeys) {  // (codes' wideners write zeros there)
             // Slots past the request's length hold anything, NaN included:
             // 0 * NaN would reach the outputs, so their values become zeros
             // (by both halves' warps, each before its own products).
@@ -468,7 +692,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
           // not finite (the other half may read them cleared as well).
           const int hidden = max(hidden0 - j * kTileKeys, 0);
           const int chunks = (min(have, kTileKeys) - hidden) * 8;  // of a column half
-          if (chunks > 0) {
+          if (!kCoded && chunks > 0) {  // (codes are finite)
             uint8_t* first = vt + hidden * 128;
             bool finite = true;
 #pragma unroll
@@ -528,13 +752,17 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
       drain(&done[x], 0, err);
     }
   } else {
-    if constexpr (H == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    if constexpr (kCoded)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    else if constexpr (H == 2)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax of half x: thread r owns row r = TMEM lane r.
     const int x = warp >> 2;
     const int r = tid - kHalf * x;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t t_o = lane_base + kColO + 128 * x, t_s = lane_base + S::kColS + 128 * x;
     uint32_t s_turn = 0, o_turn = 0;
+    int tiles_before = 0;
     bool ok = true;
     // Copies the query rows of the half's next segment with tiles, from
     // segment `seg` on, into the K-major 128-byte swizzle: row i of each
@@ -609,8 +837,11 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
     copy_queries(seg0);
     for (int seg = seg0; seg < seg1 && ok; ++seg) {
       const PagedSegment g = p.segments[seg];
-      if (kHalf * x >= g.rows) continue;
+      if (!kCoded && kHalf * x >= g.rows) continue;
       const View<H> view(g, p.group);
+      const int tile_at = tiles_before;
+      tiles_before += view.tiles;
+      if (kCoded && kHalf * x >= g.rows) continue;
       const int count = view.count[x];
       // Threads past the rows follow the last one; what they make is dropped.
       const int pr = g.row0 + min(kHalf * x + r, g.rows - 1);
@@ -619,39 +850,66 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
       const int first_limit = g.kv_len - g.new_len + (g.row0 + kHalf * x) / p.group;
       const float scale = Act<T>::kDtype == Act<C>::kDtype ? p.scale_log2 : p.scale_log2 * boost;
       float m = -INFINITY, l = 0.f;
+      float v_ref = 1.f;  // r of O
       for (int j = 0; j < count; ++j) {
         if (!(ok = wait_warp(&s_full[x], s_turn & 1, ctl, err, 90))) break;
         ++s_turn;
         tc_fence_after();
+        const TileScales& of = told[(tile_at + j) & 3];  // of codes
+        float shrink = 1.f;
+        if constexpr (kCoded) {
+          const float ref = of.v_ref;
+          if (j > 0) shrink = v_ref / ref;  // powers of two
+          v_ref = ref;
+        }
         float sc[128];
 #pragma unroll
         for (int c = 0; c < 128; c += 32) tmem_ld32_begin(t_s + c, sc + c);
 #pragma unroll
         for (int c = 0; c < 128; c += 32) tmem_wait32(sc + c);
         const int key0 = (g.tile0 + j) * kTileKeys;
-        if (key0 + kTileKeys - 1 > first_limit) {
-          const int lim = limit - key0;  // later columns are masked
+        const bool ragged = key0 + kTileKeys - 1 > first_limit;
+        const int lim = limit - key0;  // later columns are masked
+        if (ragged) {
 #pragma unroll
           for (int c = 0; c < 128; ++c) sc[c] = c > lim ? -INFINITY : sc[c];
         }
         // The maximum of the raw scores (the scale is positive), NaN kept.
         float mp[8];
+        float units[8];  // of codes: a block's factor
+        float mx;
+        if constexpr (kCoded) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mp[i] = max_nan(sc[2 * i], sc[2 * i + 1]);
+          for (int b = 0; b < 8; ++b) {
+            units[b] = scale * of.k[b];
+            if (ragged && 16 * b > lim) units[b] = 1.f;  // a hidden block's scale may be NaN
+            float most = max_nan(sc[16 * b], sc[16 * b + 1]);
 #pragma unroll
-        for (int c = 16; c < 128; c += 16)
+            for (int i = 2; i < 16; i += 2) most = max_nan(most, sc[16 * b + i], sc[16 * b + i + 1]);
+            mp[b] = most * units[b];
+          }
+          mx = max_nan(max_nan(mp[0], mp[1], mp[2]), max_nan(mp[3], mp[4], mp[5]), max_nan(mp[6], mp[7]));
+        } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) mp[i] = max_nan(mp[i], sc[c + 2 * i], sc[c + 2 * i + 1]);
-        float mx = max_nan(max_nan(mp[0], mp[1], mp[2]), max_nan(mp[3], mp[4], mp[5]), max_nan(mp[6], mp[7])) *
-                   scale;
+          for (int i = 0; i < 8; ++i) mp[i] = max_nan(sc[2 * i], sc[2 * i + 1]);
+#pragma unroll
+          for (int c = 16; c < 128; c += 16)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mp[i] = max_nan(mp[i], sc[c + 2 * i], sc[c + 2 * i + 1]);
+          mx = max_nan(max_nan(mp[0], mp[1], mp[2]), max_nan(mp[3], mp[4], mp[5]), max_nan(mp[6], mp[7])) * scale;
+        }
         if (mx == INFINITY) mx = __uint_as_float(0x7fc00000u);  // inf - inf: the row is NaN
         // Far out the product with the scale is rounded by more than the
         // exponential bears: there each score takes the maximum's rounding.
         float unit = scale;
         if (__any_sync(0xffffffffu, fabsf(mx) > kFar)) {
 #pragma unroll
-          for (int c = 0; c < 128; ++c) sc[c] *= scale;
+          for (int c = 0; c < 128; ++c) sc[c] *= kCoded ? units[c / 16] : scale;
           unit = 1.f;
+          if constexpr (kCoded) {
+#pragma unroll
+            for (int b = 0; b < 8; ++b) units[b] = 1.f;
+          }
         }
         float factor = 1.f;
         mx = lifted<C>(mx);
@@ -664,6 +922,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
         // This tile's scores were issued after the last tile's product: O is
         // stable, and P may overlay S.  (The vote is taken on the first tile too:
         // it brings the warp together for the stores of P.)
+        if (kCoded) factor *= shrink;
         if (__any_sync(0xffffffffu, factor != 1.f) && j > 0) {
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
@@ -681,7 +940,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
         // second's exponentials do.
         const float sub = m == -INFINITY ? 0.f : -m;
         const uint64_t sl2 = f2_pack(unit, unit), nm = f2_pack(sub, sub);
-        uint64_t sp[4];
+        uint64_t sp[4], block_unit = 0ull, block_offset = 0ull;
 #pragma unroll
         for (int i = 0; i < 4; ++i) sp[i] = 0ull;
 #pragma unroll
@@ -691,6 +950,26 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
           for (int c = 0; c < 32; ++c) {
             const int k0 = 64 * half + 2 * c;
             float a, b;
+            if constexpr (kCoded) {
+              const int block = k0 / 16;
+              if (c % 8 == 0) {
+                const bool hidden = ragged && 16 * block > lim;
+                const float offset = sub + (hidden ? 0.f : of.v_log[block]);
+                block_unit = f2_pack(units[block], units[block]);
+                block_offset = f2_pack(offset, offset);
+                sp[0] = sp[1] = 0ull;
+              }
+              f2_unpack(f2_fma(f2_pack(sc[k0], sc[k0 + 1]), block_unit, block_offset), a, b);
+              a = fast_exp2(a);
+              b = fast_exp2(b);
+              sp[c & 1] = f2_add(sp[c & 1], f2_pack(a, b));
+              pk[c] = pack2<C>(a, b);
+              if (c % 8 == 7) {
+                const float back = ragged && 16 * block > lim ? 0.f : of.v_inv[block];
+                sp[2 + (block & 1)] = f2_fma(f2_add(sp[0], sp[1]), f2_pack(back, back), sp[2 + (block & 1)]);
+              }
+              continue;
+            }
             f2_unpack(f2_fma(f2_pack(sc[k0], sc[k0 + 1]), sl2, nm), a, b);
             a = fast_exp2(a);
             b = fast_exp2(b);
@@ -704,7 +983,7 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
           mbar_arrive(&p_full[2 * x + half]);
         }
         float s0, s1;
-        f2_unpack(f2_add(f2_add(sp[0], sp[1]), f2_add(sp[2], sp[3])), s0, s1);
+        f2_unpack(kCoded ? f2_add(sp[2], sp[3]) : f2_add(f2_add(sp[0], sp[1]), f2_add(sp[2], sp[3])), s0, s1);
         l += s0 + s1;
       }
       if (!ok) break;
@@ -718,7 +997,8 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
       }
       const bool cleared = ctl->cleared != 0;
       // A row that has seen no key above -inf gives zeros.
-      const float inv = m == -INFINITY ? 0.f : 1.f / l;
+      float inv = m == -INFINITY ? 0.f : 1.f / l;
+      if (kCoded) inv *= v_ref;
       T* orow = static_cast<T*>(p.out) +
                 ((int64_t)(g.q_row + token) * p.heads + g.kv_head * p.group + pr % p.group) * D;
       float* prow = p.part + (int64_t)g.part * S::kRows * D + row * 4;
@@ -741,13 +1021,15 @@ __global__ void __launch_bounds__(Shape<D, H>::kThreads, 3 - H)
           }
         } else if (mine) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(prow + (c + i) * S::kRows) =
-                make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          for (int i = 0; i < 32; i += 4) {
+            float4 four = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            if (kCoded) four.x *= v_ref, four.y *= v_ref, four.z *= v_ref, four.w *= v_ref;
+            *reinterpret_cast<float4*>(prow + (c + i) * S::kRows) = four;
+          }
         }
         __syncwarp();  // the next load takes the whole warp, also where the rows end inside it
       }
-      if (cleared) {
+      if (!kCoded && cleared) {
         if (mine && m != -INFINITY)
           add_cleared<T, C, D>(p, g, limit, g.part < 0 ? orow : nullptr, prow, S::kRows);
         __syncwarp();
@@ -818,14 +1100,14 @@ struct Work {
   float* stat;
 };
 
-template <typename T, typename C, int D, int H>
+template <typename T, typename C, int D, int H, typename St>
 tf_status launch(TileParams p, const Work& w, const char* table, bool early, cudaStream_t s) {
-  using S = Shape<D, H>;
+  using S = Shape<D, H, C, St>;
   if (w.blocks == 0) return TF_OK;
   static PerDeviceOnce attr;
   int dev = 0;
   if (attr.needed(&dev)) {
-    TF_CUDA(cudaFuncSetAttribute(paged_tile_kernel<T, C, D, H>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    TF_CUDA(cudaFuncSetAttribute(paged_tile_kernel<T, C, D, H, St>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  S::kSmem));
     attr.mark(dev);
   }
@@ -843,7 +1125,7 @@ tf_status launch(TileParams p, const Work& w, const char* table, bool early, cud
   cfg.stream = s;
   cfg.attrs = &overlap;
   cfg.numAttrs = early ? 1 : 0;
-  TF_CUDA(cudaLaunchKernelEx(&cfg, paged_tile_kernel<T, C, D, H>, p));
+  TF_CUDA(cudaLaunchKernelEx(&cfg, paged_tile_kernel<T, C, D, H, St>, p));
   TF_TRY(check_launch("paged_tile"));
   if (w.cuts == 0) return TF_OK;
   // grid.z is below 65536: at most one cut item per block.
@@ -862,7 +1144,7 @@ tf_status launch(TileParams p, const Work& w, const char* table, bool early, cud
   return check_launch("paged_merge");
 }
 
-template <typename T, typename C, int D>
+template <typename T, typename C, int D, typename St>
 tf_status launch_both(const TileParams& p, const PagedArgs& a, cudaStream_t s) {
   const tf_paged_plan& plan = *a.plan;
   float* stat = reinterpret_cast<float*>(a.workspace + split_workspace_bytes(plan));
@@ -873,20 +1155,16 @@ tf_status launch_both(const TileParams& p, const PagedArgs& a, cudaStream_t s) {
                      stat + (int64_t)plan.tile_parts * kTileRows * (2 + D)};
   // The first kernel after the few-rows kernel starts on the SMs that it leaves.
   const bool after_split = plan.split_blocks > 0;
-  TF_TRY((launch<T, C, D, 2>(p, tile, a.plan_table, after_split, s)));
-  return launch<T, C, D, 1>(p, half, a.plan_table, after_split && plan.tile_blocks == 0, s);
+  TF_TRY((launch<T, C, D, 2, St>(p, tile, a.plan_table, after_split, s)));
+  return launch<T, C, D, 1, St>(p, half, a.plan_table, after_split && plan.tile_blocks == 0, s);
 }
 
-}  // namespace
-
-tf_status launch_paged_tile(const PagedArgs& a, cudaStream_t s) {
+// What all launches fill in alike.
+tf_status tile_params(const PagedArgs& a, TileParams* out) {
   const tf_paged_plan& plan = *a.plan;
-  if (plan.tile_blocks == 0 && plan.half_blocks == 0) return TF_OK;
-  TileParams p;
+  TileParams& p = *out;
   memset(&p, 0, sizeof(p));
   p.box_rows = a.kv.page_size < kTileKeys ? a.kv.page_size : kTileKeys;
-  TF_TRY(make_page_map(&p.tm_k, a.kv.k, a.kv, p.box_rows, 64));
-  TF_TRY(make_page_map(&p.tm_v, a.kv.v, a.kv, p.box_rows, 64));
   p.q = a.q;
   p.q_stride = a.q_stride;
   p.ids = a.table.ids;
@@ -902,10 +1180,46 @@ tf_status launch_paged_tile(const PagedArgs& a, cudaStream_t s) {
   p.out = a.out;
   p.scale_log2 = a.scale * kLog2e;
   TF_TRY(tc_flags(&p.err, const_cast<long long**>(&p.wait_cycles)));
-#define TF_TILE(T, C) return plan.head_dim == 128 ? launch_both<T, C, 128>(p, a, s) : launch_both<T, C, 64>(p, a, s)
+  return TF_OK;
+}
+
+}  // namespace
+
+tf_status launch_paged_tile(const PagedArgs& a, cudaStream_t s) {
+  const tf_paged_plan& plan = *a.plan;
+  if (plan.tile_blocks == 0 && plan.half_blocks == 0) return TF_OK;
+  TileParams p;
+  TF_TRY(tile_params(a, &p));
+  TF_TRY(make_page_map(&p.tm_k, a.kv.k, a.kv, p.box_rows, 64));
+  TF_TRY(make_page_map(&p.tm_v, a.kv.v, a.kv, p.box_rows, 64));
+#define TF_TILE(T, C) \
+  return plan.head_dim == 128 ? launch_both<T, C, 128, C>(p, a, s) : launch_both<T, C, 64, C>(p, a, s)
   if (a.act == TF_DTYPE_F16) TF_TILE(__half, __half);
   if (a.kv.dtype == TF_DTYPE_F16) TF_TILE(__nv_bfloat16, __half);
   TF_TILE(__nv_bfloat16, __nv_bfloat16);
+#undef TF_TILE
+}
+
+tf_status launch_paged_tile_8bit(const PagedArgs& a, cudaStream_t s) {
+  const tf_paged_plan& plan = *a.plan;
+  if (plan.tile_blocks == 0 && plan.half_blocks == 0) return TF_OK;
+  TileParams p;
+  TF_TRY(tile_params(a, &p));
+  p.box_rows = a.kv.page_size < 64 ? a.kv.page_size : 64;
+  TF_TRY(make_code_map(&p.tm_k, a.kv.k, a.kv, p.box_rows));
+  TF_TRY(make_code_map(&p.tm_v, a.kv.v, a.kv, p.box_rows));
+  p.k_scales = a.scales.k;
+  p.v_scales = a.scales.v;
+  p.scale_stride = a.scales.page_stride;
+  const bool ints = a.kv.dtype == TF_DTYPE_I8;
+#define TF_TILE(T, S)                                                                          \
+  return plan.head_dim == 128 ? launch_both<T, __half, 128, S>(p, a, s) : launch_both<T, __half, 64, S>(p, a, s)
+  if (a.act == TF_DTYPE_F16) {
+    if (ints) TF_TILE(__half, I8);
+    TF_TILE(__half, E4M3);
+  }
+  if (ints) TF_TILE(__nv_bfloat16, I8);
+  TF_TILE(__nv_bfloat16, E4M3);
 #undef TF_TILE
 }
 

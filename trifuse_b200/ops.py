@@ -12,14 +12,15 @@ allocate outputs and scratch.
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 from operator import index
 from typing import NamedTuple
 
 import torch
 from torch import Tensor
 
-from ._lib import (AffineWeight, DTYPE_BF16, DTYPE_F16, DTYPE_F32, MoeArgs, PagedKV, PagedPlanDesc, PageTable, RouterWeight,
-                   TF_ERR_CAPACITY, check, lib)
+from ._lib import (AffineWeight, CopyArray, DTYPE_BF16, DTYPE_E4M3, DTYPE_F16, DTYPE_F32, DTYPE_I8, MoeArgs, PagedKV,
+                   PagedPlanDesc, PagedScales, PageTable, RouterWeight, TF_ERR_CAPACITY, check, lib)
 
 _ACT = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
 
@@ -206,6 +207,53 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0) -> TokenLogprob
                                   entropy.data_ptr(), rank.data_ptr(), top_logprob.data_ptr(), top_token.data_ptr(),
                                   stream))
     return TokenLogprobs(logprob, entropy, rank, top_logprob, top_token)
+
+
+class BeamChoice(NamedTuple):
+    """The continuations that beam_select picks for each request, best first."""
+    score: Tensor   # float32 [requests, count], -inf where there are fewer
+    parent: Tensor  # int32 [requests, count], the beam that goes on; -1
+    token: Tensor   # int64 [requests, count]; -1
+
+
+def beam_select(logits: Tensor, scores: Tensor, count: int | None = None, finished: Tensor | None = None,
+                end: int = -1) -> BeamChoice:
+    """The ``count`` (default: as many as beams, at most 64) most probable
+    continuations of each request over its beams and the vocabulary: logits
+    [requests, beams, vocab] (float32, float16 or bfloat16), scores float32
+    [requests, beams], the beams' log probabilities so far (-inf: no beam).
+
+    A continuation's score is the beam's plus the token's log probability;
+    equal ones in order of the beam, then of the token.  A beam marked in
+    ``finished`` (bool [requests, beams]) goes on as it is, with the token
+    ``end``.  Beams whose logits are no distribution, and tokens at -inf, have
+    no continuation."""
+    if logits.dtype != torch.float32 and logits.dtype not in _ACT:
+        raise ValueError("beam_select: logits must be float32, float16 or bfloat16")
+    if logits.ndim != 3 or scores.shape != logits.shape[:2] or scores.dtype != torch.float32:
+        raise ValueError("beam_select: logits are [requests, beams, vocab], scores float32 [requests, beams]")
+    if finished is not None and (finished.shape != scores.shape or finished.dtype != torch.bool):
+        raise ValueError("beam_select: finished is bool [requests, beams]")
+    R, beams, V = logits.shape
+    count = beams if count is None else index(count)
+    end = index(end)
+    stream = _launch_stream(logits, scores, finished)
+    step = logits.stride(1) if beams > 1 else logits.stride(0) if R > 1 else V  # from row to row
+    if (V > 1 and logits.stride(2) != 1) or step < V or (R > 1 and logits.stride(0) != beams * step):
+        logits, step = logits.contiguous(), V
+    scores = scores.contiguous()
+    if finished is not None:
+        finished = finished.contiguous()
+    nb = C.c_size_t()
+    check(lib().tf_beam_select_workspace_size(R, beams, V, count, nb))
+    ws = _ws(nb.value, logits.device)
+    score = scores.new_empty((R, count))
+    parent = torch.empty_like(score, dtype=torch.int32)
+    token = torch.empty_like(score, dtype=torch.int64)
+    check(lib().tf_beam_select(logits.data_ptr(), step, R, beams, V, _ACT.get(logits.dtype, DTYPE_F32),
+                               scores.data_ptr(), None if finished is None else finished.data_ptr(), end, count,
+                               score.data_ptr(), parent.data_ptr(), token.data_ptr(), ws.data_ptr(), nb.value, stream))
+    return BeamChoice(score, parent, token)
 
 
 def native_olmoe_softmax(x: Tensor) -> Tensor:
@@ -474,13 +522,21 @@ def attention_decode(qkv: Tensor, q_norm: Tensor, k_norm: Tensor, positions: Ten
 # paged key/value cache
 
 
-def _paged_kv(k_pages: Tensor, v_pages: Tensor) -> PagedKV:
+SCALE_TOKENS = 16  # tokens of a page and head that share a scale in an 8-bit cache
+_CODES = {torch.int8: DTYPE_I8, torch.float8_e4m3fn: DTYPE_E4M3}
+
+
+def _paged_kv(k_pages: Tensor, v_pages: Tensor, types=_ACT) -> PagedKV:
     """Descriptor of [pages, kv_heads, page_size, head_dim] caches; only the
     first dimension may have a stride of its own."""
     shape, dtype, stride = k_pages.shape, k_pages.dtype, k_pages.stride()
     if len(shape) != 4 or shape != v_pages.shape or dtype != v_pages.dtype:
         raise ValueError("paged: k_pages and v_pages are [pages, kv_heads, page_size, head_dim] of one dtype")
-    if dtype not in _ACT:
+    if dtype not in types:
+        if types is _CODES:
+            raise ValueError("paged: a cache with scales must be int8 or float8_e4m3fn")
+        if dtype in _CODES:
+            raise ValueError("paged: an 8-bit cache needs k_scales and v_scales")
         raise ValueError("paged: the cache must be float16 or bfloat16")
     pages, heads, size, D = shape
     other = v_pages.stride()
@@ -490,7 +546,26 @@ def _paged_kv(k_pages: Tensor, v_pages: Tensor) -> PagedKV:
     step = stride[0]
     if stride != (step, size * D, D, 1) or stride != other:
         raise ValueError("paged: a page must be contiguous, and k_pages and v_pages laid out alike")
-    return PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), pages, step, heads, size, D, _ACT[dtype])
+    return PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), pages, step, heads, size, D, types[dtype])
+
+
+def _paged_scales(k_scales: Tensor | None, v_scales: Tensor | None, kv: PagedKV) -> PagedScales:
+    """Descriptor of the scales [pages, kv_heads, page_size / 16] of an 8-bit
+    cache; only the first dimension may have a stride of its own."""
+    if k_scales is None or v_scales is None:
+        raise ValueError("paged: k_scales and v_scales go together")
+    heads, blocks = kv.kv_heads, kv.page_size // SCALE_TOKENS
+    shape = (kv.pages, heads, blocks)
+    if k_scales.shape != shape or v_scales.shape != shape or not k_scales.dtype == v_scales.dtype == torch.float32:
+        raise ValueError("paged: scales are float32 [pages, kv_heads, page_size / 16]")
+    step = None
+    for t in (k_scales, v_scales):
+        s = t.stride()  # the stride of a dimension of one is of no meaning
+        own = s[0] if kv.pages > 1 else heads * blocks
+        if (heads > 1 and s[1] != blocks) or (blocks > 1 and s[2] != 1) or step not in (None, own):
+            raise ValueError("paged: a page's scales must be contiguous, and k_scales and v_scales laid out alike")
+        step = own
+    return PagedScales(k_scales.data_ptr(), v_scales.data_ptr(), step)
 
 
 def _page_table(page_table: Tensor) -> PageTable:
@@ -531,7 +606,8 @@ def _rows16(t: Tensor, width: int) -> Tensor:
 
 def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, positions: Tensor,
                  requests: Tensor, heads: int, q_norm: Tensor | None = None, k_norm: Tensor | None = None,
-                 eps: float = 1e-5, rope_theta: float | None = None, out: Tensor | None = None) -> Tensor:
+                 eps: float = 1e-5, rope_theta: float | None = None, out: Tensor | None = None,
+                 k_scales: Tensor | None = None, v_scales: Tensor | None = None) -> Tensor:
     """New tokens into a paged cache: q and k RMS-normalised over their full
     widths (when norms are given) and rotated by halves at ``positions`` (when
     ``rope_theta`` is given), k and v written to the pages (updated in place),
@@ -539,9 +615,18 @@ def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tens
 
     qkv: [rows, (heads + 2 kv_heads) * head_dim] rows q | k | v; positions and
     requests: int32 [rows] on the device; page_table: int32 [requests, pages].
-    A row whose slot the table does not have is not stored."""
-    stream = _launch_stream(qkv, k_pages, v_pages, page_table, positions, requests, q_norm, k_norm, out)
-    kv = _paged_kv(k_pages, v_pages)
+    A row whose slot the table does not have is not stored.
+
+    An 8-bit cache (int8 or float8_e4m3fn pages) comes with k_scales and
+    v_scales, float32 [pages, kv_heads, page_size / 16], updated in place: a
+    block of 16 tokens and a head have the scale of their largest magnitude,
+    which becomes the code 127 (int8) or 448.  Where new tokens raise it, the
+    block's earlier codes are rounded anew.  Rows of a request whose tokens
+    share a block are adjacent, in rising order."""
+    stream = _launch_stream(qkv, k_pages, v_pages, page_table, positions, requests, q_norm, k_norm, out, k_scales,
+                            v_scales)
+    coded = k_scales is not None or v_scales is not None
+    kv = _paged_kv(k_pages, v_pages, _CODES if coded else _ACT)
     D, kv_heads = kv.head_dim, kv.kv_heads
     width = (heads + 2 * kv_heads) * D
     if qkv.ndim != 2 or qkv.shape[1] != width:
@@ -568,9 +653,12 @@ def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tens
         raise ValueError("paged_append: out is a contiguous [rows, heads, head_dim] of qkv's dtype")
     elif out.data_ptr() % 16:  # the kernel cannot store there: copied over
         q = torch.empty_like(out)
-    check(lib().tf_paged_append(qkv.data_ptr(), qkv.stride(0) if rows > 1 else width, rows, heads, _act(qkv), qn, kn,
-                                eps, rope_theta or 0.0, positions.data_ptr(), requests.data_ptr(),
-                                _page_table(page_table), kv, q.data_ptr(), stream))
+    args = (qkv.data_ptr(), qkv.stride(0) if rows > 1 else width, rows, heads, _act(qkv), qn, kn, eps,
+            rope_theta or 0.0, positions.data_ptr(), requests.data_ptr(), _page_table(page_table), kv)
+    if coded:
+        check(lib().tf_paged_append_8bit(*args, _paged_scales(k_scales, v_scales, kv), q.data_ptr(), stream))
+    else:
+        check(lib().tf_paged_append(*args, q.data_ptr(), stream))
     return q if out is None or out is q else out.copy_(q)
 
 
@@ -651,12 +739,16 @@ class PagedPlan:
 
 
 def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, plan: PagedPlan,
-                    scale: float | None = None, out: Tensor | None = None) -> Tensor:
+                    scale: float | None = None, out: Tensor | None = None, k_scales: Tensor | None = None,
+                    v_scales: Tensor | None = None) -> Tensor:
     """Attention of every request's new tokens over its pages: row i of a
     request attends keys 0 .. kv_length - new_length + i; query heads share
     key heads in groups.  q: [rows, heads, head_dim] (rows may be strided);
-    returns [rows, heads, head_dim].  Rows that attend nothing give zeros."""
-    stream = _launch_stream(q, k_pages, v_pages, page_table, plan.table, out)
+    returns [rows, heads, head_dim].  Rows that attend nothing give zeros.
+
+    An 8-bit cache (int8 or float8_e4m3fn pages) comes with the k_scales and
+    v_scales that ``paged_append`` keeps; a plan serves either kind of cache."""
+    stream = _launch_stream(q, k_pages, v_pages, page_table, plan.table, out, k_scales, v_scales)
     shape = plan.shape
     if q.shape != shape:
         raise ValueError("paged_attention: q is [rows, heads, head_dim] of the plan")
@@ -672,11 +764,51 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Ten
         o = torch.empty_like(out)
     if stream != plan.made_on:
         plan.order(stream)
-    check(lib().tf_paged_attention(q.data_ptr(), q.stride(0) if rows > 1 else width, _page_table(page_table),
-                                   _paged_kv(k_pages, v_pages), plan.desc, plan.table_ptr,
-                                   D ** -0.5 if scale is None else scale, _act(q), o.data_ptr(),
-                                   plan.workspace_ptr, plan.workspace_bytes, stream))
+    q_stride = q.stride(0) if rows > 1 else width
+    rest = (plan.desc, plan.table_ptr, D ** -0.5 if scale is None else scale, _act(q), o.data_ptr(),
+            plan.workspace_ptr, plan.workspace_bytes, stream)
+    if k_scales is None and v_scales is None:
+        check(lib().tf_paged_attention(q.data_ptr(), q_stride, _page_table(page_table), _paged_kv(k_pages, v_pages),
+                                       *rest))
+    else:
+        kv = _paged_kv(k_pages, v_pages, _CODES)
+        check(lib().tf_paged_attention_8bit(q.data_ptr(), q_stride, _page_table(page_table), kv,
+                                            _paged_scales(k_scales, v_scales, kv), *rest))
     return o if out is None or out is o else out.copy_(o)
+
+
+def paged_copy(arrays, src, dst):
+    """Page dst[i] becomes page src[i] in every layer of every array (a cache's
+    keys, values and scales: up to 8 tensors [layers, pages, ...] with
+    contiguous pages, updated in place).  src and dst are sequences of ints on
+    the host.  A page may be written once, and not be read as well."""
+    arrays = list(arrays)
+    if not arrays:
+        raise ValueError("paged_copy: no arrays")
+    stream = _launch_stream(*arrays)
+    layers, pages = arrays[0].shape[:2] if arrays[0].ndim > 1 else (0, 0)
+    descs = (CopyArray * len(arrays))()
+    for d, t in zip(descs, arrays):
+        shape, stride, size = t.shape, t.stride(), t.element_size()
+        if len(shape) < 3 or shape[0] != layers or shape[1] != pages:
+            raise ValueError("paged_copy: arrays are [layers, pages, ...] with the same layers and pages")
+        n = 1  # values of a page; the stride of a dimension of one is of no meaning
+        for i in range(len(shape) - 1, 1, -1):
+            if shape[i] != 1 and stride[i] != n:
+                raise ValueError("paged_copy: a page must be contiguous")
+            n *= shape[i]
+        if (pages > 1 and stride[1] < n) or (layers > 1 and stride[0] == 0):
+            raise ValueError("paged_copy: pages share memory")
+        d.base, d.page_bytes = t.data_ptr(), n * size
+        d.layer_stride, d.page_stride = stride[0] * size if layers > 1 else 0, (stride[1] if pages > 1 else n) * size
+    try:
+        src, dst = array("i", src), array("i", dst)
+    except OverflowError:
+        raise ValueError("paged_copy: a page does not fit 32 bits") from None
+    if len(src) != len(dst):
+        raise ValueError("paged_copy: src and dst differ in length")
+    check(lib().tf_paged_copy(descs, len(arrays), layers, pages, src.buffer_info()[0], dst.buffer_info()[0], len(src),
+                              stream))
 
 
 def set_qmm_path(path: int):
