@@ -416,6 +416,11 @@ typedef struct tf_paged_plan {
   int32_t half_merges;
   int32_t split_rows;       /* most packed rows of a request in the few-rows
                                kernel                                        */
+  int32_t widened_requests; /* requests whose 8-bit codes a call widens first */
+  int64_t widened_pages;    /* their pages                                   */
+  int64_t widened_offset;   /* their list in the table                       */
+  size_t widened_bytes;     /* scratch of a call over an 8-bit cache beyond
+                               workspace_bytes                               */
 } tf_paged_plan;
 
 /* new_lengths[i] query rows and kv_lengths[i] cached tokens (the new ones
@@ -479,9 +484,11 @@ int tf_paged_append_8bit(const void* qkv, int64_t qkv_stride, int64_t rows, int3
 
 /* tf_paged_attention over an 8-bit cache; the same plans serve both.  The
  * codes enter the products as f16, which holds them exactly; the scales go to
- * the scores and weights (or, for many rows, to the f16 operands, which then
- * are rounded once).  A NaN scale makes the rows NaN that see a token of its
- * block, and only those. */
+ * the scores and weights.  Scales are not negative; a NaN scale makes the rows
+ * NaN that see a token of its block, and only those.  The workspace holds
+ * plan->workspace_bytes + plan->widened_bytes: the codes of requests with many
+ * rows are widened there first (two bytes a code, of this layer's keys and
+ * values). */
 int tf_paged_attention_8bit(const void* q, int64_t q_stride, const tf_page_table* table, const tf_paged_kv* kv,
                             const tf_paged_scales* scales, const tf_paged_plan* plan, void* plan_table, float scale,
                             int act, void* out, void* workspace, size_t workspace_bytes, void* stream);

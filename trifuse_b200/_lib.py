@@ -77,7 +77,8 @@ class PagedPlanDesc(C.Structure):
                 ("columns", C.c_int32), ("split_blocks", C.c_int32), ("split_parts", C.c_int32),
                 ("split_counters", C.c_int32), ("tile_blocks", C.c_int32), ("tile_parts", C.c_int32),
                 ("tile_merges", C.c_int32), ("half_blocks", C.c_int32), ("half_parts", C.c_int32),
-                ("half_merges", C.c_int32), ("split_rows", C.c_int32)]
+                ("half_merges", C.c_int32), ("split_rows", C.c_int32), ("widened_requests", C.c_int32),
+                ("widened_pages", C.c_int64), ("widened_offset", C.c_int64), ("widened_bytes", C.c_size_t)]
 
 
 P = C.c_void_p

@@ -251,6 +251,10 @@ int tf_paged_attention_8bit(const void* q, int64_t q_stride, const tf_page_table
   a.scales = *scales;
   TF_TRY(check_attention(a, table, workspace_bytes));
   if (plan->rows == 0) return TF_OK;
+  if (plan->widened_bytes &&
+      (!a.workspace || !aligned16(a.workspace) || workspace_bytes < plan->workspace_bytes + plan->widened_bytes))
+    return set_error(TF_ERR_INVALID_ARGUMENT, "paged_attention: workspace too small for an 8-bit cache");
+  TF_TRY(launch_paged_widen(a, st(stream)));
   TF_TRY(launch_paged_split_8bit(a, st(stream)));
   return launch_paged_tile_8bit(a, st(stream));
 }

@@ -66,12 +66,55 @@ tf_status make_code_map(void* map, const void* base, const tf_paged_kv& kv, int 
 tf_status launch_paged_split(const PagedArgs& a, cudaStream_t s);
 tf_status launch_paged_tile(const PagedArgs& a, cudaStream_t s);
 tf_status launch_paged_split_8bit(const PagedArgs& a, cudaStream_t s);
+// Widens the codes of the plan's requests with many rows into the workspace,
+// before the tensor-core kernel reads them.
+tf_status launch_paged_widen(const PagedArgs& a, cudaStream_t s);
 tf_status launch_paged_tile_8bit(const PagedArgs& a, cudaStream_t s);
 // Workspace of the few-rows kernel's parts: per part and row the maximum, the
 // sum, the outputs.  The tensor-core kernels' parts follow it.
 inline size_t split_workspace_bytes(const tf_paged_plan& p) {
   return (size_t)p.split_parts * kSplitRows * (2 + p.head_dim) * 4;
 }
+
+// A request whose codes are widened: its pages come one after the other from
+// first_page on, and so do its blocks' scales.
+struct WidenedRequest {
+  int32_t first_page;
+  int32_t request;
+  int32_t kv_len;
+  int32_t pad;
+};
+// In the table: first_page of every request (-1: not widened), then the list.
+inline size_t widened_list_offset(int requests) { return align_up((size_t)requests * 4, 16); }
+inline size_t widened_scale_bytes(const tf_paged_plan& p) {  // of the keys, and of the values
+  return align_up((size_t)p.widened_pages * (p.page_size / kScaleTokens) * p.kv_heads * 4, 256);
+}
+inline size_t widened_code_bytes(const tf_paged_plan& p) {
+  return (size_t)p.widened_pages * p.kv_heads * p.page_size * p.head_dim * 2;
+}
+// Where a call's widened codes and their scales [kv_head][block] lie.
+struct WidenedPages {
+  tf_paged_kv kv;
+  float *k_scales, *v_scales;
+  int64_t blocks;
+  const int32_t* first_page;
+  const WidenedRequest* list;
+  explicit WidenedPages(const PagedArgs& a) {
+    const tf_paged_plan& p = *a.plan;
+    char* at = a.workspace + align_up(p.workspace_bytes, 256);
+    kv = a.kv;
+    kv.dtype = TF_DTYPE_F16;
+    kv.pages = p.widened_pages;
+    kv.page_stride = (int64_t)p.kv_heads * p.page_size * p.head_dim;
+    kv.k = at;
+    kv.v = at + widened_code_bytes(p);
+    k_scales = reinterpret_cast<float*>(at + 2 * widened_code_bytes(p));
+    v_scales = reinterpret_cast<float*>(at + 2 * widened_code_bytes(p) + widened_scale_bytes(p));
+    blocks = p.widened_pages * (p.page_size / kScaleTokens);
+    first_page = reinterpret_cast<const int32_t*>(a.plan_table + p.widened_offset);
+    list = reinterpret_cast<const WidenedRequest*>(a.plan_table + p.widened_offset + widened_list_offset(p.requests));
+  }
+};
 
 struct AppendArgs {
   const void* qkv = nullptr;

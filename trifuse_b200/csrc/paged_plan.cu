@@ -299,12 +299,33 @@ void put_table(const Plans& plans, const int32_t* new_lengths, const int32_t* kv
   at = put(table, at, plans.half.starts);
   p->half_merges_offset = (int64_t)at;
   at = put(table, at, plans.half_merges);
+  p->workspace_bytes = split_workspace_bytes(*p) +
+                       ((size_t)p->tile_parts * kTileRows + (size_t)p->half_parts * kHalfRows) * (2 + p->head_dim) * 4;
+  // Requests of the tensor-core kernel with two halves, for a cache of codes.
+  std::vector<int32_t> first_page;
+  std::vector<WidenedRequest> widened;
+  int64_t pages = 0;
+  if (p->page_size >= kScaleTokens && p->tile_blocks) {
+    first_page.assign(p->requests, -1);
+    for (int r = 0; r < p->requests; ++r)
+      if ((int64_t)new_lengths[r] * (p->heads / p->kv_heads) > kHalfRows && kv_lengths[r] > 0) {
+        first_page[r] = (int32_t)pages;
+        widened.push_back({(int32_t)pages, r, kv_lengths[r], 0});
+        pages += (kv_lengths[r] + p->page_size - 1) / p->page_size;
+      }
+  }
+  p->widened_requests = (int32_t)widened.size();
+  p->widened_pages = pages;
+  p->widened_offset = (int64_t)at;
+  at = put(table, at, first_page);
+  at = put(table, at, widened);
+  p->widened_bytes = pages ? align_up(p->workspace_bytes, 256) - p->workspace_bytes + 2 * widened_code_bytes(*p) +
+                                 2 * widened_scale_bytes(*p)
+                           : 0;
   p->positions_offset = (int64_t)at;
   at = align_up(at + (size_t)p->rows * 4, 16);
   p->requests_offset = (int64_t)at;
   p->table_bytes = align_up(at + (size_t)p->rows * 4, 16);
-  p->workspace_bytes = split_workspace_bytes(*p) +
-                       ((size_t)p->tile_parts * kTileRows + (size_t)p->half_parts * kHalfRows) * (2 + p->head_dim) * 4;
   if (!table) return;
   int32_t* pos = reinterpret_cast<int32_t*>(table + p->positions_offset);
   int32_t* req = reinterpret_cast<int32_t*>(table + p->requests_offset);

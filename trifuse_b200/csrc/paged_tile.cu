@@ -53,16 +53,21 @@
 // P is rounded to the cache's 16-bit type, relative 2^-11 (f16, down to 2^-21 of
 // the row's largest) or 2^-8 (bf16), the size of the output's own rounding; l
 // sums the unrounded values.
-// An 8-bit cache (storage I8 or E4M3, C = f16) adds a warpgroup (one half: two
-// warps) that widens the tiles on their way: TMA brings codes into a small ring,
-// the wideners write them as f16, exactly, into the ring that the products read.
-// The scales of a tile's 16-token blocks go to the softmax: s_k into the factor
-// of the exponent's argument and of the block's maximum, and s_v / r into the
-// weights as a summand log2(s_v / r) of the argument, which the row's sum takes
-// out again block by block: P' = 2^(s s_k - m + log2(s_v / r)), l += (r / s_v)
-// sum P', O += P' V.  That costs a few instructions a block, none a score, and
-// rounds nothing but P'.  r is a power of two at or above all value scales of the
-// segment so far; O is rescaled where it grows, along with the maximum.
+// An 8-bit cache (C = f16): codes widen to f16 exactly, and the scales of a
+// tile's 16-token blocks go to the softmax: s_k into the factor of the exponent's
+// argument and of the block's maximum, and s_v / r into the weights as a summand
+// log2(s_v / r) of the argument, which the row's sum takes out again block by
+// block: P' = 2^(s s_k - m + log2(s_v / r)), l += (r / s_v) sum P', O += P' V.
+// That costs a few instructions a block, none a score, and rounds nothing but P'.
+// r is a power of two at or above all value scales of the segment so far; O is
+// rescaled where it grows, along with the maximum.
+//   Two halves (storage Widened): the requests' codes are widened by a kernel of
+// their own first (paged_widen.cu), for the tensor cores are the limit and a
+// tile is read by many row blocks.  (Widened in this kernel by a warpgroup more,
+// 2048 tokens of 16384 took 702 us; shared memory then carries 96 KB more a tile
+// beside the products' 192, and without that work it were 568.)
+//   One half (storage I8 or E4M3): two warps more widen the tiles on their way,
+// from a small ring of codes that TMA fills into the ring that the products read.
 //
 // Every wait is bounded; an expired one records an error code (tf_device_error)
 // and all roles stop.
@@ -99,35 +104,43 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 7.f;
 constexpr int kColBytes = kTileKeys * 128;  // 64 columns of a tile: 128 rows of 128 bytes
 
+// f16 numbers that are codes: what a request's codes were widened to.
+struct Widened {
+  uint16_t bits;
+};
+
 // A block of H halves: two of them one to an SM, or one half two to an SM.  St:
-// what the pages hold; the products' type C, or codes.
+// what is read; the products' type C, or codes (widened here, or before).
 template <int D, int H, typename C, typename St>
 struct Shape {
-  static constexpr bool kCoded = !std::is_same<St, C>::value;
+  static constexpr bool kScaled = !std::is_same<St, C>::value;
+  static constexpr bool kWiden = kScaled && !std::is_same<St, Widened>::value;
+  static_assert(!kWiden || H == 1, "two halves read widened codes");
   static constexpr int kTile = D / 64 * kColBytes;  // bytes of 128 rows or keys
   // Ring of K and V.
-  static constexpr int kSlots = kCoded ? (H == 2 ? (D == 128 ? 4 : 6) : D == 128 ? 2 : 4)
-                                       : (H == 2 ? 160 : 64) * 1024 / kTile - (H == 2 && D == 64 ? 2 : 0);
+  static constexpr int kSlots = (H == 2 ? 160 : 64) * 1024 / kTile - (H == 2 && D == 64 ? 2 : 0);
   // Ring of codes: a slot holds that many keys (or values).
-  static constexpr int kRawKeys = H == 1 && D == 128 ? 64 : kTileKeys;
+  static constexpr int kRawKeys = D == 128 ? 64 : kTileKeys;
   static constexpr int kRaw = kRawKeys * D;
-  static constexpr int kRawSlots = kCoded ? (D == 128 ? 2 : H == 2 ? 4 : 2) : 0;
+  static constexpr int kRawSlots = kWiden ? 2 : 0;
   static constexpr int kOffRing = H * kTile;        // after the halves' queries
   static constexpr int kOffRaw = kOffRing + kSlots * kTile;
   static constexpr int kOffBar = kOffRaw + kRawSlots * kRaw;
-  static constexpr int kBarBytes = kCoded ? 1024 * H : 512;
-  // + barriers + alignment slack.  (Two blocks of codes on an SM have no room for
+  static constexpr int kBarBytes = !kScaled ? 512 : H == 2 || D == 64 ? 2048 : 1024;
+  // + barriers + alignment slack.  (Two blocks with a ring of codes have no room for
   // the slack; without static shared memory the base is aligned, and checked.)
-  static constexpr int kSlack = kCoded && H == 1 ? 0 : 1024;
+  static constexpr int kSlack = kWiden ? 0 : 1024;
   static constexpr int kSmem = kOffBar + kBarBytes + kSlack;
-  static_assert(kSmem <= 227 * 1024 / (3 - H) - (2 - H) * (kCoded ? 512 : 1024), "shared memory of an SM");
+  static_assert(kSmem <= 227 * 1024 / (3 - H) - (2 - H) * (kWiden ? 512 : 1024), "shared memory of an SM");
   // Warps: softmax 0 .. 4 H - 1, then the halves' MMA warps, then the loader
   // (with two halves one more fills the third warpgroup), then the wideners.
   static constexpr int kMmaWarp = 4 * H, kLoadWarp = 5 * H;
-  static constexpr int kWidenWarp = H == 2 ? 12 : 6, kWideners = H == 2 ? 128 : 64;
-  static constexpr int kThreads = (H == 2 ? 384 : 192) + (kCoded ? kWideners : 0);
+  static constexpr int kWidenWarp = 6, kWideners = 64;
+  static constexpr int kThreads = H == 2 ? 384 : kWiden ? 256 : 192;
   static constexpr uint32_t kColumns = 256 * H, kColS = 128 * H;
   static constexpr int kRows = kHalf * H;
+  // Tiles whose scales are kept: more than lie between the loader and the softmax.
+  static constexpr int kTold = H == 2 ? 8 : D == 64 ? 4 : 2;
 };
 
 struct TileParams {
@@ -150,9 +163,10 @@ struct TileParams {
   float scale_log2;
   int* err;
   const long long* wait_cycles;
-  const float* k_scales;  // of codes
+  const float* k_scales;  // of codes: [page][kv_head][block], or of widened ones: [kv_head][block]
   const float* v_scales;
-  int64_t scale_stride;
+  int64_t scale_stride;   // from page to page, from head to head
+  const int32_t* first_page;  // of each request's widened codes
 };
 
 struct Control {
@@ -223,18 +237,42 @@ __device__ __forceinline__ float power_above(float v) {
   return __uint_as_float(min((__float_as_uint(v) + 0x7fffffu) & 0x7f800000u, 0x7f000000u));
 }
 constexpr float kLeastRef = 1.17549435e-38f;  // 2^-126
-// What the wideners say of a tile of codes.  Zero scales and ratios stay above
-// 2^-100 and 2^-60, where nothing is left of what they scale.
-struct TileScales {
-  float k[8];      // s_k of each block of 16 keys
-  float v_log[8];  // log2(s_v / r)
-  float v_inv[8];  // r / s_v
-  float v_ref;     // r
-  float pad[7];
-};
 // The reference of scales: a power of two at or above those that are finite.
 __device__ __forceinline__ float raise_ref(float ref, float scale) {
   return scale > ref && scale < INFINITY ? power_above(scale) : ref;
+}
+// What is told of a tile of codes, twice where packed pairs are worked on.  Zero
+// scales and ratios stay above 2^-100 and 2^-60, where nothing is left of what
+// they scale; scales that are not finite count as zero, and the rows that see a
+// token of their blocks as NaN.
+struct TileScales {
+  float4 block[8];  // unit, unit, offset, offset: s_k * scale * log2 e, log2(s_v / r)
+  float2 back[8];   // r / s_v
+  float v_ref;      // r
+  uint32_t odd;     // bit b: a scale of block b is not finite
+  uint32_t pad[2];
+};
+// Lane i of a warp, i < 8, has the scales of block i (the other lanes those of
+// i % 8); returns the new r.
+__device__ __forceinline__ float tell(TileScales& to, float k, float v, float scale, float ref, int lane) {
+  const bool odd = !(fabsf(k) < INFINITY && fabsf(v) < INFINITY);
+  if (odd) k = v = 0.f;
+  float most = v;
+#pragma unroll
+  for (int off = 1; off < 8; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+  ref = raise_ref(ref, most);
+  const uint32_t odds = __ballot_sync(0xffffffffu, odd) & 0xffu;
+  if (lane < 8) {
+    const float unit = fmaxf(k, 7.8886091e-31f) * scale, some = fmaxf(v * (1.f / ref), 8.6736174e-19f);
+    const float offset = log2f(some), back = 1.f / some;
+    to.block[lane] = make_float4(unit, unit, offset, offset);
+    to.back[lane] = make_float2(back, back);
+    if (lane == 0) {
+      to.v_ref = ref;
+      to.odd = odds;
+    }
+  }
+  return ref;
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
@@ -382,7 +420,7 @@ template <typename T, typename C, int D, int H, typename St>
 __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
     paged_tile_kernel(const __grid_constant__ TileParams p) {
   using S = Shape<D, H, C, St>;
-  constexpr bool kCoded = S::kCoded;
+  constexpr bool kScaled = S::kScaled, kWiden = S::kWiden;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   if (S::kSlack == 0 && base != smem_raw) {  // does not happen
@@ -404,16 +442,17 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
   uint64_t* raw_full = baton + 6;               // [raw slots] TMA, and each lane's scales
   uint64_t* raw_empty = raw_full + S::kRawSlots;  // [raw slots] each warp of the wideners
   float* scales = reinterpret_cast<float*>(raw_empty + S::kRawSlots);  // [4 tiles][k, v][8]
-  TileScales* told = reinterpret_cast<TileScales*>(scales + 64);  // [4 tiles]
+  TileScales* told = reinterpret_cast<TileScales*>(scales + (kWiden ? 64 : 0));  // [kTold tiles]
   static_assert((12 + 2 * S::kSlots + 5) * 8 + sizeof(Control) <= 512, "barrier block");
-  static_assert(!kCoded || (20 + 2 * S::kSlots + 2 * S::kRawSlots) * 8 + 256 + 4 * sizeof(TileScales) <= S::kBarBytes, "barrier block");
+  static_assert(!kScaled || (20 + 2 * S::kSlots + 2 * S::kRawSlots) * 8 + (kWiden ? 256 : 0) +
+                                    S::kTold * sizeof(TileScales) <= S::kBarBytes, "barrier block");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int* err = p.err;
   if (tid == 0) {
     for (int x = 0; x < H; ++x) {
       mbar_init(&q_full[x], kHalf);
-      mbar_init(&s_full[x], kCoded ? 2 : 1);
+      mbar_init(&s_full[x], kScaled ? 2 : 1);
       mbar_init(&p_full[2 * x], kHalf);
       mbar_init(&p_full[2 * x + 1], kHalf);
       mbar_init(&o_full[x], 2);
@@ -422,7 +461,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
       mbar_init(&baton[x], 1);
     }
     for (int i = 0; i < S::kSlots; ++i) {
-      mbar_init(&kv_full[i], kCoded ? S::kWideners : 1);
+      mbar_init(&kv_full[i], kWiden ? S::kWideners : 1);
       mbar_init(&kv_empty[i], H);
     }
     for (int i = 0; i < S::kRawSlots; ++i) {
@@ -450,14 +489,14 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
   const int seg0 = p.starts[blockIdx.x], seg1 = p.starts[blockIdx.x + 1];
 
   if (warp >= S::kMmaWarp) {
-    // 384 threads x 168 registers = 2 x 128 x 208 + 128 x 88; with codes 512 x 128 =
-    // 2 x 128 x 200 + 128 x 56 + 128 x 56, or 256 x 128 = 128 x 200 + 128 x 56.
-    if constexpr (kCoded)
+    // 384 threads x 168 registers = 2 x 128 x 208 + 128 x 88; with wideners 256 x 128 =
+    // 128 x 200 + 128 x 56.
+    if constexpr (kWiden)
       asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     else if constexpr (H == 2)
       asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (kCoded && warp == S::kLoadWarp) {
-      if constexpr (kCoded) {
+    if (kWiden && warp == S::kLoadWarp) {
+      if constexpr (kWiden) {
       constexpr int kChunks = kTileKeys / S::kRawKeys;
       int m = 0, t = 0;  // chunks and tiles fetched
       bool ok = true;
@@ -510,11 +549,19 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
       for (int i = m > S::kRawSlots ? m - S::kRawSlots : 0; i < m; ++i)
         drain(&raw_full[i % S::kRawSlots], (uint32_t)((i / S::kRawSlots) & 1), err);
       }
-    } else if (kCoded && warp >= S::kWidenWarp) {
-      if constexpr (kCoded) {
+    } else if (kWiden && warp >= S::kWidenWarp) {
+      if constexpr (kWiden) {
       constexpr int kChunks = kTileKeys / S::kRawKeys;
-      constexpr int kRowVectors = D / 16;  // 16-byte vectors of a row of codes
-      const int me = tid - 32 * S::kWidenWarp;
+      // A warp takes 8 rows by 64 columns at a time, 16 codes a thread: eight threads in a
+      // row read two rows and write them to rows whose swizzles keep both apart in the
+      // banks (of 128-byte rows r and r ^ 5, of 64-byte rows neighbours).
+      constexpr int kGroupStep = 8 * (S::kWideners / 32);  // rows from one group of a warp to its next
+      const int quarter = lane >> 3, other = (lane >> 2) & 1, vec = lane & 3;
+      const int row8 = D == 128 ? (other ? quarter ^ 5 : quarter) : 2 * quarter + other;
+      const int my_row = 8 * (warp - S::kWidenWarp) + row8;
+      const int chunk = D == 128 ? vec ^ row8 : vec ^ ((row8 >> 1) & 3);  // the second half's lies 64 bytes on or back
+      const int from_at = my_row * D + chunk * 16, flip = chunk & 4 ? -64 : 64;
+      const int to_at = my_row * 128 + (((2 * vec) ^ row8) << 4), second = (row8 & 1) ? -16 : 16;
       int n = 0, m = 0, t = 0;  // slots of the ring, chunks, tiles
       bool ok = true;
       for (int seg = seg0; seg < seg1 && ok; ++seg) {
@@ -533,54 +580,35 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
               const int raw = m % S::kRawSlots;
               if (!(ok = wait_warp(&raw_full[raw], (uint32_t)((m / S::kRawSlots) & 1), ctl, err, 95))) break;
               if (c == 0 && v == 0 && warp == S::kWidenWarp) {
-                // Lane i speaks of block i; four tiles of this are enough, because a tile's
-                // keys are overwritten only once its weights are there.
                 const float* from = scales + (t & 3) * 16;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) ref = raise_ref(ref, from[8 + i]);
-                if (lane < 8) {
-                  TileScales& to = told[t & 3];
-                  const float k = from[lane], v_scale = from[8 + lane];
-                  const float ratio = v_scale * (1.f / ref);
-                  to.k[lane] = fabsf(k) < INFINITY ? fmaxf(k, 7.8886091e-31f) : __uint_as_float(0x7fc00000u);
-                  const bool finite = fabsf(v_scale) < INFINITY;
-                  const float some = fmaxf(ratio, 8.6736174e-19f);
-                  to.v_log[lane] = finite ? log2f(some) : __uint_as_float(0x7fc00000u);
-                  to.v_inv[lane] = finite ? 1.f / some : __uint_as_float(0x7fc00000u);
-                  if (lane == 0) to.v_ref = ref;
-                }
+                ref = tell(told[t % S::kTold], from[lane & 7], from[8 + (lane & 7)], p.scale_log2, ref, lane);
               }
-              const uint8_t* src = base + S::kOffRaw + raw * S::kRaw;
-              // Vectors in flight: each thread has kRawKeys * D / 16 / kWideners of a chunk.
-              constexpr int kBatch = 4;
-              static_assert(S::kRawKeys * kRowVectors % (kBatch * S::kWideners) == 0, "batches");
-#pragma unroll 1
-              for (int i0 = me; i0 < S::kRawKeys * kRowVectors; i0 += kBatch * S::kWideners) {
-                uint4 w[kBatch];
+              const uint8_t* src = base + S::kOffRaw + raw * S::kRaw + from_at;
+              uint8_t* to = dst + c * S::kRawKeys * 128 + to_at;
+              // The thread's vectors: column halves h, groups of 8 rows.
 #pragma unroll
-                for (int b = 0; b < kBatch; ++b) {
-                  const int i = i0 + b * S::kWideners, r = i / kRowVectors, vec = i % kRowVectors;
-                  w[b] = *reinterpret_cast<const uint4*>(
-                      src + r * D + ((D == 128 ? vec ^ (r & 7) : vec ^ ((r >> 1) & 3)) << 4));
+              for (int h = 0; h < D / 64; ++h) {
+                constexpr int kGroups = S::kRawKeys / 8 / (S::kWideners / 32);
+                uint4 w[kGroups];
+#pragma unroll
+                for (int b = 0; b < kGroups; ++b)
+                  w[b] = *reinterpret_cast<const uint4*>(src + b * kGroupStep * D + (h ? flip : 0));
+                if (have < kTileKeys) {
+                  // Past the request's length anything may lie, NaN included: zeros.
+#pragma unroll
+                  for (int b = 0; b < kGroups; ++b)
+                    if (c * S::kRawKeys + my_row + b * kGroupStep >= have) w[b] = make_uint4(0, 0, 0, 0);
                 }
 #pragma unroll
-                for (int b = 0; b < kBatch; ++b) {
-                  const int i = i0 + b * S::kWideners, r = i / kRowVectors, vec = i % kRowVectors;
-                  const int row = c * S::kRawKeys + r;
-                  // Past the request's length anything may lie, NaN included: zeros.
-                  if (row >= have) w[b] = make_uint4(0, 0, 0, 0);
+                for (int b = 0; b < kGroups; ++b) {
                   uint4 out[2];
                   Code<St>::widen(w[b].x, out[0].x, out[0].y);
                   Code<St>::widen(w[b].y, out[0].z, out[0].w);
                   Code<St>::widen(w[b].z, out[1].x, out[1].y);
                   Code<St>::widen(w[b].w, out[1].z, out[1].w);
-                  // The first and second column halves lie in the same banks: their threads
-                  // store their two vectors in opposite order.
-                  const int half = vec >> 2, pair = (vec & 3) * 2;
-                  uint8_t* to = dst + half * kColBytes + row * 128;
-                  const int x = half & 1;
-                  *reinterpret_cast<uint4*>(to + (((pair + x) ^ (row & 7)) << 4)) = x ? out[1] : out[0];
-                  *reinterpret_cast<uint4*>(to + (((pair + 1 - x) ^ (row & 7)) << 4)) = x ? out[0] : out[1];
+                  uint8_t* at = to + h * kColBytes + b * kGroupStep * 128;
+                  *reinterpret_cast<uint4*>(at) = out[0];
+                  *reinterpret_cast<uint4*>(at + second) = out[1];
                 }
               }
               __syncwarp();
@@ -593,7 +621,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         }
       }
       }
-    } else if (!kCoded && warp == S::kLoadWarp) {
+    } else if (!kWiden && warp == S::kLoadWarp) {
       int n = 0;  // tiles fetched (K and V each count)
       bool ok = true;
       for (int seg = seg0; seg < seg1 && ok; ++seg) {
@@ -601,6 +629,24 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         const View<H> view(g, p.group);
         const int32_t* ids = p.ids + g.request * p.ids_stride;
         const int box_bytes = p.box_rows * 128;
+        // Of widened codes: the request's first page; lane i reads the scales of block
+        // i % 8, a tile ahead.
+        int first_page = 0;
+        const float *k_from = nullptr, *v_from = nullptr;
+        float k_scale = 0.f, v_scale = 0.f, ref = kLeastRef;
+        if constexpr (kScaled) {
+          first_page = __ldg(p.first_page + g.request);
+          const int64_t at = g.kv_head * p.scale_stride + (int64_t)first_page * (p.page_size / kScaleTokens) +
+                             g.tile0 * (kTileKeys / kScaleTokens) + (lane & 7);
+          k_from = p.k_scales + at;
+          v_from = p.v_scales + at;
+        }
+        auto look_at = [&](int j) {
+          const bool real = (g.tile0 + j) * kTileKeys + (lane & 7) * kScaleTokens < g.kv_len;
+          k_scale = real ? __ldg(k_from + 8 * j) : 0.f;
+          v_scale = real ? __ldg(v_from + 8 * j) : 0.f;
+        };
+        if (kScaled && view.tiles > 0) look_at(0);
         for (int j = 0; j < view.tiles && ok; ++j) {
           const int key0 = (g.tile0 + j) * kTileKeys;
           const int left = g.kv_len - key0;
@@ -609,13 +655,24 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
           int page = -1, row = 0;
           if (lane < boxes) {
             const int key = key0 + lane * p.box_rows, column = key >> p.page_shift;
-            if (column < p.columns) page = __ldg(ids + column);
+            if constexpr (kScaled)
+              page = first_page + column;
+            else if (column < p.columns)
+              page = __ldg(ids + column);
             row = g.kv_head * p.page_size + (key & (p.page_size - 1));
           }
 #pragma unroll
           for (int v = 0; v < 2; ++v, ++n) {
             const int slot = n % S::kSlots, turn = n / S::kSlots;
             if (turn > 0 && !(ok = wait_warp(&kv_empty[slot], (uint32_t)((turn - 1) & 1), ctl, err, 81))) break;
+            if constexpr (kScaled) {
+              if (v == 0) {  // seen with the keys
+                ref = tell(told[n / 2 % S::kTold], k_scale, v_scale, p.scale_log2, ref, lane);
+                __syncwarp();
+              } else if (j + 1 < view.tiles) {
+                look_at(j + 1);
+              }
+            }
             if (lane == 0) mbar_expect_tx(&kv_full[slot], (uint32_t)(boxes * box_bytes * (D / 64)));
             __syncwarp();
             if (lane < boxes) {
@@ -654,7 +711,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
           mma_f16(leader, t_s, sw128_desc(qa + off), sw128_desc(ka + off), id_qk, s > 0 ? 1u : 0u);
         }
         mma_commit(leader, &s_full[x]);
-        if (kCoded && lane == 0) mbar_arrive(&s_full[x]);  // what the wideners said of the tile has been seen
+        if (kScaled && lane == 0) mbar_arrive(&s_full[x]);  // what is told of the tile has been seen
         mma_commit(leader, &kv_empty[slot]);
       };
       for (int seg = seg0; seg < seg1 && ok; ++seg) {
@@ -677,7 +734,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
           const int vs = (n + 1) % S::kSlots;
           uint8_t* vt = base + S::kOffRing + vs * S::kTile;
           const int have = g.kv_len - (g.tile0 + j) * kTileKeys;
-          if (!kCoded && have < kTileKeys) {  // (codes' wideners write zeros there)
+          if (!kWiden && have < kTileKeys) {  // (the wideners write zeros there)
             // Slots past the request's length hold anything, NaN included:
             // 0 * NaN would reach the outputs, so their values become zeros
             // (by both halves' warps, each before its own products).
@@ -692,7 +749,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
           // not finite (the other half may read them cleared as well).
           const int hidden = max(hidden0 - j * kTileKeys, 0);
           const int chunks = (min(have, kTileKeys) - hidden) * 8;  // of a column half
-          if (!kCoded && chunks > 0) {  // (codes are finite)
+          if (!kScaled && chunks > 0) {  // (codes are finite)
             uint8_t* first = vt + hidden * 128;
             bool finite = true;
 #pragma unroll
@@ -752,7 +809,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
       drain(&done[x], 0, err);
     }
   } else {
-    if constexpr (kCoded)
+    if constexpr (kWiden)
       asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     else if constexpr (H == 2)
       asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -837,11 +894,11 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
     copy_queries(seg0);
     for (int seg = seg0; seg < seg1 && ok; ++seg) {
       const PagedSegment g = p.segments[seg];
-      if (!kCoded && kHalf * x >= g.rows) continue;
+      if (!kScaled && kHalf * x >= g.rows) continue;
       const View<H> view(g, p.group);
       const int tile_at = tiles_before;
       tiles_before += view.tiles;
-      if (kCoded && kHalf * x >= g.rows) continue;
+      if (kScaled && kHalf * x >= g.rows) continue;
       const int count = view.count[x];
       // Threads past the rows follow the last one; what they make is dropped.
       const int pr = g.row0 + min(kHalf * x + r, g.rows - 1);
@@ -855,9 +912,9 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         if (!(ok = wait_warp(&s_full[x], s_turn & 1, ctl, err, 90))) break;
         ++s_turn;
         tc_fence_after();
-        const TileScales& of = told[(tile_at + j) & 3];  // of codes
+        const TileScales& of = told[(tile_at + j) % S::kTold];
         float shrink = 1.f;
-        if constexpr (kCoded) {
+        if constexpr (kScaled) {
           const float ref = of.v_ref;
           if (j > 0) shrink = v_ref / ref;  // powers of two
           v_ref = ref;
@@ -868,25 +925,28 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
 #pragma unroll
         for (int c = 0; c < 128; c += 32) tmem_wait32(sc + c);
         const int key0 = (g.tile0 + j) * kTileKeys;
-        const bool ragged = key0 + kTileKeys - 1 > first_limit;
-        const int lim = limit - key0;  // later columns are masked
-        if (ragged) {
+        if constexpr (kScaled && Act<T>::kDtype != Act<C>::kDtype) {
+          if (__any_sync(0xffffffffu, boost != 1.f)) {
+#pragma unroll
+            for (int c = 0; c < 128; ++c) sc[c] *= boost;
+          }
+        }
+        if (key0 + kTileKeys - 1 > first_limit) {
+          const int lim = limit - key0;  // later columns are masked
 #pragma unroll
           for (int c = 0; c < 128; ++c) sc[c] = c > lim ? -INFINITY : sc[c];
         }
         // The maximum of the raw scores (the scale is positive), NaN kept.
         float mp[8];
-        float units[8];  // of codes: a block's factor
+        bool raw = true;  // the scores are not yet multiplied with their scale
         float mx;
-        if constexpr (kCoded) {
+        if constexpr (kScaled) {
 #pragma unroll
           for (int b = 0; b < 8; ++b) {
-            units[b] = scale * of.k[b];
-            if (ragged && 16 * b > lim) units[b] = 1.f;  // a hidden block's scale may be NaN
             float most = max_nan(sc[16 * b], sc[16 * b + 1]);
 #pragma unroll
             for (int i = 2; i < 16; i += 2) most = max_nan(most, sc[16 * b + i], sc[16 * b + i + 1]);
-            mp[b] = most * units[b];
+            mp[b] = most * of.block[b].x;
           }
           mx = max_nan(max_nan(mp[0], mp[1], mp[2]), max_nan(mp[3], mp[4], mp[5]), max_nan(mp[6], mp[7]));
         } else {
@@ -904,12 +964,9 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         float unit = scale;
         if (__any_sync(0xffffffffu, fabsf(mx) > kFar)) {
 #pragma unroll
-          for (int c = 0; c < 128; ++c) sc[c] *= kCoded ? units[c / 16] : scale;
+          for (int c = 0; c < 128; ++c) sc[c] *= kScaled ? of.block[c / 16].x : scale;
           unit = 1.f;
-          if constexpr (kCoded) {
-#pragma unroll
-            for (int b = 0; b < 8; ++b) units[b] = 1.f;
-          }
+          raw = false;
         }
         float factor = 1.f;
         mx = lifted<C>(mx);
@@ -922,7 +979,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         // This tile's scores were issued after the last tile's product: O is
         // stable, and P may overlay S.  (The vote is taken on the first tile too:
         // it brings the warp together for the stores of P.)
-        if (kCoded) factor *= shrink;
+        if (kScaled) factor *= shrink;
         if (__any_sync(0xffffffffu, factor != 1.f) && j > 0) {
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
@@ -950,13 +1007,12 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
           for (int c = 0; c < 32; ++c) {
             const int k0 = 64 * half + 2 * c;
             float a, b;
-            if constexpr (kCoded) {
+            if constexpr (kScaled) {
               const int block = k0 / 16;
               if (c % 8 == 0) {
-                const bool hidden = ragged && 16 * block > lim;
-                const float offset = sub + (hidden ? 0.f : of.v_log[block]);
-                block_unit = f2_pack(units[block], units[block]);
-                block_offset = f2_pack(offset, offset);
+                const ulonglong2 both = *reinterpret_cast<const ulonglong2*>(&of.block[block]);
+                block_unit = raw ? both.x : sl2;
+                block_offset = f2_add(nm, both.y);
                 sp[0] = sp[1] = 0ull;
               }
               f2_unpack(f2_fma(f2_pack(sc[k0], sc[k0 + 1]), block_unit, block_offset), a, b);
@@ -965,8 +1021,8 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
               sp[c & 1] = f2_add(sp[c & 1], f2_pack(a, b));
               pk[c] = pack2<C>(a, b);
               if (c % 8 == 7) {
-                const float back = ragged && 16 * block > lim ? 0.f : of.v_inv[block];
-                sp[2 + (block & 1)] = f2_fma(f2_add(sp[0], sp[1]), f2_pack(back, back), sp[2 + (block & 1)]);
+                sp[2 + (block & 1)] = f2_fma(f2_add(sp[0], sp[1]),
+                                             *reinterpret_cast<const uint64_t*>(&of.back[block]), sp[2 + (block & 1)]);
               }
               continue;
             }
@@ -983,8 +1039,14 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
           mbar_arrive(&p_full[2 * x + half]);
         }
         float s0, s1;
-        f2_unpack(kCoded ? f2_add(sp[2], sp[3]) : f2_add(f2_add(sp[0], sp[1]), f2_add(sp[2], sp[3])), s0, s1);
+        f2_unpack(kScaled ? f2_add(sp[2], sp[3]) : f2_add(f2_add(sp[0], sp[1]), f2_add(sp[2], sp[3])), s0, s1);
         l += s0 + s1;
+        if constexpr (kScaled) {
+          if (of.odd) {
+            for (int b = 0; b < 8; ++b)
+              if ((of.odd >> b & 1) && key0 + 16 * b <= limit) l = __uint_as_float(0x7fc00000u);
+          }
+        }
       }
       if (!ok) break;
       const int row = kHalf * x + r;
@@ -995,10 +1057,10 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         ++o_turn;
         tc_fence_after();
       }
-      const bool cleared = ctl->cleared != 0;
+      const bool cleared = !kScaled && ctl->cleared != 0;
       // A row that has seen no key above -inf gives zeros.
       float inv = m == -INFINITY ? 0.f : 1.f / l;
-      if (kCoded) inv *= v_ref;
+      if (kScaled) inv *= v_ref;
       T* orow = static_cast<T*>(p.out) +
                 ((int64_t)(g.q_row + token) * p.heads + g.kv_head * p.group + pr % p.group) * D;
       float* prow = p.part + (int64_t)g.part * S::kRows * D + row * 4;
@@ -1023,13 +1085,13 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
             float4 four = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-            if (kCoded) four.x *= v_ref, four.y *= v_ref, four.z *= v_ref, four.w *= v_ref;
+            if (kScaled) four.x *= v_ref, four.y *= v_ref, four.z *= v_ref, four.w *= v_ref;
             *reinterpret_cast<float4*>(prow + (c + i) * S::kRows) = four;
           }
         }
         __syncwarp();  // the next load takes the whole warp, also where the rows end inside it
       }
-      if (!kCoded && cleared) {
+      if (cleared) {
         if (mine && m != -INFINITY)
           add_cleared<T, C, D>(p, g, limit, g.part < 0 ? orow : nullptr, prow, S::kRows);
         __syncwarp();
@@ -1145,7 +1207,7 @@ tf_status launch(TileParams p, const Work& w, const char* table, bool early, cud
 }
 
 template <typename T, typename C, int D, typename St>
-tf_status launch_both(const TileParams& p, const PagedArgs& a, cudaStream_t s) {
+tf_status launch_both(const TileParams& p, const PagedArgs& a, cudaStream_t s, const TileParams& widened = TileParams()) {
   const tf_paged_plan& plan = *a.plan;
   float* stat = reinterpret_cast<float*>(a.workspace + split_workspace_bytes(plan));
   const Work tile = {plan.tile_segments_offset, plan.tile_starts_offset, plan.tile_merges_offset,
@@ -1155,7 +1217,11 @@ tf_status launch_both(const TileParams& p, const PagedArgs& a, cudaStream_t s) {
                      stat + (int64_t)plan.tile_parts * kTileRows * (2 + D)};
   // The first kernel after the few-rows kernel starts on the SMs that it leaves.
   const bool after_split = plan.split_blocks > 0;
-  TF_TRY((launch<T, C, D, 2, St>(p, tile, a.plan_table, after_split, s)));
+  if constexpr (Shape<D, 1, C, St>::kWiden) {
+    TF_TRY((launch<T, C, D, 2, Widened>(widened, tile, a.plan_table, after_split, s)));
+  } else {
+    TF_TRY((launch<T, C, D, 2, St>(p, tile, a.plan_table, after_split, s)));
+  }
   return launch<T, C, D, 1, St>(p, half, a.plan_table, after_split && plan.tile_blocks == 0, s);
 }
 
@@ -1203,17 +1269,29 @@ tf_status launch_paged_tile(const PagedArgs& a, cudaStream_t s) {
 tf_status launch_paged_tile_8bit(const PagedArgs& a, cudaStream_t s) {
   const tf_paged_plan& plan = *a.plan;
   if (plan.tile_blocks == 0 && plan.half_blocks == 0) return TF_OK;
-  TileParams p;
+  TileParams p, w;
   TF_TRY(tile_params(a, &p));
-  p.box_rows = a.kv.page_size < 64 ? a.kv.page_size : 64;
-  TF_TRY(make_code_map(&p.tm_k, a.kv.k, a.kv, p.box_rows));
-  TF_TRY(make_code_map(&p.tm_v, a.kv.v, a.kv, p.box_rows));
-  p.k_scales = a.scales.k;
-  p.v_scales = a.scales.v;
-  p.scale_stride = a.scales.page_stride;
+  w = p;
+  if (plan.half_blocks) {
+    p.box_rows = a.kv.page_size < 64 ? a.kv.page_size : 64;
+    TF_TRY(make_code_map(&p.tm_k, a.kv.k, a.kv, p.box_rows));
+    TF_TRY(make_code_map(&p.tm_v, a.kv.v, a.kv, p.box_rows));
+    p.k_scales = a.scales.k;
+    p.v_scales = a.scales.v;
+    p.scale_stride = a.scales.page_stride;
+  }
+  if (plan.tile_blocks) {
+    const WidenedPages pages(a);
+    TF_TRY(make_page_map(&w.tm_k, pages.kv.k, pages.kv, w.box_rows, 64));
+    TF_TRY(make_page_map(&w.tm_v, pages.kv.v, pages.kv, w.box_rows, 64));
+    w.k_scales = pages.k_scales;
+    w.v_scales = pages.v_scales;
+    w.scale_stride = pages.blocks;
+    w.first_page = pages.first_page;
+  }
   const bool ints = a.kv.dtype == TF_DTYPE_I8;
-#define TF_TILE(T, S)                                                                          \
-  return plan.head_dim == 128 ? launch_both<T, __half, 128, S>(p, a, s) : launch_both<T, __half, 64, S>(p, a, s)
+#define TF_TILE(T, S) \
+  return plan.head_dim == 128 ? launch_both<T, __half, 128, S>(p, a, s, w) : launch_both<T, __half, 64, S>(p, a, s, w)
   if (a.act == TF_DTYPE_F16) {
     if (ints) TF_TILE(__half, I8);
     TF_TILE(__half, E4M3);

@@ -705,7 +705,7 @@ class PagedPlan:
         self.shape = (d.rows, heads, head_dim)  # of q
         self.rows = d.rows
         self.table_ptr, self.workspace_ptr = self.table.data_ptr(), self.workspace.data_ptr()
-        self.workspace_bytes = d.workspace_bytes
+        self.workspace_bytes, self.widened_bytes = d.workspace_bytes, d.widened_bytes
         at, size = d.positions_offset, 4 * d.rows
         self._positions = self.table[at:at + size].view(torch.int32)
         at = d.requests_offset
@@ -765,15 +765,21 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Ten
     if stream != plan.made_on:
         plan.order(stream)
     q_stride = q.stride(0) if rows > 1 else width
-    rest = (plan.desc, plan.table_ptr, D ** -0.5 if scale is None else scale, _act(q), o.data_ptr(),
-            plan.workspace_ptr, plan.workspace_bytes, stream)
+    scale = D ** -0.5 if scale is None else scale
     if k_scales is None and v_scales is None:
         check(lib().tf_paged_attention(q.data_ptr(), q_stride, _page_table(page_table), _paged_kv(k_pages, v_pages),
-                                       *rest))
+                                       plan.desc, plan.table_ptr, scale, _act(q), o.data_ptr(), plan.workspace_ptr,
+                                       plan.workspace_bytes, stream))
     else:
         kv = _paged_kv(k_pages, v_pages, _CODES)
+        ws, nbytes = plan.workspace_ptr, plan.workspace_bytes
+        if plan.widened_bytes:  # of this call alone: other steps' plans need not hold it
+            nbytes += plan.widened_bytes
+            widened = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            ws = widened.data_ptr()
         check(lib().tf_paged_attention_8bit(q.data_ptr(), q_stride, _page_table(page_table), kv,
-                                            _paged_scales(k_scales, v_scales, kv), *rest))
+                                            _paged_scales(k_scales, v_scales, kv), plan.desc, plan.table_ptr, scale,
+                                            _act(q), o.data_ptr(), ws, nbytes, stream))
     return o if out is None or out is o else out.copy_(o)
 
 
