@@ -53,14 +53,13 @@ template <>
 struct Code<E4M3> {
   static constexpr tf_dtype kDtype = TF_DTYPE_E4M3;
   static constexpr float kLargest = 448.f;
-  __device__ __forceinline__ static uint32_t pair(uint32_t two) {
-    uint32_t r;
-    asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(r) : "r"(two));
-    return r;
-  }
   __device__ __forceinline__ static void widen(uint32_t w, uint32_t& a, uint32_t& b) {
-    a = pair(w & 0xffffu);
-    b = pair(w >> 16);
+    asm("{\n\t.reg .b16 lo, hi;\n\t"
+        "mov.b32 {lo, hi}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, lo;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+        : "=r"(a), "=r"(b)
+        : "r"(w));
   }
   __device__ __forceinline__ static void widen_cross(uint32_t w, uint32_t& a, uint32_t& b) {
     widen(__byte_perm(w, 0, 0x3120), a, b);

@@ -64,19 +64,21 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRowBytes = 128;                        // one swizzled row: 64 values
 
 // S: what the pages hold; the products' type C, or codes.
-template <int D, typename C, typename S>
+template <int D, int NT, typename C, typename S>
 struct Shape {
   static constexpr bool kCoded = !std::is_same<S, C>::value;
-  static constexpr int kWarps = kCoded ? 8 : 4;
+  static constexpr int kWarps = !kCoded ? 4 : NT == 1 ? 12 : 8;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kRow = kCoded ? D : kRowBytes;             // bytes of a row in shared memory
   static constexpr int kHalves = kCoded ? 1 : D / 64;             // column parts that lie apart
   static constexpr int kTile = kHalves * kSplitKeys * kRow;       // bytes of a tile's keys (and of its values)
   static constexpr int kStages = kCoded ? 256 / D : 384 / D;      // 48 KB per warp, of codes 16
   static constexpr int kRing = kStages * 2 * kTile;
-  static constexpr int kPitch = D + 4;                // joined outputs: rows 4 words apart in the banks
+  static constexpr int kJoin = kCoded ? 64 : D;       // columns that are joined at a time
+  static constexpr int kJoinRows = kCoded ? 8 * NT : kSplitRows;
+  static constexpr int kPitch = kJoin + 4;            // joined outputs: rows 4 words apart in the banks
   static constexpr int kOffJoin = kWarps * kRing;
-  static constexpr int kOffStat = kOffJoin + kWarps * kSplitRows * kPitch * 4;
+  static constexpr int kOffStat = kOffJoin + kWarps * kJoinRows * kPitch * 4;
   static constexpr int kOffScale = kOffStat + kWarps * kSplitRows * 2 * 4;  // [warp][stage] k, k, v, v
   static constexpr int kOffRef = kOffScale + (kCoded ? kWarps * kStages * 16 : 0);
   static constexpr int kOffBar = kOffRef + (kCoded ? kWarps * 4 : 0);
@@ -147,12 +149,6 @@ __device__ __forceinline__ void copy_value(float* dst, const float* src, bool re
 __device__ __forceinline__ void arrive_with_copies(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
-// 16-byte chunk `chunk` of row r of a tile of codes (128- or 64-byte swizzle).
-template <int D>
-__device__ __forceinline__ int code_at(int r, int chunk) {
-  return r * D + ((D == 128 ? chunk ^ (r & 7) : chunk ^ ((r >> 1) & 3)) << 4);
-}
-
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -241,9 +237,9 @@ struct Cursor {
 };
 
 template <typename T, typename C, int D, int NT, typename St>  // NT: groups of 8 packed rows
-__global__ void __launch_bounds__(Shape<D, C, St>::kThreads, 1)
+__global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
     paged_split_kernel(const __grid_constant__ SplitParams p) {
-  using S = Shape<D, C, St>;
+  using S = Shape<D, NT, C, St>;
   constexpr bool kCoded = S::kCoded;
   constexpr int kWarps = S::kWarps, kThreads = S::kThreads;
   extern __shared__ uint8_t smem_raw[];
@@ -331,6 +327,10 @@ __global__ void __launch_bounds__(Shape<D, C, St>::kThreads, 1)
   auto key_at = [&](int r) {
     return kCoded ? r * S::kRow : (r >> p.box_shift) * box_bytes + (r & (p.box_rows - 1)) * S::kRow;
   };
+  // Of codes, the lane's 16-byte chunk lane / 16 of row lane % 16 (128- or 64-byte
+  // swizzle); chunk + k, k even, lies at the address ^ 16 k, and 16 rows on the
+  // swizzle is the same.
+  const uint32_t code_at = (lane & 15) * D + ((lane >> 4 ^ (D == 128 ? lane & 7 : lane >> 1 & 3)) << 4);
   int k_at[2], v_at[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(Shape<D, C, St>::kThreads, 1)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t w[4];
-            ldsm4(ks + code_at<D>(16 * h + (lane & 15), k + (lane >> 4)), w);
+            ldsm4((ks + code_at ^ k << 4) + 16 * h * D, w);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               uint32_t a[4];
@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(Shape<D, C, St>::kThreads, 1)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t w[4];
-            ldsm4_t(vs + code_at<D>(16 * h + (lane & 15), d + (lane >> 4)), w);
+            ldsm4_t((vs + code_at ^ d << 4) + 16 * h * D, w);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               uint32_t a[4];
@@ -624,40 +624,48 @@ __global__ void __launch_bounds__(Shape<D, C, St>::kThreads, 1)
           stat[warp * 32 + r] = m[t][i];
           stat[warp * 32 + 16 + r] = l[t][i];
         }
-        float* row = join + (warp * kSplitRows + r) * S::kPitch;
+      }
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
-          row[16 * d + (kCoded ? 2 * g : g)] = o[d][t][i];
-          row[16 * d + (kCoded ? 2 * g + 1 : g + 8)] = o[d][t][i + 2];
+    for (int pass = 0; pass < D / S::kJoin; ++pass) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float* row = join + (warp * S::kJoinRows + 8 * t + c2 + i) * S::kPitch;
+#pragma unroll
+          for (int d = 0; d < S::kJoin / 16; ++d) {
+            row[16 * d + (kCoded ? 2 * g : g)] = o[pass * (S::kJoin / 16) + d][t][i];
+            row[16 * d + (kCoded ? 2 * g + 1 : g + 8)] = o[pass * (S::kJoin / 16) + d][t][i + 2];
+          }
+        }
+      __syncthreads();
+      for (int i = tid; i < sg.rows * S::kJoin; i += kThreads) {
+        const int r = i / S::kJoin, at = i % S::kJoin, d = pass * S::kJoin + at;
+        float M = stat[r];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) M = max_nan(M, stat[w * 32 + r]);
+        float acc = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float f = part_weight(stat[w * 32 + r], M);
+          acc = fmaf(kCoded ? f * refs[w] : f, join[(w * S::kJoinRows + r) * S::kPitch + at], acc);
+          sum = fmaf(f, stat[w * 32 + 16 + r], sum);
+        }
+        if (sg.part < 0) {
+          const int pr = sg.row0 + r;
+          T* orow = static_cast<T*>(p.out) + ((int64_t)(sg.q_row + pr / p.group) * p.heads + sg.kv_head * p.group +
+                                              pr % p.group) * D;
+          orow[d] = from_f<T>(sum == 0.f ? 0.f : acc / sum);
+        } else {
+          p.part[((int64_t)sg.part * kSplitRows + r) * D + d] = acc;
+          if (d == 0) {
+            p.stat[(int64_t)sg.part * 32 + r] = M;
+            p.stat[(int64_t)sg.part * 32 + 16 + r] = sum;
+          }
         }
       }
-    __syncthreads();
-    for (int i = tid; i < sg.rows * D; i += kThreads) {
-      const int r = i / D, d = i % D;
-      float M = stat[r];
-#pragma unroll
-      for (int w = 1; w < kWarps; ++w) M = max_nan(M, stat[w * 32 + r]);
-      float acc = 0.f, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = part_weight(stat[w * 32 + r], M);
-        acc = fmaf(kCoded ? f * refs[w] : f, join[(w * kSplitRows + r) * S::kPitch + d], acc);
-        sum = fmaf(f, stat[w * 32 + 16 + r], sum);
-      }
-      if (sg.part < 0) {
-        const int pr = sg.row0 + r;
-        T* orow = static_cast<T*>(p.out) + ((int64_t)(sg.q_row + pr / p.group) * p.heads + sg.kv_head * p.group +
-                                            pr % p.group) * D;
-        orow[d] = from_f<T>(sum == 0.f ? 0.f : acc / sum);
-      } else {
-        p.part[((int64_t)sg.part * kSplitRows + r) * D + d] = acc;
-        if (d == 0) {
-          p.stat[(int64_t)sg.part * 32 + r] = M;
-          p.stat[(int64_t)sg.part * 32 + 16 + r] = sum;
-        }
-      }
+      __syncthreads();
     }
-    __syncthreads();
     if (sg.part >= 0) {
       // The last piece of these rows to finish merges all of them, in order.
       if (tid == 0) {
@@ -698,7 +706,7 @@ __global__ void __launch_bounds__(Shape<D, C, St>::kThreads, 1)
 
 template <typename T, typename C, int D, int NT, typename St>
 tf_status launch(const SplitParams& p, int blocks, cudaStream_t s) {
-  using S = Shape<D, C, St>;
+  using S = Shape<D, NT, C, St>;
   static PerDeviceOnce attr;
   int dev = 0;
   if (attr.needed(&dev)) {
