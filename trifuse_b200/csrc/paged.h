@@ -101,7 +101,7 @@ struct WidenedPages {
   const WidenedRequest* list;
   explicit WidenedPages(const PagedArgs& a) {
     const tf_paged_plan& p = *a.plan;
-    char* at = a.workspace + align_up(p.workspace_bytes, 256);
+    char* at = reinterpret_cast<char*>(align_up(reinterpret_cast<uintptr_t>(a.workspace) + p.workspace_bytes, 256));
     kv = a.kv;
     kv.dtype = TF_DTYPE_F16;
     kv.pages = p.widened_pages;

@@ -66,238 +66,435 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return y;
 }
 
+// The largest magnitude of 16 values, NaN kept.
+__device__ __forceinline__ float largest(const float2 (&f)[2][4]) {
+  float most = 0.f;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(most) : "f"(f[j][k].x), "f"(f[j][k].y));
+  return most;
+}
+
+// A block's scale: `most` of its new tokens, `old` of its earlier ones (0: none).
+template <typename S>
+__device__ __forceinline__ float block_scale(float most, float old) {
+  float scale = __fdiv_rn(most, Code<S>::kLargest);
+  if (most > 0.f) scale = max_nan(scale, 1.17549435e-38f);  // its reciprocal is finite
+  if (!(most < INFINITY)) scale = __uint_as_float(0x7fc00000u);
+  return max_nan(scale, old);
+}
+
+// `n` vectors of earlier codes times `ratio`; lane `lane` of `lanes`.
+template <typename S>
+__device__ __forceinline__ void round_anew(uint8_t* block, int n, float ratio, int lane, int lanes) {
+  for (int i = lane; i < n; i += lanes) {
+    uint4* at = reinterpret_cast<uint4*>(block) + i;
+    uint4 v = *at;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t a, b;
+      Code<S>::widen(w[k], a, b);
+      const float2 x = __half22float2(bits_half2(a)), y = __half22float2(bits_half2(b));
+      w[k] = Code<S>::narrow(x, y, ratio);
+    }
+    *at = v;
+  }
+}
+
+// 16 values times `by` as codes: 8 at `to`, 8 half a head on.
+template <typename S, int D>
+__device__ __forceinline__ void put_codes(uint8_t* to, const float2 (&f)[2][4], bool finite, float by) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    uint2 w = make_uint2(Code<S>::narrow(f[j][0], f[j][1], by), Code<S>::narrow(f[j][2], f[j][3], by));
+    if (!finite) w = make_uint2(0, 0);
+    *reinterpret_cast<uint2*>(to + j * (D / 2)) = w;
+  }
+}
+
+// cos and sin of an angle of `turns` turns.
+__device__ __forceinline__ void turn(double turns, float& cs, float& sn) {
+  sincospif(2.f * (float)(turns - rint(turns)), &sn, &cs);
+}
+
+// Eight values of a head's first half and their partners: normalised, rotated.
+__device__ __forceinline__ void rotate_pairs(float2 (&f)[2][4], const float* cs, const float* sn) {
+#pragma unroll
+  for (int k = 0; k < 4; k += 2) {
+    const float4 c = *reinterpret_cast<const float4*>(cs + 2 * k), s = *reinterpret_cast<const float4*>(sn + 2 * k);
+#pragma unroll
+    for (int l = 0; l < 2; ++l) {
+      const float2 c2 = l ? make_float2(c.z, c.w) : make_float2(c.x, c.y);
+      const float2 s2 = l ? make_float2(s.z, s.w) : make_float2(s.x, s.y);
+      const float2 a = f[0][k + l], b = f[1][k + l];
+      f[0][k + l] = fma2(a, c2, mul2(b, make_float2(-s2.x, -s2.y)));
+      f[1][k + l] = fma2(a, s2, mul2(b, c2));
+    }
+  }
+}
+
+// The page of a token, -1 where its slot does not exist.
+__device__ __forceinline__ int64_t page_of(const Append8Params& p, int pos, int req) {
+  const int column = pos >> p.page_shift;
+  if (pos < 0 || req < 0 || req >= p.table.requests || column >= p.table.columns) return -1;
+  const int64_t id = p.table.ids[req * p.table.stride + column];
+  return id >= 0 && id < p.pages ? id : -1;
+}
+
+struct Window {
+  float rot[2][2 * kWindow][64];       // cos and sin of the rows
+  float sums[kWarps][2 * kWindow];     // a warp's share of the rows' sums of squares
+  float norm_of[2 * kWindow];
+  int64_t unit_page[kWindow];          // -1: the slot does not exist
+  int unit_slot[kWindow];
+  int unit_row[kWindow], unit_rows[kWindow];  // relative to the window; rows of the unit
+  int unit_count, row_end;
+};
+
+// One token that is a unit of its own: what a decode step brings.  All loads
+// whose addresses are known are under way at once: the token's values, its
+// position and those beside it, then the page, then the blocks' scales.  A head
+// takes kLanes threads, so a block of 8 warps 32 heads (of 128) at a time.
 template <typename T, typename S, int D>
-__global__ void __launch_bounds__(kThreads, 2) paged_append_8bit_kernel(const __grid_constant__ Append8Params p) {
+__device__ __forceinline__ bool append_one(const Append8Params& p, int part, int64_t row, Window& w) {
+  constexpr int kLanes = D / 16, kHeads = kThreads / kLanes;  // heads at a time
+  constexpr int kKept = 2;                                    // rounds of heads that stay in registers
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, at = tid % kLanes;
+  const int heads = part == 0 ? p.heads : p.kv_heads;
+  const T* x = static_cast<const T*>(p.qkv) + row * p.qkv_stride +
+               (int64_t)(part == 0 ? 0 : part == 1 ? p.heads : p.heads + p.kv_heads) * D + 8 * at;
+  uint4 raw[kKept][2];
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) {
+    const int h = tid / kLanes + i * kHeads;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      raw[i][j] = h < heads ? ld_v4(x + h * D + j * (D / 2)) : make_uint4(0, 0, 0, 0);
+  }
+  const int pos = p.positions[row], req = p.requests[row];
+  if (part != 0) {
+    const bool has_next = row + 1 < p.rows, has_last = row > 0;
+    const int next = has_next ? p.positions[row + 1] : 0, next_req = has_next ? p.requests[row + 1] : 0;
+    const int last = has_last ? p.positions[row - 1] : 0, last_req = has_last ? p.requests[row - 1] : 0;
+    const bool joins = has_last && last_req == req && (uint32_t)pos == (uint32_t)last + 1u &&
+                       (pos & (kScaleTokens - 1)) != 0;
+    if (joins) return true;  // its unit's first row brings it
+    if (has_next && next_req == req && (uint32_t)next == (uint32_t)pos + 1u && (next & (kScaleTokens - 1)) != 0)
+      return false;  // more rows in the unit
+  }
+  const __half* norm = part == 0 ? p.q_norm : part == 1 ? p.k_norm : nullptr;
+  const bool rotate = p.rotate && part < 2;
+  const int64_t page = part == 0 ? -1 : page_of(p, pos, req);
+  const int slot = pos & (p.page_size - 1), earlier = slot & (kScaleTokens - 1);
+  const auto scale_of = [&](int h) {
+    return p.scales[part - 1] + page * p.scale_stride + h * (p.page_size / kScaleTokens) + slot / kScaleTokens;
+  };
+  float old[kKept];
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) {
+    const int h = tid / kLanes + i * kHeads;
+    old[i] = page >= 0 && earlier && h < heads ? *scale_of(h) : 0.f;
+  }
+  if (rotate && tid < D / 2) turn((double)pos * p.turns[tid], w.rot[0][0][tid], w.rot[1][0][tid]);
+  if (norm) {
+    float2 sum = make_float2(0.f, 0.f);
+    for (int h = tid / kLanes, i = 0; h < heads; h += kHeads, ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float2 f[4];
+        unpack4<T>(i == 0 ? raw[0][j] : i == 1 ? raw[1][j] : ld_v4(x + h * D + j * (D / 2)), f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum = fma2(f[k], f[k], sum);
+      }
+    const float all = warp_sum_butterfly(sum.x + sum.y);
+    if (lane == 0) w.sums[warp][0] = all;
+  }
+  if (norm || rotate) __syncthreads();
+  float2 scale2 = make_float2(1.f, 1.f);
+  if (norm) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) sum += w.sums[i][0];
+    scale2.x = scale2.y = rms_scale(sum, heads * D, p.eps);
+  }
+  if (part != 0 && page < 0) return true;
+  // Whole warps go round, for the maxima of their heads.
+  for (int h0 = 0, i = 0; h0 < heads; h0 += kHeads, ++i) {
+    const int h = h0 + tid / kLanes;
+    const bool mine = h < heads;
+    float2 f[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      unpack4<T>(i == 0   ? raw[0][j]
+                 : i == 1 ? raw[1][j]
+                 : mine   ? ld_v4(x + h * D + j * (D / 2))
+                          : make_uint4(0, 0, 0, 0),
+                 f[j]);
+      if (norm && mine) {
+        float2 g[4];
+        unpack4<__half>(ld_v4(norm + h * D + j * (D / 2) + 8 * at), g);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[j][k] = mul2(mul2(f[j][k], scale2), g[k]);
+      }
+    }
+    if (rotate) rotate_pairs(f, &w.rot[0][0][8 * at], &w.rot[1][0][8 * at]);
+    if (part == 0) {
+      T* out = static_cast<T*>(p.q_out) + (row * heads + h) * D + 8 * at;
+      if (mine) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) *reinterpret_cast<uint4*>(out + j * (D / 2)) = pack4<T>(f[j]);
+      }
+      continue;
+    }
+    // Read before the head's threads meet in the shuffles, written after.
+    const float before = i == 0 ? old[0] : i == 1 ? old[1] : earlier && mine ? *scale_of(h) : 0.f;
+    float most = largest(f);
+#pragma unroll
+    for (int off = 1; off < kLanes; off <<= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, off));
+    if (!mine) continue;
+    const float scale = block_scale<S>(most, before);
+    const float inverse = scale > 0.f && scale < INFINITY ? __fdiv_rn(1.f, scale) : 0.f;
+    uint8_t* block = p.codes[part - 1] + page * p.page_stride + (int64_t)(h * p.page_size + slot - earlier) * D;
+    if (earlier && scale > before) round_anew<S>(block, earlier * (D / 16), before * inverse, at, kLanes);
+    if (at == 0) *scale_of(h) = scale;
+    put_codes<S, D>(block + earlier * D + 8 * at, f, scale < INFINITY, inverse);
+  }
+  return true;
+}
+
+// The units of a window (part 0: its rows as one), by warp 0.
+__device__ __forceinline__ void find_units(const Append8Params& p, int part, int64_t r0, int lane, Window& w) {
+  // Lane i looks at row r0 + i; a unit that begins in the window ends within
+  // the 31 rows after its start.
+  const int64_t row = r0 + lane;
+  const bool real = row < p.rows;
+  const int pos = real ? p.positions[row] : 0, req = real ? p.requests[row] : 0;
+  int before_pos = __shfl_up_sync(0xffffffffu, pos, 1), before_req = __shfl_up_sync(0xffffffffu, req, 1);
+  bool first = part == 0 && lane == 0;
+  if (part != 0 && real) {
+    if (lane == 0 && row > 0) before_pos = p.positions[row - 1], before_req = p.requests[row - 1];
+    first = row == 0 || before_req != req || (uint32_t)pos != (uint32_t)before_pos + 1u ||
+            (pos & (kScaleTokens - 1)) == 0;
+  }
+  const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+  const int end = (int)min((int64_t)32, p.rows - r0);  // rows that exist
+  if (first && lane < p.window) {
+    const uint32_t later = lane < 31 ? firsts >> (lane + 1) : 0u;
+    int next = later ? lane + __ffs(later) : end;
+    if (part == 0) next = min(p.window, end);
+    const int at = __popc(firsts & ((1u << lane) - 1u));
+    w.unit_row[at] = lane;
+    w.unit_rows[at] = next - lane;
+    w.unit_page[at] = part != 0 ? page_of(p, pos, req) : -1;
+    w.unit_slot[at] = pos & (p.page_size - 1);
+  }
+  if (lane == 0) {
+    const uint32_t mine = firsts & ((1u << p.window) - 1u);
+    w.unit_count = __popc(mine);
+    const int last = mine ? 31 - __clz(mine) : 0;
+    const uint32_t later = last < 31 ? firsts >> (last + 1) : 0u;
+    w.row_end = part == 0 ? min(p.window, end) : later ? last + __ffs(later) : end;
+  }
+}
+
+// One part of a window's rows: q (0), k (1) or v (2).
+template <typename T, typename S, int D, int kPart, bool kRotate>
+__device__ __forceinline__ void append_window(const Append8Params& p, int64_t r0, Window& w) {
   constexpr int kLanes = D / 16;          // threads of a token of a head, 8 values of either half each
   constexpr int kTokens = 32 / kLanes;    // tokens of a pass
   constexpr int kPasses = kScaleTokens / kTokens;
-  __shared__ float rot[2][2 * kWindow][D / 2];  // cos and sin of the rows
-  __shared__ float sums[kWarps][2 * kWindow];   // a warp's share of the rows' sums of squares
-  __shared__ float norm_of[2 * kWindow];
-  __shared__ int unit_row[kWindow], unit_rows[kWindow];  // relative to the window; rows of the unit
-  __shared__ int64_t unit_page[kWindow];                 // -1: the slot does not exist
-  __shared__ int unit_slot[kWindow];
-  __shared__ int unit_count, row_end;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int part = blockIdx.x < p.windows ? 1 : blockIdx.x < 2 * p.windows ? 2 : 0;  // k, v, q
-  const int64_t r0 = (int64_t)(blockIdx.x % p.windows) * p.window;
-  const int heads = part == 0 ? p.heads : p.kv_heads;
-
-  if (warp == 0) {
-    // Lane i looks at row r0 + i; a unit that begins in the window ends within
-    // the 31 rows after its start.
-    const int64_t row = r0 + lane;
-    const bool real = row < p.rows;
-    const int pos = real ? p.positions[row] : 0, req = real ? p.requests[row] : 0;
-    int before_pos = __shfl_up_sync(0xffffffffu, pos, 1), before_req = __shfl_up_sync(0xffffffffu, req, 1);
-    bool first = part == 0 && lane == 0;
-    if (part != 0 && real) {
-      if (lane == 0 && row > 0) before_pos = p.positions[row - 1], before_req = p.requests[row - 1];
-      first = row == 0 || before_req != req || (uint32_t)pos != (uint32_t)before_pos + 1u ||
-              (pos & (kScaleTokens - 1)) == 0;
-    }
-    const uint32_t firsts = __ballot_sync(0xffffffffu, first);
-    const int end = (int)min((int64_t)32, p.rows - r0);  // rows that exist
-    if (first && lane < p.window) {
-      const uint32_t later = lane < 31 ? firsts >> (lane + 1) : 0u;
-      int next = later ? lane + __ffs(later) : end;
-      if (part == 0) next = min(p.window, end);
-      const int at = __popc(firsts & ((1u << lane) - 1u));
-      unit_row[at] = lane;
-      unit_rows[at] = next - lane;
-      int64_t page = -1;
-      if (part != 0) {
-        const int column = pos >> p.page_shift;
-        if (pos >= 0 && req >= 0 && req < p.table.requests && column < p.table.columns) {
-          const int64_t id = p.table.ids[req * p.table.stride + column];
-          if (id >= 0 && id < p.pages) page = id;
-        }
-      }
-      unit_page[at] = page;
-      unit_slot[at] = pos & (p.page_size - 1);
-    }
-    if (lane == 0) {
-      const uint32_t mine = firsts & ((1u << p.window) - 1u);
-      unit_count = __popc(mine);
-      const int last = mine ? 31 - __clz(mine) : 0;
-      const uint32_t later = last < 31 ? firsts >> (last + 1) : 0u;
-      row_end = part == 0 ? min(p.window, end) : later ? last + __ffs(later) : end;
-    }
-  }
-  __syncthreads();
-  const int units = unit_count;
-  if (units == 0) return;
-  const int first_row = unit_row[0], rows = row_end - first_row;  // rows of all units
+  const int heads = kPart == 0 ? p.heads : p.kv_heads;
+  const __half* norm = kPart == 0 ? p.q_norm : p.k_norm;
   const T* src = static_cast<const T*>(p.qkv) + r0 * p.qkv_stride +
-                 (int64_t)(part == 0 ? 0 : part == 1 ? p.heads : p.heads + p.kv_heads) * D;
-  const __half* norm = part == 0 ? p.q_norm : part == 1 ? p.k_norm : nullptr;
-  const bool rotate = p.rotate && part < 2;
-  const int tasks = units * heads;
+                 (int64_t)(kPart == 0 ? 0 : kPart == 1 ? p.heads : p.heads + p.kv_heads) * D;
+  const int pairs = (heads + 1) / 2;  // a warp's task: two heads of a unit
   const int at = lane % kLanes, sub = lane / kLanes;
 
-  uint4 raw[kPasses][2];
-  auto load = [&](int task) {
-    const int u = task / heads, h = task % heads, n = unit_rows[u];
-    const T* x = src + (int64_t)unit_row[u] * p.qkv_stride + h * D + 8 * at;
+  uint4 raw[2][kPasses][2];
+  auto load_rows = [&](int row, int n, int h0) {
+    const T* x = src + (int64_t)row * p.qkv_stride + h0 * D + 8 * at;
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int t = i * kTokens + sub;
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        raw[i][j] = t < n ? ld_v4(x + t * p.qkv_stride + j * (D / 2)) : make_uint4(0, 0, 0, 0);
-    }
+      for (int i = 0; i < kPasses; ++i) {
+        const int t = i * kTokens + sub;
+        const bool mine = t < n && h0 + e < heads;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          raw[e][i][j] = mine ? ld_v4(x + t * p.qkv_stride + e * D + j * (D / 2)) : make_uint4(0, 0, 0, 0);
+      }
   };
-  const bool once = tasks <= kWarps;  // a warp's only task stays in its registers
-  if (warp < tasks) load(warp);
-
-  if (rotate) {
+  auto load = [&](int task) {
+    const int u = task / pairs;
+    load_rows(w.unit_row[u], w.unit_rows[u], task % pairs * 2);
+  };
+  // A window of a long prompt is one unit as a rule: its rows are under way while
+  // the units are found.
+  const int likely = (int)min((int64_t)p.window, p.rows - r0);
+  if (warp < pairs) load_rows(0, likely, warp * 2);
+  if (warp == 0) find_units(p, kPart, r0, lane, w);
+  __syncthreads();
+  const int units = w.unit_count;
+  if (units == 0) return;
+  const int first_row = w.unit_row[0], rows = w.row_end - first_row;  // rows of all units
+  const int tasks = units * pairs;
+  // The first task stays in the registers.
+  if (warp < tasks && !(warp < pairs && first_row == 0 && w.unit_rows[0] == likely)) load(warp);
+  if constexpr (kRotate) {
     for (int i = tid; i < rows * (D / 2); i += kThreads) {
       const int r = i / (D / 2), d = i % (D / 2);
-      const double t = (double)p.positions[r0 + first_row + r] * p.turns[d];
-      float sn, cs;
-      sincospif(2.f * (float)(t - rint(t)), &sn, &cs);
-      rot[0][r][d] = cs;
-      rot[1][r][d] = sn;
+      turn((double)p.positions[r0 + first_row + r] * p.turns[d], w.rot[0][r][d], w.rot[1][r][d]);
     }
+    __syncthreads();
   }
-  if (norm) {
-    sums[warp][lane] = 0.f;
+  float2 weight[2][4];
+  auto fetch_weight = [&](int h) {
+    if constexpr (kPart < 2) {  // without a norm ones
+      const uint32_t one = 0x3c003c00u;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        unpack4<__half>(norm ? ld_v4(norm + h * D + j * (D / 2) + 8 * at) : make_uint4(one, one, one, one), weight[j]);
+    }
+  };
+  // A token's values but for the factor of its norm.
+  auto values = [&](const uint4 (&in)[2], int row, float2 (&f)[2][4]) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      unpack4<T>(in[j], f[j]);
+      if constexpr (kPart < 2) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[j][k] = mul2(f[j][k], weight[j][k]);
+      }
+    }
+    if constexpr (kRotate) rotate_pairs(f, &w.rot[0][row][8 * at], &w.rot[1][row][8 * at]);
+  };
+
+  // First pass: the rows' sums of squares, where there is a norm.
+  if (kPart < 2 && norm) {
+    w.sums[warp][lane] = 0.f;
     __syncwarp();
     for (int task = warp; task < tasks; task += kWarps) {
       if (task != warp) load(task);
-      const int u = task / heads, n = unit_rows[u];
+      const int u = task / pairs, n = w.unit_rows[u], local = w.unit_row[u] - first_row;
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
+        if (i * kTokens >= n) break;
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float2 f[4];
-          unpack4<T>(raw[i][j], f);
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) sum = fma2(f[k], f[k], sum);
-        }
+          for (int j = 0; j < 2; ++j) {
+            float2 f[4];
+            unpack4<T>(raw[e][i][j], f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum = fma2(f[k], f[k], sum);
+          }
         float all = sum.x + sum.y;
 #pragma unroll
         for (int off = 1; off < kLanes; off <<= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
         const int t = i * kTokens + sub;
-        if (at == 0 && t < n) sums[warp][unit_row[u] - first_row + t] += all;  // a token always has the same thread
+        if (at == 0 && t < n) w.sums[warp][local + t] += all;  // a token always has the same thread
       }
     }
     __syncthreads();
     if (tid < rows) {
       float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) sum += sums[w][tid];
-      norm_of[tid] = rms_scale(sum, heads * D, p.eps);
+      for (int i = 0; i < kWarps; ++i) sum += w.sums[i][tid];
+      w.norm_of[tid] = rms_scale(sum, heads * D, p.eps);
     }
+    __syncthreads();
   }
-  if (norm || rotate) __syncthreads();
 
+  // Second pass: out.
   for (int task = warp; task < tasks; task += kWarps) {
-    if (!once && (norm || task != warp)) load(task);
-    const int u = task / heads, h = task % heads, n = unit_rows[u], local = unit_row[u] - first_row;
-    float2 weight[2][4];
-    if (norm) {
+    if (task != warp || (kPart < 2 && norm && tasks > kWarps)) load(task);
+    const int u = task / pairs, n = w.unit_rows[u], local = w.unit_row[u] - first_row;
+    const int64_t page = w.unit_page[u];
+    const int slot = w.unit_slot[u], earlier = slot & (kScaleTokens - 1);
+    if (kPart != 0 && page < 0) continue;
+    float factor[kPasses];  // of the thread's tokens
 #pragma unroll
-      for (int j = 0; j < 2; ++j) unpack4<__half>(ld_v4(norm + h * D + j * (D / 2) + 8 * at), weight[j]);
-    }
-    // Pass i's values: 8 of the first half, their partners in the second.
-    auto values = [&](int i, float2 (&f)[2][4]) {
-      const int row = min(local + i * kTokens + sub, rows - 1);
+    for (int i = 0; i < kPasses; ++i) factor[i] = kPart < 2 && norm ? w.norm_of[min(local + i * kTokens + sub, rows - 1)] : 1.f;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        unpack4<T>(raw[i][j], f[j]);
-        if (norm) {
-          const float2 scale = make_float2(norm_of[row], norm_of[row]);
+    for (int e = 0; e < 2; ++e) {
+      const int h = task % pairs * 2 + e;
+      if (h >= heads) break;
+      fetch_weight(h);
+      if constexpr (kPart == 0) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) f[j][k] = mul2(mul2(f[j][k], scale), weight[j][k]);
+        for (int i = 0; i < kPasses; ++i) {
+          if (i * kTokens >= n) break;
+          const int t = i * kTokens + sub;
+          float2 f[2][4];
+          values(raw[e][i], min(local + t, rows - 1), f);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[j][k] = mul2(f[j][k], make_float2(factor[i], factor[i]));
+          if (t < n) {
+            T* out = static_cast<T*>(p.q_out) + ((r0 + w.unit_row[u] + t) * heads + h) * D + 8 * at;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) *reinterpret_cast<uint4*>(out + j * (D / 2)) = pack4<T>(f[j]);
+          }
         }
-      }
-      if (rotate) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 cs = *reinterpret_cast<const float2*>(&rot[0][row][8 * at + 2 * k]);
-          const float2 sn = *reinterpret_cast<const float2*>(&rot[1][row][8 * at + 2 * k]);
-          const float2 a = f[0][k], b = f[1][k];
-          f[0][k] = fma2(a, cs, mul2(b, make_float2(-sn.x, -sn.y)));
-          f[1][k] = fma2(a, sn, mul2(b, cs));
-        }
-      }
-    };
-    if (part == 0) {
+      } else {
+      uint8_t* block = p.codes[kPart - 1] + page * p.page_stride + (int64_t)(h * p.page_size + slot - earlier) * D;
+      float* scale_at = p.scales[kPart - 1] + page * p.scale_stride + h * (p.page_size / kScaleTokens) +
+                        slot / kScaleTokens;
+      const float old = earlier ? *scale_at : 0.f;
+      float most = 0.f;
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
+        if (i * kTokens >= n) break;
         const int t = i * kTokens + sub;
         float2 f[2][4];
-        values(i, f);
-        if (t < n) {
-          T* out = static_cast<T*>(p.q_out) + ((r0 + unit_row[u] + t) * heads + h) * D + 8 * at;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) *reinterpret_cast<uint4*>(out + j * (D / 2)) = pack4<T>(f[j]);
-        }
+        values(raw[e][i], min(local + t, rows - 1), f);
+        if (t < n) most = max_nan(most, largest(f) * factor[i]);
       }
-      continue;
-    }
-    const int64_t page = unit_page[u];
-    if (page < 0) continue;
-    const int slot = unit_slot[u], earlier = slot & (kScaleTokens - 1);
-    uint8_t* block = p.codes[part - 1] + page * p.page_stride + (int64_t)(h * p.page_size + slot - earlier) * D;
-    float* scale_at = p.scales[part - 1] + page * p.scale_stride + h * (p.page_size / kScaleTokens) +
-                      slot / kScaleTokens;
-    const float old = earlier ? *scale_at : 0.f;
-    float2 f[kPasses][2][4];
-    float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      values(i, f[i]);
-      if (i * kTokens + sub < n) {
+      for (int off = 16; off > 0; off >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, off));
+      const float scale = block_scale<S>(most, old);
+      const float inverse = scale > 0.f && scale < INFINITY ? __fdiv_rn(1.f, scale) : 0.f;
+      if (lane == 0) *scale_at = scale;
+      if (earlier && scale > old) round_anew<S>(block, earlier * (D / 16), old * inverse, lane, 32);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+      for (int i = 0; i < kPasses; ++i) {
+        if (i * kTokens >= n) break;
+        const int t = i * kTokens + sub;
+        float2 f[2][4];
+        values(raw[e][i], min(local + t, rows - 1), f);
+        float by = factor[i] * inverse;
+        if (inverse > 1e30f) {  // the product may be beyond fp32
+          by = inverse;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) most = max_nan(most, max_nan(fabsf(f[i][j][k].x), fabsf(f[i][j][k].y)));
-      }
-    }
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, off));
-    float scale = __fdiv_rn(most, Code<S>::kLargest);
-    if (most > 0.f) scale = max_nan(scale, 1.17549435e-38f);  // its reciprocal is finite
-    if (!(most < INFINITY)) scale = __uint_as_float(0x7fc00000u);
-    scale = max_nan(scale, old);
-    const float inverse = scale > 0.f && scale < INFINITY ? __fdiv_rn(1.f, scale) : 0.f;
-    if (lane == 0) *scale_at = scale;
-    if (earlier && scale > old) {
-      const float ratio = old * inverse;
-      for (int i = lane; i < earlier * (D / 16); i += 32) {
-        uint4* at16 = reinterpret_cast<uint4*>(block) + i;
-        uint4 v = *at16;
-        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t a, b;
-          Code<S>::widen(w[k], a, b);
-          const float2 x = __half22float2(bits_half2(a)), y = __half22float2(bits_half2(b));
-          w[k] = Code<S>::narrow(x.x * ratio, x.y * ratio, y.x * ratio, y.y * ratio);
+            for (int k = 0; k < 4; ++k) f[j][k] = mul2(f[j][k], make_float2(factor[i], factor[i]));
         }
-        *at16 = v;
+        if (t < n) put_codes<S, D>(block + (earlier + t) * D + 8 * at, f, scale < INFINITY, by);
       }
-    }
-    const bool finite = scale < INFINITY;
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int t = i * kTokens + sub;
-      if (t >= n) continue;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        uint32_t w[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float2 x = f[i][j][2 * k], y = f[i][j][2 * k + 1];
-          w[k] = finite ? Code<S>::narrow(x.x * inverse, x.y * inverse, y.x * inverse, y.y * inverse) : 0u;
-        }
-        *reinterpret_cast<uint2*>(block + (earlier + t) * D + j * (D / 2) + 8 * at) = make_uint2(w[0], w[1]);
       }
     }
   }
+}
+
+template <typename T, typename S, int D>
+__global__ void __launch_bounds__(kThreads, 2) paged_append_8bit_kernel(const __grid_constant__ Append8Params p) {
+  __shared__ __align__(16) Window w;
+  const int part = blockIdx.x < p.windows ? 1 : blockIdx.x < 2 * p.windows ? 2 : 0;
+  const int64_t r0 = (int64_t)(blockIdx.x % p.windows) * p.window;
+  if (p.window == 1 && append_one<T, S, D>(p, part, r0, w)) return;
+  if (part == 2)
+    append_window<T, S, D, 2, false>(p, r0, w);
+  else if (part == 1)
+    p.rotate ? append_window<T, S, D, 1, true>(p, r0, w) : append_window<T, S, D, 1, false>(p, r0, w);
+  else
+    p.rotate ? append_window<T, S, D, 0, true>(p, r0, w) : append_window<T, S, D, 0, false>(p, r0, w);
 }
 
 }  // namespace

@@ -6,6 +6,7 @@
 #include <cuda_fp8.h>
 
 #include "common.cuh"
+#include "paged_pairs.cuh"
 
 namespace tf {
 
@@ -42,10 +43,16 @@ struct Code<I8> {
     a = lift(u, 0x4240);
     b = lift(u, 0x4341);
   }
-  // Four values -> codes, the first in the lowest byte.
-  __device__ __forceinline__ static uint32_t narrow(float x, float y, float z, float w) {
-    const auto one = [](float v) { return (uint32_t)__float2int_rn(fminf(fmaxf(v, -127.f), 127.f)) & 0xffu; };
-    return one(x) | one(y) << 8 | one(z) << 16 | one(w) << 24;
+  // Four values times `by` -> codes, the first in the lowest byte; the products
+  // lie within 127.5.  Added to 1.5 * 2^23 a number is rounded to the nearest
+  // integer, whose lowest byte is the code.
+  __device__ __forceinline__ static uint32_t narrow(float2 x, float2 y, float by) {
+    const float2 b = make_float2(by, by), magic = make_float2(12582912.f, 12582912.f);
+    x = fma2(x, b, magic);
+    y = fma2(y, b, magic);
+    const uint32_t lo = __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
   }
 };
 
@@ -64,10 +71,11 @@ struct Code<E4M3> {
   __device__ __forceinline__ static void widen_cross(uint32_t w, uint32_t& a, uint32_t& b) {
     widen(__byte_perm(w, 0, 0x3120), a, b);
   }
-  __device__ __forceinline__ static uint32_t narrow(float x, float y, float z, float w) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(z, w), __NV_SATFINITE, __NV_E4M3);
-    return lo | hi << 16;
+  __device__ __forceinline__ static uint32_t narrow(float2 x, float2 y, float by) {
+    const float2 b = make_float2(by, by);
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(mul2(x, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(mul2(y, b), __NV_SATFINITE, __NV_E4M3);
+    return __byte_perm(lo, hi, 0x5410);
   }
 };
 

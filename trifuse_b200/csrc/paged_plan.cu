@@ -319,9 +319,7 @@ void put_table(const Plans& plans, const int32_t* new_lengths, const int32_t* kv
   p->widened_offset = (int64_t)at;
   at = put(table, at, first_page);
   at = put(table, at, widened);
-  p->widened_bytes = pages ? align_up(p->workspace_bytes, 256) - p->workspace_bytes + 2 * widened_code_bytes(*p) +
-                                 2 * widened_scale_bytes(*p)
-                           : 0;
+  p->widened_bytes = pages ? 256 + 2 * widened_code_bytes(*p) + 2 * widened_scale_bytes(*p) : 0;  // from a multiple of 256
   p->positions_offset = (int64_t)at;
   at = align_up(at + (size_t)p->rows * 4, 16);
   p->requests_offset = (int64_t)at;

@@ -30,6 +30,13 @@ struct WidenParams {
   int requests;
 };
 
+// One whole 32-byte sector.
+__device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z),
+               "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
 template <typename S>
 __global__ void __launch_bounds__(kThreads) paged_widen_kernel(const __grid_constant__ WidenParams p) {
   const int page = blockIdx.x, head = blockIdx.y;
@@ -51,18 +58,27 @@ __global__ void __launch_bounds__(kThreads) paged_widen_kernel(const __grid_cons
   const int vectors = p.page_size * row;
   const int64_t from = id * p.page_stride + (int64_t)head * p.page_size * p.head_dim;
   const int64_t to = ((int64_t)page * p.kv_heads + head) * p.page_size * p.head_dim * 2;
-  for (int i = threadIdx.x; i < 2 * vectors; i += kThreads) {
-    const int side = i >= vectors, at = side ? i - vectors : i;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (at / row < have) w = ld_stream_v4(p.codes[side] + from + 16 * at);
-    uint4 out[2];
-    Code<S>::widen(w.x, out[0].x, out[0].y);
-    Code<S>::widen(w.y, out[0].z, out[0].w);
-    Code<S>::widen(w.z, out[1].x, out[1].y);
-    Code<S>::widen(w.w, out[1].z, out[1].w);
-    uint4* dst = reinterpret_cast<uint4*>(p.to[side] + to) + 2 * at;
-    dst[0] = out[0];
-    dst[1] = out[1];
+  // Four vectors of a thread are under way at a time.
+  constexpr int kBatch = 4;
+  for (int i0 = threadIdx.x; i0 < 2 * vectors; i0 += kBatch * kThreads) {
+    uint4 w[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int i = i0 + k * kThreads, side = i >= vectors, at = side ? i - vectors : i;
+      w[k] = make_uint4(0, 0, 0, 0);
+      if (i < 2 * vectors && at / row < have) w[k] = ld_stream_v4(p.codes[side] + from + 16 * at);
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int i = i0 + k * kThreads, side = i >= vectors, at = side ? i - vectors : i;
+      if (i >= 2 * vectors) break;
+      uint4 a, b;
+      Code<S>::widen(w[k].x, a.x, a.y);
+      Code<S>::widen(w[k].y, a.z, a.w);
+      Code<S>::widen(w[k].z, b.x, b.y);
+      Code<S>::widen(w[k].w, b.z, b.w);
+      store32(p.to[side] + to + 32 * at, a, b);
+    }
   }
   const int blocks = p.page_size / kScaleTokens;
   if (threadIdx.x < 2 * blocks) {

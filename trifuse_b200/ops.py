@@ -554,18 +554,17 @@ def _paged_scales(k_scales: Tensor | None, v_scales: Tensor | None, kv: PagedKV)
     cache; only the first dimension may have a stride of its own."""
     if k_scales is None or v_scales is None:
         raise ValueError("paged: k_scales and v_scales go together")
-    heads, blocks = kv.kv_heads, kv.page_size // SCALE_TOKENS
-    shape = (kv.pages, heads, blocks)
-    if k_scales.shape != shape or v_scales.shape != shape or not k_scales.dtype == v_scales.dtype == torch.float32:
+    pages, heads, blocks = kv.pages, kv.kv_heads, kv.page_size // SCALE_TOKENS
+    if (k_scales.shape != (pages, heads, blocks) or v_scales.shape != (pages, heads, blocks)
+            or k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32):
         raise ValueError("paged: scales are float32 [pages, kv_heads, page_size / 16]")
-    step = None
-    for t in (k_scales, v_scales):
-        s = t.stride()  # the stride of a dimension of one is of no meaning
-        own = s[0] if kv.pages > 1 else heads * blocks
-        if (heads > 1 and s[1] != blocks) or (blocks > 1 and s[2] != 1) or step not in (None, own):
-            raise ValueError("paged: a page's scales must be contiguous, and k_scales and v_scales laid out alike")
-        step = own
-    return PagedScales(k_scales.data_ptr(), v_scales.data_ptr(), step)
+    stride, other = k_scales.stride(), v_scales.stride()
+    if pages == 1 or heads == 1 or blocks == 1:  # the stride of a dimension of one is of no meaning
+        stride, other = ((t[0] if pages > 1 else heads * blocks, t[1] if heads > 1 else blocks, t[2] if blocks > 1 else 1)
+                         for t in (stride, other))
+    if stride != other or stride[1] != blocks or stride[2] != 1:
+        raise ValueError("paged: a page's scales must be contiguous, and k_scales and v_scales laid out alike")
+    return PagedScales(k_scales.data_ptr(), v_scales.data_ptr(), stride[0])
 
 
 def _page_table(page_table: Tensor) -> PageTable:
