@@ -249,9 +249,11 @@ struct TileScales {
   float4 block[8];  // unit, unit, offset, offset: s_k * scale * log2 e, log2(s_v / r)
   float2 back[8];   // r / s_v
   float v_ref;      // r
-  uint32_t odd;     // bit b: a scale of block b is not finite
-  uint32_t pad[2];
+  float shrink;     // r of the tile before / r
+  uint32_t events;  // bit b: a scale of block b is not finite; bit 8: r grew
+  uint32_t pad;
 };
+constexpr uint32_t kGrew = 256;
 // Lane i of a warp, i < 8, has the scales of block i (the other lanes those of
 // i % 8); returns the new r.
 __device__ __forceinline__ float tell(TileScales& to, float k, float v, float scale, float ref, int lane) {
@@ -260,16 +262,19 @@ __device__ __forceinline__ float tell(TileScales& to, float k, float v, float sc
   float most = v;
 #pragma unroll
   for (int off = 1; off < 8; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+  const float before = ref;
   ref = raise_ref(ref, most);
   const uint32_t odds = __ballot_sync(0xffffffffu, odd) & 0xffu;
   if (lane < 8) {
-    const float unit = fmaxf(k, 7.8886091e-31f) * scale, some = fmaxf(v * (1.f / ref), 8.6736174e-19f);
+    const float inverse = 1.f / ref;
+    const float unit = fmaxf(k, 7.8886091e-31f) * scale, some = fmaxf(v * inverse, 8.6736174e-19f);
     const float offset = log2f(some), back = 1.f / some;
     to.block[lane] = make_float4(unit, unit, offset, offset);
     to.back[lane] = make_float2(back, back);
     if (lane == 0) {
       to.v_ref = ref;
-      to.odd = odds;
+      to.shrink = before * inverse;  // powers of two
+      to.events = odds | (ref != before ? kGrew : 0u);
     }
   }
   return ref;
@@ -646,7 +651,20 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
           k_scale = real ? __ldg(k_from + 8 * j) : 0.f;
           v_scale = real ? __ldg(v_from + 8 * j) : 0.f;
         };
-        if (kScaled && view.tiles > 0) look_at(0);
+        if (kScaled && view.tiles > 0) {
+          look_at(0);
+          // r of the whole segment: the loader is ahead, so the softmax need not look for it
+          // to grow.
+          float most = 0.f;
+          const int blocks = min((g.kv_len + kScaleTokens - 1) / kScaleTokens - g.tile0 * 8, view.tiles * 8);
+          const float* from = v_from - (lane & 7);
+#pragma unroll 8
+          for (int i = lane; i < blocks; i += 32) {
+            const float v = __ldg(from + i);
+            most = fmaxf(most, fabsf(v) < INFINITY ? v : 0.f);
+          }
+          ref = raise_ref(ref, warp_max(most));
+        }
         for (int j = 0; j < view.tiles && ok; ++j) {
           const int key0 = (g.tile0 + j) * kTileKeys;
           const int left = g.kv_len - key0;
@@ -908,16 +926,17 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
       const float scale = Act<T>::kDtype == Act<C>::kDtype ? p.scale_log2 : p.scale_log2 * boost;
       float m = -INFINITY, l = 0.f;
       float v_ref = 1.f;  // r of O
+      bool boosted = false;
+      if constexpr (kScaled && Act<T>::kDtype != Act<C>::kDtype) boosted = __any_sync(0xffffffffu, boost != 1.f);
       for (int j = 0; j < count; ++j) {
         if (!(ok = wait_warp(&s_full[x], s_turn & 1, ctl, err, 90))) break;
         ++s_turn;
         tc_fence_after();
         const TileScales& of = told[(tile_at + j) % S::kTold];
-        float shrink = 1.f;
+        uint32_t events = 0;
         if constexpr (kScaled) {
-          const float ref = of.v_ref;
-          if (j > 0) shrink = v_ref / ref;  // powers of two
-          v_ref = ref;
+          events = of.events;
+          v_ref = of.v_ref;
         }
         float sc[128];
 #pragma unroll
@@ -926,7 +945,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         for (int c = 0; c < 128; c += 32) tmem_wait32(sc + c);
         const int key0 = (g.tile0 + j) * kTileKeys;
         if constexpr (kScaled && Act<T>::kDtype != Act<C>::kDtype) {
-          if (__any_sync(0xffffffffu, boost != 1.f)) {
+          if (boosted) {
 #pragma unroll
             for (int c = 0; c < 128; ++c) sc[c] *= boost;
           }
@@ -979,7 +998,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         // This tile's scores were issued after the last tile's product: O is
         // stable, and P may overlay S.  (The vote is taken on the first tile too:
         // it brings the warp together for the stores of P.)
-        if (kScaled) factor *= shrink;
+        if (kWiden && (events & kGrew)) factor *= of.shrink;
         if (__any_sync(0xffffffffu, factor != 1.f) && j > 0) {
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
@@ -1042,9 +1061,9 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         f2_unpack(kScaled ? f2_add(sp[2], sp[3]) : f2_add(f2_add(sp[0], sp[1]), f2_add(sp[2], sp[3])), s0, s1);
         l += s0 + s1;
         if constexpr (kScaled) {
-          if (of.odd) {
+          if (events & 0xffu) {
             for (int b = 0; b < 8; ++b)
-              if ((of.odd >> b & 1) && key0 + 16 * b <= limit) l = __uint_as_float(0x7fc00000u);
+              if ((events >> b & 1) && key0 + 16 * b <= limit) l = __uint_as_float(0x7fc00000u);
           }
         }
       }

@@ -238,21 +238,24 @@ def beam_select(logits: Tensor, scores: Tensor, count: int | None = None, finish
     count = beams if count is None else index(count)
     end = index(end)
     stream = _launch_stream(logits, scores, finished)
-    step = logits.stride(1) if beams > 1 else logits.stride(0) if R > 1 else V  # from row to row
-    if (V > 1 and logits.stride(2) != 1) or step < V or (R > 1 and logits.stride(0) != beams * step):
-        logits, step = logits.contiguous(), V
+    step = V  # from row to row
+    if not logits.is_contiguous():
+        stride = logits.stride()
+        step = stride[1] if beams > 1 else stride[0] if R > 1 else V
+        if (V > 1 and stride[2] != 1) or step < V or (R > 1 and stride[0] != beams * step):
+            logits, step = logits.contiguous(), V
     scores = scores.contiguous()
     if finished is not None:
         finished = finished.contiguous()
-    nb = C.c_size_t()
-    check(lib().tf_beam_select_workspace_size(R, beams, V, count, nb))
-    ws = _ws(nb.value, logits.device)
-    score = scores.new_empty((R, count))
+    # What tf_beam_select_workspace_size gives; checked by the call.
+    ws = torch.empty(max(R * beams * (16 + 8 * min(max(count, 0), V)), 1), dtype=torch.uint8, device=logits.device)
+    score = torch.empty_like(scores) if count == beams else scores.new_empty((R, max(count, 0)))
     parent = torch.empty_like(score, dtype=torch.int32)
     token = torch.empty_like(score, dtype=torch.int64)
     check(lib().tf_beam_select(logits.data_ptr(), step, R, beams, V, _ACT.get(logits.dtype, DTYPE_F32),
                                scores.data_ptr(), None if finished is None else finished.data_ptr(), end, count,
-                               score.data_ptr(), parent.data_ptr(), token.data_ptr(), ws.data_ptr(), nb.value, stream))
+                               score.data_ptr(), parent.data_ptr(), token.data_ptr(), ws.data_ptr(), ws.numel(),
+                               stream))
     return BeamChoice(score, parent, token)
 
 
@@ -792,27 +795,30 @@ def paged_copy(arrays, src, dst):
         raise ValueError("paged_copy: no arrays")
     stream = _launch_stream(*arrays)
     layers, pages = arrays[0].shape[:2] if arrays[0].ndim > 1 else (0, 0)
-    descs = (CopyArray * len(arrays))()
-    for d, t in zip(descs, arrays):
+    descs = []
+    for t in arrays:
         shape, stride, size = t.shape, t.stride(), t.element_size()
         if len(shape) < 3 or shape[0] != layers or shape[1] != pages:
             raise ValueError("paged_copy: arrays are [layers, pages, ...] with the same layers and pages")
-        n = 1  # values of a page; the stride of a dimension of one is of no meaning
-        for i in range(len(shape) - 1, 1, -1):
-            if shape[i] != 1 and stride[i] != n:
-                raise ValueError("paged_copy: a page must be contiguous")
-            n *= shape[i]
-        if (pages > 1 and stride[1] < n) or (layers > 1 and stride[0] == 0):
-            raise ValueError("paged_copy: pages share memory")
-        d.base, d.page_bytes = t.data_ptr(), n * size
-        d.layer_stride, d.page_stride = stride[0] * size if layers > 1 else 0, (stride[1] if pages > 1 else n) * size
+        if t.is_contiguous():
+            n = t.numel() // max(layers * pages, 1)  # values of a page
+        else:
+            n = 1
+            for i in range(len(shape) - 1, 1, -1):  # the stride of a dimension of one is of no meaning
+                if shape[i] != 1 and stride[i] != n:
+                    raise ValueError("paged_copy: a page must be contiguous")
+                n *= shape[i]
+            if (pages > 1 and stride[1] < n) or (layers > 1 and stride[0] == 0):
+                raise ValueError("paged_copy: pages share memory")
+        descs.append(CopyArray(t.data_ptr(), stride[0] * size if layers > 1 else 0,
+                               (stride[1] if pages > 1 else n) * size, n * size))
     try:
         src, dst = array("i", src), array("i", dst)
     except OverflowError:
         raise ValueError("paged_copy: a page does not fit 32 bits") from None
     if len(src) != len(dst):
         raise ValueError("paged_copy: src and dst differ in length")
-    check(lib().tf_paged_copy(descs, len(arrays), layers, pages, src.buffer_info()[0], dst.buffer_info()[0], len(src),
+    check(lib().tf_paged_copy((CopyArray * len(descs))(*descs), len(descs), layers, pages, src.buffer_info()[0], dst.buffer_info()[0], len(src),
                               stream))
 
 
