@@ -59,8 +59,8 @@
 // log2(s_v / r) of the argument, which the row's sum takes out again block by
 // block: P' = 2^(s s_k - m + log2(s_v / r)), l += (r / s_v) sum P', O += P' V.
 // That costs a few instructions a block, none a score, and rounds nothing but P'.
-// r is a power of two at or above all value scales of the segment so far; O is
-// rescaled where it grows, along with the maximum.
+// r is a power of two at or above the segment's value scales (one half: those so
+// far; O is rescaled where it grows, along with the maximum).
 //   Two halves (storage Widened): the requests' codes are widened by a kernel of
 // their own first (paged_widen.cu), for the tensor cores are the limit and a
 // tile is read by many row blocks.  (Widened in this kernel by a warpgroup more,
