@@ -86,9 +86,10 @@ __device__ __forceinline__ float block_scale(float most, float old) {
   return max_nan(scale, old);
 }
 
-// `n` vectors of earlier codes times `ratio`; lane `lane` of `lanes`.
+// `n` vectors of earlier codes at the scale `old`; lane `lane` of `lanes`.
 template <typename S>
-__device__ __forceinline__ void round_anew(uint8_t* block, int n, float ratio, int lane, int lanes) {
+__device__ __forceinline__ void round_anew(uint8_t* block, int n, float old, const Divisor& over, int lane, int lanes) {
+  const float2 old2 = make_float2(old, old);
   for (int i = lane; i < n; i += lanes) {
     uint4* at = reinterpret_cast<uint4*>(block) + i;
     uint4 v = *at;
@@ -98,18 +99,18 @@ __device__ __forceinline__ void round_anew(uint8_t* block, int n, float ratio, i
       uint32_t a, b;
       Code<S>::widen(w[k], a, b);
       const float2 x = __half22float2(bits_half2(a)), y = __half22float2(bits_half2(b));
-      w[k] = Code<S>::narrow(x, y, ratio);
+      w[k] = Code<S>::narrow(over(mul2(x, old2)), over(mul2(y, old2)));
     }
     *at = v;
   }
 }
 
-// 16 values times `by` as codes: 8 at `to`, 8 half a head on.
+// 16 values as codes: 8 at `to`, 8 half a head on.
 template <typename S, int D>
-__device__ __forceinline__ void put_codes(uint8_t* to, const float2 (&f)[2][4], bool finite, float by) {
+__device__ __forceinline__ void put_codes(uint8_t* to, const float2 (&f)[2][4], bool finite, const Divisor& over) {
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    uint2 w = make_uint2(Code<S>::narrow(f[j][0], f[j][1], by), Code<S>::narrow(f[j][2], f[j][3], by));
+    uint2 w = make_uint2(Code<S>::narrow(over(f[j][0]), over(f[j][1])), Code<S>::narrow(over(f[j][2]), over(f[j][3])));
     if (!finite) w = make_uint2(0, 0);
     *reinterpret_cast<uint2*>(to + j * (D / 2)) = w;
   }
@@ -256,11 +257,11 @@ __device__ __forceinline__ bool append_one(const Append8Params& p, int part, int
     for (int off = 1; off < kLanes; off <<= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, off));
     if (!mine) continue;
     const float scale = block_scale<S>(most, before);
-    const float inverse = scale > 0.f && scale < INFINITY ? __fdiv_rn(1.f, scale) : 0.f;
+    const Divisor over(scale);
     uint8_t* block = p.codes[part - 1] + page * p.page_stride + (int64_t)(h * p.page_size + slot - earlier) * D;
-    if (earlier && scale > before) round_anew<S>(block, earlier * (D / 16), before * inverse, at, kLanes);
+    if (earlier && scale > before) round_anew<S>(block, earlier * (D / 16), before, over, at, kLanes);
     if (at == 0) *scale_of(h) = scale;
-    put_codes<S, D>(block + earlier * D + 8 * at, f, scale < INFINITY, inverse);
+    put_codes<S, D>(block + earlier * D + 8 * at, f, scale < INFINITY, over);
   }
   return true;
 }
@@ -459,24 +460,23 @@ __device__ __forceinline__ void append_window(const Append8Params& p, int64_t r0
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, off));
       const float scale = block_scale<S>(most, old);
-      const float inverse = scale > 0.f && scale < INFINITY ? __fdiv_rn(1.f, scale) : 0.f;
+      const Divisor over(scale);
       if (lane == 0) *scale_at = scale;
-      if (earlier && scale > old) round_anew<S>(block, earlier * (D / 16), old * inverse, lane, 32);
+      if (earlier && scale > old) round_anew<S>(block, earlier * (D / 16), old, over, lane, 32);
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
         if (i * kTokens >= n) break;
         const int t = i * kTokens + sub;
         float2 f[2][4];
         values(raw[e][i], min(local + t, rows - 1), f);
-        float by = factor[i] * inverse;
-        if (inverse > 1e30f) {  // the product may be beyond fp32
-          by = inverse;
+        if constexpr (kPart == 1) {
+          const float2 by = make_float2(factor[i], factor[i]);
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) f[j][k] = mul2(f[j][k], make_float2(factor[i], factor[i]));
+            for (int k = 0; k < 4; ++k) f[j][k] = mul2(f[j][k], by);
         }
-        if (t < n) put_codes<S, D>(block + (earlier + t) * D + 8 * at, f, scale < INFINITY, by);
+        if (t < n) put_codes<S, D>(block + (earlier + t) * D + 8 * at, f, scale < INFINITY, over);
       }
       }
     }

@@ -23,6 +23,23 @@ __device__ __forceinline__ __half2 bits_half2(uint32_t w) { return *reinterpret_
 template <typename S>
 struct Code;
 
+// Division by a block's scale, given with its rounded reciprocal: the quotient
+// once improved by its remainder, so that a value that lies halfway between two
+// codes is not moved off it (16-bit values over a scale of few bits often do).
+// A scale that has no reciprocal gives zeros.
+struct Divisor {
+  float2 by, inverse;
+  __device__ __forceinline__ explicit Divisor(float scale) {
+    const float r = scale > 0.f && scale < INFINITY ? __fdiv_rn(1.f, scale) : 0.f;
+    by = make_float2(-scale, -scale);
+    inverse = make_float2(r, r);
+  }
+  __device__ __forceinline__ float2 operator()(float2 x) const {
+    const float2 y = mul2(x, inverse);
+    return fma2(fma2(y, by, x), inverse, y);
+  }
+};
+
 template <>
 struct Code<I8> {
   static constexpr tf_dtype kDtype = TF_DTYPE_I8;
@@ -43,13 +60,12 @@ struct Code<I8> {
     a = lift(u, 0x4240);
     b = lift(u, 0x4341);
   }
-  // Four values times `by` -> codes, the first in the lowest byte; the products
-  // lie within 127.5.  Added to 1.5 * 2^23 a number is rounded to the nearest
+  // Four values within 127.5 -> codes, the first in the lowest byte.  Added to 1.5 * 2^23 a number is rounded to the nearest
   // integer, whose lowest byte is the code.
-  __device__ __forceinline__ static uint32_t narrow(float2 x, float2 y, float by) {
-    const float2 b = make_float2(by, by), magic = make_float2(12582912.f, 12582912.f);
-    x = fma2(x, b, magic);
-    y = fma2(y, b, magic);
+  __device__ __forceinline__ static uint32_t narrow(float2 x, float2 y) {
+    const float2 one = make_float2(1.f, 1.f), magic = make_float2(12582912.f, 12582912.f);
+    x = fma2(x, one, magic);
+    y = fma2(y, one, magic);
     const uint32_t lo = __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x0040);
     const uint32_t hi = __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x0040);
     return __byte_perm(lo, hi, 0x5410);
@@ -71,10 +87,9 @@ struct Code<E4M3> {
   __device__ __forceinline__ static void widen_cross(uint32_t w, uint32_t& a, uint32_t& b) {
     widen(__byte_perm(w, 0, 0x3120), a, b);
   }
-  __device__ __forceinline__ static uint32_t narrow(float2 x, float2 y, float by) {
-    const float2 b = make_float2(by, by);
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(mul2(x, b), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(mul2(y, b), __NV_SATFINITE, __NV_E4M3);
+  __device__ __forceinline__ static uint32_t narrow(float2 x, float2 y) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
     return __byte_perm(lo, hi, 0x5410);
   }
 };

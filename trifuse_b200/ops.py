@@ -237,6 +237,8 @@ def beam_select(logits: Tensor, scores: Tensor, count: int | None = None, finish
     R, beams, V = logits.shape
     count = beams if count is None else index(count)
     end = index(end)
+    if not 1 <= count <= 64 or not -(1 << 63) <= end < 1 << 63:  # would wrap on the way to C
+        raise ValueError("beam_select: count is from 1 to 64, end fits 64 bits")
     stream = _launch_stream(logits, scores, finished)
     step = V  # from row to row
     if not logits.is_contiguous():
@@ -248,8 +250,8 @@ def beam_select(logits: Tensor, scores: Tensor, count: int | None = None, finish
     if finished is not None:
         finished = finished.contiguous()
     # What tf_beam_select_workspace_size gives; checked by the call.
-    ws = torch.empty(max(R * beams * (16 + 8 * min(max(count, 0), V)), 1), dtype=torch.uint8, device=logits.device)
-    score = torch.empty_like(scores) if count == beams else scores.new_empty((R, max(count, 0)))
+    ws = torch.empty(max(R * beams * (16 + 8 * min(count, V)), 1), dtype=torch.uint8, device=logits.device)
+    score = torch.empty_like(scores) if count == beams else scores.new_empty((R, count))
     parent = torch.empty_like(score, dtype=torch.int32)
     token = torch.empty_like(score, dtype=torch.int64)
     check(lib().tf_beam_select(logits.data_ptr(), step, R, beams, V, _ACT.get(logits.dtype, DTYPE_F32),
