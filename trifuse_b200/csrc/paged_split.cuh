@@ -232,6 +232,73 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // (m = -inf) weighs nothing, also where every part is empty.
 __device__ __forceinline__ float part_weight(float m, float M) { return m == -INFINITY ? 0.f : exp2_fast(m - M); }
 
+// The pieces of a segment's rows joined, in piece order within each of the groups
+// of threads that share them.  work: (parts + 1) * 16 floats of shared memory, and
+// at least four a thread.  Called by the whole block; ends with a barrier.
+constexpr int kFewParts = 8;
+template <typename T, int D, int kThreads>
+__device__ __forceinline__ void merge_many(const SplitParams& p, const PagedSegment& sg, float* work) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  float* sums = work + sg.parts * kSplitRows;  // of the rows
+  for (int r = warp; r < sg.rows; r += kThreads / 32) {
+    const float* stat = p.stat + (int64_t)sg.part0 * 32 + r;
+    float M = -INFINITY, sum = 0.f;
+    for (int k = lane; k < sg.parts; k += 32) M = max_nan(M, __ldcg(stat + (int64_t)k * 32));
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) M = max_nan(M, __shfl_xor_sync(0xffffffffu, M, off));
+    for (int k = lane; k < sg.parts; k += 32) {
+      const float f = part_weight(__ldcg(stat + (int64_t)k * 32), M);
+      sum = fmaf(f, __ldcg(stat + (int64_t)k * 32 + 16), sum);
+      work[k * kSplitRows + r] = f;
+    }
+    sum = warp_sum_butterfly(sum);
+    if (lane == 0) sums[r] = sum;
+  }
+  __syncthreads();
+  // Four values a thread; threads i, i + n, i + 2 n, ... take every g-th piece.
+  const int n = sg.rows * (D / 4), groups = max(1, min(kThreads / n, 8));
+  for (int i0 = 0; i0 < n; i0 += kThreads) {  // one round but for many rows
+    const int i = groups > 1 ? tid % n : i0 + tid, group = groups > 1 ? tid / n : 0;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const bool mine = i < n && group < groups;
+    const int r = mine ? i / (D / 4) : 0, d = i % (D / 4) * 4;
+    if (mine) {
+      const float* from = p.part + ((int64_t)sg.part0 * kSplitRows + r) * D + d;
+#pragma unroll 4
+      for (int k = group; k < sg.parts; k += groups) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(from + (int64_t)k * kSplitRows * D));
+        const float f = work[k * kSplitRows + r];
+        acc.x = fmaf(f, v.x, acc.x);
+        acc.y = fmaf(f, v.y, acc.y);
+        acc.z = fmaf(f, v.z, acc.z);
+        acc.w = fmaf(f, v.w, acc.w);
+      }
+    }
+    const float sum = sums[r];
+    if (groups > 1) {  // the weights' place is free now
+      __syncthreads();
+      float4* out = reinterpret_cast<float4*>(work);
+      if (mine && group > 0) out[(group - 1) * n + i] = acc;
+      __syncthreads();
+      if (mine && group == 0)
+        for (int g = 1; g < groups; ++g) {
+          const float4 v = out[(g - 1) * n + i];
+          acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
+        }
+    }
+    if (mine && group == 0) {
+      const int pr = sg.row0 + r;
+      T* orow = static_cast<T*>(p.out) + ((int64_t)(sg.q_row + pr / p.group) * p.heads + sg.kv_head * p.group +
+                                          pr % p.group) * D + d;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      alignas(8) const T v[4] = {from_f<T>(acc.x * inv), from_f<T>(acc.y * inv), from_f<T>(acc.z * inv),
+                                 from_f<T>(acc.w * inv)};
+      *reinterpret_cast<uint2*>(orow) = *reinterpret_cast<const uint2*>(v);
+    }
+  }
+  __syncthreads();
+}
+
 // A warp's position in its block's work: tile `tile` of segment `seg`.
 struct Cursor {
   int seg, end, tile, tile1;
@@ -758,6 +825,16 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
       __syncthreads();
       if (!last) continue;
       __threadfence();
+      if constexpr (kCoded) {
+        // Many pieces: their weights first, a warp a row, then groups of threads that
+        // share the pieces (one long request, 148 pieces: 65 -> 27 us).
+        constexpr int kRoom = kWarps * S::kJoinRows * S::kPitch;
+        static_assert(kRoom >= 4 * kThreads, "the groups' outputs");
+        if (sg.parts > kFewParts && (sg.parts + 1) * kSplitRows <= kRoom) {
+          merge_many<T, D, kThreads>(p, sg, join);
+          continue;
+        }
+      }
       for (int i = tid; i < sg.rows * D; i += kThreads) {
         const int r = i / D, d = i % D;
         float M = -INFINITY;

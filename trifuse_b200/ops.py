@@ -608,6 +608,17 @@ def _rows16(t: Tensor, width: int) -> Tensor:
     return t
 
 
+def _norm_weight(w: Tensor, n: int):
+    """A norm's n weights (or a copy of them where they start off 16 bytes) and their address."""
+    if w.dtype != torch.float16 or w.shape != (n,) or not w.is_contiguous():
+        raise ValueError("paged_append: norm weights are contiguous float16 over the full q and k widths")
+    at = w.data_ptr()
+    if at % 16:
+        w = w.clone()
+        at = w.data_ptr()
+    return w, at
+
+
 def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, positions: Tensor,
                  requests: Tensor, heads: int, q_norm: Tensor | None = None, k_norm: Tensor | None = None,
                  eps: float = 1e-5, rope_theta: float | None = None, out: Tensor | None = None,
@@ -642,14 +653,10 @@ def paged_append(qkv: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tens
             or not positions.is_contiguous() or not requests.is_contiguous()):
         raise ValueError("paged_append: positions and requests are contiguous int32 [rows]")
     qn = kn = None
-    if q_norm is not None or k_norm is not None:
-        for t, n in ((q_norm, heads * D), (k_norm, kv_heads * D)):
-            if t is not None and (t.dtype != torch.float16 or t.shape != (n,) or not t.is_contiguous()):
-                raise ValueError("paged_append: norm weights are contiguous float16 over the full q and k widths")
-        qn, kn = (None if t is None else t.data_ptr() for t in (q_norm, k_norm))
-        if (qn or 0) % 16 or (kn or 0) % 16:
-            q_norm, k_norm = (None if t is None else t.clone() for t in (q_norm, k_norm))
-            qn, kn = (None if t is None else t.data_ptr() for t in (q_norm, k_norm))
+    if q_norm is not None:
+        q_norm, qn = _norm_weight(q_norm, heads * D)
+    if k_norm is not None:
+        k_norm, kn = _norm_weight(k_norm, kv_heads * D)
     q = out
     if out is None:
         q = qkv.new_empty((rows, heads, D))
