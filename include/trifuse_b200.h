@@ -525,8 +525,8 @@ int tf_paged_copy(const tf_copy_array* arrays, int32_t count, int32_t layers, in
  * [requests][beams], may be NULL): such a beam has ended and competes with its
  * score as it is, as one continuation by the token `end`; its logits are not
  * read.  A beam whose score is not finite, or whose logits hold a NaN or +inf
- * or nothing but -inf, has no continuations.  Scores that lie within 3e-5 of
- * one another are told apart in 64 bits.  beams <= TF_MAX_BEAMS, count <=
+ * or nothing but -inf, has no continuations.  Scores closer than the sums'
+ * rounding are told apart in 64 bits.  beams <= TF_MAX_BEAMS, count <=
  * TF_MAX_TOP.  The workspace is device scratch (16-byte aligned, no initial
  * contents).  The reference generates greedily (patches/executorch.patch:
  * 1350-1353). */
