@@ -366,3 +366,72 @@ def test_append_then_attend(ops):
             check(got, *attend(c, q, [n], [at + n]))
             assert (got - want).float().norm() <= 0.05 * want.float().norm()
             at += n
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("power", [16, 100])
+@pytest.mark.parametrize("H,Hk,D,new,kv", [(4, 4, 128, [1, 1], [1, 700]), (14, 2, 64, [1, 2], [40, 9000]),
+                                           (8, 2, 64, [9, 30], [5000, 30]), (4, 2, 128, [257, 64], [257, 4000])])
+def test_queries_beyond_f16(ops, kind, power, H, Hk, D, new, kv):
+    """bf16 queries past f16's range, all rows and every third one; the scale brings the scores back, so the bounds are
+    those of ordinary ones."""
+    c = Cache(kv, Hk, D, 16, kind, seed=3)
+    plan = ops.PagedPlan(new, kv, H, Hk, D, 16)
+    q = (torch.randn(sum(new), H, D, generator=torch.Generator().manual_seed(4)) * 2).to(BF16).cuda()
+    some = q.clone()
+    some[::3, ::2] *= 2.0 ** power
+    scale = 2.0 ** -power * D ** -0.5
+    for x in (q * 2.0 ** power, some):
+        got = ops.paged_attention(x, *c.args(), plan, scale=scale, **c.scales())
+        assert ops.device_error() == 0
+        check(got, *attend(c, x, new, kv, scale), rms=False)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [1, 5, 40, 300])
+def test_an_infinite_query_stays_in_its_row(ops, kind, n):
+    """NaN and infinite queries make their own (row, head) NaN and leave the others' bits."""
+    H, Hk, D, L = 4, 2, 128, 700
+    c = Cache([L], Hk, D, 16, kind)
+    plan = ops.PagedPlan([n], [L], H, Hk, D, 16)
+    q = torch.randn(n, H, D, generator=torch.Generator().manual_seed(n)).to(BF16).cuda()
+    want = ops.paged_attention(q, *c.args(), plan, **c.scales())
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        x = q.clone()
+        x[n // 2, 1, 17] = bad
+        got = ops.paged_attention(x, *c.args(), plan, **c.scales())
+        assert torch.isnan(got[n // 2, 1]).all()
+        got[n // 2, 1] = want[n // 2, 1]
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("L", [9000, 33000])
+@pytest.mark.parametrize("H,Hk,D", [(1, 1, 64), (1, 1, 128), (7, 1, 64), (8, 1, 128), (12, 1, 128), (16, 1, 64)])
+def test_many_pieces(ops, H, Hk, D, L):
+    """One long request whose pieces lie on every SM: all ways to share them among threads."""
+    run(ops, [1], [L], H, Hk, D, 64, F16, KINDS[H % 2], seed=H)
+
+
+def test_refusals(ops):
+    from trifuse_b200 import TriFuseError
+    c = Cache([40], 2, 64, 16, I8)
+    plan = ops.PagedPlan([1], [40], 4, 2, 64, 16)
+    q = torch.zeros(1, 4, 64, dtype=F16, device="cuda")
+    qkv = torch.zeros(1, 8 * 64, dtype=F16, device="cuda")
+    before = [x.nan_to_num().clone() if x.is_floating_point() else x.clone() for x in (c.k, c.v, c.ks, c.vs)]
+    pages16 = c.k.half()
+    for k, v, ks, vs in ((c.k, c.v, None, None), (c.k, c.v, c.ks, None), (pages16, pages16, c.ks, c.vs),
+                         (c.k, c.v, c.ks[:1], c.vs), (c.k, c.v, c.ks.cpu(), c.vs), (c.k, c.v, c.ks.half(), c.vs.half()),
+                         (c.k, c.v.view(torch.float8_e4m3fn), c.ks, c.vs)):
+        kw = {n: x for n, x in (("k_scales", ks), ("v_scales", vs)) if x is not None}
+        with pytest.raises((ValueError, TriFuseError)):
+            ops.paged_attention(q, k, v, c.table, plan, **kw)
+        with pytest.raises((ValueError, TriFuseError)):
+            ops.paged_append(qkv, k, v, c.table, plan.positions, plan.requests, 4, **kw)
+    small = torch.zeros(4, 2, 8, 64, dtype=I8, device="cuda")  # pages below a block of tokens
+    with pytest.raises((ValueError, TriFuseError)):
+        ops.paged_append(qkv, small, small, c.table, plan.positions, plan.requests, 4,
+                         k_scales=torch.zeros(4, 2, 0, device="cuda"), v_scales=torch.zeros(4, 2, 0, device="cuda"))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b.nan_to_num() if b.is_floating_point() else b)
+               for a, b in zip(before, (c.k, c.v, c.ks, c.vs)))

@@ -383,7 +383,6 @@ __device__ __forceinline__ void append_window(const Append8Params& p, int64_t r0
       const int u = task / pairs, n = w.unit_rows[u], local = w.unit_row[u] - first_row;
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
-        if (i * kTokens >= n) break;
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int e = 0; e < 2; ++e)

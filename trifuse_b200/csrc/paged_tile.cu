@@ -242,8 +242,8 @@ __device__ __forceinline__ float raise_ref(float ref, float scale) {
   return scale > ref && scale < INFINITY ? power_above(scale) : ref;
 }
 // What is told of a tile of codes, twice where packed pairs are worked on.  Zero
-// scales and ratios stay above 2^-100 and 2^-60, where nothing is left of what
-// they scale; scales that are not finite count as zero, and the rows that see a
+// units become the smallest number, 2^-149 (a hidden score of -inf must not meet a
+// zero), zero ratios 2^-60, where nothing is left of what they scale; scales that are not finite count as zero, and the rows that see a
 // token of their blocks as NaN.
 struct TileScales {
   float4 block[8];  // unit, unit, offset, offset: s_k * scale * log2 e, log2(s_v / r)
@@ -267,7 +267,7 @@ __device__ __forceinline__ float tell(TileScales& to, float k, float v, float sc
   const uint32_t odds = __ballot_sync(0xffffffffu, odd) & 0xffu;
   if (lane < 8) {
     const float inverse = 1.f / ref;
-    const float unit = fmaxf(k, 7.8886091e-31f) * scale, some = fmaxf(v * inverse, 8.6736174e-19f);
+    const float unit = fmaxf(k * scale, 1.401298464e-45f), some = fmaxf(v * inverse, 8.6736174e-19f);
     const float offset = log2f(some), back = 1.f / some;
     to.block[lane] = make_float4(unit, unit, offset, offset);
     to.back[lane] = make_float2(back, back);
