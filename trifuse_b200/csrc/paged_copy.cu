@@ -6,6 +6,9 @@
 // before the first is stored; eight such blocks on an SM keep 128 KB in flight.
 // Pages below 4 KB (scales) go a warp each.  The pairs travel with the launch,
 // so a call uploads nothing, waits for nothing and can be captured.
+//
+// Measured: 301 pages of 128 KB in 8 layers, keys and values (1.26 GB moved) 190 us,
+// 6.65 TB/s; 3 pages of 32 KB in 16 layers 3.1 us.
 #include <string.h>
 
 #include <algorithm>

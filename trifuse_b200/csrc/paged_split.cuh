@@ -42,7 +42,10 @@
 // Measured: 64 decodes of 4096 tokens, 16 heads, pages of 64: 311 us, 6.9 TB/s;
 // 37 ragged decodes of up to 32768 tokens, 8 key heads, pages of 16: 279 us, 6.0
 // TB/s (277 with the products taken out: 4 KB pages set that); one decode of 600
-// tokens 7.2 us, of one token 4.0.
+// tokens 7.2 us, of one token 4.0.  Codes: the same 64 decodes 171 us, 6.3 TB/s, the
+// ragged ones 140 (int8; 124 with the arithmetic taken out), 600 tokens 8.1 or
+// 7.5 (e4m3), one token 5.7 or 5.1; 64 decodes of 1024 tokens 58 (a segment is three
+// tiles a warp there, and the warps meet at its end).
 #pragma once
 
 #include <cuda.h>

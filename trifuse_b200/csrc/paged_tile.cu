@@ -77,7 +77,9 @@
 // power cap leaves); 8 prompts of 2048 tokens (16 heads) 163 us, 0.84 PFLOP/s
 // (segments of 9 tiles on average, whose ends cost 5600 clocks each; 4 us of it
 // for looking the causal edge's values through, paged_values.cuh), 182 us with
-// bf16 queries over an f16 cache.
+// bf16 queries over an f16 cache.  Over int8 codes (bf16 queries) the first takes
+// 497 us, widening included, where f16 keys and values take 443; the prompts 240 to
+// 250 against 186.
 #include <cuda.h>
 #include <math.h>
 #include <string.h>
@@ -502,129 +504,129 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
       asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (kWiden && warp == S::kLoadWarp) {
       if constexpr (kWiden) {
-      constexpr int kChunks = kTileKeys / S::kRawKeys;
-      int m = 0, t = 0;  // chunks and tiles fetched
-      bool ok = true;
-      for (int seg = seg0; seg < seg1 && ok; ++seg) {
-        const PagedSegment g = p.segments[seg];
-        const View<H> view(g, p.group);
-        const int32_t* ids = p.ids + g.request * p.ids_stride;
-        const int box_bytes = p.box_rows * D;
-        for (int j = 0; j < view.tiles && ok; ++j, ++t) {
-          const int key0 = (g.tile0 + j) * kTileKeys;
-          // Lane i brings the scale of block i % 8 of the tile's keys (i < 8) or values
-          // (i < 16).
-          int64_t scale_page = -1;
-          const int scale_key = key0 + (lane & 7) * kScaleTokens;
-          if (lane < 16 && scale_key < g.kv_len && scale_key >> p.page_shift < p.columns)
-            scale_page = __ldg(ids + (scale_key >> p.page_shift));
+        constexpr int kChunks = kTileKeys / S::kRawKeys;
+        int m = 0, t = 0;  // chunks and tiles fetched
+        bool ok = true;
+        for (int seg = seg0; seg < seg1 && ok; ++seg) {
+          const PagedSegment g = p.segments[seg];
+          const View<H> view(g, p.group);
+          const int32_t* ids = p.ids + g.request * p.ids_stride;
+          const int box_bytes = p.box_rows * D;
+          for (int j = 0; j < view.tiles && ok; ++j, ++t) {
+            const int key0 = (g.tile0 + j) * kTileKeys;
+            // Lane i brings the scale of block i % 8 of the tile's keys (i < 8) or values
+            // (i < 16).
+            int64_t scale_page = -1;
+            const int scale_key = key0 + (lane & 7) * kScaleTokens;
+            if (lane < 16 && scale_key < g.kv_len && scale_key >> p.page_shift < p.columns)
+              scale_page = __ldg(ids + (scale_key >> p.page_shift));
 #pragma unroll 1
-          for (int c = 0; c < 2 * kChunks && ok; ++c, ++m) {
-            const bool v = c >= kChunks;
-            const int slot = m % S::kRawSlots, turn = m / S::kRawSlots;
-            const int chunk0 = key0 + c % kChunks * S::kRawKeys;
-            const int left = min(g.kv_len - chunk0, S::kRawKeys);
-            const int boxes = left > 0 ? (left + p.box_rows - 1) / p.box_rows : 0;
-            // Lane i fetches box i (at most 8 of the chunk's pages).
-            int page = -1, row = 0;
-            if (lane < boxes) {
-              const int key = chunk0 + lane * p.box_rows, column = key >> p.page_shift;
-              if (column < p.columns) page = __ldg(ids + column);
-              row = g.kv_head * p.page_size + (key & (p.page_size - 1));
+            for (int c = 0; c < 2 * kChunks && ok; ++c, ++m) {
+              const bool v = c >= kChunks;
+              const int slot = m % S::kRawSlots, turn = m / S::kRawSlots;
+              const int chunk0 = key0 + c % kChunks * S::kRawKeys;
+              const int left = min(g.kv_len - chunk0, S::kRawKeys);
+              const int boxes = left > 0 ? (left + p.box_rows - 1) / p.box_rows : 0;
+              // Lane i fetches box i (at most 8 of the chunk's pages).
+              int page = -1, row = 0;
+              if (lane < boxes) {
+                const int key = chunk0 + lane * p.box_rows, column = key >> p.page_shift;
+                if (column < p.columns) page = __ldg(ids + column);
+                row = g.kv_head * p.page_size + (key & (p.page_size - 1));
+              }
+              if (turn > 0 && !(ok = wait_warp(&raw_empty[slot], (uint32_t)((turn - 1) & 1), ctl, err, 93))) break;
+              if (lane == 0) mbar_expect_tx(&raw_full[slot], (uint32_t)(boxes * box_bytes));
+              __syncwarp();
+              if (lane < boxes)
+                tma_codes(base + S::kOffRaw + slot * S::kRaw + lane * box_bytes, v ? &p.tm_v : &p.tm_k, row, page,
+                          &raw_full[slot]);
+              if (c == 0 && lane < 16) {
+                const bool real = scale_page >= 0 && scale_page < p.pages;
+                const float* from = lane < 8 ? p.k_scales : p.v_scales;
+                if (real)
+                  from += scale_page * p.scale_stride + g.kv_head * (p.page_size / kScaleTokens) +
+                          (scale_key & (p.page_size - 1)) / kScaleTokens;
+                copy_value(scales + (t & 3) * 16 + lane, from, real);
+              }
+              arrive_with_copies(&raw_full[slot]);
             }
-            if (turn > 0 && !(ok = wait_warp(&raw_empty[slot], (uint32_t)((turn - 1) & 1), ctl, err, 93))) break;
-            if (lane == 0) mbar_expect_tx(&raw_full[slot], (uint32_t)(boxes * box_bytes));
-            __syncwarp();
-            if (lane < boxes)
-              tma_codes(base + S::kOffRaw + slot * S::kRaw + lane * box_bytes, v ? &p.tm_v : &p.tm_k, row, page,
-                        &raw_full[slot]);
-            if (c == 0 && lane < 16) {
-              const bool real = scale_page >= 0 && scale_page < p.pages;
-              const float* from = lane < 8 ? p.k_scales : p.v_scales;
-              if (real)
-                from += scale_page * p.scale_stride + g.kv_head * (p.page_size / kScaleTokens) +
-                        (scale_key & (p.page_size - 1)) / kScaleTokens;
-              copy_value(scales + (t & 3) * 16 + lane, from, real);
-            }
-            arrive_with_copies(&raw_full[slot]);
           }
         }
-      }
-      // Copies in flight land before the block exits.
-      for (int i = m > S::kRawSlots ? m - S::kRawSlots : 0; i < m; ++i)
-        drain(&raw_full[i % S::kRawSlots], (uint32_t)((i / S::kRawSlots) & 1), err);
+        // Copies in flight land before the block exits.
+        for (int i = m > S::kRawSlots ? m - S::kRawSlots : 0; i < m; ++i)
+          drain(&raw_full[i % S::kRawSlots], (uint32_t)((i / S::kRawSlots) & 1), err);
       }
     } else if (kWiden && warp >= S::kWidenWarp) {
       if constexpr (kWiden) {
-      constexpr int kChunks = kTileKeys / S::kRawKeys;
-      // A warp takes 8 rows by 64 columns at a time, 16 codes a thread: eight threads in a
-      // row read two rows and write them to rows whose swizzles keep both apart in the
-      // banks (of 128-byte rows r and r ^ 5, of 64-byte rows neighbours).
-      constexpr int kGroupStep = 8 * (S::kWideners / 32);  // rows from one group of a warp to its next
-      const int quarter = lane >> 3, other = (lane >> 2) & 1, vec = lane & 3;
-      const int row8 = D == 128 ? (other ? quarter ^ 5 : quarter) : 2 * quarter + other;
-      const int my_row = 8 * (warp - S::kWidenWarp) + row8;
-      const int chunk = D == 128 ? vec ^ row8 : vec ^ ((row8 >> 1) & 3);  // the second half's lies 64 bytes on or back
-      const int from_at = my_row * D + chunk * 16, flip = chunk & 4 ? -64 : 64;
-      const int to_at = my_row * 128 + (((2 * vec) ^ row8) << 4), second = (row8 & 1) ? -16 : 16;
-      int n = 0, m = 0, t = 0;  // slots of the ring, chunks, tiles
-      bool ok = true;
-      for (int seg = seg0; seg < seg1 && ok; ++seg) {
-        const PagedSegment g = p.segments[seg];
-        const View<H> view(g, p.group);
-        float ref = kLeastRef;  // r: of the segment's values so far
-        for (int j = 0; j < view.tiles && ok; ++j, ++t) {
-          const int have = g.kv_len - (g.tile0 + j) * kTileKeys;
+        constexpr int kChunks = kTileKeys / S::kRawKeys;
+        // A warp takes 8 rows by 64 columns at a time, 16 codes a thread: eight threads in a
+        // row read two rows and write them to rows whose swizzles keep both apart in the
+        // banks (of 128-byte rows r and r ^ 5, of 64-byte rows neighbours).
+        constexpr int kGroupStep = 8 * (S::kWideners / 32);  // rows from one group of a warp to its next
+        const int quarter = lane >> 3, other = (lane >> 2) & 1, vec = lane & 3;
+        const int row8 = D == 128 ? (other ? quarter ^ 5 : quarter) : 2 * quarter + other;
+        const int my_row = 8 * (warp - S::kWidenWarp) + row8;
+        const int chunk = D == 128 ? vec ^ row8 : vec ^ ((row8 >> 1) & 3);  // the second half's lies 64 bytes on or back
+        const int from_at = my_row * D + chunk * 16, flip = chunk & 4 ? -64 : 64;
+        const int to_at = my_row * 128 + (((2 * vec) ^ row8) << 4), second = (row8 & 1) ? -16 : 16;
+        int n = 0, m = 0, t = 0;  // slots of the ring, chunks, tiles
+        bool ok = true;
+        for (int seg = seg0; seg < seg1 && ok; ++seg) {
+          const PagedSegment g = p.segments[seg];
+          const View<H> view(g, p.group);
+          float ref = kLeastRef;  // r: of the segment's values so far
+          for (int j = 0; j < view.tiles && ok; ++j, ++t) {
+            const int have = g.kv_len - (g.tile0 + j) * kTileKeys;
 #pragma unroll 1
-          for (int v = 0; v < 2 && ok; ++v, ++n) {
-            const int slot = n % S::kSlots, turn = n / S::kSlots;
-            if (turn > 0 && !(ok = wait_warp(&kv_empty[slot], (uint32_t)((turn - 1) & 1), ctl, err, 94))) break;
-            uint8_t* dst = base + S::kOffRing + slot * S::kTile;
+            for (int v = 0; v < 2 && ok; ++v, ++n) {
+              const int slot = n % S::kSlots, turn = n / S::kSlots;
+              if (turn > 0 && !(ok = wait_warp(&kv_empty[slot], (uint32_t)((turn - 1) & 1), ctl, err, 94))) break;
+              uint8_t* dst = base + S::kOffRing + slot * S::kTile;
 #pragma unroll 1
-            for (int c = 0; c < kChunks; ++c, ++m) {
-              const int raw = m % S::kRawSlots;
-              if (!(ok = wait_warp(&raw_full[raw], (uint32_t)((m / S::kRawSlots) & 1), ctl, err, 95))) break;
-              if (c == 0 && v == 0 && warp == S::kWidenWarp) {
-                const float* from = scales + (t & 3) * 16;
-                ref = tell(told[t % S::kTold], from[lane & 7], from[8 + (lane & 7)], p.scale_log2, ref, lane);
-              }
-              const uint8_t* src = base + S::kOffRaw + raw * S::kRaw + from_at;
-              uint8_t* to = dst + c * S::kRawKeys * 128 + to_at;
-              // The thread's vectors: column halves h, groups of 8 rows.
+              for (int c = 0; c < kChunks; ++c, ++m) {
+                const int raw = m % S::kRawSlots;
+                if (!(ok = wait_warp(&raw_full[raw], (uint32_t)((m / S::kRawSlots) & 1), ctl, err, 95))) break;
+                if (c == 0 && v == 0 && warp == S::kWidenWarp) {
+                  const float* from = scales + (t & 3) * 16;
+                  ref = tell(told[t % S::kTold], from[lane & 7], from[8 + (lane & 7)], p.scale_log2, ref, lane);
+                }
+                const uint8_t* src = base + S::kOffRaw + raw * S::kRaw + from_at;
+                uint8_t* to = dst + c * S::kRawKeys * 128 + to_at;
+                // The thread's vectors: column halves h, groups of 8 rows.
 #pragma unroll
-              for (int h = 0; h < D / 64; ++h) {
-                constexpr int kGroups = S::kRawKeys / 8 / (S::kWideners / 32);
-                uint4 w[kGroups];
-#pragma unroll
-                for (int b = 0; b < kGroups; ++b)
-                  w[b] = *reinterpret_cast<const uint4*>(src + b * kGroupStep * D + (h ? flip : 0));
-                if (have < kTileKeys) {
-                  // Past the request's length anything may lie, NaN included: zeros.
+                for (int h = 0; h < D / 64; ++h) {
+                  constexpr int kGroups = S::kRawKeys / 8 / (S::kWideners / 32);
+                  uint4 w[kGroups];
 #pragma unroll
                   for (int b = 0; b < kGroups; ++b)
-                    if (c * S::kRawKeys + my_row + b * kGroupStep >= have) w[b] = make_uint4(0, 0, 0, 0);
-                }
+                    w[b] = *reinterpret_cast<const uint4*>(src + b * kGroupStep * D + (h ? flip : 0));
+                  if (have < kTileKeys) {
+                    // Past the request's length anything may lie, NaN included: zeros.
 #pragma unroll
-                for (int b = 0; b < kGroups; ++b) {
-                  uint4 out[2];
-                  Code<St>::widen(w[b].x, out[0].x, out[0].y);
-                  Code<St>::widen(w[b].y, out[0].z, out[0].w);
-                  Code<St>::widen(w[b].z, out[1].x, out[1].y);
-                  Code<St>::widen(w[b].w, out[1].z, out[1].w);
-                  uint8_t* at = to + h * kColBytes + b * kGroupStep * 128;
-                  *reinterpret_cast<uint4*>(at) = out[0];
-                  *reinterpret_cast<uint4*>(at + second) = out[1];
+                    for (int b = 0; b < kGroups; ++b)
+                      if (c * S::kRawKeys + my_row + b * kGroupStep >= have) w[b] = make_uint4(0, 0, 0, 0);
+                  }
+#pragma unroll
+                  for (int b = 0; b < kGroups; ++b) {
+                    uint4 out[2];
+                    Code<St>::widen(w[b].x, out[0].x, out[0].y);
+                    Code<St>::widen(w[b].y, out[0].z, out[0].w);
+                    Code<St>::widen(w[b].z, out[1].x, out[1].y);
+                    Code<St>::widen(w[b].w, out[1].z, out[1].w);
+                    uint8_t* at = to + h * kColBytes + b * kGroupStep * 128;
+                    *reinterpret_cast<uint4*>(at) = out[0];
+                    *reinterpret_cast<uint4*>(at + second) = out[1];
+                  }
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&raw_empty[raw]);
               }
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&raw_empty[raw]);
+              if (!ok) break;
+              fence_proxy_async();
+              mbar_arrive(&kv_full[slot]);
             }
-            if (!ok) break;
-            fence_proxy_async();
-            mbar_arrive(&kv_full[slot]);
           }
         }
-      }
       }
     } else if (!kWiden && warp == S::kLoadWarp) {
       int n = 0;  // tiles fetched (K and V each count)

@@ -6,8 +6,8 @@
 // they are read.  Slots past the request's length become zeros, and so do pages
 // that do not exist.  What bounds it: these bytes.
 //
-// Measured: 16384 tokens of 8 key heads of 128 (101 MB): see the table of the
-// operators' times.
+// Measured: 16384 tokens of 8 key heads of 128 (101 MB) 20 us of a call; 8 x 2048
+// tokens of 16 heads (201 MB) 35.
 #include "common.cuh"
 #include "paged.h"
 #include "paged_codes.cuh"
