@@ -435,3 +435,23 @@ def test_refusals(ops):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b.nan_to_num() if b.is_floating_point() else b)
                for a, b in zip(before, (c.k, c.v, c.ks, c.vs)))
+
+
+@pytest.mark.parametrize("new,kv", [([1] * 5, [700, 3000, 17, 9000, 40]), ([30, 25], [3000, 900]), ([300], [5000]),
+                                    ([1, 300, 40], [4000, 2000, 700])])
+def test_waits_that_run_out(ops, new, kv):
+    """With a limit of one cycle a wait that its first try does not meet runs out; the call ends all the same, and the
+    next ones give what they gave."""
+    from trifuse_b200._lib import check as ok, lib
+    c, q, plan, want = run(ops, new, kv, 8, 2, 128, 16, BF16, E4M3)
+    try:
+        ok(lib().tf_set_wait_limit(1))
+        for _ in range(3):
+            ops.paged_attention(q, *c.args(), plan, **c.scales())
+        torch.cuda.synchronize()
+    finally:
+        ok(lib().tf_set_wait_limit(0))
+    assert ops.device_error() in (0, 71, *range(81, 96))
+    for _ in range(3):
+        assert torch.equal(ops.paged_attention(q, *c.args(), plan, **c.scales()), want)
+    assert ops.device_error() == 0

@@ -266,3 +266,19 @@ def test_beam_search_gives_its_pages_back(copies, monkeypatch):
         with pytest.raises(ValueError):
             beam_search(model, cache, **args)
     assert beam_search(model, cache, [], 3, 4) == []
+
+
+def test_beam_search_refuses_logits_that_are_no_distribution(copies, monkeypatch):
+    """As serve does: an error, not an empty answer; its pages are free again."""
+    from trifuse_b200 import TriFuseError
+    monkeypatch.setattr(ops, "beam_select", plain_select)
+    for bad in ("at once", "later"):
+        model = Chain(11)
+        if bad == "at once":
+            model.table[:] = float("nan")
+        else:
+            model.table[3:, 3:] = float("inf")
+        cache = PagedCache(1, 90, 1, 4, 64, device="cpu")
+        with pytest.raises(TriFuseError, match="no distribution"):
+            beam_search(model, cache, [[1, 2], [5, 7]], 3, 20)
+        assert len(cache.free) == 90 and not cache.pages and not cache.lengths

@@ -256,6 +256,8 @@ struct TileScales {
   uint32_t pad;
 };
 constexpr uint32_t kGrew = 256;
+// Up to 2^9 a maximum and a logarithm add up to within 2^-15, 2e-5 of a weight.
+constexpr float kApart = 512.f;
 // Lane i of a warp, i < 8, has the scales of block i (the other lanes those of
 // i % 8); returns the new r.
 __device__ __forceinline__ float tell(TileScales& to, float k, float v, float scale, float ref, int lane) {
@@ -959,7 +961,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         }
         // The maximum of the raw scores (the scale is positive), NaN kept.
         float mp[8];
-        bool raw = true;  // the scores are not yet multiplied with their scale
+        bool raw = true;  // the scores are not yet the exponents
         float mx;
         if constexpr (kScaled) {
 #pragma unroll
@@ -983,11 +985,10 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         // Far out the product with the scale is rounded by more than the
         // exponential bears: there each score takes the maximum's rounding.
         float unit = scale;
-        if (__any_sync(0xffffffffu, fabsf(mx) > kFar)) {
+        if (!kScaled && __any_sync(0xffffffffu, fabsf(mx) > kFar)) {
 #pragma unroll
-          for (int c = 0; c < 128; ++c) sc[c] *= kScaled ? of.block[c / 16].x : scale;
+          for (int c = 0; c < 128; ++c) sc[c] *= scale;
           unit = 1.f;
-          raw = false;
         }
         float factor = 1.f;
         mx = lifted<C>(mx);
@@ -1018,6 +1019,16 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         // second's exponentials do.
         const float sub = m == -INFINITY ? 0.f : -m;
         const uint64_t sl2 = f2_pack(unit, unit), nm = f2_pack(sub, sub);
+        if constexpr (kScaled) {
+          // Away from zero -m + log2(s_v / r) would lose the logarithm's bits (and far out
+          // the product needs the maximum's rounding, as above): step by step there.
+          if (__any_sync(0xffffffffu, fabsf(sub) > kApart)) {
+            raw = false;
+#pragma unroll
+            for (int c = 0; c < 128; ++c)
+              sc[c] = __fadd_rn(__fadd_rn(__fmul_rn(sc[c], of.block[c / 16].x), sub), of.block[c / 16].z);
+          }
+        }
         uint64_t sp[4], block_unit = 0ull, block_offset = 0ull;
 #pragma unroll
         for (int i = 0; i < 4; ++i) sp[i] = 0ull;
@@ -1032,8 +1043,8 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
               const int block = k0 / 16;
               if (c % 8 == 0) {
                 const ulonglong2 both = *reinterpret_cast<const ulonglong2*>(&of.block[block]);
-                block_unit = raw ? both.x : sl2;
-                block_offset = f2_add(nm, both.y);
+                block_unit = raw ? both.x : f2_pack(1.f, 1.f);
+                block_offset = raw ? f2_add(nm, both.y) : 0ull;
                 sp[0] = sp[1] = 0ull;
               }
               f2_unpack(f2_fma(f2_pack(sc[k0], sc[k0 + 1]), block_unit, block_offset), a, b);

@@ -368,6 +368,8 @@ def beam_search(model: PagedOLMoE, cache: PagedCache, prompts, beams: int, new_t
                 found[r] = [Hypothesis(before[p].tokens + [t] * (not before[p].ended), s,
                                        before[p].ended or t == end) if p >= 0 else None
                             for p, t, s in zip(parents[r], tokens[r], scores[r])]
+                if not any(found[r]):  # as serve refuses such a row
+                    raise TriFuseError(9, "beam_search: logits that are no distribution give no continuation")
                 ended[r] = [h is None or h.ended for h in found[r]]
                 for b in range(beams):
                     if ended[r][b]:  # its tokens are all that is left of it
