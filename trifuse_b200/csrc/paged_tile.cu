@@ -78,7 +78,7 @@
 // (segments of 9 tiles on average, whose ends cost 5600 clocks each; 4 us of it
 // for looking the causal edge's values through, paged_values.cuh), 182 us with
 // bf16 queries over an f16 cache.  Over int8 codes (bf16 queries) the first takes
-// 497 us, widening included, where f16 keys and values take 443; the prompts 240 to
+// 508 us, widening included, where f16 keys and values take 443; the prompts 240 to
 // 250 against 186.
 #include <cuda.h>
 #include <math.h>
