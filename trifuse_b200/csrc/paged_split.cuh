@@ -29,23 +29,23 @@
 // to 2^-21 of the row's largest, paged_values.cuh); scores, m, l and O stay fp32.
 //
 // An 8-bit cache (storage S = I8 or E4M3, C = f16) runs through the same code with
-// twice the warps: its tiles are half the bytes and the same products.  Codes
-// become f16 on the way from shared memory to the products, exactly, and a
+// 12 warps (8 for 16 rows), since its tiles are half the bytes and the same
+// products.  Codes become f16 on the way from shared memory to the products,
+// exactly, and a
 // block's scales (16 tokens = one 16-key half of the products) go to the scores
-// and to the weights: S = (K Q^T) s_k, O += (P s_v / r) V.  Integer codes meet the
-// queries as integers, without being widened: a row of queries is 16-bit fixed
-// point to its largest value (an error of 2^-16 of that, below what f16 leaves
-// of the weights), in two bytes, so S is two exact integer products.  r is a power of two
+// and to the weights: S = (K Q^T) s_k, O += (P s_v / r) V.  r is a power of two
 // at or above the value scales that the warp has met; it grows like the running
 // maximum, O rescaled, so that the weights use f16's range whatever the scales.
 //
 // Measured: 64 decodes of 4096 tokens, 16 heads, pages of 64: 311 us, 6.9 TB/s;
 // 37 ragged decodes of up to 32768 tokens, 8 key heads, pages of 16: 279 us, 6.0
 // TB/s (277 with the products taken out: 4 KB pages set that); one decode of 600
-// tokens 7.2 us, of one token 4.0.  Codes: the same 64 decodes 171 us, 6.3 TB/s, the
-// ragged ones 140 (int8; 124 with the arithmetic taken out), 600 tokens 8.1 or
-// 7.5 (e4m3), one token 5.7 or 5.1; 64 decodes of 1024 tokens 58 (a segment is three
-// tiles a warp there, and the warps meet at its end).
+// tokens 7.2 us, of one token 4.0.  Codes: the same 64 decodes 171 us (e4m3; 6.3
+// TB/s), the ragged ones 149 (int8; 124 with the arithmetic taken out), 600 tokens
+// 7.7 or 7.5 (e4m3), one token 5.3; 64 decodes of 1024 tokens 60 and 58 (a segment
+// is three tiles a warp there, and the warps meet at its end).  Integer products of
+// int8 codes with queries in two or three bytes of fixed point took 141 or 143 on
+// the ragged ones, but 62 and 65, 8.2 and 8.4 on the short ones.
 #pragma once
 
 #include <cuda.h>
@@ -192,21 +192,6 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float* d, const uint32_t
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Integer codes (A) by the bytes of fixed-point queries (B), signed high ones
-// or unsigned low ones.
-__device__ __forceinline__ void mma16832(int* d, const uint32_t* a, uint32_t b0, uint32_t b1, bool high) {
-  if (high)
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 template <typename C>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const C a = from_f<C>(lo), b = from_f<C>(hi);
@@ -328,7 +313,7 @@ template <typename T, typename C, int D, int NT, typename St>  // NT: groups of 
 __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
     paged_split_kernel(const __grid_constant__ SplitParams p) {
   using S = Shape<D, NT, C, St>;
-  constexpr bool kCoded = S::kCoded, kInt = std::is_same<St, I8>::value;
+  constexpr bool kCoded = S::kCoded;
   constexpr int kWarps = S::kWarps, kThreads = S::kThreads;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -445,37 +430,7 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       scale[t][0] = scale[t][1] = p.scale_log2;
-      if constexpr (kInt) {
-        // A row as 16-bit fixed-point numbers of its largest: bytes 4 c .. 4 c + 3 of a
-        // chunk in one word of signed high bytes and one of low bytes.
-        float most = 0.f;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const T* v = reinterpret_cast<const T*>(&qb[k][t][j]);
-            most = max_nan(most, max_nan(fabsf(to_f(v[0])), fabsf(to_f(v[1]))));
-          }
-        most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const float step = fmaxf(most * (1.f / 32767.f), most > 0.f ? 1.17549435e-38f : 0.f) + (most - most);  // NaN stays
-        const float inverse = step > 0.f && step < INFINITY ? 1.f / step : 0.f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) scale[t][i] *= __shfl_sync(0xffffffffu, step, 4 * (c2 + i));
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          uint32_t high = 0, low = 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const T* v = reinterpret_cast<const T*>(&qb[k][t][j >> 1]);
-            const int n = __float2int_rn(to_f(v[j & 1]) * inverse);
-            high |= ((uint32_t)(n >> 8) & 0xffu) << (8 * j);
-            low |= ((uint32_t)n & 0xffu) << (8 * j);
-          }
-          qb[k][t][0] = high;
-          qb[k][t][1] = low;
-        }
-      } else if constexpr (Act<T>::kDtype != Act<C>::kDtype) {
+      if constexpr (Act<T>::kDtype != Act<C>::kDtype) {
         uint32_t most = 0;  // of row 8 t + g, whose values four lanes share
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
@@ -549,35 +504,6 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
         }
         v_scale[0] = four.z * ref_inverse;
         v_scale[1] = four.w * ref_inverse;
-        if constexpr (kInt) {
-          int dot[2][NT][2][4];  // by the high bytes, by the low ones
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-              for (int j = 0; j < 8; ++j) dot[h][t][j >> 2][j & 3] = 0;
-#pragma unroll
-          for (int k = 0; k < D / 16; k += 2) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t w[4];
-              ldsm4((ks + code_at ^ k << 4) + 16 * h * D, w);
-#pragma unroll
-              for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int part = 0; part < 2; ++part)
-                  mma16832(dot[h][t][part], w, qb[k][t][part], qb[k + 1][t][part], part == 0);
-            }
-          }
-          // Below 2^30: exact.
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) s[h][t][j] = (float)(dot[h][t][0][j] * 256 + dot[h][t][1][j]);
-        } else {
         // Bytes 4 c .. 4 c + 3 of a lane's row are taken as columns 2 c, 2 c + 1, 2 c + 8
         // and 2 c + 9 of the product, as the queries are.
 #pragma unroll
@@ -595,7 +521,6 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
               for (int t = 0; t < NT; ++t) mma16816<C>(s[h][t], a, qb[k + j][t][0], qb[k + j][t][1]);
             }
           }
-        }
         }
       } else {
 #pragma unroll
