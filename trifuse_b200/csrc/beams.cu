@@ -13,7 +13,8 @@
 // off by up to 4.4e-7 (flat to peaked rows of 1000 to 600000 logits).  Where two
 // candidates of different beams that matter lie closer than ten times the sum of
 // two such errors, their rows are summed again in fp64, so which beam goes on
-// does not hang on a rounding.  At eight beams a batch of 64 requests meets that
+// does not hang on a rounding; an exact total may lie close to another rough one,
+// so this goes on until none does (each row is summed again once at most).  At eight beams a batch of 64 requests meets that
 // about once in sixty steps, and then takes 30 us more.
 //
 // What bounds it: the logits, read once; this kernel's block is latency (some
@@ -89,8 +90,8 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_cons
   __shared__ int n_of[kMaxBeams];
   __shared__ double base[kMaxBeams];  // score - log sum: what a token's x - m is added to
   __shared__ float m_of[kMaxBeams];
-  __shared__ double best[kMaxCount + 1];
-  __shared__ int best_at[kMaxCount + 1];  // beam * each + place
+  __shared__ double best[kMaxCount];
+  __shared__ int best_at[kMaxCount];  // beam * each + place
   __shared__ int near[kMaxBeams];
   __shared__ int any_near;
   __shared__ double warps[kThreads / 32];
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_cons
     ended = a.finished && a.finished[row0 + tid];
     near[tid] = 0;
   }
-  if (tid <= count && tid <= kMaxCount) best_at[tid] = -1;
+  if (tid < count) best_at[tid] = -1;
   if (tid == 0) any_near = 0;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows are written
   if (tid < beams) {
@@ -141,13 +142,13 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_cons
       if (j >= n_of[b]) continue;
       const double total = totals[i];
       int place = j;
-      for (int o = 0; o < beams && place <= count; ++o) {
+      for (int o = 0; o < beams && place < count; ++o) {
         if (o == b) continue;
-        // More than count + 1 of another list need not be told apart.
-        const int n = min(n_of[o], count + 1 - place);
+        // More than `count` of another list need not be told apart.
+        const int n = min(n_of[o], count - place);
         place += o < b ? ahead<true>(totals + o * each, n, total) : ahead<false>(totals + o * each, n, total);
       }
-      if (place <= count) {
+      if (place < count) {
         best[place] = total;
         best_at[place] = i;
       }
@@ -155,24 +156,34 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_cons
     __syncthreads();
   };
   order();
-  if (tid < count && best_at[tid + 1] >= 0) {
-    const int b = best_at[tid] / each, c = best_at[tid + 1] / each;
-    if (b != c && best[tid] - best[tid + 1] < near_by(a.vocab)) {
-      near[b] = near[c] = 1;
-      any_near = 1;
-    }
-  }
-  __syncthreads();
-  if (any_near) {
+  // Until no pair is left that hangs on a rounding: neighbours among the picked
+  // ones, and the last of them with all that were not picked.
+  for (;;) {
+    const auto close = [&](int one, int other, double apart) {
+      const int b = one / each, c = other / each;
+      if (b == c || !(fabs(apart) < near_by(a.vocab))) return;
+      for (int beam : {b, c})
+        if (near[beam] == 0) near[beam] = any_near = 1;  // 2: summed again
+    };
+    if (tid + 1 < count && best_at[tid + 1] >= 0) close(best_at[tid], best_at[tid + 1], best[tid] - best[tid + 1]);
+    if (best_at[count - 1] >= 0)
+      for (int i = tid; i < beams * each; i += kThreads)
+        if (i % each < n_of[i / each]) close(best_at[count - 1], i, best[count - 1] - totals[i]);
+    __syncthreads();
+    if (!any_near) break;
     for (int b = 0; b < beams; ++b) {
-      if (!near[b] || m_of[b] == INFINITY) continue;
-      const double log_sum =
-          row_log_sum(static_cast<const T*>(a.logits) + (row0 + b) * a.row_stride, a.vocab, m_of[b], warps);
-      if (tid == 0) base[b] = (double)a.scores[row0 + b] - log_sum;
-      __syncthreads();
-      if (tid < n_of[b]) fill(b, tid);
+      if (near[b] != 1) continue;
+      if (m_of[b] != INFINITY) {
+        const double log_sum =
+            row_log_sum(static_cast<const T*>(a.logits) + (row0 + b) * a.row_stride, a.vocab, m_of[b], warps);
+        if (tid == 0) base[b] = (double)a.scores[row0 + b] - log_sum;
+        __syncthreads();
+        if (tid < n_of[b]) fill(b, tid);
+      }
     }
     __syncthreads();
+    if (tid < beams && near[tid] == 1) near[tid] = 2;
+    if (tid == 0) any_near = 0;
     order();
   }
   if (tid < count) {
