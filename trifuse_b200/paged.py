@@ -104,7 +104,8 @@ class PagedCache:
 
     def take_back(self, requests, counts):
         """Undoes the last grow of the same requests and counts (pages that it
-        copied stay their requests' own)."""
+        copied stay their requests' own; of an 8-bit cache, earlier tokens of
+        a block that was written to stay as it left them)."""
         for r, count in reversed(list(zip(requests, counts))):
             left = self.lengths[r] - count
             keep = -(-left // self.page_size)
@@ -350,7 +351,8 @@ def beam_search(model: PagedOLMoE, cache: PagedCache, prompts, beams: int, new_t
             row = 0
             for r, p in zip(active, parts):
                 row += len(p)
-                logits[r] = out[row - 1]
+                if fed + chunk >= len(prompts[r]):
+                    logits[r] = out[row - 1].clone()  # the rest of the step's logits may go
             fed += chunk
             active = [r for r in active if len(prompts[r]) > fed]
         got = ops.beam_select(torch.stack(logits)[:, None], torch.zeros(R, 1, device=cache.k.device), beams)
