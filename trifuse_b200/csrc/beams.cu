@@ -14,8 +14,9 @@
 // candidates of different beams that matter lie closer than ten times the sum of
 // two such errors, their rows are summed again in fp64, so which beam goes on
 // does not hang on a rounding; an exact total may lie close to another rough one,
-// so this goes on until none does (each row is summed again once at most).  At eight beams a batch of 64 requests meets that
-// about once in sixty steps, and then takes 30 us more.
+// so this goes on until none does (each row is summed again once at most).  At
+// eight beams a batch of 64 requests meets that about once in sixty steps, and then
+// takes 30 us more.
 //
 // What bounds it: the logits, read once; this kernel's block is latency (some
 // 64 candidates, a few round trips).  Measured: 64 x 8 beams over 50304 fp32 logits

@@ -44,7 +44,9 @@ struct BeamArgs {
   char* workspace = nullptr;
   int each() const { return count < vocab ? count : vocab; }  // candidates of a beam
   __host__ __device__ BeamRow* rows() const { return reinterpret_cast<BeamRow*>(workspace); }
-  __host__ __device__ uint64_t* keys() const { return reinterpret_cast<uint64_t*>(workspace + requests * beams * sizeof(BeamRow)); }
+  __host__ __device__ uint64_t* keys() const {
+    return reinterpret_cast<uint64_t*>(workspace + requests * beams * sizeof(BeamRow));
+  }
   size_t workspace_bytes() const { return (size_t)requests * beams * (sizeof(BeamRow) + 8 * (size_t)each()); }
 };
 tf_status launch_beam_rows(const BeamArgs& a, cudaStream_t s);

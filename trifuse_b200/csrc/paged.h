@@ -135,5 +135,4 @@ struct AppendArgs {
 tf_status launch_paged_append(const AppendArgs& a, cudaStream_t s);
 tf_status launch_paged_append_8bit(const AppendArgs& a, const tf_paged_scales& scales, cudaStream_t s);
 
-
 }  // namespace tf

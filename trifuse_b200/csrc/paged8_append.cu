@@ -428,7 +428,8 @@ __device__ __forceinline__ void append_window(const Append8Params& p, int64_t r0
     if (kPart != 0 && page < 0) continue;
     float factor[kPasses];  // of the thread's tokens
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) factor[i] = kPart < 2 && norm ? w.norm_of[min(local + i * kTokens + sub, rows - 1)] : 1.f;
+    for (int i = 0; i < kPasses; ++i)
+      factor[i] = kPart < 2 && norm ? w.norm_of[min(local + i * kTokens + sub, rows - 1)] : 1.f;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int h = task % pairs * 2 + e;

@@ -60,8 +60,9 @@ struct Code<I8> {
     a = lift(u, 0x4240);
     b = lift(u, 0x4341);
   }
-  // Four values within 127.5 -> codes, the first in the lowest byte.  Added to 1.5 * 2^23 a number is rounded to the nearest
-  // integer, whose lowest byte is the code.
+  // Four values within 127.5 -> codes, the first in the lowest byte.  Added to
+  // 1.5 * 2^23 a number is rounded to the nearest integer, whose lowest byte is the
+  // code.
   __device__ __forceinline__ static uint32_t narrow(float2 x, float2 y) {
     const float2 one = make_float2(1.f, 1.f), magic = make_float2(12582912.f, 12582912.f);
     x = fma2(x, one, magic);

@@ -344,7 +344,8 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
     more = in.settle(p.segments, warp);
   }
   int fetched = 0, used = 0;
-  // Box of this lane in a tile: which page's part, keys or values.  The page id of the next tile is looked up a tile ahead.
+  // Box of this lane in a tile: which page's part, keys or values.  The page id of
+  // the next tile is looked up a tile ahead.
   const int box = lane >> 1, is_v = lane & 1;
   // Of codes, box = 16-key half of the tile as far as the scales go.
   const int half_bytes = p.box_rows * S::kRow, box_bytes = half_bytes * S::kHalves;

@@ -245,8 +245,9 @@ __device__ __forceinline__ float raise_ref(float ref, float scale) {
 }
 // What is told of a tile of codes, twice where packed pairs are worked on.  Zero
 // units become the smallest number, 2^-149 (a hidden score of -inf must not meet a
-// zero), zero ratios 2^-60, where nothing is left of what they scale; scales that are not finite count as zero, and the rows that see a
-// token of their blocks as NaN.
+// zero), zero ratios 2^-60, where nothing is left of what they scale; scales that
+// are not finite count as zero, and the rows that see a token of their blocks as
+// NaN.
 struct TileScales {
   float4 block[8];  // unit, unit, offset, offset: s_k * scale * log2 e, log2(s_v / r)
   float2 back[8];   // r / s_v

@@ -827,8 +827,8 @@ def paged_copy(arrays, src, dst):
         raise ValueError("paged_copy: a page does not fit 32 bits") from None
     if len(src) != len(dst):
         raise ValueError("paged_copy: src and dst differ in length")
-    check(lib().tf_paged_copy((CopyArray * len(descs))(*descs), len(descs), layers, pages, src.buffer_info()[0], dst.buffer_info()[0], len(src),
-                              stream))
+    check(lib().tf_paged_copy((CopyArray * len(descs))(*descs), len(descs), layers, pages, src.buffer_info()[0],
+                              dst.buffer_info()[0], len(src), stream))
 
 
 def set_qmm_path(path: int):
