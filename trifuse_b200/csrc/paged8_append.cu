@@ -125,9 +125,18 @@ __device__ __forceinline__ void put_codes(uint8_t* to, const float2 (&f)[2][4], 
   }
 }
 
-// cos and sin of an angle of `turns` turns.
-__device__ __forceinline__ void turn(double turns, float& cs, float& sn) {
-  sincospif(2.f * (float)(turns - rint(turns)), &sn, &cs);
+// cos and sin of an angle of `turns` turns.  For keys, what the angle loses by its
+// rounding turns them on (half as many codes fall to the other side of a
+// rounding); q is the 16-bit append's.
+__device__ __forceinline__ void turn(double turns, bool key, float& cs, float& sn) {
+  const double half = 2. * (turns - rint(turns));  // half turns
+  const float rough = (float)half;
+  sincospif(rough, &sn, &cs);
+  if (key) {
+    const float rest = (float)(half - (double)rough) * 3.14159265f, c = cs;
+    cs = fmaf(-rest, sn, c);
+    sn = fmaf(rest, c, sn);
+  }
 }
 
 // Eight values of a head's first half and their partners: normalised, rotated.
@@ -208,7 +217,7 @@ __device__ __forceinline__ bool append_one(const Append8Params& p, int part, int
     const int h = tid / kLanes + i * kHeads;
     old[i] = page >= 0 && earlier && h < heads ? *scale_of(h) : 0.f;
   }
-  if (rotate && tid < D / 2) turn((double)pos * p.turns[tid], w.rot[0][0][tid], w.rot[1][0][tid]);
+  if (rotate && tid < D / 2) turn((double)pos * p.turns[tid], part == 1, w.rot[0][0][tid], w.rot[1][0][tid]);
   if (norm) {
     float2 sum = make_float2(0.f, 0.f);
     for (int h = tid / kLanes, i = 0; h < heads; h += kHeads, ++i)
@@ -357,7 +366,7 @@ __device__ __forceinline__ void append_window(const Append8Params& p, int64_t r0
   if constexpr (kRotate) {
     for (int i = tid; i < rows * (D / 2); i += kThreads) {
       const int r = i / (D / 2), d = i % (D / 2);
-      turn((double)p.positions[r0 + first_row + r] * p.turns[d], w.rot[0][r][d], w.rot[1][r][d]);
+      turn((double)p.positions[r0 + first_row + r] * p.turns[d], kPart == 1, w.rot[0][r][d], w.rot[1][r][d]);
     }
     __syncthreads();
   }
