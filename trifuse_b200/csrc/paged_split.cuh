@@ -33,9 +33,11 @@
 // products.  Codes become f16 on the way from shared memory to the products,
 // exactly, and a
 // block's scales (16 tokens = one 16-key half of the products) go to the scores
-// and to the weights: S = (K Q^T) s_k, O += (P s_v / r) V.  r is a power of two
-// at or above the value scales that the warp has met; it grows like the running
-// maximum, O rescaled, so that the weights use f16's range whatever the scales.
+// and to the weights: S = (K Q^T) s_k, P' = 2^(S - m + log2(s_v / r)), l += (r / s_v)
+// sum P', O += P' V.  r is a power of two at or above the value scales that the
+// warp has met; where it grows, m falls by as much.  m is the maximum of S +
+// log2(s_v / r), so the largest share of an output is a P' of 2^7 and not rounded,
+// and the weights use f16's range whatever the scales.
 //
 // Measured: 64 decodes of 4096 tokens, 16 heads, pages of 64: 311 us, 6.9 TB/s;
 // 37 ragged decodes of up to 32768 tokens, 8 key heads, pages of 16: 279 us, 6.0
@@ -491,20 +493,28 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int j = 0; j < 4; ++j) s[h][t][j] = 0.f;
-      float k_scale[2] = {1.f, 1.f}, v_scale[2] = {1.f, 1.f}, shrink = 1.f;
+      float k_scale[2] = {1.f, 1.f};
+      float offset[2], back[2], fall = 0.f;  // log2(s_v / r), r / s_v; log2 of r before / r
+      bool odd = false;  // a value scale is not finite
       if constexpr (kCoded) {
         const float4 four = *reinterpret_cast<const float4*>(scales + slot * 4);
         k_scale[0] = four.x;
         k_scale[1] = four.y;
         const float most = fmaxf(four.z, four.w);
+        odd = !(max_nan(four.z, four.w) < INFINITY);
         if (most > ref && most < INFINITY) {
-          const float up = __uint_as_float(min((__float_as_uint(most) + 0x7fffffu) & 0x7f800000u, 0x7f000000u));
-          ref_inverse = 1.f / up;
-          shrink = ref * ref_inverse;
-          ref = up;
+          const uint32_t up = min((__float_as_uint(most) + 0x7fffffu) & 0x7f800000u, 0x7f000000u);
+          fall = (float)((int)(__float_as_uint(ref) >> 23) - (int)(up >> 23));
+          ref = __uint_as_float(up);
+          ref_inverse = 1.f / ref;
         }
-        v_scale[0] = four.z * ref_inverse;
-        v_scale[1] = four.w * ref_inverse;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          // Below 2^-60 nothing is left of what it scales.
+          const float some = fmaxf((h ? four.w : four.z) * ref_inverse, 8.6736174e-19f);
+          offset[h] = __log2f(some);
+          back[h] = __fdividef(1.f, some);
+        }
         // Bytes 4 c .. 4 c + 3 of a lane's row are taken as columns 2 c, 2 c + 1, 2 c + 8
         // and 2 c + 9 of the product, as the queries are.
 #pragma unroll
@@ -539,7 +549,7 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
       const bool ragged = key0 + kSplitKeys - 1 > first_limit;
       uint32_t pb[2][NT][2];  // P^T as the B operand
       float keep[NT][2];
-      bool moved = kCoded && shrink != 1.f;
+      bool moved = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         float sub[2];
@@ -547,34 +557,57 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
         for (int i = 0; i < 2; ++i) {
           float mx = -INFINITY;
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2; ++h) {
+            float most = -INFINITY;
 #pragma unroll
             for (int j = i; j < 4; j += 2) {
               float v = s[h][t][j] * (kCoded ? scale[t][i] * k_scale[h] : scale[t][i]);
               if (ragged && key0 + 16 * h + g + 4 * (j - i) > limit[t][i]) v = -INFINITY;
               s[h][t][j] = v;
-              mx = max_nan(mx, v);
+              most = max_nan(most, v);
             }
+            // (Far out the sum's rounding would lie between m and the scores.)
+            if constexpr (kCoded) most += fabsf(most) < kFar ? offset[h] : 0.f;
+            mx = max_nan(mx, most);
+          }
           mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          const float mn = max_nan(m[t][i], lifted<C>(mx));
+          // What m stands for falls with r, of codes.
+          const float mn = max_nan(kCoded ? m[t][i] + fall : m[t][i], lifted<C>(mx));
           // Rows that have seen no key yet keep m = -inf and add nothing.
           sub[i] = mn == -INFINITY ? 0.f : mn;
-          keep[t][i] = exp2_fast(m[t][i] - sub[i]);
+          keep[t][i] = exp2_fast(kCoded ? (m[t][i] - sub[i]) + fall : m[t][i] - sub[i]);
           moved |= keep[t][i] != 1.f;
+          if (kCoded && fall != 0.f) {
+            l[t][i] *= exp2_fast(m[t][i] - sub[i]);
+            if (l[t][i] == INFINITY) l[t][i] = 3.0e38f;  // the rest is nothing beside it
+          } else {
+            l[t][i] *= keep[t][i];
+          }
           m[t][i] = mn;
-          l[t][i] *= keep[t][i];
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float e[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            e[j] = exp2_fast(s[h][t][j] - sub[j & 1]);
-            l[t][j & 1] += e[j];
-            // A dropped key's value scale may be NaN.
-            if constexpr (kCoded) e[j] = s[h][t][j] == -INFINITY ? 0.f : e[j] * v_scale[h];
+            if constexpr (kCoded) {
+              e[j] = exp2_fast((s[h][t][j] - sub[j & 1]) + offset[h]);
+            } else {
+              e[j] = exp2_fast(s[h][t][j] - sub[j & 1]);
+              l[t][j & 1] += e[j];
+            }
+          }
+          if constexpr (kCoded) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) l[t][i] = fmaf(e[i] + e[i + 2], back[h], l[t][i]);
+            if (odd) {  // the rows that see a key of such a block are NaN
+              const float v = scales[slot * 4 + 2 + h];
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (!(fabsf(v) < INFINITY) && s[h][t][j] != -INFINITY) l[t][j & 1] = __uint_as_float(0x7fc00000u);
+            }
           }
           pb[h][t][0] = transpose8(pack2<C>(e[0], e[1]));
           pb[h][t][1] = transpose8(pack2<C>(e[2], e[3]));
@@ -586,7 +619,7 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[d][t][j] *= kCoded ? keep[t][j & 1] * shrink : keep[t][j & 1];
+            for (int j = 0; j < 4; ++j) o[d][t][j] *= keep[t][j & 1];
       }
       const int have = sg.kv_len - key0;
       if (kCoded) {
