@@ -42,12 +42,12 @@
 // Measured: 64 decodes of 4096 tokens, 16 heads, pages of 64: 311 us, 6.9 TB/s;
 // 37 ragged decodes of up to 32768 tokens, 8 key heads, pages of 16: 279 us, 6.0
 // TB/s (277 with the products taken out: 4 KB pages set that); one decode of 600
-// tokens 7.2 us, of one token 4.0.  Codes: the same 64 decodes 171 us (e4m3; 6.3
-// TB/s), the ragged ones 149 (int8; 124 with the arithmetic taken out), 600 tokens
-// 7.7 or 7.5 (e4m3), one token 5.3; 64 decodes of 1024 tokens 60 and 58 (a segment
-// is three tiles a warp there, and the warps meet at its end).  Integer products of
-// int8 codes with queries in two or three bytes of fixed point took 141 or 143 on
-// the ragged ones, but 62 and 65, 8.2 and 8.4 on the short ones.
+// tokens 7.2 us, of one token 4.0.  Codes: the same 64 decodes 173 us (e4m3; 6.2
+// TB/s), the ragged ones 157 (int8; 124 with the arithmetic taken out), 600 tokens
+// 8.0 or 7.7 (e4m3), one token 5.3; 64 decodes of 1024 tokens 64 and 60 (a segment
+// is three tiles a warp there, and the warps meet at its end).  With m the scores'
+// maximum the ragged ones took 149, and f16 outputs over few keys were off by up to
+// 1.9 times their own rounding (now 1.2).
 #pragma once
 
 #include <cuda.h>

@@ -58,10 +58,10 @@
 // argument and of the block's maximum, and s_v / r into the weights as a summand
 // log2(s_v / r) of the argument, which the row's sum takes out again block by
 // block: P' = 2^(s s_k - m + log2(s_v / r)), l += (r / s_v) sum P', O += P' V.
-// With one half m is the maximum of s s_k + log2(s_v / r): the largest share of an
-// output is a P' of 2^7 and not rounded, which counts where few keys do (f16: 1.1
-// times the output's own rounding, against 1.4 to 1.6; with two halves it took 3%
-// more for 1.15 against 1.4, and m is the scores' maximum).
+// m is the maximum of s s_k + log2(s_v / r): the largest share of an output is a
+// P' of 2^7 and not rounded, which counts where few keys do (f16 outputs are off by
+// 1.1 times their own rounding; with m the scores' maximum 1.4 to 1.6, and 2048 of
+// 16384 took 3% less), and rows that see small values alone lose nothing.
 // That costs a few instructions a block, none a score, and rounds nothing but P'.
 // r is a power of two at or above the segment's value scales (one half: those so
 // far; where it grows, m falls by as much).
@@ -82,7 +82,7 @@
 // (segments of 9 tiles on average, whose ends cost 5600 clocks each; 4 us of it
 // for looking the causal edge's values through, paged_values.cuh), 182 us with
 // bf16 queries over an f16 cache.  Over int8 codes (bf16 queries) the first takes
-// 508 us, widening included, where f16 keys and values take 443; the prompts 240 to
+// 526 us, widening included, where f16 keys and values take 443; the prompts 240 to
 // 250 against 186.
 #include <cuda.h>
 #include <math.h>
@@ -974,12 +974,12 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
             float most = max_nan(sc[16 * b], sc[16 * b + 1]);
 #pragma unroll
             for (int i = 2; i < 16; i += 2) most = max_nan(most, sc[16 * b + i], sc[16 * b + i + 1]);
-            mp[b] = kWiden ? fmaf(most, of.block[b].x, of.block[b].z) : most * of.block[b].x;
+            mp[b] = fmaf(most, of.block[b].x, of.block[b].z);
           }
           mx = max_nan(max_nan(mp[0], mp[1], mp[2]), max_nan(mp[3], mp[4], mp[5]), max_nan(mp[6], mp[7]));
           // Far out the sum's rounding would lie between m and the products that it is
           // taken from: the scores' own maximum there.
-          if (kWiden && __any_sync(0xffffffffu, fabsf(mx) > kFar)) {
+          if (__any_sync(0xffffffffu, fabsf(mx) > kFar)) {
             float own = -INFINITY;
 #pragma unroll
             for (int c = 0; c < 128; ++c) own = max_nan(own, __fmul_rn(sc[c], of.block[c / 16].x));
