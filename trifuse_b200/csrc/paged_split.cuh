@@ -113,6 +113,7 @@ struct SplitParams {
   float* part;  // [part][16][D]
   void* out;
   float scale_log2;
+  int least_power;  // power_floor of the scale
   int* err;
   const long long* wait_cycles;
   const float* k_scales;  // of codes
@@ -441,7 +442,7 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
           for (int j = 0; j < 2; ++j) most = magnitude(qb[k][t][j], most);
         most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int over = beyond_f16(most);
+        const int over = beyond_f16(most, p.least_power);
         const float down = power2(-over);
 #pragma unroll
         for (int i = 0; i < 2; ++i) scale[t][i] *= power2(__shfl_sync(0xffffffffu, over, 4 * (c2 + i)));
@@ -858,6 +859,7 @@ tf_status split_params(const PagedArgs& a, SplitParams* out) {
   p.part = p.stat + (int64_t)plan.split_parts * 2 * kSplitRows;
   p.out = a.out;
   p.scale_log2 = a.scale * kLog2e;
+  p.least_power = power_floor(p.scale_log2);
   TF_TRY(tc_flags(&p.err, const_cast<long long**>(&p.wait_cycles)));
   return TF_OK;
 }

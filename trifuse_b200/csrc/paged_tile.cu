@@ -167,6 +167,7 @@ struct TileParams {
   float* part;  // [part][D / 4][rows of a block][4]: a warp's rows side by side
   void* out;
   float scale_log2;
+  int least_power;  // power_floor of the scale
   int* err;
   const long long* wait_cycles;
   const float* k_scales;  // of codes: [page][kv_head][block], or of widened ones: [kv_head][block]
@@ -870,7 +871,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
 #pragma unroll 1
         for (int i0 = 0; i0 < 32 / kRowsAt; i0 += kBatch) {
           uint4 values[kBatch];
-          uint32_t most[kBatch], all = 0;
+          uint32_t most[kBatch];
 #pragma unroll
           for (int b = 0; b < kBatch; ++b) {
             const int from = (i0 + b) * kRowsAt + lane / kChunks;  // lane whose row this is
@@ -887,21 +888,23 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
             }
           }
           if constexpr (Act<T>::kDtype != Act<C>::kDtype) {
+            bool outside = false;
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
               const uint4 v = values[b];
               most[b] = magnitude(v.w, magnitude(v.z, magnitude(v.y, magnitude(v.x, 0))));
-              all = max(all, most[b]);
+#pragma unroll
+              for (int off = 1; off < kChunks; off <<= 1)
+                most[b] = max(most[b], __shfl_xor_sync(0xffffffffu, most[b], off));
+              outside |= outside_f16(most[b]);
             }
-            const bool wide = __any_sync(0xffffffffu, beyond_f16(all) > 0);
+            outside = __any_sync(0xffffffffu, outside);
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
               float f[8];
               unpack8<T>(values[b], f);
-              if (wide) {
-#pragma unroll
-                for (int off = 1; off < kChunks; off <<= 1) most[b] = max(most[b], __shfl_xor_sync(0xffffffffu, most[b], off));
-                const int over = beyond_f16(most[b]);
+              if (outside) {
+                const int over = beyond_f16(most[b], p.least_power);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) f[k] *= power2(-over);
                 const int mine = __shfl_sync(0xffffffffu, over, lane % kRowsAt * kChunks);
@@ -935,8 +938,8 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
       const float scale = Act<T>::kDtype == Act<C>::kDtype ? p.scale_log2 : p.scale_log2 * boost;
       float m = -INFINITY, l = 0.f;
       float v_ref = 1.f;  // r of O
-      bool boosted = false;
-      if constexpr (kScaled && Act<T>::kDtype != Act<C>::kDtype) boosted = __any_sync(0xffffffffu, boost != 1.f);
+      const bool own_boost = kScaled && Act<T>::kDtype != Act<C>::kDtype && boost != 1.f;
+      const bool boosted = kScaled && Act<T>::kDtype != Act<C>::kDtype && __any_sync(0xffffffffu, own_boost);
       for (int j = 0; j < count; ++j) {
         if (!(ok = wait_warp(&s_full[x], s_turn & 1, ctl, err, 90))) break;
         ++s_turn;
@@ -955,10 +958,15 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         const int key0 = (g.tile0 + j) * kTileKeys;
         if constexpr (kScaled && Act<T>::kDtype != Act<C>::kDtype) {
           if (boosted) {
+            // Powers below one before the units, those above after them: what lies
+            // between stays in fp32's range.
+            const float before = fminf(boost, 1.f), after = fmaxf(boost, 1.f);
 #pragma unroll
-            for (int c = 0; c < 128; ++c) sc[c] *= boost;
+            for (int c = 0; c < 128; ++c) sc[c] = own_boost ? sc[c] * before * of.block[c / 16].x * after : sc[c];
           }
         }
+        // Of codes: what the scores are still to be multiplied with.
+        const auto unit_of = [&](int block) { return own_boost ? 1.f : of.block[block].x; };
         if (key0 + kTileKeys - 1 > first_limit) {
           const int lim = limit - key0;  // later columns are masked
 #pragma unroll
@@ -974,7 +982,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
             float most = max_nan(sc[16 * b], sc[16 * b + 1]);
 #pragma unroll
             for (int i = 2; i < 16; i += 2) most = max_nan(most, sc[16 * b + i], sc[16 * b + i + 1]);
-            mp[b] = fmaf(most, of.block[b].x, of.block[b].z);
+            mp[b] = fmaf(most, unit_of(b), of.block[b].z);
           }
           mx = max_nan(max_nan(mp[0], mp[1], mp[2]), max_nan(mp[3], mp[4], mp[5]), max_nan(mp[6], mp[7]));
           // Far out the sum's rounding would lie between m and the products that it is
@@ -982,7 +990,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
           if (__any_sync(0xffffffffu, fabsf(mx) > kFar)) {
             float own = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < 128; ++c) own = max_nan(own, __fmul_rn(sc[c], of.block[c / 16].x));
+            for (int c = 0; c < 128; ++c) own = max_nan(own, __fmul_rn(sc[c], unit_of(c / 16)));
             if (fabsf(mx) > kFar) mx = own;
           }
         } else {
@@ -1046,7 +1054,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
             raw = false;
 #pragma unroll
             for (int c = 0; c < 128; ++c)
-              sc[c] = __fadd_rn(__fadd_rn(__fmul_rn(sc[c], of.block[c / 16].x), sub), of.block[c / 16].z);
+              sc[c] = __fadd_rn(__fadd_rn(__fmul_rn(sc[c], unit_of(c / 16)), sub), of.block[c / 16].z);
           }
         }
         uint64_t sp[4], block_unit = 0ull, block_offset = 0ull;
@@ -1063,7 +1071,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
               const int block = k0 / 16;
               if (c % 8 == 0) {
                 const ulonglong2 both = *reinterpret_cast<const ulonglong2*>(&of.block[block]);
-                block_unit = raw ? both.x : f2_pack(1.f, 1.f);
+                block_unit = raw && !own_boost ? both.x : f2_pack(1.f, 1.f);
                 block_offset = raw ? f2_add(nm, both.y) : 0ull;
                 sp[0] = sp[1] = 0ull;
               }
@@ -1297,6 +1305,7 @@ tf_status tile_params(const PagedArgs& a, TileParams* out) {
   p.page_stride = a.kv.page_stride;
   p.out = a.out;
   p.scale_log2 = a.scale * kLog2e;
+  p.least_power = power_floor(p.scale_log2);
   TF_TRY(tc_flags(&p.err, const_cast<long long**>(&p.wait_cycles)));
   return TF_OK;
 }

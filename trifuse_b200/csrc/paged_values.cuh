@@ -7,6 +7,8 @@
 // decide alone: a sum with an infinity or a NaN in it).
 #pragma once
 
+#include <math.h>
+
 #include "common.cuh"
 
 namespace tf {
@@ -101,17 +103,35 @@ __device__ __forceinline__ void clear_not_finite(uint8_t* chunks, int n, int lan
   }
 }
 
-// Queries of bf16 for a cache of f16, whose largest value is 65504: a row with
-// larger ones goes to the product divided by a power of two, which its scores
-// get back with the scale (exact both ways).  Rows within the range, that is
-// all but unheard-of ones, are converted as they are.
+// Queries of bf16 for products in f16, which ends at 65504 and below 2^-14 has
+// steps of 2^-24: a row with larger values, or with none of kSmallQuery or more,
+// goes to the product times a power of two that brings its largest value to 2^15,
+// and its scores get the inverse back with the scale (exact both ways; what is
+// 2^-39 of the row's largest may be rounded).  A caller's scale, or an 8-bit
+// cache's, can make ordinary scores of such rows.  Other rows are converted as
+// they are: their values are off by at most 2^-25, which is 2^-21 of the largest.
 //
 // The largest magnitude, as bf16 bits, of two packed values.
 __device__ __forceinline__ uint32_t magnitude(uint32_t w, uint32_t most) {
   return max(most, max(w & 0x7fffu, w >> 16 & 0x7fffu));
 }
-// The power (0 or more) by which a row of that magnitude must be divided.
-__device__ __forceinline__ int beyond_f16(uint32_t most) { return max((int)(most >> 7) - (127 + 15), 0); }
+constexpr int kSmallQuery = 127 - 4;  // exponent of 2^-4 in bf16
+__device__ __forceinline__ bool outside_f16(uint32_t most) {
+  return (int)(most >> 7) > 127 + 15 || (most != 0u && (int)(most >> 7) < kSmallQuery);
+}
+// The power by which a row of that magnitude must be divided (0: by none), not
+// below `least` (power_floor).
+__device__ __forceinline__ int beyond_f16(uint32_t most, int least) {
+  return outside_f16(most) ? max((int)(most >> 7) - (127 + 15), least) : 0;
+}
+// The least power whose product with the scale is a normal number; 2^120 makes
+// f16 numbers of all bf16 ones that are smaller than 2^-105 (multiples of 2^-133).
+inline int power_floor(float scale_log2) {
+  int exponent;
+  frexpf(scale_log2, &exponent);
+  const int least = -125 - exponent;
+  return least < -120 ? -120 : least > 0 ? 0 : least;
+}
 // 2^n, n in [-126, 127].
 __device__ __forceinline__ float power2(int n) { return __uint_as_float((uint32_t)(127 + n) << 23); }
 
