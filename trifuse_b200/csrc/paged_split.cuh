@@ -87,9 +87,9 @@ struct Shape {
   static constexpr int kPitch = kJoin + 4;            // joined outputs: rows 4 words apart in the banks
   static constexpr int kOffJoin = kWarps * kRing;
   static constexpr int kOffStat = kOffJoin + kWarps * kJoinRows * kPitch * 4;
-  static constexpr int kOffScale = kOffStat + kWarps * kSplitRows * 2 * 4;  // [warp][stage] k, k, v, v
-  static constexpr int kOffRef = kOffScale + (kCoded ? kWarps * kStages * 16 : 0);
-  static constexpr int kOffBar = kOffRef + (kCoded ? kWarps * 4 : 0);
+  static constexpr int kStat = kSplitRows * (kCoded ? 3 : 2);  // a row's m and l, of codes also r
+  static constexpr int kOffScale = kOffStat + kWarps * kStat * 4;  // [warp][stage] k, k, v, v
+  static constexpr int kOffBar = kOffScale + (kCoded ? kWarps * kStages * 16 : 0);
   static constexpr int kSmem = kOffBar + kWarps * kStages * 8 + 16 + 1024;  // + alignment slack
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
@@ -110,7 +110,7 @@ struct SplitParams {
   const int32_t* starts;
   int* counters;
   float* stat;  // [part][2][16]: m, l
-  float* part;  // [part][16][D]
+  float* part;  // [part][16][D] (of codes divided by l)
   void* out;
   float scale_log2;
   int least_power;  // power_floor of the scale
@@ -223,14 +223,33 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // (m = -inf) weighs nothing, also where every part is empty.
 __device__ __forceinline__ float part_weight(float m, float M) { return m == -INFINITY ? 0.f : exp2_fast(m - M); }
 
+// The same times the part's sum, where a part's outputs are kept divided by it (an
+// 8-bit cache, whose values may lie anywhere in fp32's range): down to 2^-149, for
+// a small weight may stand before a large value.
+__device__ __forceinline__ float part_share(float m, float M, float sum) {
+  float f;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(f) : "f"(m - M));
+  return m == -INFINITY ? 0.f : f * sum;
+}
+// A power of two that brings up to 2^kParts shares of at most `most` each (a sum,
+// below 2^110) to a total below one, and its inverse.
+template <int kParts>
+__device__ __forceinline__ float share_unit(float most) {
+  return __uint_as_float((253u - kParts << 23) - (__float_as_uint(fmaxf(most, 0.f)) & 0x7f800000u));
+}
+template <int kParts>
+__device__ __forceinline__ float share_unit_inverse(float most) {
+  return __uint_as_float((1u + kParts << 23) + (__float_as_uint(fmaxf(most, 0.f)) & 0x7f800000u));
+}
+
 // The pieces of a segment's rows joined, in piece order within each of the groups
-// of threads that share them.  work: (parts + 1) * 16 floats of shared memory, and
-// at least four a thread.  Called by the whole block; ends with a barrier.
+// of threads that share them; each piece's outputs are divided by its sum.  work:
+// parts * 16 floats of shared memory, and at least four a thread.  Called by the
+// whole block; ends with a barrier.
 constexpr int kFewParts = 8;
 template <typename T, int D, int kThreads>
 __device__ __forceinline__ void merge_many(const SplitParams& p, const PagedSegment& sg, float* work) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  float* sums = work + sg.parts * kSplitRows;  // of the rows
   for (int r = warp; r < sg.rows; r += kThreads / 32) {
     const float* stat = p.stat + (int64_t)sg.part0 * 32 + r;
     float M = -INFINITY, sum = 0.f;
@@ -238,12 +257,13 @@ __device__ __forceinline__ void merge_many(const SplitParams& p, const PagedSegm
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) M = max_nan(M, __shfl_xor_sync(0xffffffffu, M, off));
     for (int k = lane; k < sg.parts; k += 32) {
-      const float f = part_weight(__ldcg(stat + (int64_t)k * 32), M);
-      sum = fmaf(f, __ldcg(stat + (int64_t)k * 32 + 16), sum);
+      const float f = part_share(__ldcg(stat + (int64_t)k * 32), M, __ldcg(stat + (int64_t)k * 32 + 16));
+      sum += f;
       work[k * kSplitRows + r] = f;
     }
     sum = warp_sum_butterfly(sum);
-    if (lane == 0) sums[r] = sum;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    for (int k = lane; k < sg.parts; k += 32) work[k * kSplitRows + r] *= inv;
   }
   __syncthreads();
   // Four values a thread; threads i, i + n, i + 2 n, ... take every g-th piece.
@@ -265,7 +285,6 @@ __device__ __forceinline__ void merge_many(const SplitParams& p, const PagedSegm
         acc.w = fmaf(f, v.w, acc.w);
       }
     }
-    const float sum = sums[r];
     if (groups > 1) {  // the weights' place is free now
       __syncthreads();
       float4* out = reinterpret_cast<float4*>(work);
@@ -281,9 +300,7 @@ __device__ __forceinline__ void merge_many(const SplitParams& p, const PagedSegm
       const int pr = sg.row0 + r;
       T* orow = static_cast<T*>(p.out) + ((int64_t)(sg.q_row + pr / p.group) * p.heads + sg.kv_head * p.group +
                                           pr % p.group) * D + d;
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      alignas(8) const T v[4] = {from_f<T>(acc.x * inv), from_f<T>(acc.y * inv), from_f<T>(acc.z * inv),
-                                 from_f<T>(acc.w * inv)};
+      alignas(8) const T v[4] = {from_f<T>(acc.x), from_f<T>(acc.y), from_f<T>(acc.z), from_f<T>(acc.w)};
       *reinterpret_cast<uint2*>(orow) = *reinterpret_cast<const uint2*>(v);
     }
   }
@@ -317,15 +334,14 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
     paged_split_kernel(const __grid_constant__ SplitParams p) {
   using S = Shape<D, NT, C, St>;
   constexpr bool kCoded = S::kCoded;
-  constexpr int kWarps = S::kWarps, kThreads = S::kThreads;
+  constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kStat = S::kStat;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* ring = base + warp * S::kRing;
   float* join = reinterpret_cast<float*>(base + S::kOffJoin);
-  float* stat = reinterpret_cast<float*>(base + S::kOffStat);  // [warp][2][16]
+  float* stat = reinterpret_cast<float*>(base + S::kOffStat);  // [warp][kStat / 16][16]
   float* scales = reinterpret_cast<float*>(base + S::kOffScale) + warp * S::kStages * 4;
-  float* refs = reinterpret_cast<float*>(base + S::kOffRef);  // [warp]
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + S::kOffBar) + warp * S::kStages;
   int* last_s = reinterpret_cast<int*>(base + S::kOffBar + kWarps * S::kStages * 8);
 
@@ -582,7 +598,7 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
           moved |= keep[t][i] != 1.f;
           if (kCoded && fall != 0.f) {
             l[t][i] *= exp2_fast(m[t][i] - sub[i]);
-            if (l[t][i] == INFINITY) l[t][i] = 3.0e38f;  // the rest is nothing beside it
+            if (l[t][i] > 1.0e32f) l[t][i] = 1.0e32f;  // the rest is nothing beside it
           } else {
             l[t][i] *= keep[t][i];
           }
@@ -719,7 +735,6 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
     }
 
     // Join the warps' results.
-    if (kCoded && lane == 0) refs[warp] = ref;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -729,8 +744,9 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
         l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], 16);
         const int r = 8 * t + c2 + i;
         if (g == 0) {
-          stat[warp * 32 + r] = m[t][i];
-          stat[warp * 32 + 16 + r] = l[t][i];
+          stat[warp * kStat + r] = m[t][i];
+          stat[warp * kStat + 16 + r] = l[t][i];
+          if (kCoded) stat[warp * kStat + 32 + r] = ref;
         }
       }
 #pragma unroll
@@ -751,24 +767,37 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
         const int r = i / S::kJoin, at = i % S::kJoin, d = pass * S::kJoin + at;
         float M = stat[r];
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) M = max_nan(M, stat[w * 32 + r]);
-        float acc = 0.f, sum = 0.f;
+        for (int w = 1; w < kWarps; ++w) M = max_nan(M, stat[w * kStat + r]);
+        float acc = 0.f, sum = 0.f, most = 0.f;
+        if constexpr (kCoded) {
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float f = part_weight(stat[w * 32 + r], M);
-          acc = fmaf(kCoded ? f * refs[w] : f, join[(w * S::kJoinRows + r) * S::kPitch + at], acc);
-          sum = fmaf(f, stat[w * 32 + 16 + r], sum);
+          for (int w = 0; w < kWarps; ++w) most = fmaxf(most, stat[w * kStat + 16 + r]);
+          const float unit = share_unit<4>(most);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float f = part_share(stat[w * kStat + r], M, unit);
+            acc = fmaf(f * stat[w * kStat + 32 + r], join[(w * S::kJoinRows + r) * S::kPitch + at], acc);
+            sum = fmaf(f, stat[w * kStat + 16 + r], sum);
+          }
+          acc = sum == 0.f ? 0.f : acc / sum;
+        } else {
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float f = part_weight(stat[w * kStat + r], M);
+            acc = fmaf(f, join[(w * S::kJoinRows + r) * S::kPitch + at], acc);
+            sum = fmaf(f, stat[w * kStat + 16 + r], sum);
+          }
         }
         if (sg.part < 0) {
           const int pr = sg.row0 + r;
           T* orow = static_cast<T*>(p.out) + ((int64_t)(sg.q_row + pr / p.group) * p.heads + sg.kv_head * p.group +
                                               pr % p.group) * D;
-          orow[d] = from_f<T>(sum == 0.f ? 0.f : acc / sum);
+          orow[d] = from_f<T>(kCoded ? acc : sum == 0.f ? 0.f : acc / sum);
         } else {
           p.part[((int64_t)sg.part * kSplitRows + r) * D + d] = acc;
           if (d == 0) {
             p.stat[(int64_t)sg.part * 32 + r] = M;
-            p.stat[(int64_t)sg.part * 32 + 16 + r] = sum;
+            p.stat[(int64_t)sg.part * 32 + 16 + r] = kCoded ? sum * share_unit_inverse<4>(most) : sum;
           }
         }
       }
@@ -793,21 +822,27 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
         // share the pieces (one long request, 148 pieces: 65 -> 27 us).
         constexpr int kRoom = kWarps * S::kJoinRows * S::kPitch;
         static_assert(kRoom >= 4 * kThreads, "the groups' outputs");
-        if (sg.parts > kFewParts && (sg.parts + 1) * kSplitRows <= kRoom) {
+        if (sg.parts > kFewParts && sg.parts * kSplitRows <= kRoom) {
           merge_many<T, D, kThreads>(p, sg, join);
           continue;
         }
       }
       for (int i = tid; i < sg.rows * D; i += kThreads) {
         const int r = i / D, d = i % D;
-        float M = -INFINITY;
-        for (int k = 0; k < sg.parts; ++k) M = max_nan(M, __ldcg(&p.stat[(int64_t)(sg.part0 + k) * 32 + r]));
+        float M = -INFINITY, most = 0.f;
+        for (int k = 0; k < sg.parts; ++k) {
+          const float* st = &p.stat[(int64_t)(sg.part0 + k) * 32 + r];
+          M = max_nan(M, __ldcg(st));
+          if (kCoded) most = fmaxf(most, __ldcg(st + 16));
+        }
+        const float unit = share_unit<8>(most);
         float acc = 0.f, sum = 0.f;
         for (int k = 0; k < sg.parts; ++k) {
           const int64_t at = sg.part0 + k;
-          const float f = part_weight(__ldcg(&p.stat[at * 32 + r]), M);
+          const float m = __ldcg(&p.stat[at * 32 + r]), own = __ldcg(&p.stat[at * 32 + 16 + r]);
+          const float f = kCoded ? part_share(m, M, own * unit) : part_weight(m, M);
           acc = fmaf(f, __ldcg(&p.part[(at * kSplitRows + r) * D + d]), acc);
-          sum = fmaf(f, __ldcg(&p.stat[at * 32 + 16 + r]), sum);
+          sum = kCoded ? sum + f : fmaf(f, own, sum);
         }
         const int pr = sg.row0 + r;
         T* orow = static_cast<T*>(p.out) + ((int64_t)(sg.q_row + pr / p.group) * p.heads + sg.kv_head * p.group +

@@ -1020,7 +1020,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
           if (!(mx <= m + kRescale)) m = max_nan(m, mx);
           factor = fast_exp2((before - m) + of.fall);
           l *= fast_exp2(before - m);
-          if (l == INFINITY) l = 3.0e38f;  // the rest is nothing beside it
+          if (l > 1.0e32f) l = 1.0e32f;  // the rest is nothing beside it
         } else if (!(mx <= m + kRescale)) {  // also for NaN, and for the first key seen
           mx = max_nan(m, mx);  // a NaN stays
           factor = fast_exp2(m - mx);
@@ -1119,8 +1119,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
       }
       const bool cleared = !kScaled && ctl->cleared != 0;
       // A row that has seen no key above -inf gives zeros.
-      float inv = m == -INFINITY ? 0.f : 1.f / l;
-      if (kScaled) inv *= v_ref;
+      const float inv = m == -INFINITY ? 0.f : 1.f / l;
       T* orow = static_cast<T*>(p.out) +
                 ((int64_t)(g.q_row + token) * p.heads + g.kv_head * p.group + pr % p.group) * D;
       float* prow = p.part + (int64_t)g.part * S::kRows * D + row * 4;
@@ -1133,21 +1132,23 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0.f;
         }
+        if constexpr (kScaled) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = m == -INFINITY ? 0.f : o[i] * inv * v_ref;
+        }
         if (mine && g.part < 0) {
 #pragma unroll
           for (int i = 0; i < 32; i += 16) {
             float f[16];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) f[k] = m == -INFINITY ? 0.f : o[i + k] * inv;
+            for (int k = 0; k < 16; ++k) f[k] = kScaled ? o[i + k] : m == -INFINITY ? 0.f : o[i + k] * inv;
             store32(orow + c + i, pack8<T>(f), pack8<T>(f + 8));
           }
         } else if (mine) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            float4 four = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-            if (kScaled) four.x *= v_ref, four.y *= v_ref, four.z *= v_ref, four.w *= v_ref;
-            *reinterpret_cast<float4*>(prow + (c + i) * S::kRows) = four;
-          }
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(prow + (c + i) * S::kRows) =
+                make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
         __syncwarp();  // the next load takes the whole warp, also where the rows end inside it
       }
@@ -1178,10 +1179,13 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
 }
 
 // Joins the pieces of cut row blocks, in piece order.  A warp takes 32 rows
-// and 4 columns, so the pieces' outputs arrive 512 bytes at a time.
+// and 4 columns, so the pieces' outputs arrive 512 bytes at a time.  kDivided: a
+// piece's outputs are divided by its sum (an 8-bit cache, whose values may lie
+// anywhere in fp32's range: weights count down to 2^-149, and a power of two keeps
+// their total below one).
 constexpr int kMergeWarps = 8;
 
-template <typename T, int D, int R>
+template <typename T, int D, int R, bool kDivided>
 __global__ void __launch_bounds__(32 * kMergeWarps)
     paged_merge_kernel(const PagedSegment* items, const float* stat, const float* part, int group, int heads,
                        T* out) {
@@ -1192,17 +1196,29 @@ __global__ void __launch_bounds__(32 * kMergeWarps)
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the pieces are written
   const float* st = stat + (int64_t)g.part0 * 2 * R + row;
   const float* o = part + (int64_t)g.part0 * R * D + (c * R + row) * 4;
-  float M = -INFINITY;
+  float M = -INFINITY, most = 0.f;
 #pragma unroll 4
-  for (int i = 0; i < g.parts; ++i) M = max_nan(M, st[(int64_t)i * 2 * R]);
+  for (int i = 0; i < g.parts; ++i) {
+    M = max_nan(M, st[(int64_t)i * 2 * R]);
+    if (kDivided) most = fmaxf(most, st[(int64_t)i * 2 * R + R]);
+  }
+  // 2^-10 / (the sums' largest power of two): for up to 2^8 pieces.
+  const float unit = __uint_as_float((245u << 23) - (__float_as_uint(most) & 0x7f800000u));
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
 #pragma unroll 4
   for (int i = 0; i < g.parts; ++i) {
-    const float m = st[(int64_t)i * 2 * R];
-    const float f = m == -INFINITY ? 0.f : fast_exp2(m - M);  // an empty piece holds zeros
+    const float m = st[(int64_t)i * 2 * R], own = st[(int64_t)i * 2 * R + R];
+    float f;
+    if (kDivided) {
+      asm("ex2.approx.f32 %0, %1;" : "=f"(f) : "f"(m - M));
+      f = m == -INFINITY ? 0.f : f * (own * unit);  // an empty piece holds zeros
+      sum += f;
+    } else {
+      f = m == -INFINITY ? 0.f : fast_exp2(m - M);
+      sum = fmaf(f, own, sum);
+    }
     const float4 v = *reinterpret_cast<const float4*>(o + (int64_t)i * R * D);
-    sum = fmaf(f, st[(int64_t)i * 2 * R + R], sum);
     acc.x = fmaf(f, v.x, acc.x);
     acc.y = fmaf(f, v.y, acc.y);
     acc.z = fmaf(f, v.z, acc.z);
@@ -1260,7 +1276,7 @@ tf_status launch(TileParams p, const Work& w, const char* table, bool early, cud
   cfg.stream = s;
   cfg.attrs = &overlap;
   cfg.numAttrs = 1;
-  TF_CUDA(cudaLaunchKernelEx(&cfg, paged_merge_kernel<T, D, S::kRows>,
+  TF_CUDA(cudaLaunchKernelEx(&cfg, paged_merge_kernel<T, D, S::kRows, S::kScaled>,
                              reinterpret_cast<const PagedSegment*>(table + w.merges), (const float*)p.stat,
                              (const float*)p.part, p.group, p.heads, static_cast<T*>(p.out)));
   return check_launch("paged_merge");
