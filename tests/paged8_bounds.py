@@ -50,11 +50,18 @@ class Exact:
                 self.sums[at] = a.masked_fill(hidden, 0.0).amax(-1).reshape(n, H, 1)
             row += n
 
+    def rows(self, at):
+        """The same of some rows."""
+        some = object.__new__(Exact)
+        some.__dict__.update({n: x[at] for n, x in self.__dict__.items()})
+        return some
 
-def check_rounding(got, ref, scattered=True, largest_exact=False):
+
+def check_rounding(got, ref, scattered=True, largest_exact=False, exponents=2.0 ** -18):
     """Each output: 2^-11 of sum p |v| for the weights (2^-32 of the largest share for each that lies below f16's
     normal numbers), its own rounding, and fp32's part: eight sums' roundings (2^-23) of a score's terms and the
-    offsets' 2^-18, in numerator and denominator.
+    exponents' own (the scales' logarithms, up to 2^6, are within 2^-19; up to 2^9, added up in three steps, 2^-13 for
+    the calls that say so), in numerator and denominator.
 
     All outputs together, where values and shares are scattered: independent roundings add up by their squares.  A
     relative error evenly spread up to u has u^2 / 3 times the mean of 1 / m^2 over mantissas, 0.541 where they are
@@ -64,7 +71,7 @@ def check_rounding(got, ref, scattered=True, largest_exact=False):
     assert torch.isfinite(want).all() and torch.isfinite(got).all()
     u, own = UNIT[F16], UNIT[act]
     err = (got.double() - want).abs()
-    fp32 = 2 * (2.0 ** -18 + 16 * 2.0 ** -23 * ref.sums) * ref.mass
+    fp32 = 2 * (exponents + 16 * 2.0 ** -23 * ref.sums) * ref.mass
     bound = u * ref.mass + 2.0 ** -32 * ref.share + fp32 + own * (want.abs() + u * ref.mass + fp32) + LEAST[act]
     assert (err <= bound).all(), f"worst {float((err / bound).max()):.2f} of the bound"
     if scattered:

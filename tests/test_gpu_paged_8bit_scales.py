@@ -38,3 +38,132 @@ def test_values_near_the_types_largest(ops, kind, H, Hk, D, new, kv):
     assert ops.device_error() == 0
     ref = Exact(c, q, new, kv)
     check_rounding(got, ref)
+
+
+def block_of(c, request, token):
+    """Index of the token's block of scales."""
+    return c.table[request, token // c.page].long(), slice(None), token % c.page // BLOCK
+
+
+ROWS = [(1, 1, 657), (2, 2, 657), (5, 3, 657), (40, 2, 657), (300, 2, 657), (300, 1, 300), (1, 2, 20001), (40, 1, 20001)]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("power", [30, 70, 120])
+@pytest.mark.parametrize("n,G,L", [(2, 2, 657), (5, 3, 657), (16, 1, 5009), (40, 2, 657), (40, 1, 20001), (130, 1, 657), (300, 2, 657),
+                                   (300, 1, 305)])
+def test_a_later_token_of_any_size(ops, kind, power, n, G, L):
+    """The last token's block, and one in the middle of the new ones, hold values 2^power times as large: the rows before
+    do not see them, and are as exact as without."""
+    for token in {L - 1, L - n // 2}:
+        c = Cache([L], 2, 128, 16, kind, seed=n, spread=1)
+        c.vs[block_of(c, 0, token)] *= 2.0 ** power
+        q = queries(n, 2 * G, 128, n)
+        plan = ops.PagedPlan([n], [L], 2 * G, 2, 128, 16)
+        got = ops.paged_attention(q, *c.args(), plan, **c.scales())
+        assert ops.device_error() == 0
+        ref = Exact(c, q, [n], [L])
+        check_rounding(got, ref, scattered=False, exponents=2.0 ** -13)
+        before = max(0, token // BLOCK * BLOCK - (L - n))
+        if before:
+            check_rounding(got[:before], ref.rows(slice(0, before)), exponents=2.0 ** -13)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("power", [30, 100, 118])
+@pytest.mark.parametrize("gap", [0.5, 20.0, 60.0, 88.0, 150.0, 300.0])
+@pytest.mark.parametrize("n,G,L", ROWS)
+def test_large_values_of_little_weight(ops, kind, power, gap, n, G, L):
+    """A block that every row sees has e^-gap of the weight and values 2^power times as large."""
+    D = 128
+    c = Cache([L], 2, D, 16, kind, seed=n, spread=1)
+    at = block_of(c, 0, 7)
+    c.k[..., 0] = 0
+    c.k[at[0]] = 0  # pages of 16: one block
+    c.k[at[0], ..., 0] = torch.tensor(-LARGEST[kind], device="cuda").to(kind)
+    c.ks[at] = gap * D ** 0.5 / (4 * LARGEST[kind])
+    c.vs[at] *= 2.0 ** power
+    q = queries(n, 2 * G, D, n) * 0.5
+    q[..., 0] = 4
+    plan = ops.PagedPlan([n], [L], 2 * G, 2, D, 16)
+    got = ops.paged_attention(q, *c.args(), plan, **c.scales())
+    assert ops.device_error() == 0
+    check_rounding(got, Exact(c, q, [n], [L]), scattered=False, exponents=2.0 ** -13)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("act,low,high", [(BF16, -110, 100), (BF16, -110, -50), (BF16, -60, 60), (F16, -110, 8)])
+@pytest.mark.parametrize("size", [0.5, 4.0])
+@pytest.mark.parametrize("n,G,L", ROWS + [(300, 2, 5000)])
+def test_blocks_of_every_size(ops, kind, act, low, high, size, n, G, L):
+    """Each block's values lie anywhere between 2^low and 2^high; every tenth block's scale is zero, whatever its codes."""
+    c = Cache([L], 2, 64, 16, kind, seed=n, spread=0)
+    g = torch.Generator().manual_seed(n + 1)
+    power = torch.randint(low, high + 1, c.vs.shape, generator=g).cuda()
+    c.vs *= torch.where((torch.rand(c.vs.shape, generator=g) < 0.1).cuda(), 0.0, 2.0 ** power)
+    q = (torch.randn(n, 2 * G, 64, generator=g) * size).to(act).cuda()
+    plan = ops.PagedPlan([n], [L], 2 * G, 2, 64, 16)
+    got = ops.paged_attention(q, *c.args(), plan, **c.scales())
+    assert ops.device_error() == 0
+    check_rounding(got, Exact(c, q, [n], [L]), scattered=False, exponents=2.0 ** -13)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("power", [-116, -60, 60, 110])
+@pytest.mark.parametrize("n,G,L", ROWS)
+def test_all_values_large_or_small(ops, kind, power, n, G, L):
+    """One power of two for all values: exact, so the outputs are those of ordinary ones."""
+    c = Cache([L], 2, 128, 16, kind, seed=n)
+    c.vs *= 2.0 ** power
+    q = queries(n, 2 * G, 128, n)
+    plan = ops.PagedPlan([n], [L], 2 * G, 2, 128, 16)
+    got = ops.paged_attention(q, *c.args(), plan, **c.scales())
+    assert ops.device_error() == 0
+    check_rounding(got, Exact(c, q, [n], [L]))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", [300.0, 7000.0, 40000.0])
+@pytest.mark.parametrize("n,L", [(1, 3000), (5, 700), (40, 3000), (300, 2500)])
+def test_far_scores_of_blocks_of_every_size(ops, kind, size, n, L):
+    """Keys of one direction in steps of 3 per cent, scores to 10^9: the largest visible score decides, with those equal
+    to it, whatever the other blocks' values."""
+    H, Hk, D, page = 4, 2, 64, 16
+    c = Cache([L], Hk, D, page, kind, seed=n, spread=0)
+    g = torch.Generator().manual_seed(n)
+    blocks = -(-L // BLOCK)
+    step = torch.randint(0, 40, (blocks,), generator=g).double()
+    ids = c.table[0].long()
+    c.k[ids] = int(LARGEST[kind]) if kind == I8 else torch.tensor(448.0, device="cuda").to(kind)
+    c.ks[ids, :, 0] = (size * 1.03 ** (step - 40) / LARGEST[kind]).float().cuda()[:, None]
+    c.vs[ids, :, 0] = 2.0 ** torch.randint(-100, 100, (blocks, 1), generator=g).float().cuda()
+    q = (size * (0.5 + torch.rand(n, H, 1, generator=g))).to(BF16).expand(n, H, D).contiguous().cuda()
+    plan = ops.PagedPlan([n], [L], H, Hk, D, page)
+    got = ops.paged_attention(q, *c.args(), plan, scale=1.0, **c.scales())
+    assert ops.device_error() == 0
+    ref = Exact(c, q, [n], [L], 1.0)
+    ref.sums = torch.zeros_like(ref.sums)  # one direction: no rounding of a key moves them apart
+    check_rounding(got, ref, scattered=False, exponents=2.0 ** -13)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,G,L", [(5, 3, 657), (40, 2, 657), (300, 2, 657), (300, 1, 300), (130, 2, 20001)])
+def test_nan_scales_among_blocks_of_every_size(ops, kind, n, G, L):
+    """A NaN scale of a value or a key makes the rows NaN that see its block; the others are as exact as without it."""
+    c = Cache([L], 2, 64, 16, kind, seed=n, spread=0)
+    g = torch.Generator().manual_seed(n + 1)
+    c.vs *= (2.0 ** torch.randint(-100, 100, c.vs.shape, generator=g)).cuda()
+    q = queries(n, 2 * G, 64, n)
+    ref = Exact(c, q, [n], [L])
+    plan = ops.PagedPlan([n], [L], 2 * G, 2, 64, 16)
+    for scales, token in ((c.vs, L - 1), (c.ks, L - 1), (c.vs, L - n // 2)):
+        at = block_of(c, 0, token)
+        was = scales[at].clone()
+        scales[at] = float("nan")
+        got = ops.paged_attention(q, *c.args(), plan, **c.scales())
+        assert ops.device_error() == 0
+        scales[at] = was
+        before = max(0, token // BLOCK * BLOCK - (L - n))
+        assert torch.isnan(got[before:]).all()
+        if before:
+            check_rounding(got[:before], ref.rows(slice(0, before)), scattered=False, exponents=2.0 ** -13)

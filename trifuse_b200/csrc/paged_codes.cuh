@@ -40,6 +40,19 @@ struct Divisor {
   }
 };
 
+// The reference r of value scales: a power of two at or above those that are finite
+// (2^-126 .. 2^126; beyond that, near them).  Ratios s_v / r down to 2^-61 are worked
+// with as they are; below that (or at zero, which has no logarithm) scales count as
+// far apart.
+constexpr float kLeastRef = 1.17549435e-38f, kLeastInverse = 8.50705917e37f;  // 2^-126, 2^126
+constexpr float kLeastRatio = 4.33680869e-19f;                                // 2^-61
+__device__ __forceinline__ float power_above(float v) {
+  return __uint_as_float(min((__float_as_uint(v) + 0x7fffffu) & 0x7f800000u, 0x7e800000u));
+}
+__device__ __forceinline__ float inverse_of(float power) { return __uint_as_float(0x7f000000u - __float_as_uint(power)); }
+__device__ __forceinline__ float exponent_of(float power) { return (float)((int)(__float_as_uint(power) >> 23) - 127); }
+__device__ __forceinline__ bool far_apart(float lowest, float ref) { return lowest < ref * kLeastRatio || lowest == 0.f; }
+
 template <>
 struct Code<I8> {
   static constexpr tf_dtype kDtype = TF_DTYPE_I8;

@@ -31,13 +31,16 @@
 // An 8-bit cache (storage S = I8 or E4M3, C = f16) runs through the same code with
 // 12 warps (8 for 16 rows), since its tiles are half the bytes and the same
 // products.  Codes become f16 on the way from shared memory to the products,
-// exactly, and a
-// block's scales (16 tokens = one 16-key half of the products) go to the scores
-// and to the weights: S = (K Q^T) s_k, P' = 2^(S - m + log2(s_v / r)), l += (r / s_v)
-// sum P', O += P' V.  r is a power of two at or above the value scales that the
-// warp has met; where it grows, m falls by as much.  m is the maximum of S +
-// log2(s_v / r), so the largest share of an output is a P' of 2^7 and not rounded,
-// and the weights use f16's range whatever the scales.
+// exactly, and a block's scales (16 tokens = one 16-key half of the products) go to
+// the scores and to the weights: S = (K Q^T) s_k, P' = 2^(S - m + log2(s_v / r)),
+// l += (r / s_v) sum P', O += P' V.  r is a power of two at or above the value
+// scales that the warp has met; where it grows, m falls by as much.  m is the
+// maximum of S + log2(s_v / r), so the largest share of an output is a P' of 2^7 and
+// not rounded, and the weights use f16's range whatever the scales.
+//   Once a warp has met scales more than 2^60 apart (or zero), r / s_v no longer
+// serves: keys with a tiny scale may hold all of a row's weight, or none of it beside
+// a large one that counts, or one that the row does not see.  From there on l sums
+// 2^(S - mu), mu the scores' own maximum, and m = mu + kappa is kept in two parts.
 //
 // Measured: 64 decodes of 4096 tokens, 16 heads, pages of 64: 311 us, 6.9 TB/s;
 // 37 ragged decodes of up to 32768 tokens, 8 key heads, pages of 16: 279 us, 6.0
@@ -212,11 +215,25 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// Down to 2^-149.
+__device__ __forceinline__ float exp2_far(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // max that keeps a NaN, so a row with a NaN score ends as NaN.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
+}
+
+// Of the lanes that share a row of the products.
+__device__ __forceinline__ float rows_max(float v) {
+  v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, 4));
+  v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, 8));
+  return max_nan(v, __shfl_xor_sync(0xffffffffu, v, 16));
 }
 
 // Weight of a part with maximum m against the joined maximum M: an empty part
@@ -227,8 +244,7 @@ __device__ __forceinline__ float part_weight(float m, float M) { return m == -IN
 // 8-bit cache, whose values may lie anywhere in fp32's range): down to 2^-149, for
 // a small weight may stand before a large value.
 __device__ __forceinline__ float part_share(float m, float M, float sum) {
-  float f;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(f) : "f"(m - M));
+  const float f = exp2_far(m - M);  // (before the choice, which then is no branch)
   return m == -INFINITY ? 0.f : f * sum;
 }
 // A power of two that brings up to 2^kParts shares of at most `most` each (a sum,
@@ -342,6 +358,7 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
   float* join = reinterpret_cast<float*>(base + S::kOffJoin);
   float* stat = reinterpret_cast<float*>(base + S::kOffStat);  // [warp][kStat / 16][16]
   float* scales = reinterpret_cast<float*>(base + S::kOffScale) + warp * S::kStages * 4;
+  float* kappa = stat + warp * kStat + 32;  // of the warp's rows, until its results are joined
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + S::kOffBar) + warp * S::kStages;
   int* last_s = reinterpret_cast<int*>(base + S::kOffBar + kWarps * S::kStages * 8);
 
@@ -480,7 +497,10 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
     const int first_limit = sg.kv_len - sg.new_len + sg.row0 / p.group;  // what the first row sees
     // O^T: dims 16 d + g, + 8 (of codes 16 d + 2 g, + 1), rows 8 t + c2, + 1
     float o[D / 16][NT][4];
-    float ref = 1.17549435e-38f, ref_inverse = 8.507059173e37f;  // r = 2^-126, of codes
+    float ref = kLeastRef, ref_inverse = kLeastInverse;  // r, of codes
+    float lowest = INFINITY;  // value scale so far
+    bool wide = false;        // scales so far apart that l has a reference of its own
+    float fall = 0.f;         // log2(r of the tile before / r)
 #pragma unroll
     for (int d = 0; d < D / 16; ++d)
 #pragma unroll
@@ -493,7 +513,13 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
 #pragma unroll
       for (int i = 0; i < 2; ++i) m[t][i] = -INFINITY, l[t][i] = 0.f;
 
-    for (int tile = sg.tile0 + warp; tile < sg.tile1 && ok; tile += kWarps) {
+    // Of codes two loops: the second from the first tile on with which scales lie far
+    // apart (in one loop that rare path cost 2 per cent of the time).
+    int tile = sg.tile0 + warp;
+#pragma unroll
+    for (int apart = 0; apart < (kCoded ? 2 : 1); ++apart)
+    if (apart == 0 || __builtin_expect(wide, 0))
+    for (; tile < sg.tile1 && ok; tile += kWarps) {
       const int slot = used % S::kStages;
       ok = __all_sync(0xffffffffu, wait_copy(&bars[slot], (uint32_t)((used / S::kStages) & 1), limit_cycles));
       if (!ok) {
@@ -511,26 +537,54 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 4; ++j) s[h][t][j] = 0.f;
       float k_scale[2] = {1.f, 1.f};
-      float offset[2], back[2], fall = 0.f;  // log2(s_v / r), r / s_v; log2 of r before / r
+      float offset[2], back[2];  // log2(s_v / r), r / s_v
       bool odd = false;  // a value scale is not finite
       if constexpr (kCoded) {
         const float4 four = *reinterpret_cast<const float4*>(scales + slot * 4);
         k_scale[0] = four.x;
         k_scale[1] = four.y;
-        const float most = fmaxf(four.z, four.w);
-        odd = !(max_nan(four.z, four.w) < INFINITY);
-        if (most > ref && most < INFINITY) {
-          const uint32_t up = min((__float_as_uint(most) + 0x7fffffu) & 0x7f800000u, 0x7f000000u);
-          fall = (float)((int)(__float_as_uint(ref) >> 23) - (int)(up >> 23));
-          ref = __uint_as_float(up);
-          ref_inverse = 1.f / ref;
+        float v[2] = {four.z, four.w}, some[2];
+        const auto grow = [&](float most) {
+          if (!(most > ref)) return;
+          const float next = power_above(most);
+          fall += exponent_of(ref) - exponent_of(next);
+          ref = next;
+          ref_inverse = inverse_of(next);
+        };
+        // (Of a block past the request's length the scale is zero.)
+        const float larger = fmaxf(v[0], v[1]);
+        if (larger < INFINITY) grow(larger);
+        some[0] = v[0] * ref_inverse;
+        some[1] = v[1] * ref_inverse;
+        if (__builtin_expect(!(fminf(some[0], some[1]) >= kLeastRatio && max_nan(some[0], some[1]) <= 1.f), 0)) {
+          bool real[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            real[h] = key0 + kScaleTokens * h < sg.kv_len && v[h] < INFINITY;
+            odd |= key0 + kScaleTokens * h < sg.kv_len && !real[h];
+            if (real[h]) grow(v[h]);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (!real[h]) v[h] = ref;  // any will do
+            some[h] = v[h] * ref_inverse;
+          }
+          if (apart == 0 && far_apart(fminf(lowest, fminf(v[0], v[1])), ref)) {
+            if (g == 0)
+#pragma unroll
+              for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) kappa[8 * t + c2 + i] = 0.f;
+            __syncwarp();
+            wide = true;
+            break;
+          }
         }
+        lowest = fminf(lowest, fminf(v[0], v[1]));
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          // Below 2^-60 nothing is left of what it scales.
-          const float some = fmaxf((h ? four.w : four.z) * ref_inverse, 8.6736174e-19f);
-          offset[h] = __log2f(some);
-          back[h] = __fdividef(1.f, some);
+          offset[h] = apart ? log2f(v[h]) - exponent_of(ref) : __log2f(some[h]);
+          back[h] = __fdividef(1.f, some[h]);
         }
         // Bytes 4 c .. 4 c + 3 of a lane's row are taken as columns 2 c, 2 c + 1, 2 c + 8
         // and 2 c + 9 of the product, as the queries are.
@@ -570,6 +624,56 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         float sub[2];
+        if (apart) {
+          // P' = 2^((s - mu) + log2(s_v / r) - kappa), mu the scores' maximum (in m), kappa
+          // that of the shares beside it; l has mu for its reference.
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = 8 * t + c2 + i;
+            float own = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int j = i; j < 4; j += 2) {
+                float v = s[h][t][j] * (scale[t][i] * k_scale[h]);
+                if (ragged && key0 + 16 * h + g + 4 * (j - i) > limit[t][i]) v = -INFINITY;
+                s[h][t][j] = v;
+                own = max_nan(own, v);
+              }
+            own = rows_max(own);
+            const float mu = max_nan(m[t][i], own), from = mu == -INFINITY ? 0.f : mu;
+            l[t][i] *= part_weight(m[t][i], from);
+            float most = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int j = i; j < 4; j += 2) {
+                const float v = s[h][t][j];
+                // The NaN of a key or of inf - inf stays; a hidden key is none.
+                const float d = v - from;
+                l[t][i] += exp2_fast(d);
+                s[h][t][j] = d + offset[h];
+                most = max_nan(most, s[h][t][j]);
+                if (odd && v != -INFINITY && !(fabsf(scales[slot * 4 + 2 + h]) < INFINITY))
+                  l[t][i] = __uint_as_float(0x7fc00000u);
+              }
+            most = rows_max(most) - kLift;
+            const float stands = kappa[r] + fall + (m[t][i] - from), next = max_nan(stands, most);
+            __syncwarp();
+            if (g == 0) kappa[r] = next;
+            __syncwarp();
+            sub[i] = next == -INFINITY ? 0.f : next;
+            keep[t][i] = stands == -INFINITY ? 1.f : exp2_fast(stands - sub[i]);  // nothing stands in O yet
+            moved |= keep[t][i] != 1.f;
+            m[t][i] = mu;
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            pb[h][t][0] = transpose8(pack2<C>(exp2_fast(s[h][t][0] - sub[0]), exp2_fast(s[h][t][1] - sub[1])));
+            pb[h][t][1] = transpose8(pack2<C>(exp2_fast(s[h][t][2] - sub[0]), exp2_fast(s[h][t][3] - sub[1])));
+          }
+          continue;
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float mx = -INFINITY;
@@ -587,21 +691,17 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
             if constexpr (kCoded) most += fabsf(most) < kFar ? offset[h] : 0.f;
             mx = max_nan(mx, most);
           }
-          mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          mx = rows_max(mx);
           // What m stands for falls with r, of codes.
           const float mn = max_nan(kCoded ? m[t][i] + fall : m[t][i], lifted<C>(mx));
           // Rows that have seen no key yet keep m = -inf and add nothing.
           sub[i] = mn == -INFINITY ? 0.f : mn;
           keep[t][i] = exp2_fast(kCoded ? (m[t][i] - sub[i]) + fall : m[t][i] - sub[i]);
           moved |= keep[t][i] != 1.f;
-          if (kCoded && fall != 0.f) {
-            l[t][i] *= exp2_fast(m[t][i] - sub[i]);
-            if (l[t][i] > 1.0e32f) l[t][i] = 1.0e32f;  // the rest is nothing beside it
-          } else {
+          if (kCoded && __builtin_expect(fall != 0.f, 0))
+            l[t][i] *= exp2_fast(m[t][i] - sub[i]);  // 2^61 at most: else the scales are far apart
+          else
             l[t][i] *= keep[t][i];
-          }
           m[t][i] = mn;
         }
 #pragma unroll
@@ -732,6 +832,7 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
       __syncwarp();
       ++used;
       if (more) fetch();
+      fall = 0.f;
     }
 
     // Join the warps' results.
@@ -743,10 +844,15 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
         l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], 8);
         l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], 16);
         const int r = 8 * t + c2 + i;
+        float gain = ref;  // of codes: what O is to be multiplied with
+        if (kCoded && wide) {
+          gain = exp2_far(kappa[r] + exponent_of(ref));
+          __syncwarp();  // it takes kappa's place
+        }
         if (g == 0) {
           stat[warp * kStat + r] = m[t][i];
           stat[warp * kStat + 16 + r] = l[t][i];
-          if (kCoded) stat[warp * kStat + 32 + r] = ref;
+          if (kCoded) stat[warp * kStat + 32 + r] = gain;
         }
       }
 #pragma unroll
@@ -775,9 +881,11 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
           const float unit = share_unit<4>(most);
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) {
-            const float f = part_share(stat[w * kStat + r], M, unit);
-            acc = fmaf(f * stat[w * kStat + 32 + r], join[(w * S::kJoinRows + r) * S::kPitch + at], acc);
-            sum = fmaf(f, stat[w * kStat + 16 + r], sum);
+            // O has the sum's size, so a large gain goes with the unit, a small one apart from
+            // it: nothing on the way lies outside fp32's range that does not in the end.
+            const float f = part_share(stat[w * kStat + r], M, 1.f), gain = stat[w * kStat + 32 + r];
+            acc = fmaf(join[(w * S::kJoinRows + r) * S::kPitch + at] * (unit * fmaxf(gain, 1.f)), f * fminf(gain, 1.f), acc);
+            sum = fmaf(f, stat[w * kStat + 16 + r] * unit, sum);
           }
           acc = sum == 0.f ? 0.f : acc / sum;
         } else {

@@ -64,7 +64,12 @@
 // 16384 took 3% less), and rows that see small values alone lose nothing.
 // That costs a few instructions a block, none a score, and rounds nothing but P'.
 // r is a power of two at or above the segment's value scales (one half: those so
-// far; where it grows, m falls by as much).
+// far; where it grows, m falls by as much).  Where they lie more than 2^60 apart
+// (or are zero), r / s_v no longer serves: keys with a tiny scale may hold all of a
+// row's weight, or none of it beside a large one that counts, or one that the row
+// does not see.  Then l sums 2^(s s_k - m) itself, m is the scores' own maximum, and
+// O stands at 2^(m + kappa), kappa the largest (s s_k - m) + log2(s_v / r): twice the
+// exponentials, on such segments (one half: from such a tile on).
 //   Two halves (storage Widened): the requests' codes are widened by a kernel of
 // their own first (paged_widen.cu), for the tensor cores are the limit and a
 // tile is read by many row blocks.  (Widened in this kernel by a warpgroup more,
@@ -239,55 +244,65 @@ __device__ __forceinline__ void arrive_with_copies(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
-// The power of two at or above a positive finite value (at most 2^127).
-__device__ __forceinline__ float power_above(float v) {
-  return __uint_as_float(min((__float_as_uint(v) + 0x7fffffu) & 0x7f800000u, 0x7f000000u));
-}
-constexpr float kLeastRef = 1.17549435e-38f;  // 2^-126
-// The reference of scales: a power of two at or above those that are finite.
-__device__ __forceinline__ float raise_ref(float ref, float scale) {
-  return scale > ref && scale < INFINITY ? power_above(scale) : ref;
-}
 // What is told of a tile of codes, twice where packed pairs are worked on.  Zero
 // units become the smallest number, 2^-149 (a hidden score of -inf must not meet a
-// zero), zero ratios 2^-60, where nothing is left of what they scale; scales that
-// are not finite count as zero, and the rows that see a token of their blocks as
-// NaN.
+// zero); of blocks past the request's length, or with scales that are not finite
+// (the rows that see a token of theirs become NaN), the rest is 1.
 struct TileScales {
   float4 block[8];  // unit, unit, offset, offset: s_k * scale * log2 e, log2(s_v / r)
   float2 back[8];   // r / s_v
   float v_ref;      // r
   float fall;       // log2(r of the tile before / r)
-  uint32_t events;  // bit b: a scale of block b is not finite; bit 8: r grew
+  uint32_t events;  // bit b: a scale of block b is not finite; bit 8: r grew; bit 9: scales are far apart
   uint32_t pad;
 };
-constexpr uint32_t kGrew = 256;
+constexpr uint32_t kGrew = 256, kWide = 512;
 // Up to 2^9 a maximum and a logarithm add up to within 2^-15, 2e-5 of a weight.
 constexpr float kApart = 512.f;
+// The value scales of a segment (one half: those so far).
+struct ScalesSeen {
+  float ref = kLeastRef;    // r
+  float lowest = INFINITY;
+  bool wide = false;        // from here on l has a reference of its own
+  __device__ __forceinline__ void add(float most, float least) {
+    if (most > ref) ref = power_above(most);
+    lowest = fminf(lowest, least);
+    wide = wide || far_apart(lowest, ref);
+  }
+};
 // Lane i of a warp, i < 8, has the scales of block i (the other lanes those of
-// i % 8); returns the new r.
-__device__ __forceinline__ float tell(TileScales& to, float k, float v, float scale, float ref, int lane) {
-  const bool odd = !(fabsf(k) < INFINITY && fabsf(v) < INFINITY);
-  if (odd) k = v = 0.f;
-  float most = v;
+// i % 8); the request's length ends in or after block `blocks` - 1.
+__device__ __forceinline__ void tell(TileScales& to, float k, float v, float scale, ScalesSeen& seen, int blocks, int lane) {
+  const bool there = (lane & 7) < blocks;
+  const bool odd = there && !(fabsf(k) < INFINITY && fabsf(v) < INFINITY);
+  const bool real = there && !odd;
+  if (odd) k = 0.f;
+  float most = real ? v : 0.f, least = real ? v : INFINITY;
 #pragma unroll
-  for (int off = 1; off < 8; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-  const float before = ref;
-  ref = raise_ref(ref, most);
+  for (int off = 1; off < 8; off <<= 1) {
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+    least = fminf(least, __shfl_xor_sync(0xffffffffu, least, off));
+  }
+  const float before = seen.ref;
+  seen.add(most, least);
   const uint32_t odds = __ballot_sync(0xffffffffu, odd) & 0xffu;
   if (lane < 8) {
-    const float inverse = 1.f / ref;
-    const float unit = fmaxf(k * scale, 1.401298464e-45f), some = fmaxf(v * inverse, 8.6736174e-19f);
-    const float offset = log2f(some), back = 1.f / some;
+    const float unit = fmaxf(k * scale, 1.401298464e-45f), some = real ? v * inverse_of(seen.ref) : 1.f;
+    const float offset = real && seen.wide ? log2f(v) - exponent_of(seen.ref) : log2f(some), back = 1.f / some;
     to.block[lane] = make_float4(unit, unit, offset, offset);
     to.back[lane] = make_float2(back, back);
     if (lane == 0) {
-      to.v_ref = ref;
-      to.fall = (float)((int)(__float_as_uint(before) >> 23) - (int)(__float_as_uint(ref) >> 23));
-      to.events = odds | (ref != before ? kGrew : 0u);
+      to.v_ref = seen.ref;
+      to.fall = exponent_of(before) - exponent_of(seen.ref);
+      to.events = odds | (seen.ref != before ? kGrew : 0u) | (seen.wide ? kWide : 0u);
     }
   }
-  return ref;
+}
+
+// Whether a row that sees the tile's first `last` + 1 keys sees one of a block whose
+// scale is not finite.
+__device__ __forceinline__ bool sees_odd(uint32_t events, int last) {
+  return last >= 0 && (events & ((2u << min(last / kScaleTokens, 7)) - 1u) & 0xffu);
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
@@ -328,9 +343,30 @@ __device__ __forceinline__ void tmem_wait32(float* v) {
                  "+f"(v[29]), "+f"(v[30]), "+f"(v[31])::"memory");
 }
 
+// A warp's rows of O times a factor each.
+template <int D>
+__device__ __forceinline__ void rescale(uint32_t t_o, float factor) {
+#pragma unroll 1
+  for (int c = 0; c < D; c += 32) {
+    float o[32];
+    tmem_ld32(t_o + c, o);
+    uint32_t w[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * factor);
+    tmem_st16(t_o + c, w);
+    tmem_st16(t_o + c + 16, w + 16);
+  }
+}
+
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Down to 2^-149.
+__device__ __forceinline__ float far_exp2(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -504,10 +540,13 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
   const int seg0 = p.starts[blockIdx.x], seg1 = p.starts[blockIdx.x + 1];
 
   if (warp >= S::kMmaWarp) {
-    // 384 threads x 168 registers = 2 x 128 x 208 + 128 x 88; with wideners 256 x 128 =
-    // 128 x 200 + 128 x 56.
+    // 384 threads x 168 registers = 2 x 128 x 208 + 128 x 88, of codes 2 x 128 x 200 +
+    // 128 x 104 (with 208 the softmax of f16 queries spilled); with wideners 256 x 128 =
+    // 128 x 192 + 128 x 64.
     if constexpr (kWiden)
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    else if constexpr (H == 2 && kScaled)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     else if constexpr (H == 2)
       asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (kWiden && warp == S::kLoadWarp) {
@@ -582,7 +621,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         for (int seg = seg0; seg < seg1 && ok; ++seg) {
           const PagedSegment g = p.segments[seg];
           const View<H> view(g, p.group);
-          float ref = kLeastRef;  // r: of the segment's values so far
+          ScalesSeen seen;
           for (int j = 0; j < view.tiles && ok; ++j, ++t) {
             const int have = g.kv_len - (g.tile0 + j) * kTileKeys;
 #pragma unroll 1
@@ -596,7 +635,8 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
                 if (!(ok = wait_warp(&raw_full[raw], (uint32_t)((m / S::kRawSlots) & 1), ctl, err, 95))) break;
                 if (c == 0 && v == 0 && warp == S::kWidenWarp) {
                   const float* from = scales + (t & 3) * 16;
-                  ref = tell(told[t % S::kTold], from[lane & 7], from[8 + (lane & 7)], p.scale_log2, ref, lane);
+                  tell(told[t % S::kTold], from[lane & 7], from[8 + (lane & 7)], p.scale_log2, seen,
+                       (have + kScaleTokens - 1) / kScaleTokens, lane);
                 }
                 const uint8_t* src = base + S::kOffRaw + raw * S::kRaw + from_at;
                 uint8_t* to = dst + c * S::kRawKeys * 128 + to_at;
@@ -648,7 +688,8 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         // i % 8, a tile ahead.
         int first_page = 0;
         const float *k_from = nullptr, *v_from = nullptr;
-        float k_scale = 0.f, v_scale = 0.f, ref = kLeastRef;
+        float k_scale = 0.f, v_scale = 0.f;
+        ScalesSeen seen;
         if constexpr (kScaled) {
           first_page = __ldg(p.first_page + g.request);
           const int64_t at = g.kv_head * p.scale_stride + (int64_t)first_page * (p.page_size / kScaleTokens) +
@@ -663,17 +704,18 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         };
         if (kScaled && view.tiles > 0) {
           look_at(0);
-          // r of the whole segment: the loader is ahead, so the softmax need not look for it
-          // to grow.
-          float most = 0.f;
+          // Those of the whole segment: the loader is ahead, so the softmax need not look for
+          // r to grow.
+          float most = 0.f, least = INFINITY;
           const int blocks = min((g.kv_len + kScaleTokens - 1) / kScaleTokens - g.tile0 * 8, view.tiles * 8);
           const float* from = v_from - (lane & 7);
 #pragma unroll 8
           for (int i = lane; i < blocks; i += 32) {
             const float v = __ldg(from + i);
             most = fmaxf(most, fabsf(v) < INFINITY ? v : 0.f);
+            least = fminf(least, fabsf(v) < INFINITY ? v : INFINITY);
           }
-          ref = raise_ref(ref, warp_max(most));
+          seen.add(warp_max(most), -warp_max(-least));
         }
         for (int j = 0; j < view.tiles && ok; ++j) {
           const int key0 = (g.tile0 + j) * kTileKeys;
@@ -695,7 +737,8 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
             if (turn > 0 && !(ok = wait_warp(&kv_empty[slot], (uint32_t)((turn - 1) & 1), ctl, err, 81))) break;
             if constexpr (kScaled) {
               if (v == 0) {  // seen with the keys
-                ref = tell(told[n / 2 % S::kTold], k_scale, v_scale, p.scale_log2, ref, lane);
+                tell(told[n / 2 % S::kTold], k_scale, v_scale, p.scale_log2, seen,
+                     (left + kScaleTokens - 1) / kScaleTokens, lane);
                 __syncwarp();
               } else if (j + 1 < view.tiles) {
                 look_at(j + 1);
@@ -838,6 +881,8 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
     }
   } else {
     if constexpr (kWiden)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    else if constexpr (H == 2 && kScaled)
       asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     else if constexpr (H == 2)
       asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -938,24 +983,100 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
       const float scale = Act<T>::kDtype == Act<C>::kDtype ? p.scale_log2 : p.scale_log2 * boost;
       float m = -INFINITY, l = 0.f;
       float v_ref = 1.f;  // r of O
+      float kappa = 0.f;  // O stands at 2^(m + kappa)
       const bool own_boost = kScaled && Act<T>::kDtype != Act<C>::kDtype && boost != 1.f;
       const bool boosted = kScaled && Act<T>::kDtype != Act<C>::kDtype && __any_sync(0xffffffffu, own_boost);
-      for (int j = 0; j < count; ++j) {
-        if (!(ok = wait_warp(&s_full[x], s_turn & 1, ctl, err, 90))) break;
-        ++s_turn;
+      // Of codes two loops: the second from the first tile on with which scales lie far
+      // apart (in one loop that rare path cost 2 to 9 per cent of the time; with two halves
+      // it is known of the segment's first tile).  The next tile's scores are awaited at a
+      // tile's end, for a second wait before the loops made it spill.
+      int j = 0;
+      bool wide = false;
+      if (kScaled && count > 0 && (ok = wait_warp(&s_full[x], s_turn & 1, ctl, err, 90)) && H == 2)
+        wide = told[tile_at % S::kTold].events & kWide;
+#pragma unroll
+      for (int apart = 0; apart < (kScaled ? 2 : 1); ++apart)
+      if (apart == 0 ? H == 1 || !wide : __builtin_expect(wide, 0))
+      for (; j < count && ok; ++j) {
+        if (!kScaled && !(ok = wait_warp(&s_full[x], s_turn & 1, ctl, err, 90))) break;
         tc_fence_after();
         const TileScales& of = told[(tile_at + j) % S::kTold];
         uint32_t events = 0;
         if constexpr (kScaled) {
           events = of.events;
+          if (H == 1 && apart == 0 && __builtin_expect(events & kWide, 0)) {
+            wide = true;
+            break;
+          }
           v_ref = of.v_ref;
+        }
+        ++s_turn;
+        const int key0 = (g.tile0 + j) * kTileKeys;
+        float factor = 1.f;
+        if (apart) {
+          // The scores are read three times, 32 at a time (what is rare takes little code): for
+          // their maximum, for the sum and the largest share, for P.
+          const float down = fminf(boost, 1.f), up = fmaxf(boost, 1.f), before = m;
+          float own = -INFINITY, most = -INFINITY, from = 0.f, sub = 0.f;
+#pragma unroll 1
+          for (int pass = 0; pass < 3; ++pass) {
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 32) {
+              float s[32];
+              __syncwarp();
+              tmem_ld32(t_s + c, s);
+              const float4 first = of.block[c / 16], second = of.block[c / 16 + 1];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                s[i] = s[i] * down * (i < 16 ? first.x : second.x) * up;
+                s[i] = key0 + c + i > limit ? -INFINITY : s[i] - from;
+              }
+              if (pass == 0) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) own = max_nan(own, s[i]);
+              } else if (pass == 1) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                  l += fast_exp2(s[i]);
+                  most = max_nan(most, s[i] + (i < 16 ? first.z : second.z));
+                }
+              } else {
+                uint32_t pk[16];
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                  const float offset = i < 16 ? first.z : second.z;
+                  pk[i / 2] = pack2<C>(fast_exp2(s[i] + offset - sub), fast_exp2(s[i + 1] + offset - sub));
+                }
+                __syncwarp();
+                tmem_st16(t_s + c / 2, pk);  // over scores that have been read
+                if (c & 32) {
+                  tmem_st_wait();
+                  tc_fence_before();
+                  mbar_arrive(&p_full[2 * x + c / 64]);
+                }
+              }
+            }
+            if (pass == 0) {
+              m = max_nan(m, own);
+              from = m == -INFINITY ? 0.f : m;
+              l *= before == -INFINITY ? 0.f : fast_exp2(before - from);
+            } else if (pass == 1) {
+              const float stands = kappa + of.fall + (before - from);
+              kappa = max_nan(stands, most - kLift);
+              sub = kappa == -INFINITY ? 0.f : kappa;
+              if (stands != -INFINITY) factor = fast_exp2(stands - sub);  // else nothing stands in O yet
+              if (__any_sync(0xffffffffu, factor != 1.f) && j > 0) rescale<D>(t_o, factor);
+            }
+          }
+          if (kScaled && (events & 0xffu) && sees_odd(events, limit - key0)) l = __uint_as_float(0x7fc00000u);
+          if (j + 1 < count) ok = wait_warp(&s_full[x], s_turn & 1, ctl, err, 90);
+          continue;
         }
         float sc[128];
 #pragma unroll
         for (int c = 0; c < 128; c += 32) tmem_ld32_begin(t_s + c, sc + c);
 #pragma unroll
         for (int c = 0; c < 128; c += 32) tmem_wait32(sc + c);
-        const int key0 = (g.tile0 + j) * kTileKeys;
         if constexpr (kScaled && Act<T>::kDtype != Act<C>::kDtype) {
           if (boosted) {
             // Powers below one before the units, those above after them: what lies
@@ -1011,7 +1132,6 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
           for (int c = 0; c < 128; ++c) sc[c] *= scale;
           unit = 1.f;
         }
-        float factor = 1.f;
         mx = lifted<C>(mx);
         if (kWiden && (events & kGrew) && m != -INFINITY) {
           // What m stands for fell with r; O stays, l is in the old units.
@@ -1019,8 +1139,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
           m += of.fall;
           if (!(mx <= m + kRescale)) m = max_nan(m, mx);
           factor = fast_exp2((before - m) + of.fall);
-          l *= fast_exp2(before - m);
-          if (l > 1.0e32f) l = 1.0e32f;  // the rest is nothing beside it
+          l *= fast_exp2(before - m);  // 2^61 at most: else the scales are far apart
         } else if (!(mx <= m + kRescale)) {  // also for NaN, and for the first key seen
           mx = max_nan(m, mx);  // a NaN stays
           factor = fast_exp2(m - mx);
@@ -1030,18 +1149,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         // This tile's scores were issued after the last tile's product: O is
         // stable, and P may overlay S.  (The vote is taken on the first tile too:
         // it brings the warp together for the stores of P.)
-        if (__any_sync(0xffffffffu, factor != 1.f) && j > 0) {
-#pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            float o[32];
-            tmem_ld32(t_o + c, o);
-            uint32_t w[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * factor);
-            tmem_st16(t_o + c, w);
-            tmem_st16(t_o + c + 16, w + 16);
-          }
-        }
+        if (__any_sync(0xffffffffu, factor != 1.f) && j > 0) rescale<D>(t_o, factor);
         // Exponent arguments and sums on packed pairs.  P goes out in two
         // parts of 64 keys, so the product of the first runs while the
         // second's exponentials do.
@@ -1101,12 +1209,8 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         float s0, s1;
         f2_unpack(kScaled ? f2_add(sp[2], sp[3]) : f2_add(f2_add(sp[0], sp[1]), f2_add(sp[2], sp[3])), s0, s1);
         l += s0 + s1;
-        if constexpr (kScaled) {
-          if (events & 0xffu) {
-            for (int b = 0; b < 8; ++b)
-              if ((events >> b & 1) && key0 + 16 * b <= limit) l = __uint_as_float(0x7fc00000u);
-          }
-        }
+        if (kScaled && (events & 0xffu) && sees_odd(events, limit - key0)) l = __uint_as_float(0x7fc00000u);
+        if (kScaled && j + 1 < count) ok = wait_warp(&s_full[x], s_turn & 1, ctl, err, 90);
       }
       if (!ok) break;
       const int row = kHalf * x + r;
@@ -1120,6 +1224,8 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
       const bool cleared = !kScaled && ctl->cleared != 0;
       // A row that has seen no key above -inf gives zeros.
       const float inv = m == -INFINITY ? 0.f : 1.f / l;
+      // 2^kappa r may lie anywhere, but not what it makes of O / l.
+      const float half = kScaled ? far_exp2(0.5f * kappa) : 1.f;
       T* orow = static_cast<T*>(p.out) +
                 ((int64_t)(g.q_row + token) * p.heads + g.kv_head * p.group + pr % p.group) * D;
       float* prow = p.part + (int64_t)g.part * S::kRows * D + row * 4;
@@ -1134,7 +1240,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
         }
         if constexpr (kScaled) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = m == -INFINITY ? 0.f : o[i] * inv * v_ref;
+          for (int i = 0; i < 32; ++i) o[i] = m == -INFINITY ? 0.f : o[i] * inv * half * (v_ref * half);
         }
         if (mine && g.part < 0) {
 #pragma unroll
@@ -1211,7 +1317,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps)
     const float m = st[(int64_t)i * 2 * R], own = st[(int64_t)i * 2 * R + R];
     float f;
     if (kDivided) {
-      asm("ex2.approx.f32 %0, %1;" : "=f"(f) : "f"(m - M));
+      f = far_exp2(m - M);
       f = m == -INFINITY ? 0.f : f * (own * unit);  // an empty piece holds zeros
       sum += f;
     } else {
