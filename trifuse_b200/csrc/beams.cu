@@ -38,6 +38,9 @@ constexpr int kMaxCount = TF_MAX_TOP;
 // values or more, so for vocabularies of millions the sums' own rounding counts).
 __device__ __forceinline__ double near_by(int V) { return fmax(1e-5, 1e-11 * V); }
 
+// From here down totals are -inf in fp32: -(2^128 - 2^103).
+constexpr double kNone = -3.4028235677973366e38;
+
 struct SelectParams {
   BeamArgs a;
   int each;
@@ -131,10 +134,12 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_cons
     if (j < n_of[b]) fill(b, j);
   }
   __syncthreads();
-  // Tokens at -inf cannot follow; they end their lists.
+  // Tokens at -inf cannot follow, nor those whose score fp32 does not hold; they end
+  // their lists.  (Rows that are summed again below move by less than fp64's steps
+  // there.)
   if (tid < beams) {
     const double* list = totals + tid * each;
-    n_of[tid] = ahead<false>(list, n_of[tid], -INFINITY);
+    n_of[tid] = ahead<false>(list, n_of[tid], kNone);
   }
   __syncthreads();
   const auto order = [&]() {
