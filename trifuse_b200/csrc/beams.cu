@@ -10,13 +10,14 @@
 // the number of entries ahead of it (a binary search).
 //
 // Totals are formed in fp64, but the pass sums fp32 exponentials: a log sum was
-// off by up to 4.4e-7 (flat to peaked rows of 1000 to 600000 logits).  Where two
-// candidates of different beams that matter lie closer than ten times the sum of
-// two such errors, their rows are summed again in fp64, so which beam goes on
-// does not hang on a rounding; an exact total may lie close to another rough one,
-// so this goes on until none does (each row is summed again once at most).  At
-// eight beams a batch of 64 requests meets that about once in sixty steps, and then
-// takes 30 us more.
+// off by up to 4.6e-7 (flat, rising, scattered and peaked rows of 1000 to 600000
+// logits; 1.0e-6 at two million, rising in steps).  Where two candidates of
+// different beams that matter lie closer than ten times the sum of two such errors,
+// their rows are summed again in fp64, so which beam goes on does not hang on a
+// rounding; an exact total may lie close to another rough one, so this goes on
+// until none does (each row is summed again once at most, one after the other).  At
+// eight beams a batch of 64 requests meets that about once in sixty steps, and a
+// pair of rows then takes 30 us more; 64 beams with equal totals sum 64 rows.
 //
 // What bounds it: the logits, read once; this kernel's block is latency (some
 // 64 candidates, a few round trips).  Measured: 64 x 8 beams over 50304 fp32 logits
@@ -34,9 +35,10 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxBeams = TF_MAX_BEAMS;
 constexpr int kMaxCount = TF_MAX_TOP;
-// Closer than this, totals are told apart in fp64 (a thread adds up V / 1024
-// values or more, so for vocabularies of millions the sums' own rounding counts).
-__device__ __forceinline__ double near_by(int V) { return fmax(1e-5, 1e-11 * V); }
+// Closer than this, totals are told apart in fp64.  Of the roundings only a thread's
+// additions to its sum grow with the row: V / 4096 of them (a tile each), of 2^-24
+// at most and possibly all one way, in two rows 2.9e-11 V.
+__device__ __forceinline__ double near_by(int V) { return fmax(1e-5, 3e-11 * V); }
 
 // From here down totals are -inf in fp32: -(2^128 - 2^103).
 constexpr double kNone = -3.4028235677973366e38;
