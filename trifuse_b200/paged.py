@@ -181,18 +181,25 @@ class PagedCache:
         return len(used)
 
     def resize(self, pages: int):
-        """Another number of pages, no fewer than are in use."""
+        """Another number of pages, no fewer than are in use.  Where memory does
+        not suffice for all arrays, each keeps the smaller number."""
         used = len({p for lists in self.pages.values() for p in lists})
         if pages < used:
             raise ValueError(f"paged cache: {used} pages are in use")
         used = self.compact()
-        for name in ("k", "v", "k_scales", "v_scales"):
-            old = getattr(self, name)
-            if old is not None:
+        names = [n for n in ("k", "v", "k_scales", "v_scales") if getattr(self, n) is not None]
+        try:
+            for name in names:  # one after the other: each takes the old one's place
+                old = getattr(self, name)
                 new = old.new_empty((old.shape[0], pages, *old.shape[2:]))
                 new[:, :used] = old[:, :used]
                 setattr(self, name, new)
-        self.free = list(range(pages - 1, used - 1, -1))
+        finally:
+            pages = min(getattr(self, n).shape[1] for n in names)
+            for name in names:
+                if getattr(self, name).shape[1] > pages:
+                    setattr(self, name, getattr(self, name)[:, :pages])
+            self.free = list(range(pages - 1, used - 1, -1))
 
     def table(self, requests) -> Tensor:
         """Page table of the requests, on the cache's device."""
