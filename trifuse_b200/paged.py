@@ -104,8 +104,11 @@ class PagedCache:
 
     def take_back(self, requests, counts):
         """Undoes the last grow of the same requests and counts (pages that it
-        copied stay their requests' own; of an 8-bit cache, earlier tokens of
-        a block that was written to stay as it left them)."""
+        copied stay their requests' own).  What was written to an 8-bit cache
+        meanwhile is not undone in blocks that hold earlier tokens: a scale that
+        rose stays, with the earlier codes rounded to it, and one that a NaN or
+        an infinity made NaN does too, so these up to 15 tokens are lost until
+        they are appended again, from the block's first on."""
         for r, count in reversed(list(zip(requests, counts))):
             left = self.lengths[r] - count
             keep = -(-left // self.page_size)
