@@ -19,7 +19,9 @@
 // registers (with more than 16 heads to 8 warps it reads them again, from L1);
 // what it makes of them is made twice, for the block's maximum and for the
 // codes, which is less than to keep it.  A norm's factor is the same for a
-// token's values, so the maximum is taken before it.  A window's rows are under
+// token's values, so the maximum is taken before it; here it comes after the weight
+// and the rotation, on the path of single tokens before them, as in the 16-bit
+// append: the last bit of a value may depend on the number of rows of a call.  A window's rows are under
 // way before its units are known, for in a long prompt they are all one unit.
 // One token (a decode step) takes a path without windows: three dependent round
 // trips to memory, a head on 8 threads.
@@ -127,7 +129,7 @@ __device__ __forceinline__ void put_codes(uint8_t* to, const float2 (&f)[2][4], 
 
 // cos and sin of an angle of `turns` turns.  For keys, what the angle loses by its
 // rounding turns them on (half as many codes fall to the other side of a
-// rounding); q is the 16-bit append's.
+// rounding); q's angle is the 16-bit append's.
 __device__ __forceinline__ void turn(double turns, bool key, float& cs, float& sn) {
   const double half = 2. * (turns - rint(turns));  // half turns
   const float rough = (float)half;
