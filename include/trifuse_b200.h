@@ -484,11 +484,13 @@ int tf_paged_append_8bit(const void* qkv, int64_t qkv_stride, int64_t rows, int3
 
 /* tf_paged_attention over an 8-bit cache; the same plans serve both.  The
  * codes enter the products as f16, which holds them exactly; the scales go to
- * the scores and weights.  Scales are not negative; a NaN scale makes the rows
- * NaN that see a token of its block, and only those.  The workspace holds
- * plan->workspace_bytes + plan->widened_bytes: the codes of requests with many
- * rows are widened there first (two bytes a code, of this layer's keys and
- * values). */
+ * the scores and weights, and may lie anywhere in f32's normal range, as bf16
+ * queries may, where the scores do not leave it.  Scales are not negative; a NaN
+ * scale makes the rows NaN that see a token of its block, and
+ * only those.  The workspace holds plan->workspace_bytes + plan->widened_bytes:
+ * the codes of requests with many rows are widened there first (two bytes a
+ * code, of this layer's keys and values; pages that requests share once for each
+ * of them). */
 int tf_paged_attention_8bit(const void* q, int64_t q_stride, const tf_page_table* table, const tf_paged_kv* kv,
                             const tf_paged_scales* scales, const tf_paged_plan* plan, void* plan_table, float scale,
                             int act, void* out, void* workspace, size_t workspace_bytes, void* stream);
@@ -525,9 +527,9 @@ int tf_paged_copy(const tf_copy_array* arrays, int32_t count, int32_t layers, in
  * [requests][beams], may be NULL): such a beam has ended and competes with its
  * score as it is, as one continuation by the token `end`; its logits are not
  * read.  A beam whose score is not finite, or whose logits hold a NaN or +inf
- * or nothing but -inf, has no continuations.  Scores closer than the sums'
- * rounding are told apart in 64 bits.  beams <= TF_MAX_BEAMS, count <=
- * TF_MAX_TOP.  The workspace is device scratch (16-byte aligned, no initial
+ * or nothing but -inf, has no continuations; a score below f32's range is none.
+ * Scores closer than the sums' rounding are told apart in 64 bits.
+ * beams <= TF_MAX_BEAMS, count <= TF_MAX_TOP.  The workspace is device scratch (16-byte aligned, no initial
  * contents).  The reference generates greedily (patches/executorch.patch:
  * 1350-1353). */
 #define TF_MAX_BEAMS 64

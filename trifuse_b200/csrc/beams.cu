@@ -16,13 +16,14 @@
 // their rows are summed again in fp64, so which beam goes on does not hang on a
 // rounding; an exact total may lie close to another rough one, so this goes on
 // until none does (each row is summed again once at most, one after the other).  At
-// eight beams a batch of 64 requests meets that about once in sixty steps, and a
-// pair of rows then takes 30 us more; 64 beams with equal totals sum 64 rows.
+// eight beams a batch of 64 requests meets that about once in fifty steps, and a
+// pair of rows of 50304 then takes 120 to 135 us more; 64 beams with equal totals
+// sum 64 rows, 3.8 ms.
 //
 // What bounds it: the logits, read once; this kernel's block is latency (some
 // 64 candidates, a few round trips).  Measured: 64 x 8 beams over 50304 fp32 logits
 // 29.5 us, of which the pass 26 (3.9 TB/s: 512 rows are 3 or 4 to an SM, and a row's
-// prunes meet at barriers); one request of 4 beams 11.4.
+// prunes meet at barriers), f16 or bf16 ones 24.5; one request of 4 beams 11.2 to 11.7.
 #include <math.h>
 
 #include "beams.h"

@@ -45,12 +45,13 @@
 // Measured: 64 decodes of 4096 tokens, 16 heads, pages of 64: 311 us, 6.9 TB/s;
 // 37 ragged decodes of up to 32768 tokens, 8 key heads, pages of 16: 279 us, 6.0
 // TB/s (277 with the products taken out: 4 KB pages set that); one decode of 600
-// tokens 7.2 us, of one token 4.0.  Codes: the same 64 decodes 173 us (e4m3; 6.2
-// TB/s), the ragged ones 157 (int8; 124 with the arithmetic taken out), 600 tokens
-// 8.0 or 7.7 (e4m3), one token 5.3; 64 decodes of 1024 tokens 64 and 60 (a segment
+// tokens 7.2 us, of one token 4.0.  Codes: the same 64 decodes 175 us (e4m3; 6.1
+// TB/s), the ragged ones 158 (int8; 124 with the arithmetic taken out), 600 tokens
+// 8.4 or 8.2 (e4m3), one token 6; 64 decodes of 1024 tokens 65 and 62 (a segment
 // is three tiles a warp there, and the warps meet at its end).  With m the scores'
 // maximum the ragged ones took 149, and f16 outputs over few keys were off by up to
-// 1.9 times their own rounding (now 1.2).
+// 1.9 times their own rounding (now 1.2).  Joins and references that hold any scales
+// cost 1 per cent of the long ones, half a microsecond of the short ones.
 #pragma once
 
 #include <cuda.h>

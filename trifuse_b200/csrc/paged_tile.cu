@@ -59,9 +59,9 @@
 // log2(s_v / r) of the argument, which the row's sum takes out again block by
 // block: P' = 2^(s s_k - m + log2(s_v / r)), l += (r / s_v) sum P', O += P' V.
 // m is the maximum of s s_k + log2(s_v / r): the largest share of an output is a
-// P' of 2^7 and not rounded, which counts where few keys do (f16 outputs are off by
-// 1.1 times their own rounding; with m the scores' maximum 1.4 to 1.6, and 2048 of
-// 16384 took 3% less), and rows that see small values alone lose nothing.
+// P' of 2^7 and not rounded in the tile that sets m, which counts where few keys do
+// (f16 outputs are off by 1.1 to 1.3 times their own rounding; with m the scores'
+// maximum 1.4 to 1.6, and 2048 of 16384 took 3% less).
 // That costs a few instructions a block, none a score, and rounds nothing but P'.
 // r is a power of two at or above the segment's value scales (one half: those so
 // far; where it grows, m falls by as much).  Where they lie more than 2^60 apart
@@ -87,8 +87,9 @@
 // (segments of 9 tiles on average, whose ends cost 5600 clocks each; 4 us of it
 // for looking the causal edge's values through, paged_values.cuh), 182 us with
 // bf16 queries over an f16 cache.  Over int8 codes (bf16 queries) the first takes
-// 526 us, widening included, where f16 keys and values take 443; the prompts 240 to
-// 250 against 186.
+// 539 us, widening included, where f16 keys and values take 443; the prompts 252 to
+// 262 against 182, with f16 queries 230 against 166; 35 rows each of 24 requests (8
+// heads of 128, 8011 tokens, one half) 188 to 197 against 142 to 150.
 #include <cuda.h>
 #include <math.h>
 #include <string.h>
