@@ -72,17 +72,20 @@ def test_a_later_token_of_any_size(ops, kind, power, n, G, L):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("power", [30, 100, 118])
 @pytest.mark.parametrize("gap", [0.5, 20.0, 60.0, 88.0, 150.0, 300.0])
+@pytest.mark.parametrize("blocks", [[0], [14, 15, 16, 17]])
 @pytest.mark.parametrize("n,G,L", ROWS)
-def test_large_values_of_little_weight(ops, kind, power, gap, n, G, L):
-    """A block that every row sees has e^-gap of the weight and values 2^power times as large."""
+def test_large_values_of_little_weight(ops, kind, power, gap, blocks, n, G, L):
+    """Blocks of e^-gap of the weight with values 2^power times as large: the first one, which every row sees, and
+    several after others (tiles of nothing but such)."""
     D = 128
     c = Cache([L], 2, D, 16, kind, seed=n, spread=1)
-    at = block_of(c, 0, 7)
     c.k[..., 0] = 0
-    c.k[at[0]] = 0  # pages of 16: one block
-    c.k[at[0], ..., 0] = torch.tensor(-LARGEST[kind], device="cuda").to(kind)
-    c.ks[at] = gap * D ** 0.5 / (4 * LARGEST[kind])
-    c.vs[at] *= 2.0 ** power
+    for block in blocks:
+        at = block_of(c, 0, block * BLOCK)
+        c.k[at[0]] = 0  # pages of 16: one block
+        c.k[at[0], ..., 0] = torch.tensor(-LARGEST[kind], device="cuda").to(kind)
+        c.ks[at] = gap * D ** 0.5 / (4 * LARGEST[kind])
+        c.vs[at] *= 2.0 ** power
     q = queries(n, 2 * G, D, n) * 0.5
     q[..., 0] = 4
     plan = ops.PagedPlan([n], [L], 2 * G, 2, D, 16)
@@ -124,8 +127,9 @@ def test_all_values_large_or_small(ops, kind, power, n, G, L):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("size", [300.0, 7000.0, 40000.0])
-@pytest.mark.parametrize("n,L", [(1, 3000), (5, 700), (40, 3000), (300, 2500)])
-def test_far_scores_of_blocks_of_every_size(ops, kind, size, n, L):
+@pytest.mark.parametrize("spread", [8, 16, 40, 200])
+@pytest.mark.parametrize("n,L", [(1, 3000), (5, 700), (40, 3000), (300, 2500), (300, 300)])
+def test_far_scores_of_blocks_of_every_size(ops, kind, size, spread, n, L):
     """Keys of one direction in steps of 3 per cent, scores to 10^9: the largest visible score decides, with those equal
     to it, whatever the other blocks' values."""
     H, Hk, D, page = 4, 2, 64, 16
@@ -136,7 +140,7 @@ def test_far_scores_of_blocks_of_every_size(ops, kind, size, n, L):
     ids = c.table[0].long()
     c.k[ids] = int(LARGEST[kind]) if kind == I8 else torch.tensor(448.0, device="cuda").to(kind)
     c.ks[ids, :, 0] = (size * 1.03 ** (step - 40) / LARGEST[kind]).float().cuda()[:, None]
-    c.vs[ids, :, 0] = 2.0 ** torch.randint(-100, 100, (blocks, 1), generator=g).float().cuda()
+    c.vs[ids, :, 0] = 2.0 ** (torch.randint(0, spread + 1, (blocks, 1), generator=g).float() - spread / 2).cuda()
     q = (size * (0.5 + torch.rand(n, H, 1, generator=g))).to(BF16).expand(n, H, D).contiguous().cuda()
     plan = ops.PagedPlan([n], [L], H, Hk, D, page)
     got = ops.paged_attention(q, *c.args(), plan, scale=1.0, **c.scales())

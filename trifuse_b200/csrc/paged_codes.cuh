@@ -43,9 +43,12 @@ struct Divisor {
 // The reference r of value scales: a power of two at or above those that are finite
 // (2^-126 .. 2^126; beyond that, near them).  Ratios s_v / r down to 2^-61 are worked
 // with as they are; below that (or at zero, which has no logarithm) scales count as
-// far apart.
+// far apart.  So they do below 2^-13 where scores are so far out (kFar) that a row's
+// reference cannot take in log2(s_v / r): the ratio itself then has to leave a weight
+// f16's 11 bits.
 constexpr float kLeastRef = 1.17549435e-38f, kLeastInverse = 8.50705917e37f;  // 2^-126, 2^126
 constexpr float kLeastRatio = 4.33680869e-19f;                                // 2^-61
+constexpr float kFarRatio = 1.220703125e-4f;                                  // 2^-13
 __device__ __forceinline__ float power_above(float v) {
   return __uint_as_float(min((__float_as_uint(v) + 0x7fffffu) & 0x7f800000u, 0x7e800000u));
 }

@@ -37,8 +37,8 @@
 // scales that the warp has met; where it grows, m falls by as much.  m is the
 // maximum of S + log2(s_v / r), so the largest share of an output is a P' of 2^7 and
 // not rounded, and the weights use f16's range whatever the scales.
-//   Once a warp has met scales more than 2^60 apart (or zero), r / s_v no longer
-// serves: keys with a tiny scale may hold all of a row's weight, or none of it beside
+//   Once a warp has met scales more than 2^61 apart (or zero; 2^13 where scores are
+// far out), r / s_v no longer serves: keys with a tiny scale may hold all of a row's weight, or none of it beside
 // a large one that counts, or one that the row does not see.  From there on l sums
 // 2^(S - mu), mu the scores' own maximum, and m = mu + kappa is kept in two parts.
 //
@@ -518,8 +518,12 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
     // apart (in one loop that rare path cost 2 per cent of the time).
     int tile = sg.tile0 + warp;
 #pragma unroll
-    for (int apart = 0; apart < (kCoded ? 2 : 1); ++apart)
-    if (apart == 0 || __builtin_expect(wide, 0))
+    for (int apart = 0; apart < (kCoded ? 2 : 1); ++apart) {
+    if (apart == 1) {
+      if (__builtin_expect(!wide, 1)) break;
+      if (lane < 16) kappa[lane] = 0.f;
+      __syncwarp();
+    }
     for (; tile < sg.tile1 && ok; tile += kWarps) {
       const int slot = used % S::kStages;
       ok = __all_sync(0xffffffffu, wait_copy(&bars[slot], (uint32_t)((used / S::kStages) & 1), limit_cycles));
@@ -539,7 +543,8 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
           for (int j = 0; j < 4; ++j) s[h][t][j] = 0.f;
       float k_scale[2] = {1.f, 1.f};
       float offset[2], back[2];  // log2(s_v / r), r / s_v
-      bool odd = false;  // a value scale is not finite
+      bool odd = false;     // a value scale is not finite
+      bool spread = false;  // scales too far apart for scores far out
       if constexpr (kCoded) {
         const float4 four = *reinterpret_cast<const float4*>(scales + slot * 4);
         k_scale[0] = four.x;
@@ -557,7 +562,8 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
         if (larger < INFINITY) grow(larger);
         some[0] = v[0] * ref_inverse;
         some[1] = v[1] * ref_inverse;
-        if (__builtin_expect(!(fminf(some[0], some[1]) >= kLeastRatio && max_nan(some[0], some[1]) <= 1.f), 0)) {
+        const float low = fminf(fminf(some[0], some[1]), lowest * ref_inverse);
+        if (__builtin_expect(!(low >= kFarRatio && max_nan(some[0], some[1]) <= 1.f), 0)) {
           bool real[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -570,16 +576,12 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
             if (!real[h]) v[h] = ref;  // any will do
             some[h] = v[h] * ref_inverse;
           }
-          if (apart == 0 && far_apart(fminf(lowest, fminf(v[0], v[1])), ref)) {
-            if (g == 0)
-#pragma unroll
-              for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) kappa[8 * t + c2 + i] = 0.f;
-            __syncwarp();
+          const float least = fminf(lowest, fminf(v[0], v[1]));
+          if (apart == 0 && far_apart(least, ref)) {
             wide = true;
             break;
           }
+          spread = least < ref * kFarRatio;
         }
         lowest = fminf(lowest, fminf(v[0], v[1]));
 #pragma unroll
@@ -616,6 +618,19 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
 #pragma unroll
             for (int t = 0; t < NT; ++t) mma16816<C>(s[h][t], a, qb[k][t][0], qb[k][t][1]);
           }
+        }
+      }
+      if (kCoded && apart == 0 && __builtin_expect(spread, 0)) {
+        bool far = false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) far |= fabsf(s[h][t][j] * (scale[t][j & 1] * k_scale[h])) >= kFar;
+        if (__any_sync(0xffffffffu, far)) {
+          wide = true;
+          break;
         }
       }
       const bool ragged = key0 + kSplitKeys - 1 > first_limit;
@@ -834,6 +849,7 @@ __global__ void __launch_bounds__(Shape<D, NT, C, St>::kThreads, 1)
       ++used;
       if (more) fetch();
       fall = 0.f;
+    }
     }
 
     // Join the warps' results.

@@ -64,10 +64,10 @@
 // maximum 1.4 to 1.6, and 2048 of 16384 took 3% less).
 // That costs a few instructions a block, none a score, and rounds nothing but P'.
 // r is a power of two at or above the segment's value scales (one half: those so
-// far; where it grows, m falls by as much).  Where they lie more than 2^60 apart
+// far; where it grows, m falls by as much).  Where they lie more than 2^61 apart
 // (or are zero), r / s_v no longer serves: keys with a tiny scale may hold all of a
 // row's weight, or none of it beside a large one that counts, or one that the row
-// does not see.  Then l sums 2^(s s_k - m) itself, m is the scores' own maximum, and
+// does not see.  (Where scores are far out, from 2^13 on.)  Then l sums 2^(s s_k - m) itself, m is the scores' own maximum, and
 // O stands at 2^(m + kappa), kappa the largest (s s_k - m) + log2(s_v / r): twice the
 // exponentials, on such segments (one half: from such a tile on).
 //   Two halves (storage Widened): the requests' codes are widened by a kernel of
@@ -254,10 +254,11 @@ struct TileScales {
   float2 back[8];   // r / s_v
   float v_ref;      // r
   float fall;       // log2(r of the tile before / r)
-  uint32_t events;  // bit b: a scale of block b is not finite; bit 8: r grew; bit 9: scales are far apart
+  uint32_t events;  // bit b: a scale of block b is not finite; bit 8: r grew; bit 9: scales are far apart; bit 10:
+                    // too far for scores far out
   uint32_t pad;
 };
-constexpr uint32_t kGrew = 256, kWide = 512;
+constexpr uint32_t kGrew = 256, kWide = 512, kSpread = 1024;
 // Up to 2^9 a maximum and a logarithm add up to within 2^-15, 2e-5 of a weight.
 constexpr float kApart = 512.f;
 // The value scales of a segment (one half: those so far).
@@ -295,7 +296,8 @@ __device__ __forceinline__ void tell(TileScales& to, float k, float v, float sca
     if (lane == 0) {
       to.v_ref = seen.ref;
       to.fall = exponent_of(before) - exponent_of(seen.ref);
-      to.events = odds | (seen.ref != before ? kGrew : 0u) | (seen.wide ? kWide : 0u);
+      to.events = odds | (seen.ref != before ? kGrew : 0u) | (seen.wide ? kWide : 0u) |
+                  (seen.lowest < seen.ref * kFarRatio ? kSpread : 0u);
     }
   }
 }
@@ -1110,6 +1112,11 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
           // Far out the sum's rounding would lie between m and the products that it is
           // taken from: the scores' own maximum there.
           if (__any_sync(0xffffffffu, fabsf(mx) > kFar)) {
+            if (events & kSpread) {  // nothing has changed yet: this tile again
+              wide = true;
+              --s_turn;
+              break;
+            }
             float own = -INFINITY;
 #pragma unroll
             for (int c = 0; c < 128; ++c) own = max_nan(own, __fmul_rn(sc[c], unit_of(c / 16)));
