@@ -72,15 +72,15 @@ def test_a_later_token_of_any_size(ops, kind, power, n, G, L):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("power", [30, 100, 118])
 @pytest.mark.parametrize("gap", [0.5, 20.0, 60.0, 88.0, 150.0, 300.0])
-@pytest.mark.parametrize("blocks", [[0], [14, 15, 16, 17]])
+@pytest.mark.parametrize("blocks", [[0], [14, 15, 16, 17], [38, 39]])
 @pytest.mark.parametrize("n,G,L", ROWS)
 def test_large_values_of_little_weight(ops, kind, power, gap, blocks, n, G, L):
     """Blocks of e^-gap of the weight with values 2^power times as large: the first one, which every row sees, and
-    several after others (tiles of nothing but such)."""
+    several after others (tiles of nothing but such, a warp's first of the few-rows kernel and its second)."""
     D = 128
     c = Cache([L], 2, D, 16, kind, seed=n, spread=1)
     c.k[..., 0] = 0
-    for block in blocks:
+    for block in (b for b in blocks if b < L // BLOCK):
         at = block_of(c, 0, block * BLOCK)
         c.k[at[0]] = 0  # pages of 16: one block
         c.k[at[0], ..., 0] = torch.tensor(-LARGEST[kind], device="cuda").to(kind)
@@ -171,3 +171,25 @@ def test_nan_scales_among_blocks_of_every_size(ops, kind, n, G, L):
         assert torch.isnan(got[before:]).all()
         if before:
             check_rounding(got[:before], ref.rows(slice(0, before)), scattered=False, exponents=2.0 ** -13)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("power", [30, 70, 118])
+@pytest.mark.parametrize("gap", [20.0, 60.0, 150.0])
+@pytest.mark.parametrize("n,G", [(1, 1), (4, 4)])
+def test_scales_that_rise_within_a_warps_tiles(ops, kind, power, gap, n, G):
+    """Requests enough that a block of warps has a whole history: each warp meets large values after small ones."""
+    R, L, D = 80, 817, 128
+    c = Cache([L] * R, 2, D, 16, kind, seed=n, spread=1)
+    c.k[..., 0] = 0
+    at = c.table[:, 26:50].long().flatten()  # the second tiles of the warps
+    c.k[at] = 0
+    c.k[at, ..., 0] = torch.tensor(-LARGEST[kind], device="cuda").to(kind)
+    c.ks[at] = gap * D ** 0.5 / (4 * LARGEST[kind])
+    c.vs[at] *= 2.0 ** power
+    q = queries(R * n, 2 * G, D, n) * 0.5
+    q[..., 0] = 4
+    plan = ops.PagedPlan([n] * R, [L] * R, 2 * G, 2, D, 16)
+    got = ops.paged_attention(q, *c.args(), plan, **c.scales())
+    assert ops.device_error() == 0
+    check_rounding(got, Exact(c, q, [n] * R, [L] * R), scattered=False, exponents=2.0 ** -13)
