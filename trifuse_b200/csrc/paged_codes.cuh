@@ -1,12 +1,15 @@
-// Codes of an 8-bit cache: the storage types I8 and E4M3, narrowing and
-// widening.  Both widen to f16 without rounding (integers up to 127; e4m3 has
-// 4 bits of precision and magnitudes from 2^-9 to 448).
+// Codes of an 8-bit cache: the storage types I8 and E4M3, narrowing and widening,
+// the reference of value scales, and what both attention kernels fetch codes with.
+// Both types widen to f16 without rounding (integers up to 127; e4m3 has 4 bits of
+// precision and magnitudes from 2^-9 to 448).
 #pragma once
 
+#include <cuda.h>
 #include <cuda_fp8.h>
 
 #include "common.cuh"
 #include "paged_pairs.cuh"
+#include "tc_ptx.cuh"
 
 namespace tf {
 
@@ -39,6 +42,13 @@ struct Divisor {
     return fma2(fma2(y, by, x), inverse, y);
   }
 };
+
+// 2^x down to 2^-149.
+__device__ __forceinline__ float exp2_far(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // The reference r of value scales: a power of two at or above those that are finite
 // (2^-126 .. 2^126; beyond that, near them).  Ratios s_v / r down to 2^-61 are worked
@@ -110,5 +120,23 @@ struct Code<E4M3> {
     return __byte_perm(lo, hi, 0x5410);
   }
 };
+
+// `row` .. of a page of codes, all columns.
+__device__ __forceinline__ void tma_codes(void* dst, const CUtensorMap* map, int row, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          tc::smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(page), "r"(tc::smem_addr(bar))
+      : "memory");
+}
+// One value, or zero, into shared memory; the barrier's phase waits for the
+// copies that a thread has begun before it arrives.
+__device__ __forceinline__ void copy_value(float* dst, const float* src, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(tc::smem_addr(dst)), "l"(src), "r"(real ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void arrive_with_copies(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(tc::smem_addr(bar)) : "memory");
+}
 
 }  // namespace tf

@@ -145,23 +145,6 @@ __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int 
       : "memory");
 }
 
-// `row` .. of a page of codes, all columns.
-__device__ __forceinline__ void tma_codes(void* dst, const CUtensorMap* map, int row, int page, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(page), "r"(smem_addr(bar))
-      : "memory");
-}
-// One value, or zero, into shared memory; the barrier's phase waits for the
-// copies that a thread has begun before it arrives.
-__device__ __forceinline__ void copy_value(float* dst, const float* src, bool real) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(real ? 4 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void arrive_with_copies(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -213,13 +196,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Down to 2^-149.
-__device__ __forceinline__ float exp2_far(float x) {
-  float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 

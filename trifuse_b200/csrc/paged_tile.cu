@@ -227,24 +227,6 @@ __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int 
       : "memory");
 }
 
-// `row` .. of a page of codes, all columns.
-__device__ __forceinline__ void tma_codes(void* dst, const CUtensorMap* map, int row, int page, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(page), "r"(smem_addr(bar))
-      : "memory");
-}
-// One value, or zero, into shared memory; the barrier's phase waits for the
-// copies that a thread has begun before it arrives.
-__device__ __forceinline__ void copy_value(float* dst, const float* src, bool real) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(real ? 4 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void arrive_with_copies(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
-}
-
 // What is told of a tile of codes, twice where packed pairs are worked on.  Zero
 // units become the smallest number, 2^-149 (a hidden score of -inf must not meet a
 // zero); of blocks past the request's length, or with scales that are not finite
@@ -364,12 +346,6 @@ __device__ __forceinline__ void rescale(uint32_t t_o, float factor) {
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// Down to 2^-149.
-__device__ __forceinline__ float far_exp2(float x) {
-  float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -1233,7 +1209,7 @@ __global__ void __launch_bounds__(Shape<D, H, C, St>::kThreads, 3 - H)
       // A row that has seen no key above -inf gives zeros.
       const float inv = m == -INFINITY ? 0.f : 1.f / l;
       // 2^kappa r may lie anywhere, but not what it makes of O / l.
-      const float half = kScaled ? far_exp2(0.5f * kappa) : 1.f;
+      const float half = kScaled ? exp2_far(0.5f * kappa) : 1.f;
       T* orow = static_cast<T*>(p.out) +
                 ((int64_t)(g.q_row + token) * p.heads + g.kv_head * p.group + pr % p.group) * D;
       float* prow = p.part + (int64_t)g.part * S::kRows * D + row * 4;
@@ -1325,7 +1301,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps)
     const float m = st[(int64_t)i * 2 * R], own = st[(int64_t)i * 2 * R + R];
     float f;
     if (kDivided) {
-      f = far_exp2(m - M);
+      f = exp2_far(m - M);
       f = m == -INFINITY ? 0.f : f * (own * unit);  // an empty piece holds zeros
       sum += f;
     } else {
